@@ -492,6 +492,65 @@ MCN_API int mcn_softmax_backward(mcn_stream_t stream, float* derInput, const flo
                                  int C, int N);
 
 /* ------------------------------------------------------------------------------------------------
+ * operators with no counterpart in the reference, for training classifiers with very many classes: layer normalisation, a fully
+ * connected layer and its loss as one operator, orthogonalised updates.  Where a call takes a data type, x, y and their
+ * derivatives (and the filters and theirs) are of it; moments, multipliers, biases, labels and weights are single
+ * precision.  Pointers of bfloat16 tensors are 2-byte aligned at least, of single-precision ones 4-byte.
+ * ---------------------------------------------------------------------------------------------- */
+enum { MCN_FLOAT = 0, MCN_BFLOAT16 = 1 };
+
+/* dst[i] = src[i], rounded to nearest (ties to even) where bits are lost; dst and src of two different data types or of one */
+MCN_API int mcn_convert(mcn_stream_t stream, void* dst, int dstType, const void* src, int srcType, size_t n);
+
+/* Layer normalisation: every pixel's C channels, y = multipliers .* (x - mu)/sigma + biases with mu the mean of the channels and
+   sigma = sqrt(their variance + epsilon).  multipliers (NULL: ones) and biases (NULL: zeros) are C values.  `moments` is
+   H x W x N x 2: all mu, then all sigma; givenMoments == 0: written if non-NULL; givenMoments != 0: an input, used as
+   it stands (the derivatives are those of moments taken from x all the same).  Outputs overlap no input. */
+MCN_API int mcn_lnorm_forward(mcn_stream_t stream, int dataType, void* y, float* moments, const void* x, const float* multipliers,
+                              const float* biases, int H, int W, int C, int N, double epsilon, int givenMoments);
+/* derInput (shape of x), derMultipliers, derBiases (C each), all fully overwritten; any of them may be NULL and is not made then.
+   The sums over the pixels are taken in one order for one shape on one kind of device: the same bits every time. */
+MCN_API size_t mcn_lnorm_workspace_bytes(int H, int W, int C, int N);
+MCN_API int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput, float* derMultipliers, float* derBiases, float* moments,
+                               const void* x, const float* multipliers, const void* derOutput, int H, int W, int C, int N,
+                               double epsilon, int givenMoments, void* workspace, size_t workspaceBytes);
+
+/* A fully connected layer and the loss 'softmaxlog' behind it, in pieces of the classes: what mcn_conv_forward and mcn_loss_forward give
+   one after the other, without the N x K tensor of scores.  x: D values per image (H x W x C x N with H*W*C = D), filters: D
+   values per class (a bank of K filters of x's size), biases: K values or NULL, labels: one per image as for mcn_loss_forward (0:
+   the image does not count; of such an image -- or one of weight 0 -- nothing reaches a result, whatever x holds, but its own
+   logSums).  Biases of -infinity take classes out.
+     y[0]      sum over the images of weight * (log sum exp scores - score of the label), over N if normalise
+     logSums   (N values, may be NULL) log sum exp of the scores, for the backward call
+   backward: derInput (shape of x), derFilters (shape of filters), derBiases (K), all fully overwritten, any may be NULL; logSums as the
+   forward call left them, or NULL (made again, a third more work); derOutput the scalar derivative of y.
+   Single precision: products on pairs of half-precision values, as exact as single-precision ones; P = softmax - 1 at the label is held
+   to 2^-39.  bfloat16: products of the bfloat16 values in single precision, P times the image's weight rounded to bfloat16.
+   workspace: mcn_fcloss_workspace_bytes(g, 0 forward / 1 backward). */
+typedef struct mcn_fcloss_geom {
+  int D, K, N;
+  int normalise;   /* reference default: true */
+  int dataType;    /* MCN_FLOAT or MCN_BFLOAT16 */
+} mcn_fcloss_geom;
+MCN_API size_t mcn_fcloss_workspace_bytes(const mcn_fcloss_geom* g, int backward);
+MCN_API int mcn_fcloss_forward(mcn_stream_t stream, const mcn_fcloss_geom* g, float* y, float* logSums, const void* x, const void* filters,
+                               const float* biases, const float* labels, size_t nLabels, const float* instanceWeights,
+                               size_t nWeights, void* workspace, size_t workspaceBytes);
+MCN_API int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, void* derInput, void* derFilters, float* derBiases,
+                                const float* logSums, const void* x, const void* filters, const float* biases, const float* labels,
+                                size_t nLabels, const float* instanceWeights, size_t nWeights, double derOutput, void* workspace,
+                                size_t workspaceBytes);
+
+/* `count` matrices of K x D single-precision values (filter banks: K filters of D = FH*FW*FC values each, as they lie in memory), one behind
+   the other: each is divided by its Frobenius norm and taken `steps` times (5 is usual) through
+     X <- a X + b (X X') X + c (X X')^2 X,  a = 3.4445, b = -4.7750, c = 2.0315,
+   which brings its singular values close to 1 (within [0.68, 1.21] for those above 1/200 of the norm).  The zero matrix stays zero.
+   Products on pairs of half-precision values, as exact as single-precision ones.  y does not overlap x. */
+MCN_API size_t mcn_orthogonalise_workspace_bytes(int K, int D, int count);
+MCN_API int mcn_orthogonalise(mcn_stream_t stream, float* y, const float* x, int K, int D, int count, int steps, void* workspace,
+                              size_t workspaceBytes);
+
+/* ------------------------------------------------------------------------------------------------
  * double precision -- the operators' VLDT_Double instantiation (bits/impl/dispatcher.hpp:60-98 switches on the
  * tensors' data type; bits/nnconv.cu:444-469, bits/nnbnorm.cu:388-442, bits/nnpooling.cu:270-282 instantiate
  * every product for float and double).  Same arguments and meaning as the single-precision calls above.  Pooling

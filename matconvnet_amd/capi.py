@@ -34,6 +34,12 @@ class LossGeom(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("H", "W", "C", "N", "loss", "topK", "normalise")] + [("threshold", C.c_double)]
 
 
+class FcLossGeom(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("D", "K", "N", "normalise", "dataType")]
+
+
+FLOAT, BFLOAT16 = 0, 1   # MCN_FLOAT, MCN_BFLOAT16
+
 LOSSES = ("classerror", "topkerror", "log", "softmaxlog", "mhinge", "mshinge", "binaryerror", "binarylog", "logistic",
           "hinge")
 
@@ -117,6 +123,15 @@ PROTOTYPES = {
     "mcn_loss_workspace_bytes": (_sz, [C.POINTER(LossGeom)]),
     "mcn_loss_forward": (_i, [_vp, C.POINTER(LossGeom), _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz]),
     "mcn_loss_backward": (_i, [_vp, C.POINTER(LossGeom), _vp, _vp, _vp, _sz, _vp, _sz, _d]),
+    "mcn_convert": (_i, [_vp, _vp, _i, _vp, _i, _sz]),
+    "mcn_lnorm_forward": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _d, _i]),
+    "mcn_lnorm_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "mcn_lnorm_backward": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _d, _i, _vp, _sz]),
+    "mcn_fcloss_workspace_bytes": (_sz, [C.POINTER(FcLossGeom), _i]),
+    "mcn_fcloss_forward": (_i, [_vp, C.POINTER(FcLossGeom), _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz]),
+    "mcn_fcloss_backward": (_i, [_vp, C.POINTER(FcLossGeom), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _d, _vp, _sz]),
+    "mcn_orthogonalise_workspace_bytes": (_sz, [_i, _i, _i]),
+    "mcn_orthogonalise": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz]),
     "mcn_conv_forward_f64": (_i, [_vp, C.POINTER(ConvGeom), _vp, _d, _vp, _d, _vp, _vp]),
     "mcn_conv_backward_data_f64": (_i, [_vp, C.POINTER(ConvGeom), _vp, _vp, _vp]),
     "mcn_conv_backward_filter_f64": (_i, [_vp, C.POINTER(ConvGeom), _vp, _vp, _vp]),
@@ -679,6 +694,146 @@ def loss_backward(x, c, dzdy, g, instance_weights=None):
     check(lib().mcn_loss_backward(stream(), C.byref(g), ptr(dx), ptr(x), ptr(c), c.numel(), ptr(instance_weights),
                                   0 if instance_weights is None else instance_weights.numel(), float(dzdy)))
     return dx
+
+
+def data_type(*tensors):
+    """MCN_FLOAT or MCN_BFLOAT16: the data type of all the given tensors (None is passed over)."""
+    torch = _torch()
+    kinds = {t.dtype for t in tensors if t is not None}
+    if len(kinds) != 1:
+        raise TypeError("tensors of different data types: %s" % sorted(str(k) for k in kinds))
+    kind = kinds.pop()
+    if kind not in (torch.float32, torch.bfloat16):
+        raise TypeError("neither single precision nor bfloat16: %s" % kind)
+    return BFLOAT16 if kind == torch.bfloat16 else FLOAT
+
+
+def _single(**tensors):
+    for name, t in tensors.items():
+        if t is not None and t.dtype != _torch().float32:
+            raise TypeError("%s is not single precision: %s" % (name, t.dtype))
+
+
+def _dense(**tensors):
+    for name, t in tensors.items():
+        if t is not None and not (t.is_cuda and t.is_contiguous()):
+            raise ValueError("%s is not a contiguous tensor on the device" % name)
+
+
+def convert(x, dtype):
+    """x as float32 or bfloat16 (include/mcn_hip.h: mcn_convert)."""
+    _dense(x=x)
+    y = _torch().empty_like(x, dtype=dtype)
+    check(lib().mcn_convert(stream(), ptr(y), data_type(y), ptr(x), data_type(x), x.numel()))
+    return y
+
+
+def _per_channel(C_, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.numel() != C_:
+            raise ValueError("%s does not have one value per channel" % name)
+
+
+def lnorm_forward(x, g, b, eps=1e-5, moments=None):
+    """Layer normalisation (include/mcn_hip.h: mcn_lnorm_forward): (y, moments).  x: float32 or bfloat16; g, b: float32 or None;
+    moments (2, N, W, H) in float32: all means, then all sigmas; given ones are used as they stand."""
+    H, W, Cc, N = _hwcn(x)
+    _single(g=g, b=b, moments=moments)
+    _dense(x=x, g=g, b=b, moments=moments)
+    _per_channel(Cc, g=g, b=b)
+    given = moments is not None
+    if given and moments.numel() != 2 * H * W * N:
+        raise ValueError("moments does not have two values per pixel")
+    y = _torch().empty_like(x)
+    mom = moments if given else empty((H, W, N, 2))
+    check(lib().mcn_lnorm_forward(stream(), data_type(x), ptr(y), ptr(mom), ptr(x), ptr(g), ptr(b), H, W, Cc, N, eps, int(given)))
+    return y, mom
+
+
+def lnorm_backward(x, g, dy, eps=1e-5, moments=None, want=(True, True, True), ws=None):
+    """(dzdx, dzdg, dzdb) of layer normalisation; those not wanted are None.  moments: as lnorm_forward left them, or None."""
+    ws = ws or _ws
+    H, W, Cc, N = _hwcn(x)
+    _single(g=g, moments=moments)
+    _dense(x=x, g=g, dy=dy, moments=moments)
+    _per_channel(Cc, g=g)
+    if dy.numel() != x.numel():
+        raise ValueError("x and dy do not have the same number of elements")
+    if moments is not None and moments.numel() != 2 * H * W * N:
+        raise ValueError("moments does not have two values per pixel")
+    dx = _torch().empty_like(x) if want[0] else None
+    dg = empty((Cc,)) if want[1] else None
+    db = empty((Cc,)) if want[2] else None
+    wp, wn = ws.get(lib().mcn_lnorm_workspace_bytes(H, W, Cc, N))
+    check(lib().mcn_lnorm_backward(stream(), data_type(x, dy), ptr(dx), ptr(dg), ptr(db), ptr(moments), ptr(x), ptr(g), ptr(dy), H, W, Cc, N,
+                                   eps, int(moments is not None), wp, wn))
+    return dx, dg, db
+
+
+def fcloss_geom(x, f, normalise=True):
+    """Geometry of mcn_fcloss_*: x (N, ...) and f (K, ...), of as many values per instance as per class."""
+    N, K = int(x.shape[0]), int(f.shape[0])
+    D = x.numel() // N if N else (f.numel() // K if K else 0)
+    if D * N != x.numel() or D * K != f.numel():
+        raise ValueError("the filters do not cover the instances' values")
+    return FcLossGeom(D, K, N, int(bool(normalise)), data_type(x, f))
+
+
+def _fcloss_check(x, f, b, c, instance_weights, log_sums):
+    _single(b=b, c=c, instance_weights=instance_weights, log_sums=log_sums)
+    _dense(x=x, f=f, b=b, c=c, instance_weights=instance_weights, log_sums=log_sums)
+    if b is not None and b.numel() != f.shape[0]:
+        raise ValueError("b does not have one value per class")
+    if log_sums is not None and log_sums.numel() != x.shape[0]:
+        raise ValueError("log_sums does not have one value per instance")
+
+
+def fcloss_forward(x, f, b, c, instance_weights=None, normalise=True, ws=None):
+    """Softmax cross entropy of the scores x.f + b against the labels c (1..K as floats, 0: does not count), without a tensor of
+    scores (include/mcn_hip.h: mcn_fcloss_forward): (y, log_sums).  x, f: float32 or bfloat16, b, c: float32."""
+    ws = ws or _ws
+    _fcloss_check(x, f, b, c, instance_weights, None)
+    g = fcloss_geom(x, f, normalise)
+    y, log_sums = empty((1,)), empty((g.N,))
+    wp, wn = ws.get(lib().mcn_fcloss_workspace_bytes(C.byref(g), 0))
+    check(lib().mcn_fcloss_forward(stream(), C.byref(g), ptr(y), ptr(log_sums), ptr(x), ptr(f), ptr(b), ptr(c), c.numel(), ptr(instance_weights),
+                                   0 if instance_weights is None else instance_weights.numel(), wp, wn))
+    return y, log_sums
+
+
+def fcloss_backward(x, f, b, c, dzdy=1.0, instance_weights=None, normalise=True, log_sums=None, want=(True, True, True), ws=None):
+    """(dzdx, dzdf, dzdb) of fcloss_forward; those not wanted are None.  log_sums: as fcloss_forward left them, or None."""
+    ws = ws or _ws
+    _fcloss_check(x, f, b, c, instance_weights, log_sums)
+    g = fcloss_geom(x, f, normalise)
+    torch = _torch()
+    dx = torch.empty_like(x) if want[0] else None
+    df = torch.empty_like(f) if want[1] else None
+    db = empty((g.K,)) if want[2] else None
+    wp, wn = ws.get(lib().mcn_fcloss_workspace_bytes(C.byref(g), 1))
+    check(lib().mcn_fcloss_backward(stream(), C.byref(g), ptr(dx), ptr(df), ptr(db), ptr(log_sums), ptr(x), ptr(f), ptr(b), ptr(c), c.numel(),
+                                    ptr(instance_weights), 0 if instance_weights is None else instance_weights.numel(), float(dzdy), wp, wn))
+    return dx, df, db
+
+
+def _banks(x):
+    """count, K, D of filter banks one behind the other: a tensor (count, K, ...)"""
+    if x.dim() < 3:
+        raise ValueError("filter banks one behind the other are a tensor (count, K, ...)")
+    count, K = int(x.shape[0]), int(x.shape[1])
+    return count, K, (x.numel() // (count * K) if count * K else 0)
+
+
+def orthogonalise(x, steps=5, ws=None):
+    """Filter banks (count, K, ...) in float32, each orthogonalised by Newton-Schulz products (include/mcn_hip.h: mcn_orthogonalise)."""
+    ws = ws or _ws
+    _single(x=x)
+    _dense(x=x)
+    count, K, D = _banks(x)
+    y = _torch().empty_like(x)
+    wp, wn = ws.get(lib().mcn_orthogonalise_workspace_bytes(K, D, count))
+    check(lib().mcn_orthogonalise(stream(), ptr(y), ptr(x), K, D, count, int(steps), wp, wn))
+    return y
 
 
 def relu_forward(x, leak=None):

@@ -129,6 +129,17 @@ __global__ __launch_bounds__(256) void taccum64_kernel(double* __restrict__ y, d
   }
 }
 
+// single precision <-> bfloat16, four values a step
+template <class D, class S>
+__global__ __launch_bounds__(256) void convert_kernel(D* __restrict__ dst, const S* __restrict__ src, size_t n, bool vec) {
+  typedef S from4 __attribute__((ext_vector_type(4)));
+  typedef D to4 __attribute__((ext_vector_type(4)));
+  const size_t stride = (size_t)gridDim.x * 256, t = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t whole = vec ? n / 4 : 0;
+  for (size_t i = t; i < whole; i += stride) ((to4*)dst)[i] = __builtin_convertvector(((const from4*)src)[i], to4);
+  for (size_t i = whole * 4 + t; i < n; i += stride) dst[i] = (D)src[i];
+}
+
 }  // namespace
 }  // namespace mcn
 
@@ -178,6 +189,22 @@ int mcn_sgd_momentum(mcn_stream_t stream, float* value, float* state, const floa
   hipLaunchKernelGGL(sgd_momentum_kernel, dim3((unsigned)chunks), dim3(256), 0, as_stream(stream), value, state, der,
                      chunkParam, rates, learningRate, weightDecay, (float)momentum, (float)derScale, nesterov ? 1 : 0);
   return check_launch("mcn_sgd_momentum");
+}
+int mcn_convert(mcn_stream_t stream, void* dst, int dstType, const void* src, int srcType, size_t n) {
+  if ((dstType != MCN_FLOAT && dstType != MCN_BFLOAT16) || (srcType != MCN_FLOAT && srcType != MCN_BFLOAT16))
+    return fail(MCN_ILLEGAL_ARGUMENT, "mcn_convert: unknown data type");
+  if (n == 0) return MCN_SUCCESS;
+  if (!dst || !src) return fail(MCN_ILLEGAL_ARGUMENT, "mcn_convert: null tensor");
+  const size_t blocks = std::min<size_t>((n + 1023) / 1024, 256u * 32u);
+  hipStream_t s = as_stream(stream);
+  KernelTimer timer("convert_kernel", s);
+  const bool vec = aligned16(dst) && aligned16(src);
+  const dim3 grid((unsigned)blocks), block(256);
+  if (dstType == MCN_FLOAT && srcType == MCN_FLOAT) hipLaunchKernelGGL((convert_kernel<float, float>), grid, block, 0, s, (float*)dst, (const float*)src, n, vec);
+  else if (dstType == MCN_FLOAT) hipLaunchKernelGGL((convert_kernel<float, __bf16>), grid, block, 0, s, (float*)dst, (const __bf16*)src, n, vec);
+  else if (srcType == MCN_FLOAT) hipLaunchKernelGGL((convert_kernel<__bf16, float>), grid, block, 0, s, (__bf16*)dst, (const float*)src, n, vec);
+  else hipLaunchKernelGGL((convert_kernel<__bf16, __bf16>), grid, block, 0, s, (__bf16*)dst, (const __bf16*)src, n, vec);
+  return check_launch("mcn_convert");
 }
 int mcn_fill(mcn_stream_t stream, float* y, float value, size_t n) {
   return launch<OP_FILL>("mcn_fill", stream, y, nullptr, nullptr, value, n);

@@ -1,0 +1,657 @@
+// Layer normalisation: the C channels of every pixel (of every image) are brought to mean 0 and deviation 1, then scaled and shifted per
+// channel.
+//   mu = mean_c x, sigma = sqrt(mean_c (x - mu)^2 + epsilon), xh = (x - mu)/sigma, y = g xh + b
+//   a = g dzdy:  dzdx = (a - mean_c a - xh mean_c(a xh))/sigma,  dzdg = sum over pixels of dzdy xh,  dzdb = sum of dzdy
+// Bound by memory: x is read once (it stays in registers between the mean, the squares about the mean and the output), x and dzdy
+// once in the backward pass.  The derivatives of g and b are sums over all pixels: every workgroup walks over many pixels with its
+// share of the sums in registers and leaves one partial sum per channel, which a second launch adds up in a fixed order.
+//
+// Two layouts.  "Rows": H = W = 1, a pixel's channels are neighbours; T lanes (16, 64, 256 or 1024) share a row.  "Planes": channels are a
+// plane apart; a lane is a pixel and the wavefronts of a workgroup share the channels.  Pixels with more channels than a workgroup
+// holds in registers are walked three times (lnorm_long_*).
+#include "mcn_internal.hpp"
+
+#include <algorithm>
+
+namespace mcn {
+namespace {
+
+typedef unsigned short bf16;
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return __builtin_bit_cast(float, (unsigned)v << 16); }
+template <class V> __device__ __forceinline__ V from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 from_float<bf16>(float v) { return __builtin_bit_cast(bf16, (__bf16)v); }
+
+template <class V, int N> struct alignas(sizeof(V) * N) Pack { V v[N]; };
+
+struct LnP {
+  int C, HW;
+  size_t items;        // pixels of all images
+  float epsilon;
+  int given;           // moments are an input
+};
+
+// The sums of two values over the T threads of a group; T > 64: over the wavefronts by local memory, with a barrier that the whole
+// workgroup reaches (two sets of slots in turn: one barrier per sum).
+template <int T>
+__device__ __forceinline__ void group_sum(float& a, float& b, float2* slots) {
+#pragma unroll
+  for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o, kWave);
+    b += __shfl_xor(b, o, kWave);
+  }
+  if (T > 64) {
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) slots[wave] = make_float2(a, b);
+    __syncthreads();
+    const int first = wave / (T / 64) * (T / 64);
+    a = b = 0.f;
+#pragma unroll
+    for (int k = 0; k < T / 64; ++k) {
+      const float2 s = slots[first + k];
+      a += s.x;
+      b += s.y;
+    }
+  }
+}
+
+// A row's values this thread holds: NCH packs of VEC neighbours, T packs apart.  What is behind the row's end is zero.
+template <class V, int VEC, int T, int NCH>
+__device__ __forceinline__ void load_row(float (&out)[NCH * VEC], const V* __restrict__ row, int C, int t) {
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = (i * T + t) * VEC;
+    Pack<V, VEC> p = {};
+    if (c < C) p = *(const Pack<V, VEC>*)(row + c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) out[i * VEC + e] = to_float(p.v[e]);
+  }
+}
+template <class V, int VEC, int T, int NCH>
+__device__ __forceinline__ void store_row(V* __restrict__ row, const float (&v)[NCH * VEC], int C, int t) {
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = (i * T + t) * VEC;
+    if (c >= C) continue;
+    Pack<V, VEC> p;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) p.v[e] = from_float<V>(v[i * VEC + e]);
+    *(Pack<V, VEC>*)(row + c) = p;
+  }
+}
+
+// mean and sigma of a row held by a group; the squares are taken about the mean
+template <int VEC, int T, int NCH>
+__device__ __forceinline__ void row_moments(const float (&x)[NCH * VEC], int C, float epsilon, int t, float2* slots, float* mu, float* sigma) {
+  float s = 0.f, none = 0.f;
+#pragma unroll
+  for (int i = 0; i < NCH * VEC; ++i) s += x[i];
+  group_sum<T>(s, none, slots);
+  const float m = s / C;
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = (i * T + t) * VEC < C ? x[i * VEC + e] - m : 0.f;
+      q += d * d;
+    }
+  group_sum<T>(q, none, slots + 16);
+  *mu = m;
+  *sigma = sqrtf(q / C + epsilon);
+}
+
+template <class V, int VEC, int T, int NCH>
+__global__ __launch_bounds__(T > 256 ? T : 256) void lnorm_rows_forward(V* __restrict__ y, float* __restrict__ moments, const V* __restrict__ x,
+                                                                        const float* __restrict__ g, const float* __restrict__ b, LnP p) {
+  constexpr int kThreads = T > 256 ? T : 256;
+  __shared__ float2 slots[32];
+  const size_t row = (size_t)blockIdx.x * (kThreads / T) + threadIdx.x / T;
+  const bool live = row < p.items;   // (whole groups; they stay for the barriers)
+  const int t = threadIdx.x % T;
+  float v[NCH * VEC];
+  load_row<V, VEC, T, NCH>(v, x + (live ? row : 0) * (size_t)p.C, p.C, t);
+  float mu, sigma;
+  if (p.given) {
+    mu = moments[live ? row : 0];
+    sigma = moments[p.items + (live ? row : 0)];
+  } else {
+    row_moments<VEC, T, NCH>(v, p.C, p.epsilon, t, slots, &mu, &sigma);
+  }
+  if (!live) return;
+  if (!p.given && moments && t == 0) {
+    moments[row] = mu;
+    moments[p.items + row] = sigma;
+  }
+  const float inv = 1.f / sigma;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = (i * T + t) * VEC;
+    Pack<float, VEC> pg = {}, pb = {};
+    if (c < p.C) {
+      if (g) pg = *(const Pack<float, VEC>*)(g + c);
+      if (b) pb = *(const Pack<float, VEC>*)(b + c);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[i * VEC + e] = (v[i * VEC + e] - mu) * inv * (g ? pg.v[e] : 1.f) + pb.v[e];
+  }
+  store_row<V, VEC, T, NCH>(y + row * (size_t)p.C, v, p.C, t);
+}
+
+// partials: [workgroups][2][C]
+template <class V, int VEC, int T, int NCH>
+__global__ __launch_bounds__(1024) void lnorm_rows_backward(V* __restrict__ dx, float* __restrict__ partials, float* __restrict__ moments,
+                                                            const V* __restrict__ x, const float* __restrict__ g, const V* __restrict__ dy,
+                                                            LnP p) {
+  constexpr int kGroups = 1024 / T, W = NCH * VEC;
+  __shared__ float2 slots[64];
+  __shared__ float join[T * W > 1024 ? T * W : 1024];
+  const int t = threadIdx.x % T, group = threadIdx.x / T;
+  float scale[W], sumG[W], sumB[W];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = (i * T + t) * VEC;
+    Pack<float, VEC> pg = {};
+    if (g && c < p.C) pg = *(const Pack<float, VEC>*)(g + c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) scale[i * VEC + e] = g ? pg.v[e] : 1.f;
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i) sumG[i] = sumB[i] = 0.f;
+  const size_t step = (size_t)gridDim.x * kGroups;
+  int turn = 0;
+  for (size_t first = (size_t)blockIdx.x * kGroups; first < p.items; first += step) {
+    const size_t row = first + group;
+    const bool live = row < p.items;
+    const size_t at = (live ? row : 0) * (size_t)p.C;
+    float v[W], d[W];
+    load_row<V, VEC, T, NCH>(v, x + at, p.C, t);
+    load_row<V, VEC, T, NCH>(d, dy + at, p.C, t);
+    float mu, sigma;
+    if (p.given) {
+      mu = moments[live ? row : 0];
+      sigma = moments[p.items + (live ? row : 0)];
+    } else {
+      row_moments<VEC, T, NCH>(v, p.C, p.epsilon, t, slots, &mu, &sigma);
+      if (moments && live && t == 0) {
+        moments[row] = mu;
+        moments[p.items + row] = sigma;
+      }
+    }
+    const float inv = 1.f / sigma;
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      v[i] = (v[i] - mu) * inv;   // (behind the row's end d is zero)
+      const float a = d[i] * scale[i];
+      s1 += a;
+      s2 += a * v[i];
+    }
+    group_sum<T>(s1, s2, slots + 32 + 16 * turn);
+    turn ^= 1;
+    s1 /= p.C;
+    s2 /= p.C;
+    if (!live) continue;   // (nobody waits for anybody in what is left of this turn)
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      sumG[i] += d[i] * v[i];
+      sumB[i] += d[i];
+      d[i] = (d[i] * scale[i] - s1 - v[i] * s2) * inv;
+    }
+    if (dx) store_row<V, VEC, T, NCH>(dx + at, d, p.C, t);
+  }
+  if (!partials) return;
+  // the groups' sums, in the order of the groups
+  float* out = partials + (size_t)blockIdx.x * 2 * p.C;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    for (int k = 0; k < kGroups; ++k) {
+      __syncthreads();
+      if (group == k) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float mine = which ? sumB[i] : sumG[i];
+          join[i * T + t] = k ? join[i * T + t] + mine : mine;
+        }
+      }
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const int c = ((i / VEC) * T + t) * VEC + i % VEC;
+        if (c < p.C) out[which * p.C + c] = join[i * T + t];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- planes
+
+__device__ __forceinline__ size_t pixel_base(size_t item, const LnP& p) {
+  const size_t n = item / p.HW;
+  return n * (size_t)p.HW * p.C + (item - n * p.HW);
+}
+
+// sums over the W wavefronts of what each lane (a pixel) has
+template <int W>
+__device__ __forceinline__ void waves_sum(float& a, float& b, float2* slots) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  slots[wave * 64 + lane] = make_float2(a, b);
+  __syncthreads();
+  a = b = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float2 s = slots[w * 64 + lane];
+    a += s.x;
+    b += s.y;
+  }
+}
+
+template <int W, int K>
+__device__ __forceinline__ void pixel_moments(const float (&v)[K], int C, float epsilon, float2* slots, float* mu, float* sigma) {
+  const int wave = threadIdx.x >> 6;
+  float s = 0.f, none = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) s += v[k];
+  waves_sum<W>(s, none, slots);
+  const float m = s / C;
+  float q = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const float d = k * W + wave < C ? v[k] - m : 0.f;
+    q += d * d;
+  }
+  waves_sum<W>(q, none, slots + W * 64);
+  *mu = m;
+  *sigma = sqrtf(q / C + epsilon);
+}
+
+// K channels per wavefront: c = k W + wave
+template <class V, int W, int K>
+__global__ __launch_bounds__(64 * W) void lnorm_planes_forward(V* __restrict__ y, float* __restrict__ moments, const V* __restrict__ x,
+                                                               const float* __restrict__ g, const float* __restrict__ b, LnP p) {
+  __shared__ float2 slots[2 * W * 64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const size_t item = (size_t)blockIdx.x * 64 + lane;
+  const bool live = item < p.items;
+  const size_t base = pixel_base(live ? item : 0, p);
+  float v[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = k * W + wave < p.C ? to_float(x[base + (size_t)(k * W + wave) * p.HW]) : 0.f;
+  float mu, sigma;
+  if (p.given) {
+    mu = moments[live ? item : 0];
+    sigma = moments[p.items + (live ? item : 0)];
+  } else {
+    pixel_moments<W, K>(v, p.C, p.epsilon, slots, &mu, &sigma);
+  }
+  if (!live) return;
+  if (!p.given && moments && wave == 0) {
+    moments[item] = mu;
+    moments[p.items + item] = sigma;
+  }
+  const float inv = 1.f / sigma;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = k * W + wave;
+    if (c < p.C) y[base + (size_t)c * p.HW] = from_float<V>((v[k] - mu) * inv * (g ? g[c] : 1.f) + (b ? b[c] : 0.f));
+  }
+}
+
+template <class V, int W, int K>
+__global__ __launch_bounds__(64 * W) void lnorm_planes_backward(V* __restrict__ dx, float* __restrict__ partials, float* __restrict__ moments,
+                                                                const V* __restrict__ x, const float* __restrict__ g, const V* __restrict__ dy,
+                                                                LnP p) {
+  __shared__ float2 slots[4 * W * 64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  float sumG[K], sumB[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) sumG[k] = sumB[k] = 0.f;
+  int turn = 0;
+  for (size_t first = (size_t)blockIdx.x * 64; first < p.items; first += (size_t)gridDim.x * 64) {
+    const size_t item = first + lane;
+    const bool live = item < p.items;
+    const size_t base = pixel_base(live ? item : 0, p);
+    float v[K], d[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = k * W + wave;
+      v[k] = c < p.C ? to_float(x[base + (size_t)c * p.HW]) : 0.f;
+      d[k] = c < p.C && live ? to_float(dy[base + (size_t)c * p.HW]) : 0.f;
+    }
+    float mu, sigma;
+    if (p.given) {
+      mu = moments[live ? item : 0];
+      sigma = moments[p.items + (live ? item : 0)];
+    } else {
+      pixel_moments<W, K>(v, p.C, p.epsilon, slots, &mu, &sigma);
+      if (moments && live && wave == 0) {
+        moments[item] = mu;
+        moments[p.items + item] = sigma;
+      }
+    }
+    const float inv = 1.f / sigma;
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = k * W + wave;
+      v[k] = (v[k] - mu) * inv;
+      const float a = c < p.C && g ? d[k] * g[c] : d[k];
+      s1 += a;
+      s2 += a * v[k];
+    }
+    waves_sum<W>(s1, s2, slots + (2 + turn) * W * 64);
+    turn ^= 1;
+    s1 /= p.C;
+    s2 /= p.C;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = k * W + wave;
+      if (c >= p.C) continue;
+      if (live) sumG[k] += d[k] * v[k];   // (a pixel behind the last may hold anything)
+      sumB[k] += d[k];
+      if (dx && live) dx[base + (size_t)c * p.HW] = from_float<V>((d[k] * (g ? g[c] : 1.f) - s1 - v[k] * s2) * inv);
+    }
+  }
+  if (!partials) return;
+  float* out = partials + (size_t)blockIdx.x * 2 * p.C;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = k * W + wave;
+    const float a = wave_sum(sumG[k]), b = wave_sum(sumB[k]);
+    if (lane == 0 && c < p.C) {
+      out[c] = a;
+      out[p.C + c] = b;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- any number of channels
+
+// Rows: a workgroup per pixel, threads along the channels.  Planes: a lane per pixel, four wavefronts share the channels.
+template <bool ROWS>
+__device__ __forceinline__ void long_sum(float& a, float& b, float2* slots) {
+  if (ROWS) {
+    group_sum<256>(a, b, slots);
+  } else {
+    waves_sum<4>(a, b, slots);
+  }
+  __syncthreads();
+}
+
+template <class V, bool ROWS, bool BACKWARD>
+__global__ __launch_bounds__(256) void lnorm_long(V* __restrict__ out, float* __restrict__ moments, const V* __restrict__ x,
+                                                  const float* __restrict__ g, const float* __restrict__ b, const V* __restrict__ dy, LnP p) {
+  __shared__ float2 slots[256];
+  const size_t item = ROWS ? (size_t)blockIdx.x : (size_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const bool live = item < p.items;
+  const size_t base = ROWS ? item * p.C : pixel_base(live ? item : 0, p), step = ROWS ? 1 : p.HW;
+  const int c0 = ROWS ? threadIdx.x : threadIdx.x >> 6, cs = ROWS ? 256 : 4;
+  float mu, sigma, none = 0.f;
+  if (p.given) {
+    mu = moments[live ? item : 0];
+    sigma = moments[p.items + (live ? item : 0)];
+  } else {
+    float s = 0.f, q = 0.f;
+    for (int c = c0; c < p.C; c += cs) s += to_float(x[base + c * step]);
+    long_sum<ROWS>(s, none, slots);
+    mu = s / p.C;
+    for (int c = c0; c < p.C; c += cs) {
+      const float d = to_float(x[base + c * step]) - mu;
+      q += d * d;
+    }
+    long_sum<ROWS>(q, none, slots);
+    sigma = sqrtf(q / p.C + p.epsilon);
+    if (moments && live && c0 == 0) {
+      moments[item] = mu;
+      moments[p.items + item] = sigma;
+    }
+  }
+  const float inv = 1.f / sigma;
+  if (!BACKWARD) {
+    if (live)
+      for (int c = c0; c < p.C; c += cs)
+        out[base + c * step] = from_float<V>((to_float(x[base + c * step]) - mu) * inv * (g ? g[c] : 1.f) + (b ? b[c] : 0.f));
+    return;
+  }
+  if (!out) return;   // (only the moments were wanted)
+  float s1 = 0.f, s2 = 0.f;
+  for (int c = c0; c < p.C; c += cs) {
+    const float a = to_float(dy[base + c * step]) * (g ? g[c] : 1.f);
+    s1 += a;
+    s2 += a * ((to_float(x[base + c * step]) - mu) * inv);
+  }
+  long_sum<ROWS>(s1, s2, slots);
+  s1 /= p.C;
+  s2 /= p.C;
+  if (live)
+    for (int c = c0; c < p.C; c += cs) {
+      const float v = (to_float(x[base + c * step]) - mu) * inv;
+      out[base + c * step] = from_float<V>((to_float(dy[base + c * step]) * (g ? g[c] : 1.f) - s1 - v * s2) * inv);
+    }
+}
+
+// Partial sums of dzdg and dzdb from stored moments.  Rows: a thread per channel, blockIdx.y a run of pixels.  Planes: a workgroup per
+// channel and run of pixels.
+template <class V, bool ROWS>
+__global__ __launch_bounds__(256) void lnorm_long_sums(float* __restrict__ partials, const float* __restrict__ moments, const V* __restrict__ x,
+                                                       const V* __restrict__ dy, LnP p, size_t run) {
+  const size_t first = (size_t)blockIdx.y * run, last = std::min(first + run, p.items);
+  float a = 0.f, b = 0.f;
+  int c;
+  if (ROWS) {
+    c = (int)blockIdx.x * 256 + threadIdx.x;
+    if (c >= p.C) return;
+    for (size_t i = first; i < last; ++i) {
+      const float d = to_float(dy[i * p.C + c]);
+      a += d * ((to_float(x[i * p.C + c]) - moments[i]) / moments[p.items + i]);
+      b += d;
+    }
+  } else {
+    __shared__ float2 slots[16];
+    c = (int)blockIdx.x;
+    for (size_t i = first + threadIdx.x; i < last; i += 256) {
+      const size_t at = pixel_base(i, p) + (size_t)c * p.HW;
+      const float d = to_float(dy[at]);
+      a += d * ((to_float(x[at]) - moments[i]) / moments[p.items + i]);
+      b += d;
+    }
+    group_sum<256>(a, b, slots);
+    if (threadIdx.x) return;
+  }
+  float* out = partials + (size_t)blockIdx.y * 2 * p.C;
+  out[c] = a;
+  out[p.C + c] = b;
+}
+
+// dzdg and dzdb from the workgroups' partial sums: 16 lanes x 16 channels per workgroup, in double, in a fixed order
+__global__ __launch_bounds__(256) void lnorm_join(float* __restrict__ dg, float* __restrict__ db, const float* __restrict__ partials, int C, int parts) {
+  __shared__ double slots[16][17];
+  const int t = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int c = (int)blockIdx.x * 16 + t;   // of the 2 C sums
+  double s = 0.0;
+  if (c < 2 * C)
+    for (int k = r; k < parts; k += 16) s += (double)partials[(size_t)k * 2 * C + c];
+  slots[r][t] = s;
+  __syncthreads();
+  if (r || c >= 2 * C) return;
+  for (int k = 1; k < 16; ++k) s += slots[k][t];
+  float* out = c < C ? dg : db;
+  if (out) out[c < C ? c : c - C] = (float)s;
+}
+
+// ---------------------------------------------------------------------------------------------- host
+
+constexpr int kMostRow = 16384, kMostPlane = 512;   // channels that a workgroup of 1024 holds, 16 (32) a thread
+constexpr int kRuns = 256;                          // runs of pixels in lnorm_long_sums
+
+bool in_registers(int C, size_t HW) { return HW == 1 ? C <= kMostRow : C <= kMostPlane; }
+
+// workgroups of a backward pass that sums as it goes: one per compute unit, and no more than there is work for
+int backward_groups(int C, size_t HW, size_t items) {
+  const size_t cus = std::max(1, device_compute_units());
+  const size_t per = HW == 1 ? (C <= 64 ? 64 : C <= 1024 ? 16 : C <= 4096 ? 4 : 1) : 64;
+  return (int)std::max<size_t>(1, std::min(cus, (items + per - 1) / per));
+}
+
+struct LnArgs {
+  void* out;
+  float *partials, *moments;
+  const void* x;
+  const float *g, *b;
+  const void* dy;
+  LnP p;
+  int groups;
+};
+
+template <class V, int VEC, int T, int NCH>
+void launch_rows(hipStream_t s, const LnArgs& a, bool backward) {
+  if (backward)
+    hipLaunchKernelGGL((lnorm_rows_backward<V, VEC, T, NCH>), dim3((unsigned)a.groups), dim3(1024), 0, s, (V*)a.out, a.partials, a.moments,
+                       (const V*)a.x, a.g, (const V*)a.dy, a.p);
+  else
+    hipLaunchKernelGGL((lnorm_rows_forward<V, VEC, T, NCH>), dim3((unsigned)((a.p.items * T + (T > 256 ? T : 256) - 1) / (T > 256 ? T : 256))),
+                       dim3(T > 256 ? T : 256), 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, a.p);
+}
+
+// the narrowest group that holds a row with 16 values a thread, and the fewest packs
+template <class V, int VEC, int T>
+void choose_packs(hipStream_t s, const LnArgs& a, bool backward) {
+  const int packs = div_up(a.p.C, T * VEC);
+  if (packs <= 1) launch_rows<V, VEC, T, 1>(s, a, backward);
+  else if (16 / VEC > 1 && packs <= 2) launch_rows<V, VEC, T, 16 / VEC >= 2 ? 2 : 1>(s, a, backward);
+  else if (16 / VEC > 2 && packs <= 4) launch_rows<V, VEC, T, 16 / VEC >= 4 ? 4 : 1>(s, a, backward);
+  else launch_rows<V, VEC, T, 16 / VEC>(s, a, backward);
+}
+template <class V, int VEC>
+void choose_group(hipStream_t s, const LnArgs& a, bool backward) {
+  if (a.p.C <= 64) choose_packs<V, VEC, 16>(s, a, backward);
+  else if (a.p.C <= 1024) choose_packs<V, VEC, 64>(s, a, backward);
+  else if (a.p.C <= 4096) choose_packs<V, VEC, 256>(s, a, backward);
+  else choose_packs<V, VEC, 1024>(s, a, backward);
+}
+
+template <class V, int K>
+void launch_planes(hipStream_t s, const LnArgs& a, bool backward) {
+  if (backward)
+    hipLaunchKernelGGL((lnorm_planes_backward<V, 16, K>), dim3((unsigned)a.groups), dim3(1024), 0, s, (V*)a.out, a.partials, a.moments,
+                       (const V*)a.x, a.g, (const V*)a.dy, a.p);
+  else
+    hipLaunchKernelGGL((lnorm_planes_forward<V, 16, K>), dim3((unsigned)((a.p.items + 63) / 64)), dim3(1024), 0, s, (V*)a.out, a.moments, (const V*)a.x,
+                       a.g, a.b, a.p);
+}
+
+template <class V>
+int launch(hipStream_t s, const char* who, LnArgs& a, bool backward, float* dg, float* db) {
+  constexpr int VEC = 16 / sizeof(V);
+  const bool rows = a.p.HW == 1;
+  if (in_registers(a.p.C, a.p.HW)) {
+    KernelTimer timer(backward ? "lnorm_backward" : "lnorm_forward", s);
+    if (rows) {
+      const bool wide = a.p.C % VEC == 0 && aligned16(a.x) && aligned16(a.out) && aligned16(a.dy) && aligned16(a.g) && aligned16(a.b);
+      if (wide) choose_group<V, VEC>(s, a, backward);
+      else choose_group<V, 1>(s, a, backward);
+    } else {
+      if (a.p.C <= 64) launch_planes<V, 4>(s, a, backward);
+      else if (a.p.C <= 128) launch_planes<V, 8>(s, a, backward);
+      else if (a.p.C <= 256) launch_planes<V, 16>(s, a, backward);
+      else launch_planes<V, 32>(s, a, backward);
+    }
+  } else {
+    KernelTimer timer(backward ? "lnorm_backward" : "lnorm_forward", s);
+    const dim3 grid((unsigned)(rows ? a.p.items : (a.p.items + 63) / 64)), block(256);
+    if (!backward) {
+      if (rows) hipLaunchKernelGGL((lnorm_long<V, true, false>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
+      else hipLaunchKernelGGL((lnorm_long<V, false, false>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
+    } else {
+      if (rows) hipLaunchKernelGGL((lnorm_long<V, true, true>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
+      else hipLaunchKernelGGL((lnorm_long<V, false, true>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
+      if (a.partials) {
+        const size_t run = (a.p.items + a.groups - 1) / a.groups;
+        const dim3 sums((unsigned)(rows ? div_up(a.p.C, 256) : a.p.C), (unsigned)a.groups);
+        if (rows) hipLaunchKernelGGL((lnorm_long_sums<V, true>), sums, block, 0, s, a.partials, a.moments, (const V*)a.x, (const V*)a.dy, a.p, run);
+        else hipLaunchKernelGGL((lnorm_long_sums<V, false>), sums, block, 0, s, a.partials, a.moments, (const V*)a.x, (const V*)a.dy, a.p, run);
+      }
+    }
+  }
+  int rc = check_launch(who);
+  if (rc || !backward || !a.partials) return rc;
+  KernelTimer timer("lnorm_join", s);
+  hipLaunchKernelGGL(lnorm_join, dim3((unsigned)div_up(2ll * a.p.C, 16)), dim3(256), 0, s, dg, db, a.partials, a.p.C, a.groups);
+  return check_launch(who);
+}
+
+int setup(const char* who, int dataType, int H, int W, int C, int N, double epsilon, int given, LnP* p) {
+  if (dataType != MCN_FLOAT && dataType != MCN_BFLOAT16) return fail(MCN_ILLEGAL_ARGUMENT, "%s: unknown data type %d", who, dataType);
+  if (H < 0 || W < 0 || C < 0 || N < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative tensor extent", who);
+  if (!(epsilon >= 0)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: EPSILON is negative", who);
+  if ((long long)H * W >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: plane too large", who);
+  if (C > (1 << 24) || (size_t)H * W * N >= (1ull << 31)) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
+  p->C = C;
+  p->HW = H * W;
+  p->items = (size_t)H * W * N;
+  p->epsilon = (float)epsilon;
+  p->given = given != 0;
+  return MCN_SUCCESS;
+}
+
+int long_groups(size_t items) { return (int)std::max<size_t>(1, std::min<size_t>(kRuns, items)); }
+
+}  // namespace
+}  // namespace mcn
+
+using namespace mcn;
+
+extern "C" {
+
+size_t mcn_lnorm_workspace_bytes(int H, int W, int C, int N) {
+  if (H <= 0 || W <= 0 || C <= 0 || N <= 0) return 0;
+  const size_t items = (size_t)H * W * N;
+  const bool regs = in_registers(C, (size_t)H * W);
+  const size_t groups = regs ? backward_groups(C, (size_t)H * W, items) : long_groups(items);
+  return groups * 2 * C * sizeof(float) + (regs ? 0 : 2 * items * sizeof(float));
+}
+
+int mcn_lnorm_forward(mcn_stream_t stream, int dataType, void* y, float* moments, const void* x, const float* multipliers, const float* biases, int H,
+                      int W, int C, int N, double epsilon, int givenMoments) {
+  const char* who = "mcn_lnorm_forward";
+  LnArgs a = {};
+  int rc = setup(who, dataType, H, W, C, N, epsilon, givenMoments, &a.p);
+  if (rc || a.p.items == 0 || C == 0) return rc;
+  if (!y || !x) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null tensor", who);
+  if (givenMoments && !moments) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null moments", who);
+  a.out = y; a.moments = moments; a.x = x; a.g = multipliers; a.b = biases;
+  hipStream_t s = as_stream(stream);
+  return dataType == MCN_BFLOAT16 ? launch<bf16>(s, who, a, false, nullptr, nullptr) : launch<float>(s, who, a, false, nullptr, nullptr);
+}
+
+int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput, float* derMultipliers, float* derBiases, float* moments, const void* x,
+                       const float* multipliers, const void* derOutput, int H, int W, int C, int N, double epsilon, int givenMoments, void* workspace,
+                       size_t workspaceBytes) {
+  const char* who = "mcn_lnorm_backward";
+  LnArgs a = {};
+  int rc = setup(who, dataType, H, W, C, N, epsilon, givenMoments, &a.p);
+  if (rc || C == 0 || (!derInput && !derMultipliers && !derBiases && !moments)) return rc;
+  hipStream_t s = as_stream(stream);
+  const bool sums = derMultipliers || derBiases;
+  if (a.p.items == 0) {   // no pixels: the sums over them are zero
+    if (!sums) return MCN_SUCCESS;
+    hipLaunchKernelGGL(lnorm_join, dim3((unsigned)div_up(2ll * C, 16)), dim3(256), 0, s, derMultipliers, derBiases, (const float*)nullptr, C, 0);
+    return check_launch(who);
+  }
+  if (!x || !derOutput) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null tensor", who);
+  if (givenMoments && !moments) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null moments", who);
+  const size_t need = mcn_lnorm_workspace_bytes(H, W, C, N);
+  if (!workspace || workspaceBytes < need)
+    return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, need);
+  a.out = derInput; a.moments = moments; a.x = x; a.g = multipliers; a.dy = derOutput;
+  a.partials = sums ? (float*)workspace : nullptr;
+  const bool regs = in_registers(C, a.p.HW);
+  a.groups = regs ? backward_groups(C, a.p.HW, a.p.items) : long_groups(a.p.items);
+  if (!regs && !moments) a.moments = (float*)workspace + (size_t)a.groups * 2 * C;   // (the sums read them back)
+  return dataType == MCN_BFLOAT16 ? launch<bf16>(s, who, a, true, derMultipliers, derBiases) : launch<float>(s, who, a, true, derMultipliers, derBiases);
+}
+
+}  // extern "C"

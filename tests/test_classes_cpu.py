@@ -1,0 +1,136 @@
+"""Refusals of the operators for classifiers with many classes: layer normalisation, the fully connected loss, orthogonalised updates,
+conversion.  All of it is decided on the host, before anything is launched."""
+import ctypes as C
+
+import pytest
+
+from matconvnet_amd import capi
+
+P = C.c_void_p(4096)   # stands for a device pointer: nothing is launched
+BIG = 1 << 50
+
+
+def refused(rc, code, text):
+    assert rc == code, rc
+    assert text in capi.lib().mcn_last_error_message().decode()
+
+
+def lnorm_forward(**k):
+    a = dict(type=0, y=P, mom=None, x=P, H=1, W=1, C=8, N=4, eps=1e-5, given=0)
+    a.update(k)
+    return capi.lib().mcn_lnorm_forward(None, a["type"], a["y"], a["mom"], a["x"], P, P, a["H"], a["W"], a["C"], a["N"], a["eps"], a["given"])
+
+
+def lnorm_backward(**k):
+    a = dict(type=0, dx=P, mom=None, x=P, dy=P, H=1, W=1, C=8, N=4, eps=1e-5, given=0, ws=P, bytes=BIG)
+    a.update(k)
+    return capi.lib().mcn_lnorm_backward(None, a["type"], a["dx"], P, P, a["mom"], a["x"], P, a["dy"], a["H"], a["W"], a["C"], a["N"], a["eps"], a["given"], a["ws"], a["bytes"])
+
+
+@pytest.mark.parametrize("call", [lnorm_forward, lnorm_backward])
+def test_lnorm(call):
+    ill = capi.ILLEGAL_ARGUMENT
+    refused(call(type=2), ill, "unknown data type")
+    refused(call(H=-1), ill, "negative tensor extent")
+    refused(call(eps=-1.0), ill, "EPSILON")
+    refused(call(eps=float("nan")), ill, "EPSILON")
+    refused(call(x=None), ill, "null tensor")
+    refused(call(given=1), ill, "null moments")
+    refused(call(H=1 << 16, W=1 << 16), capi.UNSUPPORTED, "too large")
+    refused(call(C=(1 << 24) + 1), capi.UNSUPPORTED, "too large")
+    assert call(C=0) == 0
+
+
+def test_lnorm_of_its_own():
+    ill = capi.ILLEGAL_ARGUMENT
+    refused(lnorm_forward(y=None), ill, "null tensor")
+    assert lnorm_forward(N=0) == 0
+    refused(lnorm_backward(dy=None), ill, "null tensor")
+    refused(lnorm_backward(ws=None), ill, "workspace too small")
+    refused(lnorm_backward(bytes=16), ill, "workspace too small")
+    assert capi.lib().mcn_lnorm_workspace_bytes(1, 1, 0, 4) == 0 and capi.lib().mcn_lnorm_workspace_bytes(1, 1, 100, 4) > 0
+
+
+def fc(backward, **k):
+    a = dict(D=16, K=10, N=4, type=0, y=P, x=P, f=P, c=P, labels=4, w=None, nw=0, ws=P, bytes=BIG)
+    a.update(k)
+    g = capi.FcLossGeom(a["D"], a["K"], a["N"], 1, a["type"])
+    L = capi.lib()
+    if backward:
+        return L.mcn_fcloss_backward(None, C.byref(g), a["y"], P, P, None, a["x"], a["f"], None, a["c"], a["labels"], a["w"], a["nw"], 1.0, a["ws"], a["bytes"])
+    return L.mcn_fcloss_forward(None, C.byref(g), a["y"], None, a["x"], a["f"], None, a["c"], a["labels"], a["w"], a["nw"], a["ws"], a["bytes"])
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+def test_fcloss(backward):
+    ill = capi.ILLEGAL_ARGUMENT
+    refused(fc(backward, type=7), ill, "unknown data type")
+    refused(fc(backward, D=-1), ill, "negative tensor extent")
+    refused(fc(backward, labels=5), ill, "one label per image")
+    refused(fc(backward, w=P, nw=3), ill, "cannot be broadcast")
+    refused(fc(backward, w=P, nw=0), ill, "cannot be broadcast")
+    refused(fc(backward, D=0), ill, "without features or classes")
+    refused(fc(backward, K=0), ill, "without features or classes")
+    refused(fc(backward, D=(1 << 20) + 1), capi.UNSUPPORTED, "2^20")
+    refused(fc(backward, K=(1 << 24) + 1), capi.UNSUPPORTED, "2^24")
+    for name in ("x", "f", "c"):
+        refused(fc(backward, **{name: None}), ill, "null tensor")
+    refused(fc(backward, ws=None), ill, "workspace too small")
+    refused(fc(backward, bytes=1000), ill, "workspace too small")
+    L = capi.lib()
+    assert L.mcn_fcloss_workspace_bytes(None, backward) == 0
+    small, large = capi.FcLossGeom(16, 10, 4, 1, 0), capi.FcLossGeom(64, 100000, 512, 1, 1)
+    assert 0 < L.mcn_fcloss_workspace_bytes(C.byref(small), backward) < (1 << 20)
+    # (a piece of the classes, not all of them: less than the 512 x 100000 scores in single precision)
+    assert L.mcn_fcloss_workspace_bytes(C.byref(large), backward) < 512 * 100000 * 4
+
+
+def test_fcloss_forward_needs_its_value():
+    refused(fc(0, y=None), capi.ILLEGAL_ARGUMENT, "null output")
+
+
+def ortho(**k):
+    a = dict(y=P, x=P, K=8, D=20, count=1, steps=5, ws=P, bytes=BIG)
+    a.update(k)
+    return capi.lib().mcn_orthogonalise(None, a["y"], a["x"], a["K"], a["D"], a["count"], a["steps"], a["ws"], a["bytes"])
+
+
+def test_orthogonalise():
+    ill = capi.ILLEGAL_ARGUMENT
+    refused(ortho(K=-1), ill, "negative tensor extent")
+    refused(ortho(steps=-1), ill, "number of steps")
+    refused(ortho(steps=101), ill, "number of steps")
+    refused(ortho(x=None), ill, "null tensor")
+    refused(ortho(y=None), ill, "null tensor")
+    refused(ortho(ws=None), ill, "workspace too small")
+    refused(ortho(bytes=100), ill, "workspace too small")
+    refused(ortho(K=1 << 16, D=1 << 16), capi.UNSUPPORTED, "too large")
+    refused(ortho(count=70000), capi.UNSUPPORTED, "too large")
+    assert ortho(count=0) == 0 and ortho(D=0) == 0
+
+
+def test_convert():
+    L = capi.lib()
+    refused(L.mcn_convert(None, P, 2, P, 0, 4), capi.ILLEGAL_ARGUMENT, "unknown data type")
+    refused(L.mcn_convert(None, None, 1, P, 0, 4), capi.ILLEGAL_ARGUMENT, "null tensor")
+    assert L.mcn_convert(None, None, 1, None, 0, 0) == 0
+
+
+def test_binding_refuses_what_the_library_cannot_see():
+    """Tensors on the host, of other types, strided or of other sizes are refused in Python."""
+    import torch
+    x = torch.zeros((2, 4, 1, 1))
+    with pytest.raises(ValueError):
+        capi.lnorm_forward(x, None, None)
+    with pytest.raises(TypeError):
+        capi.lnorm_forward(x, torch.zeros(4, dtype=torch.float64), None)
+    with pytest.raises(ValueError):
+        capi.fcloss_geom(torch.zeros((2, 4)), torch.zeros((3, 5)))
+    with pytest.raises(TypeError):
+        capi.fcloss_geom(torch.zeros((2, 4)), torch.zeros((3, 4), dtype=torch.bfloat16))
+    with pytest.raises(TypeError):
+        capi.data_type(torch.zeros(2, dtype=torch.float16))
+    with pytest.raises(ValueError):
+        capi.orthogonalise(x)
+    with pytest.raises(TypeError):
+        capi.orthogonalise(x.double())
