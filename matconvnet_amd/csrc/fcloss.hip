@@ -66,8 +66,9 @@ __global__ __launch_bounds__(256) void fc_magnitude(unsigned* __restrict__ bits,
   if (threadIdx.x == 0) atomicMax(bits, max(max(lds[0], lds[1]), max(lds[2], lds[3])));
 }
 
-__global__ void fc_clear(unsigned* p, int n) {
-  if ((int)threadIdx.x < n) p[threadIdx.x] = 0;
+// the magnitudes, and the products' counters behind them
+__global__ __launch_bounds__(256) void fc_clear(unsigned* p, int n) {
+  for (int i = threadIdx.x; i < n; i += 256) p[i] = 0;
 }
 
 // (K D / 1024 workgroups: at most 2^34)
@@ -140,30 +141,49 @@ __global__ __launch_bounds__(256) void fc_pack(unsigned short* __restrict__ out,
 
 // ---------------------------------------------------------------------------------------------- products
 
-// What the scores need: z = acc * unscale[m] * 1/scale(filters) + bias[n]
+// What the scores need: z = acc * unscale[m] * 1/scale(filters) + bias[n], -infinity behind the piece's last class
 struct Scores {
   const float *unscale, *bias;     // unscale: null for bfloat16
   const unsigned* magnitude;       // of the filters
   int N, K, first;                 // instances, classes in this piece, the piece's first class
   template <class S>
-  __device__ __forceinline__ void make(floatx16p (&acc)[S::TM][S::TN], int m0, int n0, int lane) const {
-    const float f = unscale ? pair_unscale(*magnitude) : 1.f;
+  __device__ __forceinline__ void make(floatx16p (&acc)[S::TM][S::TN], int m0, int n0, int tileEnd) const {
+    if (unscale) {
+      const float f = pair_unscale(*magnitude);
 #pragma unroll
-    for (int i = 0; i < S::TM; ++i) {
-      const float u = unscale ? unscale[min(m0 + 32 * i, N - 1)] : 1.f;
+      for (int i = 0; i < S::TM; ++i) {
+        // (both are powers of two: one product, kept from infinity, where the sums are nothing but zeros or past the range)
+        const float u = fminf(unscale[min(m0 + 32 * i, N - 1)] * f, 3.0e38f);
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc[i][j] *= u;
+      }
+    }
+    if (bias) {
 #pragma unroll
       for (int j = 0; j < S::TN; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int n = n0 + 32 * j + 8 * (r / 4) + r % 4;
-          float z = acc[i][j][r];
-          if (unscale) z = z * u * f;
-          if (bias) z += n < K ? bias[first + n] : 0.f;
-          acc[i][j][r] = n < K ? z : -__builtin_inff();
+          const float b = n < K ? bias[first + n] : 0.f;
+#pragma unroll
+          for (int i = 0; i < S::TM; ++i) acc[i][j][r] += b;
         }
+    }
+    if (tileEnd > K) {             // (the last column of tiles alone)
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (n0 + 32 * j + 8 * (r / 4) + r % 4 >= K) {
+#pragma unroll
+            for (int i = 0; i < S::TM; ++i) acc[i][j][r] = -__builtin_inff();
+          }
     }
   }
 };
+// whether column c (against a lane's first one) is among the lane's: of a block of 32, eight times four from 4 (lane / 32) on
+template <class S>
+__device__ __forceinline__ bool has_column(int c) { return c >= 0 && c < 32 * S::TN && (c & 4) == 0; }
 
 // Forward: (largest score, sum of exponentials against it) per instance and tile, the score of the instance's class
 struct StatsEnd {
@@ -175,10 +195,19 @@ struct StatsEnd {
   template <class S>
   __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
     const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
-    z.make<S>(acc, m0, n0, lane);
+    z.make<S>(acc, m0, n0, (tn + 1) * S::BN);
     float2* rows = (float2*)lds;   // [WN][BM]
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
+      const int m = m0 + 32 * i;
+      const int c = m < z.N ? class_of(labels[m], classes) - z.first - n0 : -1;
+      if (__any(has_column<S>(c) && n0 + c < z.K)) {   // (few tiles have the class of one of their instances)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (c == 32 * j + 8 * (r / 4) + r % 4 && n0 + c < z.K) own[m] = acc[i][j][r];
+      }
       float most = -__builtin_inff();
 #pragma unroll
       for (int j = 0; j < S::TN; ++j)
@@ -193,15 +222,6 @@ struct StatsEnd {
         for (int r = 0; r < 16; ++r) sum += __expf(acc[i][j][r] - from);
       sum += __shfl_xor(sum, 32, kWave);
       if (lane < 32) rows[wn * S::BM + 32 * (wm * S::TM + i) + lane] = make_float2(most, sum);
-      const int m = m0 + 32 * i;
-      if (m < z.N) {
-        const int c = class_of(labels[m], classes) - z.first - n0;   // (against this lane's first column)
-#pragma unroll
-        for (int j = 0; j < S::TN; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (c == 32 * j + 8 * (r / 4) + r % 4 && n0 + c < z.K) own[m] = acc[i][j][r];
-      }
     }
     __syncthreads();
     for (int t = threadIdx.x; t < S::BM; t += S::threads) {
@@ -252,7 +272,7 @@ struct ProbabilitiesEnd {
   template <class S>
   __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
     const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
-    z.make<S>(acc, m0, n0, lane);
+    z.make<S>(acc, m0, n0, (tn + 1) * S::BN);
     float* columns = (float*)lds;  // [WM][BN]
     float weight[S::TM];
 #pragma unroll
@@ -261,18 +281,26 @@ struct ProbabilitiesEnd {
       const bool live = m < z.N;
       const float w = live ? instance_weight(labels, weights, nWeights, m) : 0.f;
       const float lse = live ? logSums[m] : 0.f;
-      const int c = (live ? class_of(labels[m], classes) : -1) - z.first - n0;
+      const int c = live ? class_of(labels[m], classes) - z.first - n0 : -1;
       weight[i] = w;
+      // (classes behind the piece's last one have a score of -infinity: 0)
 #pragma unroll
       for (int j = 0; j < S::TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int n = 32 * j + 8 * (r / 4) + r % 4;
-          float p = __expf(acc[i][j][r] - lse);
-          if (c == n) p -= 1.f;
-          if (w == 0.f || n0 + n >= z.K) p = 0.f;
-          acc[i][j][r] = p;
-        }
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = __expf(acc[i][j][r] - lse);
+      if (__any(has_column<S>(c) && n0 + c < z.K)) {
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (c == 32 * j + 8 * (r / 4) + r % 4 && n0 + c < z.K) acc[i][j][r] -= 1.f;
+      }
+      if (__any(w == 0.f)) {       // (such an instance's scores may be anything)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = w == 0.f ? 0.f : acc[i][j][r];
+      }
     }
     if (sums) {
       // value v of a block's 16: column 8 (v / 4) + v % 4 (+ 4 in the upper half-wavefront)
@@ -328,58 +356,57 @@ struct ProbabilitiesEnd {
   }
 };
 
-// out[m][n] (+)= acc * factor * 1/scale of an operand * the instance's weight
+// out[m][n] = sum[m][n] + acc * factor * 1/scale of an operand * the instance's weight
 struct StoreEnd {
   void* out;
-  int M, Ncols, bf16Out, add;
-  long long slicePitch;               // from one cut of the reduction to the next
+  int bf16Out;
+  const float* sum;                   // what other pieces gave, may be null (and may be `out`)
+  int M, Ncols;
   float factor;
   const unsigned* magnitude;          // may be null
   const float *labels, *weights;      // may be null: rows are instances
   int nWeights;
   template <class S>
-  __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int slice, int lane, int wm, int wn, char*) const {
+  __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char*) const {
     const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
     const float u = magnitude ? pair_unscale(*magnitude) : 1.f;
-    const bool wide = (Ncols & 3) == 0 && ((uintptr_t)out & 15) == 0;
+    const bool wide = (Ncols & 3) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)sum & 15) == 0;
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
       const int m = m0 + 32 * i;
       if (m >= M) continue;
       const float w = labels ? instance_weight(labels, weights, nWeights, m) * factor : factor;
+      const size_t row = (size_t)m * Ncols;
 #pragma unroll
-      for (int j = 0; j < S::TN; ++j)
+      for (int j = 0; j < S::TN; ++j) {
+        const int n1 = n0 + 32 * j;
+        if (wide) {
+          float4 s[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + 32 * j + 8 * q;
-          float v[4];
+          for (int q = 0; q < 4; ++q)
+            s[q] = sum && n1 + 8 * q < Ncols ? *(const float4*)(sum + row + n1 + 8 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r] * u * w;
-          if (bf16Out) {
-            unsigned short* o = (unsigned short*)out + (size_t)m * Ncols + n;
-            if (wide && n < Ncols) {
-              *(uintx2p*)o = (uintx2p){(unsigned)to_bf16(v[0]) | (unsigned)to_bf16(v[1]) << 16, (unsigned)to_bf16(v[2]) | (unsigned)to_bf16(v[3]) << 16};
-            } else {
+          for (int q = 0; q < 4; ++q) {
+            if (n1 + 8 * q >= Ncols) continue;
+            const float4 v = make_float4(s[q].x + acc[i][j][4 * q] * u * w, s[q].y + acc[i][j][4 * q + 1] * u * w,
+                                         s[q].z + acc[i][j][4 * q + 2] * u * w, s[q].w + acc[i][j][4 * q + 3] * u * w);
+            if (bf16Out)
+              *(uintx2p*)((unsigned short*)out + row + n1 + 8 * q) =
+                  (uintx2p){(unsigned)to_bf16(v.x) | (unsigned)to_bf16(v.y) << 16, (unsigned)to_bf16(v.z) | (unsigned)to_bf16(v.w) << 16};
+            else
+              *(float4*)((float*)out + row + n1 + 8 * q) = v;
+          }
+        } else {
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (n + r < Ncols) o[r] = to_bf16(v[r]);
-            }
-          } else {
-            float* o = (float*)out + (size_t)slice * slicePitch + (size_t)m * Ncols + n;
-            if (wide && n < Ncols) {
-              float4 t = make_float4(v[0], v[1], v[2], v[3]);
-              if (add) {
-                const float4 b = *(const float4*)o;
-                t.x += b.x; t.y += b.y; t.z += b.z; t.w += b.w;
-              }
-              *(float4*)o = t;
-            } else {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (n + r < Ncols) o[r] = add ? o[r] + v[r] : v[r];
-            }
+          for (int r = 0; r < 16; ++r) {
+            const int n = n1 + 8 * (r / 4) + r % 4;
+            if (n >= Ncols) continue;
+            const float v = (sum ? sum[row + n] : 0.f) + acc[i][j][r] * u * w;
+            if (bf16Out) ((unsigned short*)out)[row + n] = to_bf16(v);
+            else ((float*)out)[row + n] = v;
           }
         }
+      }
     }
   }
 };
@@ -429,16 +456,6 @@ __global__ __launch_bounds__(256) void fc_join_columns(float* __restrict__ db, c
   db[c] = (float)s * factor;
 }
 
-// The cuts of a reduction summed, in order
-__global__ __launch_bounds__(256) void fc_join(void* __restrict__ out, const float* __restrict__ parts, size_t n, size_t pitch, int slices, int bf16Out) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float s = parts[i];
-  for (int k = 1; k < slices; ++k) s += parts[(size_t)k * pitch + i];
-  if (bf16Out) ((unsigned short*)out)[i] = to_bf16(s);
-  else ((float*)out)[i] = s;
-}
-
 // ---------------------------------------------------------------------------------------------- host
 
 // What a call keeps in the caller's workspace
@@ -446,15 +463,16 @@ struct Plan {
   int type;
   bool xInPlace, fInPlace;         // bfloat16 rows of whole stages are read where they are
   long long xPitch, fPitch, pPitch;
-  int piece, pieces, tile, tiles;  // classes per piece; the scores' tile; tiles over all classes
-  int dxTile, dxSlices;
-  size_t x, xUnscale, xw, f, magnitudes, parts, own, terms, logSums, p, dx, columns, total;
+  int piece, pieces, tiles;        // classes per piece; tiles of scores over all classes
+  ProductPlan scores, dx, df;      // of a whole piece; the last one, if smaller, is cut as they are
+  size_t x, xUnscale, xw, f, magnitudes, counters, parts, own, terms, logSums, p, sum, columns, products, total;
+  int nCounters;
   // whether rows of D values can be read 16 bytes at a time; workgroups that pack rows
   int wide(const void* t, const mcn_fcloss_geom* g) const { return g->D % (type == kPairs ? 4 : 8) == 0 && aligned16(t); }
   unsigned pack_blocks(int rows, long long pitch) const { return (unsigned)(((size_t)rows * (pitch / (type == kPairs ? 16 : 8)) + 255) / 256); }
 };
 
-constexpr size_t kPieceBytes = 128u << 20;   // of P
+size_t kPieceBytes_() { return (size_t)std::max(1, tunable("fcloss_piece", 128)) << 20; }
 
 Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool backward) {
   Plan p;
@@ -464,33 +482,32 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   p.xInPlace = whole && aligned16(x);
   p.xPitch = row_halves(p.type, g->D);
   p.fPitch = p.fInPlace ? g->D : row_halves(p.type, g->D);
-  p.tile = choose_tile(g->N, g->K);
-  const int t = kTileSize[p.tile];
   // a piece: P (backward) and the packed filters stay within kPieceBytes, whole tiles
-  const long long perClass = std::max<long long>((backward ? g->N * 2ll * (p.type == kPairs ? 2 : 1) : 0), p.fInPlace ? 0 : p.fPitch * 2);
-  long long piece = perClass ? (long long)kPieceBytes / perClass / t * t : g->K;
-  piece = std::max<long long>(piece, t);
-  if (piece >= g->K) piece = (long long)(g->K + t - 1) / t * t;
-  else {                           // equal pieces
-    const long long n = (g->K + piece - 1) / piece;
-    piece = ((g->K + n - 1) / n + t - 1) / t * t;
+  const long long most = (g->K + 255ll) / 256 * 256;
+  const long long perClass = std::max<long long>(backward ? g->N * 2ll * (p.type == kPairs ? 2 : 1) : 0, p.fInPlace ? 0 : p.fPitch * 2);
+  long long piece = perClass ? std::max(256ll, (long long)kPieceBytes_() / perClass / 256 * 256) : most;
+  if (piece < most) {              // equal pieces
+    const long long n = (most + piece - 1) / piece;
+    piece = ((most + n - 1) / n + 255) / 256 * 256;
   }
-  p.piece = (int)std::min<long long>(piece, (1ll << 30));
+  p.piece = (int)std::min(piece, most);
   p.pieces = (int)((g->K + (long long)p.piece - 1) / p.piece);
-  p.tiles = div_up(g->K, t);
+  const int classes = std::min(p.piece, g->K);
+  p.scores = plan_product(p.type, g->N, classes, g->D);
+  p.dx = plan_product(p.type, g->N, g->D, classes);
+  p.df = plan_product(p.type, classes, g->D, g->N);
+  p.tiles = div_up(g->K, kTileSize[p.scores.tile]);
   p.pPitch = row_halves(p.type, std::min<long long>(p.piece, (g->K + 63) / 64 * 64));
-  // dzdx has few tiles when there are few instances: its reduction over the classes is cut then
-  p.dxTile = choose_tile(g->N, g->D);
-  const long long dxTiles = (long long)div_up(g->N, kTileSize[p.dxTile]) * div_up(g->D, kTileSize[p.dxTile]);
-  const int stages = div_up(std::min(p.piece, g->K), stage_depth(p.type));
-  p.dxSlices = (int)std::max<long long>(1, std::min<long long>({2ll * std::max(1, device_compute_units()) / std::max(1ll, dxTiles), stages / 4, 64}));
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t here = at;
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  p.magnitudes = take(256);
+  p.nCounters = (int)(backward ? std::max({p.scores.counters(), p.dx.counters(), p.df.counters()}) : p.scores.counters());
+  p.magnitudes = take(8 + 4 * p.nCounters);
+  p.counters = p.magnitudes + 8;
+  p.products = take(backward ? std::max({p.scores.partBytes(), p.dx.partBytes(), p.df.partBytes()}) : p.scores.partBytes());
   p.x = take(p.xInPlace ? 0 : (size_t)g->N * p.xPitch * 2);
   p.xUnscale = take(p.type == kPairs ? (size_t)g->N * 4 : 0);
   p.f = take(p.fInPlace ? 0 : (size_t)std::min(p.piece, g->K) * p.fPitch * 2);
@@ -498,12 +515,12 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   p.own = take((size_t)g->N * 4);
   p.terms = take((size_t)g->N * 4);
   p.logSums = take((size_t)g->N * 4);
-  p.xw = p.p = p.dx = p.columns = 0;
+  p.xw = p.p = p.sum = p.columns = 0;
   if (backward) {
     p.xw = take((size_t)g->N * p.xPitch * 2);
-    p.columns = take((size_t)div_up(g->N, t) * g->K * 4);
+    p.columns = take((size_t)div_up(g->N, kTileSize[p.scores.tile]) * g->K * 4);
     p.p = take((size_t)g->N * p.pPitch * 2);
-    p.dx = take(p.dxSlices > 1 || p.type == kBf16 ? (size_t)p.dxSlices * g->N * g->D * 4 : 0);
+    p.sum = take(p.type == kBf16 && p.pieces > 1 ? (size_t)g->N * g->D * 4 : 0);
   }
   p.total = at;
   return p;
@@ -523,11 +540,14 @@ int check(const char* who, const mcn_fcloss_geom* g, size_t nLabels, const float
 
 // x as the operand of the scores, and the magnitudes of the filters and of the weighted features
 int pack_x(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geom* g, char* ws, const void* x, const void* f, const float* labels,
-           const float* weights, int nWeights, bool weighted, Operand* op) {
-  *op = {p.xInPlace ? x : ws + p.x, p.xPitch, g->N};
+           const float* weights, int nWeights, bool weighted, Matrix* op) {
+  *op = {p.xInPlace ? x : ws + p.x, p.xPitch, 0, g->N};
   unsigned* m = (unsigned*)(ws + p.magnitudes);
+  if (p.type == kPairs || p.nCounters) {
+    KernelTimer timer("fc_clear", s);
+    hipLaunchKernelGGL(fc_clear, dim3(1), dim3(256), 0, s, m, 2 + p.nCounters);
+  }
   if (p.type == kPairs) {
-    hipLaunchKernelGGL(fc_clear, dim3(1), dim3(64), 0, s, m, 2);
     const size_t n = (size_t)g->K * g->D;
     KernelTimer timer("fc_magnitude", s);
     hipLaunchKernelGGL(fc_magnitude, dim3((unsigned)((n + kMagnitudeStep - 1) / kMagnitudeStep)), dim3(256), 0, s, m, (const float*)f, n, (int)aligned16(f));
@@ -554,25 +574,26 @@ void pack(hipStream_t s, const Plan& p, const mcn_fcloss_geom* g, char* out, con
 
 // the filters of a piece
 template <int TYPE>
-Operand pack_f(hipStream_t s, const Plan& p, const mcn_fcloss_geom* g, char* ws, const void* f, int first, int count) {
+Matrix pack_f(hipStream_t s, const Plan& p, const mcn_fcloss_geom* g, char* ws, const void* f, int first, int count) {
   const char* from = (const char*)f + (size_t)first * g->D * (TYPE == kPairs ? 4 : 2);
   if (!p.fInPlace) pack<TYPE>(s, p, g, ws + p.f, (const unsigned*)(ws + p.magnitudes), from, count, p.fPitch, nullptr, nullptr, 1);
-  return {p.fInPlace ? from : ws + p.f, p.fPitch, count};
+  return {p.fInPlace ? from : ws + p.f, p.fPitch, 0, count};
 }
 
 template <int TYPE>
 int forward(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geom* g, float* logSums, const void* f, const float* biases,
-            const float* labels, const float* weights, int nWeights, char* ws, const Operand& X) {
+            const float* labels, const float* weights, int nWeights, char* ws, const Matrix& X) {
+  const Scratch scratch = {(float*)(ws + p.products), (unsigned*)(ws + p.counters)};
   for (int k = 0; k < p.pieces; ++k) {
     const int first = k * p.piece, count = std::min(p.piece, g->K - first);
-    const Operand F = pack_f<TYPE>(s, p, g, ws, f, first, count);
+    const Matrix F = pack_f<TYPE>(s, p, g, ws, f, first, count);
     StatsEnd e;
     e.z = {TYPE == kPairs ? (const float*)(ws + p.xUnscale) : nullptr, biases, (const unsigned*)(ws + p.magnitudes), g->N, count, first};
     e.parts = (float2*)(ws + p.parts);
     e.own = (float*)(ws + p.own);
     e.labels = labels;
-    e.tiles = p.tiles; e.firstTile = first / kTileSize[p.tile]; e.classes = g->K;
-    const int rc = product<TYPE, false, false>(s, who, "fc_scores", X, F, g->N, count, g->D, 1, e, p.tile);
+    e.tiles = p.tiles; e.firstTile = first / kTileSize[p.scores.tile]; e.classes = g->K;
+    const int rc = product<TYPE, false, false>(s, who, "fc_scores", X, F, g->N, count, p.scores.of(g->N, count), scratch, e);
     if (rc) return rc;
   }
   KernelTimer timer("fc_log_sums", s);
@@ -584,15 +605,15 @@ int forward(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geom
 template <int TYPE>
 int backward(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geom* g, void* derInput, void* derFilters, float* derBiases,
              const float* logSums, const void* f, const float* biases, const float* labels, const float* weights, int nWeights, float factor,
-             char* ws, const Operand& X, const void* x) {
+             char* ws, const Matrix& X, const void* x) {
   const unsigned* mag = (const unsigned*)(ws + p.magnitudes);
-  const Operand Xw = {ws + p.xw, p.xPitch, g->N};
+  const Matrix Xw = {ws + p.xw, p.xPitch, 0, g->N};
+  const Scratch scratch = {(float*)(ws + p.products), (unsigned*)(ws + p.counters)};
   if (derFilters) pack<TYPE>(s, p, g, ws + p.xw, mag + 1, x, g->N, p.xPitch, labels, weights, nWeights);
-  const bool joined = p.dxSlices > 1 || TYPE == kBf16;
-  const size_t dxSize = (size_t)g->N * g->D, elem = TYPE == kPairs ? 4 : 2;
+  const float times = TYPE == kPairs ? factor / kProbability : factor;
   for (int k = 0; k < p.pieces; ++k) {
     const int first = k * p.piece, count = std::min(p.piece, g->K - first);
-    const Operand F = pack_f<TYPE>(s, p, g, ws, f, first, count);
+    const Matrix F = pack_f<TYPE>(s, p, g, ws, f, first, count);
     ProbabilitiesEnd e;
     e.z = {TYPE == kPairs ? (const float*)(ws + p.xUnscale) : nullptr, biases, mag, g->N, count, first};
     e.out = (unsigned short*)(ws + p.p);
@@ -600,31 +621,31 @@ int backward(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geo
     e.labels = labels; e.weights = weights; e.logSums = logSums;
     e.nWeights = nWeights; e.classes = g->K;
     e.sums = derBiases ? (float*)(ws + p.columns) : nullptr;
-    int rc = product<TYPE, false, false>(s, who, "fc_probabilities", X, F, g->N, (count + 63) / 64 * 64, g->D, 1, e, p.tile);
+    int rc = product<TYPE, false, false>(s, who, "fc_probabilities", X, F, g->N, (count + 63) / 64 * 64, p.scores.of(g->N, (count + 63) / 64 * 64), scratch, e);
     if (rc) return rc;
-    const Operand P = {ws + p.p, p.pPitch, g->N};
+    const Matrix P = {ws + p.p, p.pPitch, 0, g->N};
     if (derInput) {
-      StoreEnd d = {joined ? ws + p.dx : derInput, g->N, g->D, 0, k > 0, (long long)dxSize, TYPE == kPairs ? factor / kProbability : factor,
-                    TYPE == kPairs ? mag : nullptr, labels, weights, nWeights};
-      rc = product<TYPE, false, true>(s, who, "fc_derivative_x", P, F, g->N, g->D, count, p.dxSlices, d, p.dxTile);
+      // (the pieces add up in single precision: in derInput itself, or beside it)
+      float* sum = TYPE == kPairs ? (float*)derInput : (float*)(ws + p.sum);
+      const bool last = k == p.pieces - 1;
+      const StoreEnd d = {TYPE == kPairs || last ? derInput : sum, TYPE == kBf16 && last, k > 0 ? sum : nullptr, g->N, g->D, times,
+                          TYPE == kPairs ? mag : nullptr, labels, weights, nWeights};
+      ProductPlan q = p.dx;
+      q.stages = div_up(count, stage_depth(TYPE));
+      rc = product<TYPE, false, true>(s, who, "fc_derivative_x", P, F, g->N, g->D, q, scratch, d);
       if (rc) return rc;
     }
     if (derFilters) {
-      StoreEnd d = {(char*)derFilters + (size_t)first * g->D * elem, count, g->D, TYPE == kBf16, 0, 0, TYPE == kPairs ? factor / kProbability : factor,
-                    TYPE == kPairs ? mag + 1 : nullptr, nullptr, nullptr, 1};
-      rc = product<TYPE, true, true>(s, who, "fc_derivative_f", P, Xw, count, g->D, g->N, 1, d, choose_tile(count, g->D));
+      const StoreEnd d = {(char*)derFilters + (size_t)first * g->D * (TYPE == kPairs ? 4 : 2), TYPE == kBf16, nullptr, count, g->D, times,
+                          TYPE == kPairs ? mag + 1 : nullptr, nullptr, nullptr, 1};
+      rc = product<TYPE, true, true>(s, who, "fc_derivative_f", P, Xw, count, g->D, p.df.of(count, g->D), scratch, d);
       if (rc) return rc;
     }
   }
   if (derBiases) {
     KernelTimer timer("fc_join", s);
     hipLaunchKernelGGL(fc_join_columns, dim3((unsigned)div_up(g->K, 256)), dim3(256), 0, s, derBiases, (const float*)(ws + p.columns), g->K,
-                       div_up(g->N, kTileSize[p.tile]), factor);
-  }
-  if (derInput && joined) {
-    KernelTimer timer("fc_join", s);
-    hipLaunchKernelGGL(fc_join, dim3((unsigned)((dxSize + 255) / 256)), dim3(256), 0, s, derInput, (const float*)(ws + p.dx), dxSize, dxSize, p.dxSlices,
-                       TYPE == kBf16);
+                       div_up(g->N, kTileSize[p.scores.tile]), factor);
   }
   return check_launch(who);
 }
@@ -659,7 +680,7 @@ int mcn_fcloss_forward(mcn_stream_t stream, const mcn_fcloss_geom* g, float* y, 
     p = make_plan(g, x, filters, false);
     if (!workspace || workspaceBytes < p.total)
       return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, p.total);
-    Operand X;
+    Matrix X;
     rc = pack_x(s, who, p, g, ws, x, filters, labels, instanceWeights, (int)nWeights, false, &X);
     if (rc) return rc;
     float* sums = logSums ? logSums : (float*)(ws + p.logSums);
@@ -694,7 +715,7 @@ int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, void* der
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, p.total);
   hipStream_t s = as_stream(stream);
   char* ws = (char*)workspace;
-  Operand X;
+  Matrix X;
   rc = pack_x(s, who, p, g, ws, x, filters, labels, instanceWeights, (int)nWeights, true, &X);
   if (rc) return rc;
   const float factor = (float)(g->normalise ? derOutput / g->N : derOutput);

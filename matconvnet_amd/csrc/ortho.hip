@@ -18,8 +18,11 @@ constexpr int kNormParts = 256;   // workgroups per matrix that sum squares, at 
 // ---------------------------------------------------------------------------------------------- G to pairs
 
 // sums of squares, in double (single-precision squares of small gradients vanish)
-__global__ __launch_bounds__(256) void ortho_squares(double* __restrict__ parts, const float* __restrict__ x, size_t size) {
+__global__ __launch_bounds__(256) void ortho_squares(double* __restrict__ parts, const float* __restrict__ x, size_t size, unsigned* __restrict__ counters,
+                                                     int nCounters) {
   __shared__ double lds[4];
+  // (the products' counters are cleared on the way)
+  for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < nCounters; i += gridDim.x * gridDim.y * 256) counters[i] = 0;
   const float* v = x + (size_t)blockIdx.y * size;
   double s[4] = {};
   const size_t step = (size_t)gridDim.x * 256;
@@ -66,14 +69,6 @@ __global__ __launch_bounds__(256) void ortho_pack(unsigned short* __restrict__ o
 
 // ---------------------------------------------------------------------------------------------- products
 
-// The matrices of a call: one per slice of the grid
-struct Matrix {
-  const unsigned short* base;
-  long long pitch, size;   // 16-bit values from row to row, matrix to matrix
-  int rows;
-  __device__ __forceinline__ Operand of(int slice) const { return {base + slice * size, pitch, rows}; }
-};
-
 // D = add * C + times * A B, as pairs or as single-precision values
 struct OrthoEnd {
   unsigned short* out;      // pairs, at outPitch / outSize
@@ -84,7 +79,7 @@ struct OrthoEnd {
   float add, times;         // (times: with the scales of the two operands)
   int symmetric;            // tiles below the diagonal are written a second time, turned
   template <class S>
-  __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int slice, int lane, int wm, int wn, char*) const {
+  __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int which, int lane, int wm, int wn, char*) const {
     const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
@@ -97,7 +92,7 @@ struct OrthoEnd {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int n = n0 + 32 * j + 8 * q;
-          const long long at = slice * size + m * pitch + (n / 32) * 64 + n % 32;
+          const long long at = which * size + m * pitch + (n / 32) * 64 + n % 32;
           if (n / 32 * 64 >= pitch) continue;
           float v[4];
 #pragma unroll
@@ -111,7 +106,7 @@ struct OrthoEnd {
             }
           }
           if (result) {
-            float* o = result + ((long long)slice * rows + m) * cols + n;
+            float* o = result + ((long long)which * rows + m) * cols + n;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (n + r < cols) o[r] = v[r] * kUnscale;
@@ -129,7 +124,7 @@ struct OrthoEnd {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               if (n + r >= rows) continue;
-              unsigned short* o = out + slice * size + (n + r) * pitch + (m / 32) * 64 + m % 32;
+              unsigned short* o = out + which * size + (n + r) * pitch + (m / 32) * 64 + m % 32;
               o[0] = (unsigned short)p[r];
               o[32] = (unsigned short)(p[r] >> 16);
             }
@@ -139,61 +134,20 @@ struct OrthoEnd {
   }
 };
 
-template <class S, bool A_ACROSS, bool B_ACROSS>
-__global__ __launch_bounds__(S::threads, 2) void ortho_product(Matrix A, Matrix B, TileGrid g, int stages, OrthoEnd e) {
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  int tm, tn, slice;
-  if (e.symmetric) {
-    // the tiles of a triangle, row by row
-    const int per = g.tilesM * (g.tilesM + 1) / 2;
-    const int id = xcd_contiguous_id((int)blockIdx.x, (int)gridDim.x);
-    slice = id / per;
-    const int t = id - slice * per;
-    tm = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    while (tm * (tm + 1) / 2 > t) --tm;
-    while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
-    tn = t - tm * (tm + 1) / 2;
-  } else {
-    tile_of(g, &tm, &tn, &slice);
-  }
-  floatx16p acc[S::TM][S::TN];
-  product_tile<S, A_ACROSS, B_ACROSS>(A.of(slice), B.of(slice), (long long)tm * S::BM, (long long)tn * S::BN, 0, stages, lds, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  e.finish<S>(acc, tm, tn, slice, lane, wave % S::WM, wave / S::WM, lds);
-}
-
-template <class S, bool A_ACROSS, bool B_ACROSS>
-int launch_product(hipStream_t s, const char* who, const Matrix& A, const Matrix& B, int M, int N, int depth, int count, const OrthoEnd& e) {
-  const TileGrid g = {div_up(M, S::BM), div_up(N, S::BN), count};
-  const long long per = e.symmetric ? (long long)g.tilesM * (g.tilesM + 1) / 2 : (long long)g.tilesM * g.tilesN;
-  if (per * count >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
-  const auto kernel = ortho_product<S, A_ACROSS, B_ACROSS>;
-  int rc = allow_lds<S>(who, (const void*)kernel);
-  if (rc) return rc;
-  KernelTimer timer("ortho_product", s);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(per * count)), dim3(S::threads), S::ldsBytes, s, A, B, g, div_up(depth, stage_depth(kPairs)), e);
-  return check_launch(who);
-}
-
-template <bool A_ACROSS, bool B_ACROSS>
-int ortho_multiply(hipStream_t s, const char* who, const Matrix& A, const Matrix& B, int M, int N, int depth, int count, const OrthoEnd& e) {
-  switch (choose_tile(M, N, count, e.symmetric != 0)) {
-    case kTile256: return launch_product<ProductShape<kPairs, 256, 256, 2, 4>, A_ACROSS, B_ACROSS>(s, who, A, B, M, N, depth, count, e);
-    case kTile128: return launch_product<ProductShape<kPairs, 128, 128, 2, 2>, A_ACROSS, B_ACROSS>(s, who, A, B, M, N, depth, count, e);
-    default: return launch_product<ProductShape<kPairs, 64, 64, 2, 2>, A_ACROSS, B_ACROSS>(s, who, A, B, M, N, depth, count, e);
-  }
-}
-
 struct OrthoPlan {
   int m;                          // the shorter side
   int normParts;
   long long pitch, mPitch;
-  size_t x[2], a, b, parts, total;
+  ProductPlan gram, square, update;   // A = X X', B = b A + c A A, X <- a X + B X
+  size_t x[2], a, b, parts, sums, counters, total;
 };
 
 OrthoPlan ortho_plan(int K, int D, int count) {
   OrthoPlan p;
   p.m = std::min(K, D);
+  p.gram = plan_product(kPairs, p.m, p.m, std::max(K, D), count, true);
+  p.square = plan_product(kPairs, p.m, p.m, p.m, count, true);
+  p.update = plan_product(kPairs, K, D, p.m, count);
   p.normParts = (int)std::max<size_t>(1, std::min<size_t>(kNormParts, (size_t)K * D / 2048));
   p.pitch = row_halves(kPairs, D);
   p.mPitch = row_halves(kPairs, p.m);
@@ -208,6 +162,8 @@ OrthoPlan ortho_plan(int K, int D, int count) {
   p.a = take((size_t)count * p.m * p.mPitch * 2);
   p.b = take((size_t)count * p.m * p.mPitch * 2);
   p.parts = take((size_t)count * kNormParts * sizeof(double));
+  p.sums = take(std::max({p.gram.partBytes(), p.square.partBytes(), p.update.partBytes()}));
+  p.counters = take(4 * std::max({p.gram.counters(), p.square.counters(), p.update.counters()}));
   p.total = at;
   return p;
 }
@@ -223,7 +179,8 @@ int orthogonalise(hipStream_t s, const char* who, const OrthoPlan& p, float* y, 
   double* parts = (double*)(ws + p.parts);
   {
     KernelTimer timer("ortho_squares", s);
-    hipLaunchKernelGGL(ortho_squares, dim3((unsigned)p.normParts, (unsigned)count), dim3(256), 0, s, parts, x, (size_t)K * D);
+    hipLaunchKernelGGL(ortho_squares, dim3((unsigned)p.normParts, (unsigned)count), dim3(256), 0, s, parts, x, (size_t)K * D,
+                       (unsigned*)(ws + p.counters), (int)std::max({p.gram.counters(), p.square.counters(), p.update.counters()}));
   }
   {
     KernelTimer timer("ortho_pack", s);
@@ -232,21 +189,24 @@ int orthogonalise(hipStream_t s, const char* who, const OrthoPlan& p, float* y, 
   }
   int rc = check_launch(who);
   const bool tall = K > D;
+  const Scratch scratch = {(float*)(ws + p.sums), (unsigned*)(ws + p.counters)};
+  const Matrix A = {ws + p.a, p.mPitch, p.m * p.mPitch, p.m};
+  const Matrix B = {ws + p.b, p.mPitch, p.m * p.mPitch, p.m};
   for (int step = 0; step < steps && !rc; ++step) {
-    const Matrix X = {(unsigned short*)(ws + p.x[step & 1]), p.pitch, K * p.pitch, K};
-    const Matrix A = {(unsigned short*)(ws + p.a), p.mPitch, p.m * p.mPitch, p.m};
-    const Matrix B = {(unsigned short*)(ws + p.b), p.mPitch, p.m * p.mPitch, p.m};
+    const Matrix X = {ws + p.x[step & 1], p.pitch, K * p.pitch, K};
     OrthoEnd e = {(unsigned short*)(ws + p.a), nullptr, nullptr, p.mPitch, p.m * p.mPitch, p.m, p.m, 0.f, kUnscale, 1};
-    rc = tall ? ortho_multiply<true, true>(s, who, X, X, p.m, p.m, K, count, e) : ortho_multiply<false, false>(s, who, X, X, p.m, p.m, D, count, e);
+    rc = tall ? product<kPairs, true, true>(s, who, "ortho_gram", X, X, p.m, p.m, p.gram, scratch, e, count, true)
+              : product<kPairs, false, false>(s, who, "ortho_gram", X, X, p.m, p.m, p.gram, scratch, e, count, true);
     if (rc) break;
     e.out = (unsigned short*)(ws + p.b);
-    e.c = A.base;
+    e.c = (const unsigned short*)A.base;
     e.add = kB;
     e.times = kC * kUnscale;
-    rc = ortho_multiply<false, false>(s, who, A, A, p.m, p.m, p.m, count, e);
+    rc = product<kPairs, false, false>(s, who, "ortho_square", A, A, p.m, p.m, p.square, scratch, e, count, true);
     if (rc) break;
-    e = {(unsigned short*)(ws + p.x[~step & 1]), step == steps - 1 ? y : nullptr, X.base, p.pitch, K * p.pitch, K, D, kA, kUnscale, 0};
-    rc = tall ? ortho_multiply<false, false>(s, who, X, B, K, D, p.m, count, e) : ortho_multiply<false, true>(s, who, B, X, K, D, p.m, count, e);
+    e = {(unsigned short*)(ws + p.x[~step & 1]), step == steps - 1 ? y : nullptr, (const unsigned short*)X.base, p.pitch, K * p.pitch, K, D, kA, kUnscale, 0};
+    rc = tall ? product<kPairs, false, false>(s, who, "ortho_update", X, B, K, D, p.update, scratch, e, count)
+              : product<kPairs, false, true>(s, who, "ortho_update", B, X, K, D, p.update, scratch, e, count);
   }
   return rc;
 }
@@ -282,7 +242,7 @@ int mcn_orthogonalise(mcn_stream_t stream, float* y, const float* x, int K, int 
   hipStream_t s = as_stream(stream);
   if (steps == 0) {
     double* parts = (double*)((char*)workspace + p.parts);
-    hipLaunchKernelGGL(ortho_squares, dim3((unsigned)p.normParts, (unsigned)count), dim3(256), 0, s, parts, x, (size_t)K * D);
+    hipLaunchKernelGGL(ortho_squares, dim3((unsigned)p.normParts, (unsigned)count), dim3(256), 0, s, parts, x, (size_t)K * D, (unsigned*)nullptr, 0);
     hipLaunchKernelGGL(ortho_normalise, dim3((unsigned)p.normParts, (unsigned)count), dim3(256), 0, s, y, x, parts, p.normParts, (size_t)K * D);
     return check_launch(who);
   }

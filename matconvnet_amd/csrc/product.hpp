@@ -49,20 +49,21 @@ struct Operand {
   long long rows;    // rows that exist: what is behind them reads as zero
 };
 
-template <int TYPE, int BM_, int BN_, int WM_, int WN_>
+template <int TYPE, int BM_, int BN_, int WM_, int WN_, int BUFFERS>
 struct ProductShape {
   static constexpr int type = TYPE;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;      // tile, wavefronts along m and n
   static constexpr int threads = 64 * WM * WN;
   static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;         // blocks of 32 x 32 per wavefront
   static constexpr int stageBytes = (BM + BN) * 128;
-  static constexpr int ldsBytes = 2 * stageBytes;
+  static constexpr int buffers = BUFFERS;                            // stages in LDS at a time
+  static constexpr int ldsBytes = BUFFERS * stageBytes;
 };
 
 typedef __attribute__((address_space(3))) char* lds_bytes;
 
-// Where 16 bytes of a stage lie.  ALONG: row r's eight chunks are exchanged by r & 7, so that eight lanes that read the same chunk
-// of eight rows meet all banks.  ACROSS: a row of the stage is one reduction index, R values; 64-byte granules (32 values of m, h
+// Where 16 bytes of a stage lie.  ALONG: row r's eight chunks are exchanged by r / 2 % 8, so that sixteen lanes that read the same chunk
+// of sixteen rows meet all 64 banks (by r % 8 rows r and r + 8 met: half of the cycles of these reads were conflicts).  ACROSS: a row of the stage is one reduction index, R values; 64-byte granules (32 values of m, h
 // or l) are exchanged so that the four indices a transposing read takes lie in different banks.
 template <int TYPE, bool ACROSS, int R>
 struct Stage {
@@ -78,14 +79,14 @@ struct Stage {
       *chunk = c ^ (turn(*row) << 2);
     } else {
       *row = t >> 3;
-      *chunk = (t & 7) ^ (*row & 7);
+      *chunk = (t & 7) ^ (*row >> 1 & 7);
     }
   }
   // eight reduction indices from 16 s + 8 (lane / 32) of row 32 b + lane % 32, part (0: h, 1: l)
   __device__ static __forceinline__ uintx4p fragment(const char* lds, int lane, int b, int s, int part) {
     if (!ACROSS) {
       const int chunk = (TYPE == kPairs ? 4 * part : 0) + 2 * s + (lane >> 5);
-      return *(const uintx4p*)(lds + (lane & 31) * 128 + ((chunk ^ (lane & 7)) << 4) + b * 4096);
+      return *(const uintx4p*)(lds + (lane & 31) * 128 + ((chunk ^ (lane >> 1 & 7)) << 4) + b * 4096);
     } else {
       // a group of 16 lanes gives four indices x 16 values of m and takes, lane by lane, one m and four indices
       const int k = 16 * s + 8 * (lane >> 5) + ((lane >> 2) & 3);
@@ -118,9 +119,11 @@ struct Loader {
   const char* base;
   unsigned long long left;   // bytes from base to the end of the operand
   unsigned long long step;
+  int more;                  // stages to come: the loads behind the last one go out all the same (their number is what is waited for) and
+                             // find nothing
 
   // first: first row (ALONG) or first value of m (ACROSS) of the tile; stage0: first stage
-  __device__ __forceinline__ void begin(const Operand& o, long long first, long long stage0, int tid) {
+  __device__ __forceinline__ void begin(const Operand& o, long long first, long long stage0, int stages, int tid) {
 #pragma unroll
     for (int i = 0; i < loads; ++i) {
       int row, chunk;
@@ -132,50 +135,93 @@ struct Loader {
                                          : (unsigned long long)first * o.pitch * 2 + stage0 * 128;
     base = (const char*)o.base + at;
     left = at < all ? all - at : 0;
+    more = stages;
     step = ACROSS ? (unsigned long long)stage_depth(S::type) * o.pitch * 2 : 128;
   }
-  __device__ __forceinline__ void load(char* lds, int wave) {
+  // load i of a stage; after the last one the next stage's are due
+  __device__ __forceinline__ void load(char* lds, int wave, int i) {
     typedef __attribute__((address_space(3))) void* lds_ptr;
-    const unsigned records = left > 0xfffffff0ull ? 0xfffffff0u : (unsigned)left;
+    const unsigned records = more <= 0 ? 0u : left > 0xfffffff0ull ? 0xfffffff0u : (unsigned)left;
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)records, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (i * S::threads + wave * 64) * 16), 16, (int)offset[i], 0, 0, 0);
+    if (i == loads - 1) {
+      --more;
+      base += step;
+      left = left > step ? left - step : 0;
+    }
+  }
+  __device__ __forceinline__ void load_all(char* lds, int wave) {
 #pragma unroll
-    for (int i = 0; i < loads; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (i * S::threads + wave * 64) * 16), 16, (int)offset[i], 0, 0, 0);
-    base += step;
-    left = left > step ? left - step : 0;
+    for (int i = 0; i < loads; ++i) load(lds, wave, i);
   }
 };
 
-// (a function of its own with `restrict` pointers: that the loads fill another buffer than the one read is what lets the reads go
-// without waiting for them)
-template <class S, bool A_ACROSS, bool B_ACROSS, class LA, class LB>
-__device__ __forceinline__ void product_stage(const char* __restrict__ from, char* __restrict__ to, bool more, LA& la, LB& lb, int wave, int lane,
-                                              int wm, int wn, floatx16p (&acc)[S::TM][S::TN]) {
-  if (more) {
-    la.load(to, wave);
-    lb.load(to + S::BM * 128, wave);
-  }
-  typedef Stage<S::type, A_ACROSS, S::BM> SA;
-  typedef Stage<S::type, B_ACROSS, S::BN> SB;
-  constexpr int parts = S::type == kPairs ? 2 : 1;
-#pragma unroll
-  for (int s = 0; s < stage_depth(S::type) / 16; ++s) {
-    uintx4p a[parts][S::TM], b[parts][S::TN];
+// The fragments of one step of 16 reduction indices
+template <class S>
+struct Fragments {
+  static constexpr int parts = S::type == kPairs ? 2 : 1;
+  uintx4p a[parts][S::TM], b[parts][S::TN];
+  template <bool A_ACROSS, bool B_ACROSS>
+  __device__ __forceinline__ void read(const char* lds, int lane, int wm, int wn, int s) {
 #pragma unroll
     for (int q = 0; q < parts; ++q) {
 #pragma unroll
-      for (int i = 0; i < S::TM; ++i) a[q][i] = SA::fragment(from, lane, wm * S::TM + i, s, q);
+      for (int i = 0; i < S::TM; ++i) a[q][i] = Stage<S::type, A_ACROSS, S::BM>::fragment(lds, lane, wm * S::TM + i, s, q);
 #pragma unroll
-      for (int j = 0; j < S::TN; ++j) b[q][j] = SB::fragment(from + S::BM * 128, lane, wn * S::TN + j, s, q);
+      for (int j = 0; j < S::TN; ++j) b[q][j] = Stage<S::type, B_ACROSS, S::BN>::fragment(lds + S::BM * 128, lane, wn * S::TN + j, s, q);
     }
+  }
+  // the matrix instructions of a step, with load(0), load(1) ... load(LOADS - 1) spread among them
+  template <int LOADS, class Load>
+  __device__ __forceinline__ void multiply_into(floatx16p (&acc)[S::TM][S::TN], Load load) const {
+    constexpr int products = parts == 2 ? 3 : 1, all = products * S::TM * S::TN, every = all / (LOADS + 1) > 0 ? all / (LOADS + 1) : 1;
+    int done = 0, loaded = 0;
 #pragma unroll
-    for (int t = parts == 2 ? 0 : 2; t < 3; ++t)   // lh, hl, hh: the small ones first
+    for (int t = 0; t < products; ++t)   // lh, hl, hh: the small ones first
 #pragma unroll
       for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j)
+        for (int j = 0; j < S::TN; ++j) {
           acc[i][j] = multiply<S::type>(b[parts == 2 && t == 1 ? 1 : 0][j], a[parts == 2 && t == 0 ? 1 : 0][i], acc[i][j]);
+          if (++done % every == 0 && loaded < LOADS) {
+            __builtin_amdgcn_sched_barrier(0);
+            load(loaded++);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+    for (; loaded < LOADS; ++loaded) load(loaded);
   }
+};
+
+// One stage: `f` holds the fragments of its first step and is left with those of the next stage's.  The reads of a step go out before the
+// matrix instructions of the step before it; the barrier, which every wavefront reaches with its last reads of this stage done,
+// stands before the last step's, behind it the stage's buffer (`to`) is filled again: with A's share among the matrix
+// instructions of the last step, B's among those of the next stage's first.  (All of a stage's loads in a row behind the
+// barrier held the wavefronts up for as long as the CU's 64 bytes a clock take: 8192 x 8192 x 4096 bfloat16 475 -> 446 us.)
+// (A function of its own with `restrict` pointers: that the loads fill none of what is read is what lets the reads go without waiting
+// for them.  `to` is `from`, filled behind the barrier that ends its reads; `filled` holds what the barrier then waits for.)
+template <class S, bool A_ACROSS, bool B_ACROSS, class LA, class LB>
+__device__ __forceinline__ void product_stage(const char* __restrict__ from, const char* __restrict__ next, char* __restrict__ to, char* __restrict__ filled,
+                                              LA& la, LB& lb, int wave, int lane, int wm, int wn, Fragments<S>& f, floatx16p (&acc)[S::TM][S::TN]) {
+  constexpr int steps = stage_depth(S::type) / 16;
+#pragma unroll
+  for (int s = 1; s < steps; ++s) {
+    Fragments<S> g;
+    g.template read<A_ACROSS, B_ACROSS>(from, lane, wm, wn, s);
+    __builtin_amdgcn_sched_barrier(0);   // (the compiler would move the reads down to their first use)
+    if (s == 1) f.template multiply_into<LB::loads>(acc, [&](int i) __attribute__((always_inline)) { lb.load(filled + S::BM * 128, wave, i); });
+    else f.template multiply_into<0>(acc, [](int) {});
+    __builtin_amdgcn_sched_barrier(0);
+    f = g;
+  }
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::buffers - 2) * (LA::loads + LB::loads)) : "memory");
+  Fragments<S> g;
+  g.template read<A_ACROSS, B_ACROSS>(next, lane, wm, wn, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  f.template multiply_into<LA::loads>(acc, [&](int i) __attribute__((always_inline)) { la.load(to, wave, i); });
+  __builtin_amdgcn_sched_barrier(0);
+  f = g;
 }
 
 // acc[i][j][r]: row m0 + 32 (wm TM + i) + lane % 32, column n0 + 32 (wn TN + j) + 8 (r / 4) + 4 (lane / 32) + r % 4.
@@ -193,38 +239,24 @@ __device__ __forceinline__ void product_tile(const Operand& A, const Operand& B,
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   Loader<S, A_ACROSS, S::BM> la;
   Loader<S, B_ACROSS, S::BN> lb;
-  la.begin(A, m0, stage0, tid);
-  lb.begin(B, n0, stage0, tid);
-  if (stages > 0) {
-    la.load(lds, wave);
-    lb.load(lds + S::BM * 128, wave);
+  la.begin(A, m0, stage0, stages, tid);
+  lb.begin(B, n0, stage0, stages, tid);
+#pragma unroll
+  for (int k = 0; k < S::buffers; ++k) {
+    la.load_all(lds + k * S::stageBytes, wave);
+    if (k < S::buffers - 1) lb.load_all(lds + k * S::stageBytes + S::BM * 128, wave);
   }
-  int at = 0;
-  for (int s = 1; s <= stages; ++s) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    product_stage<S, A_ACROSS, B_ACROSS>(lds + at, lds + (S::stageBytes - at), s < stages, la, lb, wave, lane, wm, wn, acc);
-    at = S::stageBytes - at;
+  Fragments<S> f;
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S::buffers - 2) * (la.loads + lb.loads) + la.loads) : "memory");
+  f.template read<A_ACROSS, B_ACROSS>(lds, lane, wm, wn, 0);
+  int at = 0, filled = S::ldsBytes - S::stageBytes;
+  for (int s = 0; s < stages; ++s) {
+    const int next = at + S::stageBytes == S::ldsBytes ? 0 : at + S::stageBytes;
+    product_stage<S, A_ACROSS, B_ACROSS>(lds + at, lds + next, lds + at, lds + filled, la, lb, wave, lane, wm, wn, f, acc);
+    filled = at;
+    at = next;
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
-// The tiles of a grid of workgroups: consecutive workgroups of one XCD take kTileRows rows of tiles by as many columns as fit, so that
-// the tiles in flight on an XCD share operands in its L2.
-struct TileGrid {
-  int tilesM, tilesN;
-  int slices;          // independent products, or cuts of the reduction, one behind the other
-};
-constexpr int kTileRows = 4;
-__device__ __forceinline__ void tile_of(const TileGrid& g, int* tm, int* tn, int* slice) {
-  const int per = g.tilesM * g.tilesN;
-  const int id = xcd_contiguous_id((int)blockIdx.x, (int)gridDim.x);
-  *slice = id / per;
-  const int t = id - *slice * per;
-  const int band = kTileRows * g.tilesN;
-  const int first = t / band * kTileRows, rows = min(kTileRows, g.tilesM - first);
-  const int within = t - t / band * band;
-  *tm = first + within % rows;
-  *tn = within / rows;
 }
 
 // The power of two s that puts a magnitude (its bits) into [2^14, 2^15), and 1 / s.  1 for zero and what is not finite.
@@ -279,32 +311,170 @@ __device__ __forceinline__ void store8_pairs(unsigned short* row, int c, const f
   at[4] = l;
 }
 
-// What to do with a finished tile is E's: e.finish<S>(acc, tile row, tile column, slice, lane, wavefront along m, along n, LDS).
+// A reduction cut into slices: every workgroup of a tile leaves its part in memory, the one that comes last adds them up in the order of the
+// slices (its own among them: the same bits whichever is last) and goes on to finish the tile.  `counters`: one per tile, zero
+// before and after.  The XCDs' L2s are not coherent: the parts are written and read by relaxed atomic accesses at the scope of the
+// device, which go past them, and are counted once they have arrived.  (Plain accesses, and a count that releases and acquires, write
+// back and empty an L2 per workgroup: a quarter of a microsecond each, one at a time on an XCD.)
+struct Slices {
+  float* parts;
+  unsigned* counters;
+  int slices, perSlice;   // (slices == 1: neither pointer is used)
+};
+template <class S>
+__device__ __forceinline__ bool join_slices(const Slices& j, int tile, int slice, floatx16p (&acc)[S::TM][S::TN], char* lds) {
+  if (j.slices == 1) return true;
+  constexpr size_t size = (size_t)S::BM * S::BN / 2;   // in pairs of values
+  typedef unsigned long long two;
+  two* mine = (two*)j.parts + ((size_t)tile * j.slices + slice) * size + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+    for (int k = 0; k < S::TN; ++k)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float2 v = make_float2(acc[i][k][2 * q], acc[i][k][2 * q + 1]);
+        __hip_atomic_store(mine + ((i * S::TN + k) * 8 + q) * S::threads, __builtin_bit_cast(two, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the parts have arrived where every XCD reads them,
+  __syncthreads();                                     // those of all wavefronts,
+  if (threadIdx.x == 0) {                              // before they are counted
+    const unsigned before = __hip_atomic_fetch_add(j.counters + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool last = before == (unsigned)j.slices - 1u;
+    if (last) __hip_atomic_store(j.counters + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *(unsigned*)lds = last;
+  }
+  __syncthreads();
+  const bool last = *(volatile unsigned*)lds != 0;
+  __syncthreads();   // (the LDS is the finishing code's again)
+  if (!last) return false;
+  two* from = (two*)j.parts + (size_t)tile * j.slices * size + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+    for (int k = 0; k < S::TN; ++k)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][k][r] = 0.f;
+  for (int s = 0; s < j.slices; ++s)
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int k = 0; k < S::TN; ++k) {
+        two v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          v[q] = __hip_atomic_load(from + s * size + ((i * S::TN + k) * 8 + q) * S::threads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float2 f = __builtin_bit_cast(float2, v[q]);
+          acc[i][k][2 * q] += f.x;
+          acc[i][k][2 * q + 1] += f.y;
+        }
+      }
+  return true;
+}
+
+// The matrices of a grid of products: one or more of one shape, `size` 16-bit values apart
+struct Matrix {
+  const void* base;
+  long long pitch, size;
+  long long rows;
+  __device__ __forceinline__ Operand of(int k) const { return {(const char*)base + k * size * 2, pitch, rows}; }
+};
+
+struct TileGrid {
+  int tilesM, tilesN;
+  int count;           // products of one shape
+  int triangle;        // only the tiles on and below the diagonal
+};
+// Consecutive workgroups of one XCD take kTileRows rows of tiles by as many columns as fit, so that the tiles in flight on an XCD share
+// operands in its L2; the slices of a tile are neighbours.
+constexpr int kTileRows = 4;
+
+// What to do with a finished tile is E's: e.finish<S>(acc, tile row, tile column, which product, lane, wavefront along m, along n, LDS).
 template <class S, bool A_ACROSS, bool B_ACROSS, class E>
-__global__ __launch_bounds__(S::threads, 2) void product_kernel(Operand A, Operand B, TileGrid g, int stages, int perSlice, E e) {
+__global__ __launch_bounds__(S::threads, 2) void product_kernel(Matrix A, Matrix B, TileGrid g, int stages, Slices j, E e) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  int tm, tn, slice;
-  tile_of(g, &tm, &tn, &slice);
-  const int s0 = slice * perSlice;
+  const int id = xcd_contiguous_id((int)blockIdx.x, (int)gridDim.x);
+  const int tile = id / j.slices, slice = id - tile * j.slices;
+  const int per = g.triangle ? g.tilesM * (g.tilesM + 1) / 2 : g.tilesM * g.tilesN;
+  const int which = tile / per, t = tile - which * per;
+  int tm, tn;
+  if (g.triangle) {
+    tm = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while (tm * (tm + 1) / 2 > t) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
+    tn = t - tm * (tm + 1) / 2;
+  } else {
+    const int band = kTileRows * g.tilesN;
+    const int first = t / band * kTileRows, rows = min(kTileRows, g.tilesM - first);
+    const int within = t - t / band * band;
+    tm = first + within % rows;
+    tn = within / rows;
+  }
+  const int s0 = slice * j.perSlice;
   floatx16p acc[S::TM][S::TN];
-  product_tile<S, A_ACROSS, B_ACROSS>(A, B, (long long)tm * S::BM, (long long)tn * S::BN, s0, max(0, min(perSlice, stages - s0)), lds, acc);
+  product_tile<S, A_ACROSS, B_ACROSS>(A.of(which), B.of(which), (long long)tm * S::BM, (long long)tn * S::BN, s0, max(0, min(j.perSlice, stages - s0)), lds, acc);
+  if (!join_slices<S>(j, tile, slice, acc, lds)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  e.template finish<S>(acc, tm, tn, slice, lane, wave % S::WM, wave / S::WM, lds);
+  e.template finish<S>(acc, tm, tn, which, lane, wave % S::WM, wave / S::WM, lds);
 }
 
 // ---------------------------------------------------------------------------------------------- host
 
-// Which tile: the largest that still gives every compute unit one
 enum { kTile256, kTile128, kTile64 };
-inline int choose_tile(long long M, long long N, int count = 1, bool symmetric = false) {
+constexpr int kTileSize[3] = {256, 128, 64};
+
+// How a product is cut: the tile, and how many workgroups share a tile's reduction.
+struct ProductPlan {
+  int tile, slices, perSlice, stages;
+  long long tiles;
+  size_t partBytes() const { return slices > 1 ? (size_t)tiles * slices * kTileSize[tile] * kTileSize[tile] * 4 : 0; }
+  size_t counters() const { return slices > 1 ? (size_t)tiles : 0; }
+  // the same cut for fewer rows or columns
+  ProductPlan of(long long M, long long N) const {
+    ProductPlan p = *this;
+    p.tiles = (M + kTileSize[tile] - 1) / kTileSize[tile] * ((N + kTileSize[tile] - 1) / kTileSize[tile]);
+    return p;
+  }
+};
+
+// The cheapest of the cuts by a model in microseconds, measured on products of 2^10 to 2^13 indices: a stage takes `alone` where a
+// workgroup has its CU (nearly) to itself, `shared` per workgroup where several keep it busy; `ends` is what a tile's first loads and
+// its end cost; a join costs kJoin, its parts' way to memory and back (all together at 5 TB/s, a tile's at 0.1).  (bfloat16, tiles of
+// 64 / 128 / 256: 650 / 1040 / 1240 TFLOP/s with the chip full; pairs: 850 / 1140 / 1260.  P f of 2048 x 1024 over 16000 classes, pairs,
+// in us: 891, 288, 225 by tiles of 256 in 1, 4, 8 slices, 412, 196, 244 by tiles of 128, 234, 338, 497 by tiles of 64; chosen: 128 in 4.)
+struct StageCost { double alone, shared, ends; };
+constexpr StageCost kStageCost[2][3] = {{{1.5, 1.6, 8.0}, {0.62, 0.50, 3.0}, {0.29, 0.20, 1.0}},     // kBf16: 256, 128, 64
+                                        {{2.3, 2.5, 8.0}, {0.86, 0.70, 3.0}, {0.30, 0.24, 1.0}}};    // kPairs
+constexpr double kJoin = 4.0;
+constexpr int kMostSlices = 32;
+inline ProductPlan plan_product(int type, long long M, long long N, long long depth, int count = 1, bool triangle = false) {
   const int cus = std::max(1, device_compute_units());
-  const auto tiles = [&](int t) {
-    const long long rows = (M + t - 1) / t;
-    return count * (symmetric ? rows * (rows + 1) / 2 : rows * ((N + t - 1) / t));
-  };
-  if (tiles(256) >= cus) return kTile256;
-  if (tiles(128) >= cus) return kTile128;
-  return kTile64;
+  const int forced = tunable("product_tile", 0), cut = tunable("product_slices", 0);
+  const int stages = (int)((depth + stage_depth(type) - 1) / stage_depth(type));
+  ProductPlan best = {};
+  double least = 1e300;
+  for (int tile = 0; tile < 3; ++tile) {
+    if (forced && forced != kTileSize[tile]) continue;
+    const long long rows = (M + kTileSize[tile] - 1) / kTileSize[tile], columns = (N + kTileSize[tile] - 1) / kTileSize[tile];
+    const long long tiles = count * (triangle ? rows * (rows + 1) / 2 : rows * columns);
+    const StageCost& c = kStageCost[type][tile];
+    const double part = 4.0 * kTileSize[tile] * kTileSize[tile];
+    for (int slices = 1; slices <= kMostSlices && slices <= std::max(1, stages); ++slices) {
+      if (cut && slices != div_up(std::max(1, stages), div_up(std::max(1, stages), cut))) continue;
+      const int perSlice = std::max(1, div_up(stages, slices));
+      if (slices > 1 && ((slices - 1) * perSlice >= stages || (!cut && tiles * slices > 4ll * cus))) continue;   // (no empty slice; parts stay small)
+      const double waves = (double)((tiles * slices + cus - 1) / cus);
+      const double cost = perSlice * std::max(c.alone, waves * c.shared) + c.ends * std::max(1.0, waves / 2) +
+                          (slices > 1 ? kJoin + slices * part * (2.0 * tiles / 5.0e6 + 1.0 / 1.0e5) : 0.0);
+      if (cost < least) {
+        least = cost;
+        best = {tile, slices, perSlice, stages, tiles};
+      }
+    }
+  }
+  return best;
 }
 
 // A kernel with more than 64 KiB of local memory has to be told so once per device.
@@ -325,28 +495,34 @@ int allow_lds(const char* who, const void* kernel) {
   return MCN_SUCCESS;
 }
 
+// Where a call's products leave their parts
+struct Scratch {
+  float* parts;
+  unsigned* counters;
+};
+
 template <class S, bool A_ACROSS, bool B_ACROSS, class E>
-int run_product(hipStream_t s, const char* who, const char* name, const Operand& A, const Operand& B, long long M, long long N, int stages, int slices, const E& e) {
-  TileGrid g = {div_up(M, S::BM), div_up(N, S::BN), slices};
-  const long long blocks = (long long)g.tilesM * g.tilesN * slices;
-  if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
+int run_product(hipStream_t s, const char* who, const char* name, const Matrix& A, const Matrix& B, long long M, long long N, int count, bool triangle,
+                const ProductPlan& p, const Scratch& scratch, const E& e) {
+  if (p.tiles * p.slices >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
+  const TileGrid g = {div_up(M, S::BM), div_up(N, S::BN), count, triangle};
   const auto kernel = product_kernel<S, A_ACROSS, B_ACROSS, E>;
-  int rc = allow_lds<S>(who, (const void*)kernel);
+  const int rc = allow_lds<S>(who, (const void*)kernel);
   if (rc) return rc;
   KernelTimer timer(name, s);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(S::threads), S::ldsBytes, s, A, B, g, stages, div_up(stages, slices), e);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tiles * p.slices)), dim3(S::threads), S::ldsBytes, s, A, B, g, p.stages,
+                     Slices{scratch.parts, scratch.counters, p.slices, p.perSlice}, e);
   return check_launch(who);
 }
 
 template <int TYPE, bool A_ACROSS, bool B_ACROSS, class E>
-int product(hipStream_t s, const char* who, const char* name, const Operand& A, const Operand& B, long long M, long long N, long long depth, int slices, const E& e, int tile) {
-  const int stages = (int)((depth + stage_depth(TYPE) - 1) / stage_depth(TYPE));
-  switch (tile) {
-    case kTile256: return run_product<ProductShape<TYPE, 256, 256, 2, 4>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, stages, slices, e);
-    case kTile128: return run_product<ProductShape<TYPE, 128, 128, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, stages, slices, e);
-    default: return run_product<ProductShape<TYPE, 64, 64, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, stages, slices, e);
+int product(hipStream_t s, const char* who, const char* name, const Matrix& A, const Matrix& B, long long M, long long N, const ProductPlan& p,
+            const Scratch& scratch, const E& e, int count = 1, bool triangle = false) {
+  switch (p.tile) {
+    case kTile256: return run_product<ProductShape<TYPE, 256, 256, 4, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+    case kTile128: return run_product<ProductShape<TYPE, 128, 128, 2, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+    default: return run_product<ProductShape<TYPE, 64, 64, 2, 2, 4>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
   }
 }
-constexpr int kTileSize[3] = {256, 128, 64};
 
 }  // namespace mcn

@@ -308,3 +308,23 @@ def test_layers_of_maps(capi):
     assert torch.equal(y, y2)
     dx, df, db = capi.fcloss_backward(x.view(9, 16, 6, 6), f.view(50, 16, 6, 6), b, c)
     assert dx.shape == (9, 16, 6, 6) and df.shape == (50, 16, 6, 6)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("slices", [1, 2, 5])
+def test_every_cut_of_the_products(capi, dtype, tile, slices):
+    """Each tile, and reductions in one piece and in several: odd sizes that leave part of every tile, and tiles of several rows and
+    columns; a second call finds its counters as the first left them."""
+    try:
+        capi.set_tunable("product_tile", tile)
+        capi.set_tunable("product_slices", slices)
+        for size in [(130, 261, 70), (333, 515, 300), (700, 33, 1)]:
+            args = make(*size, dtype, 15)
+            one = check(capi, *args)
+            two = check(capi, *args)
+            for p, q in zip(one, two):
+                assert torch.equal(p, q)
+    finally:
+        capi.set_tunable("product_tile", 0)
+        capi.set_tunable("product_slices", 0)

@@ -158,3 +158,19 @@ def test_captured(capi):
 
 def test_empty(capi):
     assert capi.orthogonalise(torch.empty((0, 4, 4), device="cuda")).numel() == 0
+
+
+@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("slices", [1, 2, 5])
+def test_every_cut_of_the_products(capi, tile, slices):
+    try:
+        capi.set_tunable("product_tile", tile)
+        capi.set_tunable("product_slices", slices)
+        r = torch.Generator(device="cuda")
+        r.manual_seed(7)
+        for count, K, D in [(2, 70, 333), (1, 515, 300), (1, 290, 290), (3, 33, 40)]:
+            g = torch.randn((count, K, D), generator=r, device="cuda")
+            assert torch.equal(check(capi, g), check(capi, g))
+    finally:
+        capi.set_tunable("product_tile", 0)
+        capi.set_tunable("product_slices", 0)
