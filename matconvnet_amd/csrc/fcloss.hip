@@ -35,8 +35,16 @@ __device__ __forceinline__ float wave_max(float v) {
 
 // ---------------------------------------------------------------------------------------------- operands
 
-// The largest magnitude of n values, as the bits of a float (whole numbers: the order of the atomics does not matter; a NaN or an
-// infinity wins, and pair_scale leaves such a tensor as it is)
+// What a call's first launches leave: per workgroup of fc_magnitudes the largest magnitude of its filters, or of its instances' weighted
+// features, as the bits of floats (a NaN or an infinity wins, and pair_scale leaves such a tensor as it is); every instance's own;
+// and, from fc_pack, the two tensors'.
+constexpr int kFilterParts = 1024, kFeatureParts = 512;
+struct Magnitudes {
+  unsigned filters, features;                                     // (what the products' ends read)
+  unsigned filterParts[kFilterParts], featureParts[kFeatureParts];
+};
+constexpr int kMagnitudeStep = 256 * 4 * 8;   // values a workgroup takes at a time
+
 __device__ __forceinline__ unsigned magnitude4(uintx4p v) {
   return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
 }
@@ -45,30 +53,129 @@ __device__ __forceinline__ unsigned wave_most(unsigned m) {
   for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, kWave));
   return m;
 }
-constexpr int kMagnitudeStep = 256 * 4 * 8;   // values of a workgroup
-__global__ __launch_bounds__(256) void fc_magnitude(unsigned* __restrict__ bits, const float* __restrict__ x, size_t n, int vec) {
-  __shared__ unsigned lds[4];
-  unsigned m = 0;
-  const size_t first = (size_t)blockIdx.x * kMagnitudeStep;
-  if (vec && first + kMagnitudeStep <= n) {
-    const uintx4p* x4 = (const uintx4p*)(x + first) + threadIdx.x;
-    uintx4p v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x4[256 * i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, magnitude4(v[i]));
-  } else {
-    for (size_t i = first + threadIdx.x; i < std::min(first + kMagnitudeStep, n); i += 256) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-  }
+__device__ __forceinline__ unsigned group_most(unsigned m, unsigned* lds) {   // of 256 threads
   m = wave_most(m);
+  __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) atomicMax(bits, max(max(lds[0], lds[1]), max(lds[2], lds[3])));
+  return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
 }
 
-// the magnitudes, and the products' counters behind them
-__global__ __launch_bounds__(256) void fc_clear(unsigned* p, int n) {
-  for (int i = threadIdx.x; i < n; i += 256) p[i] = 0;
+// Workgroups [0, filterGroups): the filters; the rest: a wavefront per instance.
+__global__ __launch_bounds__(256) void fc_magnitudes(Magnitudes* __restrict__ out, unsigned* __restrict__ rows, const float* __restrict__ f, size_t n,
+                                                     int filterGroups, int vec, const float* __restrict__ x, int D, int N,
+                                                     const float* __restrict__ labels, const float* __restrict__ weights, int nWeights, int wide) {
+  __shared__ unsigned lds[4];
+  unsigned most = 0;
+  if ((int)blockIdx.x < filterGroups) {
+    for (size_t first = (size_t)blockIdx.x * kMagnitudeStep; first < n; first += (size_t)filterGroups * kMagnitudeStep) {
+      if (vec && first + kMagnitudeStep <= n) {
+        const uintx4p* f4 = (const uintx4p*)(f + first) + threadIdx.x;
+        uintx4p v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = f4[256 * i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, magnitude4(v[i]));
+      } else {
+        for (size_t i = first + threadIdx.x; i < std::min(first + kMagnitudeStep, n); i += 256) most = max(most, __float_as_uint(f[i]) & 0x7fffffffu);
+      }
+    }
+    most = group_most(most, lds);
+    if (threadIdx.x == 0) out->filterParts[blockIdx.x] = most;
+    return;
+  }
+  const int group = blockIdx.x - filterGroups, groups = gridDim.x - filterGroups, lane = threadIdx.x & 63;
+  for (int row = group * 4 + (int)(threadIdx.x >> 6); row < N; row += groups * 4) {
+    unsigned m = 0;
+    for (int c = 8 * lane; c < D; c += 512) {
+      float v[8];
+      load8(v, x + (size_t)row * D, c, D, wide);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+    }
+    m = wave_most(m);
+    if (lane == 0) rows[row] = m;
+    const float w = instance_weight(labels, weights, nWeights, row);
+    if (w != 0.f) most = max(most, __float_as_uint(fabsf(__uint_as_float(m) * w)));
+  }
+  most = group_most(most, lds);
+  if (threadIdx.x == 0) out->featureParts[group] = most;
+}
+
+// Rows brought into the form the products read: pairs by a magnitude, or bfloat16 at a pitch of whole stages.
+enum { kFilters, kFeatures, kWeighted };   // by the tensor's magnitude; each row by its own; times the instance's weight (zeros for instances
+                                           // that do not count, whatever they hold), by the tensor's
+struct PackPart {
+  const void* x;
+  unsigned short* out;
+  long long pitch;
+  int rows, form, wide;                    // wide: rows can be read 16 bytes at a time
+  unsigned firstGroup;
+};
+struct PackJob {
+  PackPart parts[3];
+  int nParts, D;
+  Magnitudes* magnitudes;                  // pairs
+  int filterGroups, featureGroups;         // 0: `filters` and `features` are there already
+  const unsigned* rowMagnitudes;
+  float* unscale;                          // of the rows by their own magnitudes
+  const float *labels, *weights;
+  int nWeights;
+  unsigned* counters;                      // cleared on the way
+  int nCounters;
+};
+constexpr int kPackSteps = 4;              // times eight values a thread
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void fc_pack(PackJob j) {
+  __shared__ unsigned lds[4];
+  const int which = j.nParts > 2 && blockIdx.x >= j.parts[2].firstGroup ? 2 : j.nParts > 1 && blockIdx.x >= j.parts[1].firstGroup ? 1 : 0;
+  const PackPart p = j.parts[which];
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < j.nCounters; i += 256) j.counters[i] = 0;
+  float scale = 1.f;
+  if (TYPE == kPairs && p.form != kFeatures) {
+    unsigned m = 0;
+    const int parts = p.form == kFilters ? j.filterGroups : j.featureGroups;
+    const unsigned* from = p.form == kFilters ? j.magnitudes->filterParts : j.magnitudes->featureParts;
+    if (parts) {
+      for (int i = threadIdx.x; i < parts; i += 256) m = max(m, from[i]);
+      m = group_most(m, lds);
+      if (blockIdx.x == p.firstGroup && threadIdx.x == 0) (p.form == kFilters ? j.magnitudes->filters : j.magnitudes->features) = m;
+    } else {
+      m = j.magnitudes->filters;
+    }
+    scale = pair_scale(m);
+  }
+  const int per = (int)(p.pitch / (TYPE == kPairs ? 16 : 8));
+#pragma unroll
+  for (int step = 0; step < kPackSteps; ++step) {
+    const size_t i = ((size_t)(blockIdx.x - p.firstGroup) * kPackSteps + step) * 256 + threadIdx.x;
+    if (i >= (size_t)p.rows * per) return;
+    const int row = (int)(i / per), c = (int)(i - (size_t)row * per) * 8;
+    const float w = p.form == kWeighted ? instance_weight(j.labels, j.weights, j.nWeights, row) : 1.f;
+    float v[8] = {};
+    if (TYPE == kPairs) {
+      if (p.form == kFeatures) {
+        scale = pair_scale(j.rowMagnitudes[row]);
+        if (c == 0) j.unscale[row] = pair_unscale(j.rowMagnitudes[row]);
+      }
+      if (w != 0.f) {
+        load8(v, (const float*)p.x + (size_t)row * j.D, c, j.D, p.wide);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = v[k] * w * scale;
+      }
+      store8_pairs(p.out + (size_t)row * p.pitch, c, v);
+    } else {
+      if (w != 0.f) load8(v, (const unsigned short*)p.x + (size_t)row * j.D, c, j.D, p.wide);
+      uintx4p h = {0, 0, 0, 0};
+      if (w != 0.f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = (unsigned)to_bf16(v[2 * k] * w) | (unsigned)to_bf16(v[2 * k + 1] * w) << 16;
+      }
+      *(uintx4p*)(p.out + (size_t)row * p.pitch + c) = h;
+    }
+  }
 }
 
 // (K D / 1024 workgroups: at most 2^34)
@@ -77,65 +184,6 @@ __global__ __launch_bounds__(256) void fc_zero(void* __restrict__ p, size_t n, i
   for (size_t i = first; i < std::min(first + 1024, n); i += 256) {
     if (is16) ((unsigned short*)p)[i] = 0;
     else ((float*)p)[i] = 0.f;
-  }
-}
-
-// Rows of single-precision values as pairs, each by its own largest magnitude: 1 / scale in unscale[row]; the largest magnitude of all
-// rows times their instances' weights in `all` (not null).  A wavefront per row.
-__global__ __launch_bounds__(256) void fc_pack_rows(unsigned short* __restrict__ out, float* __restrict__ unscale, unsigned* __restrict__ all,
-                                                    const float* __restrict__ x, int D, int rows, long long pitch, const float* __restrict__ labels,
-                                                    const float* __restrict__ weights, int nWeights, int wide) {
-  const int row = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  const float* from = x + (size_t)row * D;
-  unsigned m = 0;
-  float v[8];
-  for (int c = 8 * lane; c < D; c += 512) {
-    load8(v, from, c, D, wide);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
-  }
-  m = wave_most(m);
-  const float scale = pair_scale(m);
-  if (lane == 0) {
-    unscale[row] = pair_unscale(m);
-    const float w = all ? instance_weight(labels, weights, nWeights, row) : 0.f;
-    if (w != 0.f) atomicMax(all, __float_as_uint(fabsf(__uint_as_float(m) * w)));
-  }
-  for (int c = 8 * lane; c < pitch / 2; c += 512) {
-    load8(v, from, c, D, wide);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= scale;
-    store8_pairs(out + (size_t)row * pitch, c, v);
-  }
-}
-
-// Rows as the operand of a product: single precision as pairs by the tensor's magnitude, bfloat16 at a pitch of whole stages.  With
-// labels, times the instance's weight, and zeros for instances that do not count, whatever they hold.  A thread per eight
-// values.
-template <int TYPE>
-__global__ __launch_bounds__(256) void fc_pack(unsigned short* __restrict__ out, const unsigned* __restrict__ magnitude, const void* __restrict__ x,
-                                               int D, int rows, long long pitch, const float* __restrict__ labels, const float* __restrict__ weights,
-                                               int nWeights, int wide) {
-  const int per = (int)(pitch / (TYPE == kPairs ? 16 : 8));
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (size_t)rows * per) return;
-  const int row = (int)(i / per), c = (int)(i - (size_t)row * per) * 8;
-  const float w = labels ? instance_weight(labels, weights, nWeights, row) : 1.f;
-  float v[8] = {};
-  if (TYPE == kPairs) {
-    const float scale = pair_scale(*magnitude);
-    if (w != 0.f) load8(v, (const float*)x + (size_t)row * D, c, D, wide);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = w != 0.f ? v[k] * w * scale : 0.f;
-    store8_pairs(out + (size_t)row * pitch, c, v);
-  } else {
-    if (w != 0.f) load8(v, (const unsigned short*)x + (size_t)row * D, c, D, wide);
-    uintx4p h;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = (unsigned)to_bf16(v[2 * k] * w) | (unsigned)to_bf16(v[2 * k + 1] * w) << 16;
-    if (w == 0.f) h = (uintx4p){0, 0, 0, 0};
-    *(uintx4p*)(out + (size_t)row * pitch + c) = h;
   }
 }
 
@@ -268,7 +316,8 @@ struct ProbabilitiesEnd {
   long long pitch;
   const float *labels, *weights, *logSums;
   int nWeights, classes;
-  float* sums;                     // [tile rows][classes]; may be null
+  float* sums;                     // [tile rows][classes], times `factor`; may be null
+  float factor;
   template <class S>
   __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
     const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
@@ -324,7 +373,7 @@ struct ProbabilitiesEnd {
         float s = columns[t];
 #pragma unroll
         for (int w = 1; w < S::WM; ++w) s += columns[w * S::BN + t];
-        sums[(size_t)tm * classes + z.first + n] = s;
+        sums[(size_t)tm * classes + z.first + n] = s * factor;
       }
     }
 #pragma unroll
@@ -413,33 +462,64 @@ struct StoreEnd {
 
 // ---------------------------------------------------------------------------------------------- what follows a product
 
-// log sums of an instance from its tiles, and its term of the value; a wavefront per instance
-__global__ __launch_bounds__(256) void fc_log_sums(float* __restrict__ logSums, float* __restrict__ terms, const float2* __restrict__ parts,
-                                                   const float* __restrict__ own, const float* __restrict__ labels,
-                                                   const float* __restrict__ weights, int nWeights, int N, int tiles) {
-  const int n = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (n >= N) return;
-  const float2* p = parts + (size_t)n * tiles;
-  float most = -__builtin_inff();
-  for (int t = lane; t < tiles; t += 64) most = fmaxf(most, p[t].x);
-  most = wave_max(most);
-  const float from = most == -__builtin_inff() ? 0.f : most;
-  float sum = 0.f;
-  for (int t = lane; t < tiles; t += 64) sum += p[t].y * expf(p[t].x - from);
-  sum = wave_sum(sum);
-  if (lane) return;
-  const float lse = from + logf(sum);
-  logSums[n] = lse;
-  const float w = instance_weight(labels, weights, nWeights, n);
-  terms[n] = w != 0.f ? w * (lse - own[n]) : 0.f;
+// (largest, sum of exponentials against it) of two sets of scores together
+__device__ __forceinline__ float2 both(float2 a, float2 b) {
+  const float most = fmaxf(a.x, b.x), from = most == -__builtin_inff() ? 0.f : most;
+  return make_float2(most, a.y * expf(a.x - from) + b.y * expf(b.x - from));
 }
-
-__global__ __launch_bounds__(256) void fc_total(float* __restrict__ y, const float* __restrict__ terms, int n, int divide) {
+// log sums of an instance from its tiles, WAVES wavefronts per instance, and its term of the value; the workgroup that comes last adds
+// the terms up, in double and in order (they go past the XCDs' L2s, as the parts of a product do)
+template <int WAVES>
+__global__ __launch_bounds__(256) void fc_log_sums(float* __restrict__ y, float* __restrict__ logSums, float* __restrict__ terms, unsigned* __restrict__ counter,
+                                                   const float2* __restrict__ parts, const float* __restrict__ own, const float* __restrict__ labels,
+                                                   const float* __restrict__ weights, int nWeights, int N, int tiles, int divide) {
   __shared__ double lds[4];
+  __shared__ float2 joint[4];
+  __shared__ unsigned last;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = threadIdx.x % (64 * WAVES);
+  constexpr int kPer = 4 / WAVES;
+  for (int first = (int)blockIdx.x * kPer; first < N; first += (int)gridDim.x * kPer) {
+    const int n = first + wave / WAVES;
+    // four at a time, and the four among each other: a chain of as few exponentials as there are steps
+    float2 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = make_float2(-__builtin_inff(), 0.f);
+    if (n < N) {
+      const float2* p = parts + (size_t)n * tiles;
+      for (int i = t; i < tiles; i += 64 * WAVES * 4)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + 64 * WAVES * k < tiles) v[k] = both(v[k], p[i + 64 * WAVES * k]);
+    }
+    float2 s = both(both(v[0], v[1]), both(v[2], v[3]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s = both(s, make_float2(__shfl_xor(s.x, o, kWave), __shfl_xor(s.y, o, kWave)));
+    if (WAVES > 1) {
+      __syncthreads();
+      if (lane == 0) joint[wave] = s;
+      __syncthreads();
+      s = both(both(joint[0], joint[1]), both(joint[2], joint[3]));
+    }
+    if (t == 0 && n < N) {
+      const float lse = (s.x == -__builtin_inff() ? 0.f : s.x) + logf(s.y);
+      logSums[n] = lse;
+      const float w = instance_weight(labels, weights, nWeights, n);
+      __hip_atomic_store(terms + n, w != 0.f ? w * (lse - own[n]) : 0.f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (!y) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
   double acc = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) acc += (double)terms[i];
+  for (int i = threadIdx.x; i < N; i += 256) acc += (double)__hip_atomic_load(terms + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   acc = wave_sum(acc);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = acc;
+  if (lane == 0) lds[threadIdx.x >> 6] = acc;
   __syncthreads();
   if (threadIdx.x == 0) {
     const double s = (lds[0] + lds[1]) + (lds[2] + lds[3]);
@@ -448,12 +528,12 @@ __global__ __launch_bounds__(256) void fc_total(float* __restrict__ y, const flo
 }
 
 // dzdb: the tiles' column sums added up
-__global__ __launch_bounds__(256) void fc_join_columns(float* __restrict__ db, const float* __restrict__ sums, int K, int tileRows, float factor) {
+__global__ __launch_bounds__(256) void fc_join_columns(float* __restrict__ db, const float* __restrict__ sums, int K, int tileRows) {
   const int c = (int)blockIdx.x * 256 + threadIdx.x;
   if (c >= K) return;
   double s = 0.0;
   for (int t = 0; t < tileRows; ++t) s += (double)sums[(size_t)t * K + c];
-  db[c] = (float)s * factor;
+  db[c] = (float)s;
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -465,14 +545,16 @@ struct Plan {
   long long xPitch, fPitch, pPitch;
   int piece, pieces, tiles;        // classes per piece; tiles of scores over all classes
   ProductPlan scores, dx, df;      // of a whole piece; the last one, if smaller, is cut as they are
-  size_t x, xUnscale, xw, f, magnitudes, counters, parts, own, terms, logSums, p, sum, columns, products, total;
-  int nCounters;
+  size_t x, xUnscale, xw, f, magnitudes, rowMagnitudes, counters, parts, own, terms, logSums, p, sum, columns, products, total;
+  int nCounters, tileRows;         // (counters: the last is fc_log_sums')
   // whether rows of D values can be read 16 bytes at a time; workgroups that pack rows
   int wide(const void* t, const mcn_fcloss_geom* g) const { return g->D % (type == kPairs ? 4 : 8) == 0 && aligned16(t); }
-  unsigned pack_blocks(int rows, long long pitch) const { return (unsigned)(((size_t)rows * (pitch / (type == kPairs ? 16 : 8)) + 255) / 256); }
+  unsigned pack_groups(int rows, long long pitch) const {
+    return (unsigned)(((size_t)rows * (pitch / (type == kPairs ? 16 : 8)) + 256 * kPackSteps - 1) / (256 * kPackSteps));
+  }
 };
 
-size_t kPieceBytes_() { return (size_t)std::max(1, tunable("fcloss_piece", 128)) << 20; }
+constexpr size_t kPieceBytes = 128u << 20;
 
 Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool backward) {
   Plan p;
@@ -485,7 +567,7 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   // a piece: P (backward) and the packed filters stay within kPieceBytes, whole tiles
   const long long most = (g->K + 255ll) / 256 * 256;
   const long long perClass = std::max<long long>(backward ? g->N * 2ll * (p.type == kPairs ? 2 : 1) : 0, p.fInPlace ? 0 : p.fPitch * 2);
-  long long piece = perClass ? std::max(256ll, (long long)kPieceBytes_() / perClass / 256 * 256) : most;
+  long long piece = perClass ? std::max(256ll, (long long)kPieceBytes / perClass / 256 * 256) : most;
   if (piece < most) {              // equal pieces
     const long long n = (most + piece - 1) / piece;
     piece = ((most + n - 1) / n + 255) / 256 * 256;
@@ -504,9 +586,11 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  p.nCounters = (int)(backward ? std::max({p.scores.counters(), p.dx.counters(), p.df.counters()}) : p.scores.counters());
-  p.magnitudes = take(8 + 4 * p.nCounters);
-  p.counters = p.magnitudes + 8;
+  p.tileRows = div_up(g->N, kTileSize[p.scores.tile]);
+  p.nCounters = 1 + (int)(backward ? std::max({p.scores.counters(), p.dx.counters(), p.df.counters()}) : p.scores.counters());
+  p.magnitudes = take(p.type == kPairs ? sizeof(Magnitudes) : 0);
+  p.rowMagnitudes = take(p.type == kPairs ? (size_t)g->N * 4 : 0);
+  p.counters = take(4 * (size_t)p.nCounters);
   p.products = take(backward ? std::max({p.scores.partBytes(), p.dx.partBytes(), p.df.partBytes()}) : p.scores.partBytes());
   p.x = take(p.xInPlace ? 0 : (size_t)g->N * p.xPitch * 2);
   p.xUnscale = take(p.type == kPairs ? (size_t)g->N * 4 : 0);
@@ -518,7 +602,7 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   p.xw = p.p = p.sum = p.columns = 0;
   if (backward) {
     p.xw = take((size_t)g->N * p.xPitch * 2);
-    p.columns = take((size_t)div_up(g->N, kTileSize[p.scores.tile]) * g->K * 4);
+    p.columns = take(p.tileRows > 1 ? (size_t)p.tileRows * g->K * 4 : 0);
     p.p = take((size_t)g->N * p.pPitch * 2);
     p.sum = take(p.type == kBf16 && p.pieces > 1 ? (size_t)g->N * g->D * 4 : 0);
   }
@@ -538,116 +622,149 @@ int check(const char* who, const mcn_fcloss_geom* g, size_t nLabels, const float
   return MCN_SUCCESS;
 }
 
-// x as the operand of the scores, and the magnitudes of the filters and of the weighted features
-int pack_x(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geom* g, char* ws, const void* x, const void* f, const float* labels,
-           const float* weights, int nWeights, bool weighted, Matrix* op) {
-  *op = {p.xInPlace ? x : ws + p.x, p.xPitch, 0, g->N};
-  unsigned* m = (unsigned*)(ws + p.magnitudes);
-  if (p.type == kPairs || p.nCounters) {
-    KernelTimer timer("fc_clear", s);
-    hipLaunchKernelGGL(fc_clear, dim3(1), dim3(256), 0, s, m, 2 + p.nCounters);
+struct Call {
+  hipStream_t s;
+  const char* who;
+  const mcn_fcloss_geom* g;
+  const void *x, *filters;
+  const float *biases, *labels, *weights;
+  int nWeights;
+  char* ws;
+  Plan p;
+  Magnitudes* magnitudes() const { return (Magnitudes*)(ws + p.magnitudes); }
+  Scratch scratch() const { return {(float*)(ws + p.products), (unsigned*)(ws + p.counters)}; }
+  Matrix X() const { return {p.xInPlace ? x : ws + p.x, p.xPitch, 0, g->N}; }
+  const char* piece_of(const void* t, int first) const { return (const char*)t + (size_t)first * g->D * (p.type == kPairs ? 4 : 2); }
+  int classes(int piece) const { return std::min(p.piece, g->K - piece * p.piece); }
+  Matrix F(int piece) const { return {p.fInPlace ? piece_of(filters, piece * p.piece) : ws + p.f, p.fPitch, 0, classes(piece)}; }
+};
+
+void launch_pack(const Call& c, PackJob& j) {
+  unsigned groups = 0;
+  for (int k = 0; k < j.nParts; ++k) {
+    j.parts[k].firstGroup = groups;
+    j.parts[k].wide = c.p.wide(j.parts[k].x, c.g);
+    groups += c.p.pack_groups(j.parts[k].rows, j.parts[k].pitch);
   }
+  if (groups == 0) {               // (the counters alone)
+    j.parts[0] = {};
+    groups = 1;
+  }
+  KernelTimer timer("fc_pack", c.s);
+  if (c.p.type == kPairs) hipLaunchKernelGGL(fc_pack<kPairs>, dim3(groups), dim3(256), 0, c.s, j);
+  else hipLaunchKernelGGL(fc_pack<kBf16>, dim3(groups), dim3(256), 0, c.s, j);
+}
+
+// What comes before the products: magnitudes, the features (and, for dzdf, the weighted ones), the first piece of the filters, counters
+int prepare(const Call& c, bool weighted) {
+  const Plan& p = c.p;
+  PackJob j = {};
+  j.D = c.g->D;
+  j.labels = c.labels; j.weights = c.weights; j.nWeights = c.nWeights;
+  j.counters = (unsigned*)(c.ws + p.counters); j.nCounters = p.nCounters;
   if (p.type == kPairs) {
-    const size_t n = (size_t)g->K * g->D;
-    KernelTimer timer("fc_magnitude", s);
-    hipLaunchKernelGGL(fc_magnitude, dim3((unsigned)((n + kMagnitudeStep - 1) / kMagnitudeStep)), dim3(256), 0, s, m, (const float*)f, n, (int)aligned16(f));
+    const size_t n = (size_t)c.g->K * c.g->D;
+    j.magnitudes = c.magnitudes();
+    j.rowMagnitudes = (unsigned*)(c.ws + p.rowMagnitudes);
+    j.unscale = (float*)(c.ws + p.xUnscale);
+    j.filterGroups = (int)std::min<size_t>(kFilterParts, (n + kMagnitudeStep - 1) / kMagnitudeStep);
+    j.featureGroups = std::min(kFeatureParts, div_up(c.g->N, 4));
+    KernelTimer timer("fc_magnitudes", c.s);
+    hipLaunchKernelGGL(fc_magnitudes, dim3((unsigned)(j.filterGroups + j.featureGroups)), dim3(256), 0, c.s, j.magnitudes, (unsigned*)(c.ws + p.rowMagnitudes),
+                       (const float*)c.filters, n, j.filterGroups, (int)aligned16(c.filters), (const float*)c.x, c.g->D, c.g->N, c.labels, c.weights,
+                       c.nWeights, p.wide(c.x, c.g));
   }
-  if (p.xInPlace) return MCN_SUCCESS;
-  KernelTimer timer("fc_pack", s);
-  if (p.type == kPairs)
-    hipLaunchKernelGGL(fc_pack_rows, dim3((unsigned)div_up(g->N, 4)), dim3(256), 0, s, (unsigned short*)(ws + p.x), (float*)(ws + p.xUnscale),
-                       weighted ? m + 1 : nullptr, (const float*)x, g->D, g->N, p.xPitch, labels, weights, nWeights, p.wide(x, g));
-  else
-    hipLaunchKernelGGL(fc_pack<kBf16>, dim3(p.pack_blocks(g->N, p.xPitch)), dim3(256), 0, s, (unsigned short*)(ws + p.x), (const unsigned*)nullptr, x, g->D,
-                       g->N, p.xPitch, (const float*)nullptr, (const float*)nullptr, 1, p.wide(x, g));
-  return check_launch(who);
+  if (!p.fInPlace) j.parts[j.nParts++] = {c.filters, (unsigned short*)(c.ws + p.f), p.fPitch, c.classes(0), kFilters, 0, 0};
+  if (!p.xInPlace) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.x), p.xPitch, c.g->N, kFeatures, 0, 0};
+  if (weighted) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.xw), p.xPitch, c.g->N, kWeighted, 0, 0};
+  launch_pack(c, j);
+  return check_launch(c.who);
 }
 
-// rows of x or the filters as an operand of all products (by the tensor's magnitude), or times the instances' weights
-template <int TYPE>
-void pack(hipStream_t s, const Plan& p, const mcn_fcloss_geom* g, char* out, const unsigned* magnitude, const void* x, int rows, long long pitch,
-          const float* labels, const float* weights, int nWeights) {
-  KernelTimer timer("fc_pack", s);
-  hipLaunchKernelGGL(fc_pack<TYPE>, dim3(p.pack_blocks(rows, pitch)), dim3(256), 0, s, (unsigned short*)out, magnitude, x, g->D, rows, pitch, labels, weights,
-                     nWeights, p.wide(x, g));
-}
-
-// the filters of a piece
-template <int TYPE>
-Matrix pack_f(hipStream_t s, const Plan& p, const mcn_fcloss_geom* g, char* ws, const void* f, int first, int count) {
-  const char* from = (const char*)f + (size_t)first * g->D * (TYPE == kPairs ? 4 : 2);
-  if (!p.fInPlace) pack<TYPE>(s, p, g, ws + p.f, (const unsigned*)(ws + p.magnitudes), from, count, p.fPitch, nullptr, nullptr, 1);
-  return {p.fInPlace ? from : ws + p.f, p.fPitch, 0, count};
+// the filters of a piece, where its products read them (`there`: prepare() has done it)
+void pack_piece(const Call& c, int piece, bool there) {
+  if (c.p.fInPlace || there) return;
+  PackJob j = {};
+  j.D = c.g->D;
+  j.magnitudes = c.magnitudes();
+  j.parts[j.nParts++] = {c.piece_of(c.filters, piece * c.p.piece), (unsigned short*)(c.ws + c.p.f), c.p.fPitch, c.classes(piece), kFilters, 0, 0};
+  launch_pack(c, j);
 }
 
 template <int TYPE>
-int forward(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geom* g, float* logSums, const void* f, const float* biases,
-            const float* labels, const float* weights, int nWeights, char* ws, const Matrix& X) {
-  const Scratch scratch = {(float*)(ws + p.products), (unsigned*)(ws + p.counters)};
+Scores scores_of(const Call& c, int piece) {
+  return {TYPE == kPairs ? (const float*)(c.ws + c.p.xUnscale) : nullptr, c.biases, TYPE == kPairs ? &c.magnitudes()->filters : nullptr, c.g->N,
+          c.classes(piece), piece * c.p.piece};
+}
+
+// y may be null (the log sums alone)
+template <int TYPE>
+int forward(const Call& c, float* y, float* logSums) {
+  const Plan& p = c.p;
+  const int N = c.g->N;
   for (int k = 0; k < p.pieces; ++k) {
-    const int first = k * p.piece, count = std::min(p.piece, g->K - first);
-    const Matrix F = pack_f<TYPE>(s, p, g, ws, f, first, count);
+    pack_piece(c, k, k == 0);
     StatsEnd e;
-    e.z = {TYPE == kPairs ? (const float*)(ws + p.xUnscale) : nullptr, biases, (const unsigned*)(ws + p.magnitudes), g->N, count, first};
-    e.parts = (float2*)(ws + p.parts);
-    e.own = (float*)(ws + p.own);
-    e.labels = labels;
-    e.tiles = p.tiles; e.firstTile = first / kTileSize[p.scores.tile]; e.classes = g->K;
-    const int rc = product<TYPE, false, false>(s, who, "fc_scores", X, F, g->N, count, p.scores.of(g->N, count), scratch, e);
+    e.z = scores_of<TYPE>(c, k);
+    e.parts = (float2*)(c.ws + p.parts);
+    e.own = (float*)(c.ws + p.own);
+    e.labels = c.labels;
+    e.tiles = p.tiles; e.firstTile = k * p.piece / kTileSize[p.scores.tile]; e.classes = c.g->K;
+    const int rc = product<TYPE, false, false>(c.s, c.who, "fc_scores", c.X(), c.F(k), N, c.classes(k), p.scores.of(N, c.classes(k)), c.scratch(), e);
     if (rc) return rc;
   }
-  KernelTimer timer("fc_log_sums", s);
-  hipLaunchKernelGGL(fc_log_sums, dim3((unsigned)div_up(g->N, 4)), dim3(256), 0, s, logSums, (float*)(ws + p.terms), (const float2*)(ws + p.parts),
-                     (const float*)(ws + p.own), labels, weights, nWeights, g->N, p.tiles);
-  return check_launch(who);
+  KernelTimer timer("fc_log_sums", c.s);
+  // (few instances: four wavefronts each.  More than 256 workgroups wait for each other at the counter.)
+  const bool few = N <= 256;
+  hipLaunchKernelGGL(few ? fc_log_sums<4> : fc_log_sums<1>, dim3((unsigned)std::min(256, div_up(N, few ? 1 : 4))), dim3(256), 0, c.s, y, logSums,
+                     (float*)(c.ws + p.terms), (unsigned*)(c.ws + p.counters) + p.nCounters - 1, (const float2*)(c.ws + p.parts),
+                     (const float*)(c.ws + p.own), c.labels, c.weights, c.nWeights, N, p.tiles, c.g->normalise ? N : 0);
+  return check_launch(c.who);
 }
 
 template <int TYPE>
-int backward(hipStream_t s, const char* who, const Plan& p, const mcn_fcloss_geom* g, void* derInput, void* derFilters, float* derBiases,
-             const float* logSums, const void* f, const float* biases, const float* labels, const float* weights, int nWeights, float factor,
-             char* ws, const Matrix& X, const void* x) {
-  const unsigned* mag = (const unsigned*)(ws + p.magnitudes);
-  const Matrix Xw = {ws + p.xw, p.xPitch, 0, g->N};
-  const Scratch scratch = {(float*)(ws + p.products), (unsigned*)(ws + p.counters)};
-  if (derFilters) pack<TYPE>(s, p, g, ws + p.xw, mag + 1, x, g->N, p.xPitch, labels, weights, nWeights);
+int backward(const Call& c, void* derInput, void* derFilters, float* derBiases, const float* logSums, float factor, bool firstThere) {
+  const Plan& p = c.p;
+  const int N = c.g->N, D = c.g->D;
+  const Matrix Xw = {c.ws + p.xw, p.xPitch, 0, N};
   const float times = TYPE == kPairs ? factor / kProbability : factor;
   for (int k = 0; k < p.pieces; ++k) {
-    const int first = k * p.piece, count = std::min(p.piece, g->K - first);
-    const Matrix F = pack_f<TYPE>(s, p, g, ws, f, first, count);
+    const int first = k * p.piece, count = c.classes(k), columns = (count + 63) / 64 * 64;
+    pack_piece(c, k, k == 0 && firstThere);
     ProbabilitiesEnd e;
-    e.z = {TYPE == kPairs ? (const float*)(ws + p.xUnscale) : nullptr, biases, mag, g->N, count, first};
-    e.out = (unsigned short*)(ws + p.p);
+    e.z = scores_of<TYPE>(c, k);
+    e.out = (unsigned short*)(c.ws + p.p);
     e.pitch = p.pPitch;
-    e.labels = labels; e.weights = weights; e.logSums = logSums;
-    e.nWeights = nWeights; e.classes = g->K;
-    e.sums = derBiases ? (float*)(ws + p.columns) : nullptr;
-    int rc = product<TYPE, false, false>(s, who, "fc_probabilities", X, F, g->N, (count + 63) / 64 * 64, p.scores.of(g->N, (count + 63) / 64 * 64), scratch, e);
+    e.labels = c.labels; e.weights = c.weights; e.logSums = logSums;
+    e.nWeights = c.nWeights; e.classes = c.g->K;
+    e.sums = !derBiases ? nullptr : p.tileRows > 1 ? (float*)(c.ws + p.columns) : derBiases;
+    e.factor = factor;
+    int rc = product<TYPE, false, false>(c.s, c.who, "fc_probabilities", c.X(), c.F(k), N, columns, p.scores.of(N, columns), c.scratch(), e);
     if (rc) return rc;
-    const Matrix P = {ws + p.p, p.pPitch, 0, g->N};
+    const Matrix P = {c.ws + p.p, p.pPitch, 0, N};
     if (derInput) {
       // (the pieces add up in single precision: in derInput itself, or beside it)
-      float* sum = TYPE == kPairs ? (float*)derInput : (float*)(ws + p.sum);
+      float* sum = TYPE == kPairs ? (float*)derInput : (float*)(c.ws + p.sum);
       const bool last = k == p.pieces - 1;
-      const StoreEnd d = {TYPE == kPairs || last ? derInput : sum, TYPE == kBf16 && last, k > 0 ? sum : nullptr, g->N, g->D, times,
-                          TYPE == kPairs ? mag : nullptr, labels, weights, nWeights};
+      const StoreEnd d = {TYPE == kPairs || last ? derInput : sum, TYPE == kBf16 && last, k > 0 ? sum : nullptr, N, D, times,
+                          TYPE == kPairs ? &c.magnitudes()->filters : nullptr, c.labels, c.weights, c.nWeights};
       ProductPlan q = p.dx;
       q.stages = div_up(count, stage_depth(TYPE));
-      rc = product<TYPE, false, true>(s, who, "fc_derivative_x", P, F, g->N, g->D, q, scratch, d);
+      rc = product<TYPE, false, true>(c.s, c.who, "fc_derivative_x", P, c.F(k), N, D, q, c.scratch(), d);
       if (rc) return rc;
     }
     if (derFilters) {
-      const StoreEnd d = {(char*)derFilters + (size_t)first * g->D * (TYPE == kPairs ? 4 : 2), TYPE == kBf16, nullptr, count, g->D, times,
-                          TYPE == kPairs ? mag + 1 : nullptr, nullptr, nullptr, 1};
-      rc = product<TYPE, true, true>(s, who, "fc_derivative_f", P, Xw, count, g->D, p.df.of(count, g->D), scratch, d);
+      const StoreEnd d = {(void*)c.piece_of(derFilters, first), TYPE == kBf16, nullptr, count, D, times,
+                          TYPE == kPairs ? &c.magnitudes()->features : nullptr, nullptr, nullptr, 1};
+      rc = product<TYPE, true, true>(c.s, c.who, "fc_derivative_f", P, Xw, count, D, p.df.of(count, D), c.scratch(), d);
       if (rc) return rc;
     }
   }
-  if (derBiases) {
-    KernelTimer timer("fc_join", s);
-    hipLaunchKernelGGL(fc_join_columns, dim3((unsigned)div_up(g->K, 256)), dim3(256), 0, s, derBiases, (const float*)(ws + p.columns), g->K,
-                       div_up(g->N, kTileSize[p.scores.tile]), factor);
+  if (derBiases && p.tileRows > 1) {
+    KernelTimer timer("fc_join", c.s);
+    hipLaunchKernelGGL(fc_join_columns, dim3((unsigned)div_up(c.g->K, 256)), dim3(256), 0, c.s, derBiases, (const float*)(c.ws + p.columns), c.g->K, p.tileRows);
   }
-  return check_launch(who);
+  return check_launch(c.who);
 }
 
 }  // namespace
@@ -660,9 +777,11 @@ extern "C" {
 size_t mcn_fcloss_workspace_bytes(const mcn_fcloss_geom* g, int backward) {
   if (!g || g->D <= 0 || g->K <= 0 || g->N <= 0 || g->D > (1 << 20) || g->K > (1 << 24)) return 0;
   if (g->dataType != MCN_FLOAT && g->dataType != MCN_BFLOAT16) return 0;
-  // (the larger of the two ways tensors can be aligned)
+  // (the largest of the ways the tensors can be aligned)
   const void* odd = (const void*)2;
-  return std::max(make_plan(g, nullptr, nullptr, backward != 0).total, make_plan(g, odd, odd, backward != 0).total);
+  size_t most = 0;
+  for (int k = 0; k < 4; ++k) most = std::max(most, make_plan(g, k & 1 ? odd : nullptr, k & 2 ? odd : nullptr, backward != 0).total);
+  return most;
 }
 
 int mcn_fcloss_forward(mcn_stream_t stream, const mcn_fcloss_geom* g, float* y, float* logSums, const void* x, const void* filters,
@@ -672,25 +791,18 @@ int mcn_fcloss_forward(mcn_stream_t stream, const mcn_fcloss_geom* g, float* y, 
   int rc = check(who, g, nLabels, instanceWeights, nWeights);
   if (rc) return rc;
   if (!y) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null output", who);
-  hipStream_t s = as_stream(stream);
-  char* ws = (char*)workspace;
-  Plan p;
-  if (g->N > 0) {
-    if (!x || !filters || !labels) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null tensor", who);
-    p = make_plan(g, x, filters, false);
-    if (!workspace || workspaceBytes < p.total)
-      return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, p.total);
-    Matrix X;
-    rc = pack_x(s, who, p, g, ws, x, filters, labels, instanceWeights, (int)nWeights, false, &X);
-    if (rc) return rc;
-    float* sums = logSums ? logSums : (float*)(ws + p.logSums);
-    rc = p.type == kPairs ? forward<kPairs>(s, who, p, g, sums, filters, biases, labels, instanceWeights, (int)nWeights, ws, X)
-                          : forward<kBf16>(s, who, p, g, sums, filters, biases, labels, instanceWeights, (int)nWeights, ws, X);
-    if (rc) return rc;
+  if (g->N == 0) {
+    hipLaunchKernelGGL(fc_zero, dim3(1), dim3(256), 0, as_stream(stream), y, (size_t)1, 0);
+    return check_launch(who);
   }
-  KernelTimer timer("fc_total", s);
-  hipLaunchKernelGGL(fc_total, dim3(1), dim3(256), 0, s, y, g->N > 0 ? (const float*)(ws + p.terms) : nullptr, g->N, g->normalise ? g->N : 0);
-  return check_launch(who);
+  if (!x || !filters || !labels) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null tensor", who);
+  const Call c = {as_stream(stream), who, g, x, filters, biases, labels, instanceWeights, (int)nWeights, (char*)workspace, make_plan(g, x, filters, false)};
+  if (!workspace || workspaceBytes < c.p.total)
+    return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, c.p.total);
+  rc = prepare(c, false);
+  if (rc) return rc;
+  float* sums = logSums ? logSums : (float*)(c.ws + c.p.logSums);
+  return c.p.type == kPairs ? forward<kPairs>(c, y, sums) : forward<kBf16>(c, y, sums);
 }
 
 int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, void* derInput, void* derFilters, float* derBiases, const float* logSums,
@@ -701,35 +813,31 @@ int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, void* der
   if (rc) return rc;
   if (!derInput && !derFilters && !derBiases) return MCN_SUCCESS;
   if (g->N == 0) {   // sums over no images
-    if (derFilters && (size_t)g->K * g->D) {
-      hipLaunchKernelGGL(fc_zero, dim3((unsigned)(((size_t)g->K * g->D + 1023) / 1024)), dim3(256), 0, as_stream(stream), derFilters,
-                         (size_t)g->K * g->D, g->dataType == MCN_BFLOAT16);
-    }
+    const size_t n = (size_t)g->K * g->D;
+    if (derFilters && n)
+      hipLaunchKernelGGL(fc_zero, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, as_stream(stream), derFilters, n, g->dataType == MCN_BFLOAT16);
     if (derBiases && g->K)
       hipLaunchKernelGGL(fc_zero, dim3((unsigned)((g->K + 1023) / 1024)), dim3(256), 0, as_stream(stream), derBiases, (size_t)g->K, 0);
     return check_launch(who);
   }
   if (!x || !filters || !labels) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null tensor", who);
-  const Plan p = make_plan(g, x, filters, true);
-  if (!workspace || workspaceBytes < p.total)
-    return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, p.total);
-  hipStream_t s = as_stream(stream);
-  char* ws = (char*)workspace;
-  Matrix X;
-  rc = pack_x(s, who, p, g, ws, x, filters, labels, instanceWeights, (int)nWeights, true, &X);
+  const Call c = {as_stream(stream), who, g, x, filters, biases, labels, instanceWeights, (int)nWeights, (char*)workspace, make_plan(g, x, filters, true)};
+  if (!workspace || workspaceBytes < c.p.total)
+    return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, c.p.total);
+  rc = prepare(c, derFilters != nullptr);
   if (rc) return rc;
   const float factor = (float)(g->normalise ? derOutput / g->N : derOutput);
-  if (!logSums) {
-    float* sums = (float*)(ws + p.logSums);
-    rc = p.type == kPairs ? forward<kPairs>(s, who, p, g, sums, filters, biases, labels, instanceWeights, (int)nWeights, ws, X)
-                          : forward<kBf16>(s, who, p, g, sums, filters, biases, labels, instanceWeights, (int)nWeights, ws, X);
+  const bool recompute = logSums == nullptr;
+  if (recompute) {
+    float* sums = (float*)(c.ws + c.p.logSums);
+    rc = c.p.type == kPairs ? forward<kPairs>(c, nullptr, sums) : forward<kBf16>(c, nullptr, sums);
     if (rc) return rc;
     logSums = sums;
   }
-  return p.type == kPairs ? backward<kPairs>(s, who, p, g, derInput, derFilters, derBiases, logSums, filters, biases, labels, instanceWeights,
-                                             (int)nWeights, factor, ws, X, x)
-                          : backward<kBf16>(s, who, p, g, derInput, derFilters, derBiases, logSums, filters, biases, labels, instanceWeights,
-                                            (int)nWeights, factor, ws, X, x);
+  // (with more than one piece the log sums' pass leaves the last one's filters behind)
+  const bool there = !recompute || c.p.pieces == 1;
+  return c.p.type == kPairs ? backward<kPairs>(c, derInput, derFilters, derBiases, logSums, factor, there)
+                            : backward<kBf16>(c, derInput, derFilters, derBiases, logSums, factor, there);
 }
 
 }  // extern "C"

@@ -478,16 +478,15 @@ inline ProductPlan plan_product(int type, long long M, long long N, long long de
 }
 
 // A kernel with more than 64 KiB of local memory has to be told so once per device.
-template <class S>
-int allow_lds(const char* who, const void* kernel) {
-  if (S::ldsBytes <= 65536) return MCN_SUCCESS;
+inline int allow_lds(const char* who, const void* kernel, int bytes) {
+  if (bytes <= 65536) return MCN_SUCCESS;
   static std::mutex mutex;
   static std::set<std::pair<const void*, int>> raised;
   const int dev = current_device();
   if (dev < 0) return fail(MCN_DEVICE_ERROR, "%s: no device", who);
   std::lock_guard<std::mutex> lock(mutex);
   if (raised.count({kernel, dev})) return MCN_SUCCESS;
-  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::ldsBytes) != hipSuccess) {
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
     (void)hipGetLastError();
     return fail(MCN_DEVICE_ERROR, "%s: local memory", who);
   }
@@ -507,7 +506,7 @@ int run_product(hipStream_t s, const char* who, const char* name, const Matrix& 
   if (p.tiles * p.slices >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
   const TileGrid g = {div_up(M, S::BM), div_up(N, S::BN), count, triangle};
   const auto kernel = product_kernel<S, A_ACROSS, B_ACROSS, E>;
-  const int rc = allow_lds<S>(who, (const void*)kernel);
+  const int rc = allow_lds(who, (const void*)kernel, S::ldsBytes);
   if (rc) return rc;
   KernelTimer timer(name, s);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tiles * p.slices)), dim3(S::threads), S::ldsBytes, s, A, B, g, p.stages,

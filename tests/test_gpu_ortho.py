@@ -166,6 +166,7 @@ def test_every_cut_of_the_products(capi, tile, slices):
     try:
         capi.set_tunable("product_tile", tile)
         capi.set_tunable("product_slices", slices)
+        capi.set_tunable("ortho_no_narrow", 1)
         r = torch.Generator(device="cuda")
         r.manual_seed(7)
         for count, K, D in [(2, 70, 333), (1, 515, 300), (1, 290, 290), (3, 33, 40)]:
@@ -174,3 +175,20 @@ def test_every_cut_of_the_products(capi, tile, slices):
     finally:
         capi.set_tunable("product_tile", 0)
         capi.set_tunable("product_slices", 0)
+        capi.set_tunable("ortho_no_narrow", 0)
+
+
+@pytest.mark.parametrize("count,K,D", [(1, 1, 1), (2, 64, 576), (2, 576, 64), (1, 63, 575), (1, 65, 64), (1, 33, 1), (1, 1, 576), (3, 31, 129), (1, 64, 577), (70, 8, 24),
+                                       (1, 576, 33), (1, 64, 64)])
+def test_narrow_matrices_in_one_launch(capi, count, K, D):
+    """Up to 64 x 576 either way: all steps in one launch, within the same bound as the products launch by launch."""
+    r = torch.Generator(device="cuda")
+    r.manual_seed(8)
+    g = torch.randn((count, K, D), generator=r, device="cuda")
+    for steps in (1, 5):
+        check(capi, g, steps)
+        try:
+            capi.set_tunable("ortho_no_narrow", 1)
+            check(capi, g, steps)
+        finally:
+            capi.set_tunable("ortho_no_narrow", 0)
