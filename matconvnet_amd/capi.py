@@ -708,39 +708,38 @@ def data_type(*tensors):
     return BFLOAT16 if kind == torch.bfloat16 else FLOAT
 
 
-def _single(**tensors):
-    for name, t in tensors.items():
-        if t is not None and t.dtype != _torch().float32:
-            raise TypeError("%s is not single precision: %s" % (name, t.dtype))
-
-
-def _dense(**tensors):
-    for name, t in tensors.items():
+def _device(names, *tensors):
+    """Contiguous tensors on the device, or an error that names the one that is not."""
+    for name, t in zip(names.split(), tensors):
         if t is not None and not (t.is_cuda and t.is_contiguous()):
             raise ValueError("%s is not a contiguous tensor on the device" % name)
 
 
+def _single(names, *tensors):
+    """... in single precision"""
+    single = _torch().float32
+    for name, t in zip(names.split(), tensors):
+        if t is not None and t.dtype != single:
+            raise TypeError("%s is not single precision: %s" % (name, t.dtype))
+    _device(names, *tensors)
+
+
 def convert(x, dtype):
     """x as float32 or bfloat16 (include/mcn_hip.h: mcn_convert)."""
-    _dense(x=x)
+    _device("x", x)
     y = _torch().empty_like(x, dtype=dtype)
     check(lib().mcn_convert(stream(), ptr(y), data_type(y), ptr(x), data_type(x), x.numel()))
     return y
-
-
-def _per_channel(C_, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.numel() != C_:
-            raise ValueError("%s does not have one value per channel" % name)
 
 
 def lnorm_forward(x, g, b, eps=1e-5, moments=None):
     """Layer normalisation (include/mcn_hip.h: mcn_lnorm_forward): (y, moments).  x: float32 or bfloat16; g, b: float32 or None;
     moments (2, N, W, H) in float32: all means, then all sigmas; given ones are used as they stand."""
     H, W, Cc, N = _hwcn(x)
-    _single(g=g, b=b, moments=moments)
-    _dense(x=x, g=g, b=b, moments=moments)
-    _per_channel(Cc, g=g, b=b)
+    _single("g b moments", g, b, moments)
+    _device("x", x)
+    if (g is not None and g.numel() != Cc) or (b is not None and b.numel() != Cc):
+        raise ValueError("g or b does not have one value per channel")
     given = moments is not None
     if given and moments.numel() != 2 * H * W * N:
         raise ValueError("moments does not have two values per pixel")
@@ -754,9 +753,10 @@ def lnorm_backward(x, g, dy, eps=1e-5, moments=None, want=(True, True, True), ws
     """(dzdx, dzdg, dzdb) of layer normalisation; those not wanted are None.  moments: as lnorm_forward left them, or None."""
     ws = ws or _ws
     H, W, Cc, N = _hwcn(x)
-    _single(g=g, moments=moments)
-    _dense(x=x, g=g, dy=dy, moments=moments)
-    _per_channel(Cc, g=g)
+    _single("g moments", g, moments)
+    _device("x dy", x, dy)
+    if g is not None and g.numel() != Cc:
+        raise ValueError("g does not have one value per channel")
     if dy.numel() != x.numel():
         raise ValueError("x and dy do not have the same number of elements")
     if moments is not None and moments.numel() != 2 * H * W * N:
@@ -780,8 +780,8 @@ def fcloss_geom(x, f, normalise=True):
 
 
 def _fcloss_check(x, f, b, c, instance_weights, log_sums):
-    _single(b=b, c=c, instance_weights=instance_weights, log_sums=log_sums)
-    _dense(x=x, f=f, b=b, c=c, instance_weights=instance_weights, log_sums=log_sums)
+    _single("b c instance_weights log_sums", b, c, instance_weights, log_sums)
+    _device("x f", x, f)
     if b is not None and b.numel() != f.shape[0]:
         raise ValueError("b does not have one value per class")
     if log_sums is not None and log_sums.numel() != x.shape[0]:
@@ -827,8 +827,7 @@ def _banks(x):
 def orthogonalise(x, steps=5, ws=None):
     """Filter banks (count, K, ...) in float32, each orthogonalised by Newton-Schulz products (include/mcn_hip.h: mcn_orthogonalise)."""
     ws = ws or _ws
-    _single(x=x)
-    _dense(x=x)
+    _single("x", x)
     count, K, D = _banks(x)
     y = _torch().empty_like(x)
     wp, wn = ws.get(lib().mcn_orthogonalise_workspace_bytes(K, D, count))

@@ -62,6 +62,7 @@ Tunable g_tunables[] = {
     {"conv_pix_multi", 1},             // the stride classes of a strided backward-data product share one launch where they can
     {"conv_force_direct", 0},          // 1: always use the direct (non-MFMA) convolution kernels
     {"conv_no_uniform_tap", 0},        // 1: disable the uniform-tap variant of the pixel-major kernel (and the kernels with split operands)
+    {"fcloss_piece_kib", 0},           // > 0: so many KiB for a piece of the classes instead of 256 MiB
     {"ortho_no_narrow", 0},            // 1: narrow matrices through the launches of the others too
     {"product_tile", 0},               // 64, 128, 256: force the tile of the products of fcloss.hip and ortho.hip; 0 = choose
     {"product_slices", 0},             // > 0: cut their reductions among so many workgroups (as far as there are stages)

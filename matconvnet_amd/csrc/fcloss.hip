@@ -322,7 +322,7 @@ struct ProbabilitiesEnd {
   __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
     const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
     z.make<S>(acc, m0, n0, (tn + 1) * S::BN);
-    float* columns = (float*)lds;  // [WM][BN]
+    float* columns = (float*)(lds + S::ldsBytes - S::WM * S::BN * 4);  // [WM][BN]
     float weight[S::TM];
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
@@ -376,32 +376,37 @@ struct ProbabilitiesEnd {
         sums[(size_t)tm * classes + z.first + n] = s * factor;
       }
     }
+    constexpr int size = S::type == kPairs ? 4 : 2, J = turned_blocks<S, size>();
+    const RowTurn<J * 32 * size> turn(lds, wn * S::WM + wm);
+    static_assert(S::WM * S::WN * RowTurn<J * 32 * size>::size + S::WM * S::BN * 4 <= S::ldsBytes, "beside the columns");
+    const int half = lane >> 5, l32 = lane & 31, first = tn * S::BN + 32 * wn * S::TN;
 #pragma unroll
-    for (int i = 0; i < S::TM; ++i) {
-      const int m = m0 + 32 * i;
-      if (m >= z.N) continue;
-      unsigned short* row = out + (size_t)m * pitch;
+    for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-      for (int j = 0; j < S::TN; ++j)
+      for (int j0 = 0; j0 < S::TN; j0 += J) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + 32 * j + 8 * q;
-          const floatx16p& a = acc[i][j];
-          if ((S::type == kPairs ? 2 * (n / 32 * 32) : n) >= pitch) continue;
-          unsigned h[4];
-          if (S::type == kPairs) {
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) h[r] = split_pair(a[4 * q + r] * kProbability);
-            uintx2p* at = (uintx2p*)(row + (n / 32) * 64 + n % 32);
-            at[0] = (uintx2p){(h[0] & 0xffffu) | h[1] << 16, (h[2] & 0xffffu) | h[3] << 16};
-            at[8] = (uintx2p){h[0] >> 16 | (h[1] & 0xffff0000u), h[2] >> 16 | (h[3] & 0xffff0000u)};
-          } else {
+          for (int q = 0; q < 4; ++q) {
+            const floatx16p& a = acc[i][j0 + j];
+            const int column = 8 * q + 4 * half;
+            unsigned h[4];
+            if (S::type == kPairs) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) h[r] = to_bf16(a[4 * q + r]);
-            *(uintx2p*)(row + n) = (uintx2p){h[0] | h[1] << 16, h[2] | h[3] << 16};
+              for (int r = 0; r < 4; ++r) h[r] = split_pair(a[4 * q + r] * kProbability);
+              *(uintx2p*)turn.at(l32, 128 * j + 2 * column) = (uintx2p){(h[0] & 0xffffu) | h[1] << 16, (h[2] & 0xffffu) | h[3] << 16};
+              *(uintx2p*)turn.at(l32, 128 * j + 64 + 2 * column) = (uintx2p){h[0] >> 16 | (h[1] & 0xffff0000u), h[2] >> 16 | (h[3] & 0xffff0000u)};
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) h[r] = to_bf16(a[4 * q + r]);
+              *(uintx2p*)turn.at(l32, 64 * j + 2 * column) = (uintx2p){h[0] | h[1] << 16, h[2] | h[3] << 16};
+            }
           }
-        }
-    }
+        const int m1 = tm * S::BM + 32 * (wm * S::TM + i), start = (first + 32 * j0) * size;   // bytes from the row's first class
+        turn.each(lane, [&](int row, int offset, uintx4p v) {
+          if (m1 + row < z.N && start + offset < 2 * pitch) *(uintx4p*)((char*)(out + (size_t)(m1 + row) * pitch) + start + offset) = v;
+        });
+      }
   }
 };
 
@@ -416,44 +421,53 @@ struct StoreEnd {
   const float *labels, *weights;      // may be null: rows are instances
   int nWeights;
   template <class S>
-  __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char*) const {
-    const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
-    const float u = magnitude ? pair_unscale(*magnitude) : 1.f;
+  __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
+    const float u = (magnitude ? pair_unscale(*magnitude) : 1.f);
     const bool wide = (Ncols & 3) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)sum & 15) == 0;
+    constexpr int J = turned_blocks<S, 4>();
+    const RowTurn<J * 128> turn(lds, wn * S::WM + wm);
+    const int half = lane >> 5, l32 = lane & 31;
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
-      const int m = m0 + 32 * i;
-      if (m >= M) continue;
-      const float w = labels ? instance_weight(labels, weights, nWeights, m) * factor : factor;
-      const size_t row = (size_t)m * Ncols;
+      const int m1 = tm * S::BM + 32 * (wm * S::TM + i);
+      const float w = labels && m1 + l32 < M ? instance_weight(labels, weights, nWeights, m1 + l32) * factor : factor;
 #pragma unroll
-      for (int j = 0; j < S::TN; ++j) {
-        const int n1 = n0 + 32 * j;
-        if (wide) {
-          float4 s[4];
+      for (int j0 = 0; j0 < S::TN; j0 += J) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            s[q] = sum && n1 + 8 * q < Ncols ? *(const float4*)(sum + row + n1 + 8 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < J; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            if (n1 + 8 * q >= Ncols) continue;
-            const float4 v = make_float4(s[q].x + acc[i][j][4 * q] * u * w, s[q].y + acc[i][j][4 * q + 1] * u * w,
-                                         s[q].z + acc[i][j][4 * q + 2] * u * w, s[q].w + acc[i][j][4 * q + 3] * u * w);
+            const floatx16p& a = acc[i][j0 + j];
+            *(float4*)turn.at(l32, 128 * j + 32 * q + 16 * half) =
+                make_float4(a[4 * q] * u * w, a[4 * q + 1] * u * w, a[4 * q + 2] * u * w, a[4 * q + 3] * u * w);
+          }
+        const int n1 = tn * S::BN + 32 * (wn * S::TN + j0);
+        if (wide) {
+          turn.each(lane, [&](int row, int offset, uintx4p bits) {
+            const int n = n1 + offset / 4;
+            if (m1 + row >= M || n >= Ncols) return;
+            const size_t at = (size_t)(m1 + row) * Ncols + n;
+            float4 v = __builtin_bit_cast(float4, bits);
+            if (sum) {
+              const float4 s = *(const float4*)(sum + at);
+              v = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+            }
             if (bf16Out)
-              *(uintx2p*)((unsigned short*)out + row + n1 + 8 * q) =
+              *(uintx2p*)((unsigned short*)out + at) =
                   (uintx2p){(unsigned)to_bf16(v.x) | (unsigned)to_bf16(v.y) << 16, (unsigned)to_bf16(v.z) | (unsigned)to_bf16(v.w) << 16};
             else
-              *(float4*)((float*)out + row + n1 + 8 * q) = v;
-          }
+              *(float4*)((float*)out + at) = v;
+          });
         } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int n = n1 + 8 * (r / 4) + r % 4;
-            if (n >= Ncols) continue;
-            const float v = (sum ? sum[row + n] : 0.f) + acc[i][j][r] * u * w;
-            if (bf16Out) ((unsigned short*)out)[row + n] = to_bf16(v);
-            else ((float*)out)[row + n] = v;
-          }
+          // (rows that start anywhere: a value a lane, J * 32 lanes along a row)
+          turn.single(lane, [&](int row, int column, float v) {
+            const int n = n1 + column;
+            if (m1 + row >= M || n >= Ncols) return;
+            const size_t at = (size_t)(m1 + row) * Ncols + n;
+            if (sum) v += sum[at];
+            if (bf16Out) ((unsigned short*)out)[at] = to_bf16(v);
+            else ((float*)out)[at] = v;
+          });
         }
       }
     }
@@ -527,6 +541,20 @@ __global__ __launch_bounds__(256) void fc_log_sums(float* __restrict__ y, float*
   }
 }
 
+// the value from the terms of many instances
+__global__ __launch_bounds__(1024) void fc_total(float* __restrict__ y, const float* __restrict__ terms, int n, int divide) {
+  __shared__ double lds[16];
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) acc += (double)terms[i];
+  acc = wave_sum(acc);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x) return;
+  double s = 0.0;
+  for (int w = 0; w < 16; ++w) s += lds[w];
+  y[0] = (float)(divide ? s / divide : s);
+}
+
 // dzdb: the tiles' column sums added up
 __global__ __launch_bounds__(256) void fc_join_columns(float* __restrict__ db, const float* __restrict__ sums, int K, int tileRows) {
   const int c = (int)blockIdx.x * 256 + threadIdx.x;
@@ -554,7 +582,12 @@ struct Plan {
   }
 };
 
-constexpr size_t kPieceBytes = 128u << 20;
+// A piece's P, or packed filters: larger ones save passes over the sums of dzdx (128, 256, 512 MiB: 29.5, 29.5, 29.2 ms for 128000 classes in
+// bfloat16, 1.76, 1.72, 1.72 ms for 32000 in single precision)
+size_t piece_bytes() {
+  const int kib = tunable("fcloss_piece_kib", 0);
+  return kib > 0 ? (size_t)kib << 10 : (size_t)256 << 20;
+}
 
 Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool backward) {
   Plan p;
@@ -564,10 +597,10 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   p.xInPlace = whole && aligned16(x);
   p.xPitch = row_halves(p.type, g->D);
   p.fPitch = p.fInPlace ? g->D : row_halves(p.type, g->D);
-  // a piece: P (backward) and the packed filters stay within kPieceBytes, whole tiles
+  // a piece: P (backward) and the packed filters stay within piece_bytes(), whole tiles
   const long long most = (g->K + 255ll) / 256 * 256;
   const long long perClass = std::max<long long>(backward ? g->N * 2ll * (p.type == kPairs ? 2 : 1) : 0, p.fInPlace ? 0 : p.fPitch * 2);
-  long long piece = perClass ? std::max(256ll, (long long)kPieceBytes / perClass / 256 * 256) : most;
+  long long piece = perClass ? std::max(256ll, (long long)piece_bytes() / perClass / 256 * 256) : most;
   if (piece < most) {              // equal pieces
     const long long n = (most + piece - 1) / piece;
     piece = ((most + n - 1) / n + 255) / 256 * 256;
@@ -713,12 +746,21 @@ int forward(const Call& c, float* y, float* logSums) {
     const int rc = product<TYPE, false, false>(c.s, c.who, "fc_scores", c.X(), c.F(k), N, c.classes(k), p.scores.of(N, c.classes(k)), c.scratch(), e);
     if (rc) return rc;
   }
-  KernelTimer timer("fc_log_sums", c.s);
-  // (few instances: four wavefronts each.  More than 256 workgroups wait for each other at the counter.)
-  const bool few = N <= 256;
-  hipLaunchKernelGGL(few ? fc_log_sums<4> : fc_log_sums<1>, dim3((unsigned)std::min(256, div_up(N, few ? 1 : 4))), dim3(256), 0, c.s, y, logSums,
-                     (float*)(c.ws + p.terms), (unsigned*)(c.ws + p.counters) + p.nCounters - 1, (const float2*)(c.ws + p.parts),
-                     (const float*)(c.ws + p.own), c.labels, c.weights, c.nWeights, N, p.tiles, c.g->normalise ? N : 0);
+  // Few instances: four wavefronts each.  Up to 1024 of them, the value is added up on the way (256 workgroups that count themselves in take
+  // less than a launch, 2048 of them, for 8192 instances, 30 us more than one).
+  const bool few = N <= 256, joined = N <= 1024;
+  const int divide = c.g->normalise ? N : 0;
+  float* const terms = (float*)(c.ws + p.terms);
+  {
+    KernelTimer timer("fc_log_sums", c.s);
+    hipLaunchKernelGGL(few ? fc_log_sums<4> : fc_log_sums<1>, dim3((unsigned)div_up(N, few ? 1 : 4)), dim3(256), 0, c.s, joined ? y : nullptr, logSums, terms,
+                       (unsigned*)(c.ws + p.counters) + p.nCounters - 1, (const float2*)(c.ws + p.parts), (const float*)(c.ws + p.own), c.labels, c.weights,
+                       c.nWeights, N, p.tiles, divide);
+  }
+  if (y && !joined) {
+    KernelTimer timer("fc_total", c.s);
+    hipLaunchKernelGGL(fc_total, dim3(1), dim3(1024), 0, c.s, y, terms, N, divide);
+  }
   return check_launch(c.who);
 }
 

@@ -374,6 +374,48 @@ __device__ __forceinline__ bool join_slices(const Slices& j, int tile, int slice
   return true;
 }
 
+// Rows out through LDS.  A lane holds four neighbouring columns of a row here and there: stored as they are they are 8 or 16 bytes in each of
+// 32 rows.  A wavefront turns 32 rows of `bytes` in a corner of LDS of its own (nobody waits for anybody) and takes them back 16 bytes
+// a lane along the rows.
+template <int BYTES>
+struct RowTurn {
+  static constexpr int pitch = BYTES + 16, size = 32 * pitch;   // (16 bytes more: sixteen lanes that write a column meet all banks)
+  char* base;
+  __device__ __forceinline__ RowTurn(char* lds, int wave) : base(lds + wave * size) {}
+  __device__ __forceinline__ char* at(int row, int offset) const { return base + row * pitch + offset; }
+  // take(row, offset, 16 bytes) for all of the 32 rows
+  template <class Take>
+  __device__ __forceinline__ void each(int lane, Take take) const {
+    order();
+#pragma unroll
+    for (int k = 0; k < BYTES / 32; ++k) {
+      const int chunk = lane + 64 * k, row = chunk / (BYTES / 16), offset = chunk % (BYTES / 16) * 16;
+      take(row, offset, *(const uintx4p*)at(row, offset));
+    }
+    order();
+  }
+  // take(row, column, value) for all of the single-precision values
+  template <class Take>
+  __device__ __forceinline__ void single(int lane, Take take) const {
+    order();
+#pragma unroll 4
+    for (int k = 0; k < BYTES / 8; ++k) {
+      const int i = lane + 64 * k, row = i / (BYTES / 4), column = i % (BYTES / 4);
+      take(row, column, *(const float*)at(row, 4 * column));
+    }
+    order();
+  }
+  // (what a wavefront's lanes have written its other lanes may read: LDS accesses of a wavefront are in order, the compiler's too)
+  __device__ static __forceinline__ void order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+};
+// blocks of 32 columns that are turned together: 256 bytes a row where there are as many
+template <class S, int SIZE>
+constexpr int turned_blocks() { return S::TN * 32 * SIZE <= 256 ? S::TN : 256 / (32 * SIZE); }
+
 // The matrices of a grid of products: one or more of one shape, `size` 16-bit values apart
 struct Matrix {
   const void* base;

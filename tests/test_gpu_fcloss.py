@@ -112,8 +112,15 @@ def test_options(capi, dtype, bias, skipped, weights, normalise):
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_many_pieces(capi, dtype):
-    """More classes than one piece takes (a piece's P is at most 128 MiB): 8192 images."""
-    check(capi, *make(40, 9000, 8192, dtype, 4))
+    """More classes than one piece takes (256 MiB of P): 8192 images; and pieces of 256 classes, the last one of 1, 7, 200 classes, aligned
+    and unaligned filters."""
+    check(capi, *make(40, 17000, 8192, dtype, 4))
+    try:
+        capi.set_tunable("fcloss_piece_kib", 16)
+        for size in [(64, 513, 33), (100, 775, 40), (128, 1224, 300), (64, 256, 65)]:
+            check(capi, *make(*size, dtype, 5))
+    finally:
+        capi.set_tunable("fcloss_piece_kib", 0)
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -15,7 +15,7 @@ SHAPES = [  # (H, W, C, N)
     (1, 1, 1, 5), (1, 1, 2, 1), (1, 1, 7, 100), (1, 1, 16, 33), (1, 1, 64, 130), (1, 1, 65, 9), (1, 1, 257, 70), (1, 1, 1000, 32), (1, 1, 1024, 17),
     (1, 1, 1023, 2100), (1, 1, 2048, 32), (1, 1, 2501, 9), (1, 1, 4096, 300), (1, 1, 5000, 11), (1, 1, 8192, 7), (1, 1, 9999, 3), (1, 1, 16384, 2),
     (1, 1, 16385, 3), (1, 1, 40000, 2),
-    (2, 1, 3, 4), (5, 7, 64, 3), (7, 7, 65, 2), (3, 1, 130, 40), (14, 14, 256, 2), (56, 56, 256, 1), (9, 9, 512, 2), (3, 5, 513, 2), (4, 4, 1500, 1), (1, 63, 8, 70),
+    (2, 1, 3, 4), (5, 7, 64, 3), (7, 7, 65, 2), (3, 1, 130, 40), (14, 14, 256, 2), (56, 56, 256, 1), (9, 9, 512, 2), (3, 5, 513, 2), (4, 4, 1500, 1), (1, 63, 8, 70), (5, 3, 300, 7), (3, 3, 1024, 2), (2, 9, 700, 33), (7, 1, 1025, 2),
 ]
 TYPES = [torch.float32, torch.bfloat16]
 
