@@ -4,6 +4,7 @@
 #include "accumulate.hpp"
 
 #include <cctype>
+#include <climits>
 #include <cstdio>
 #include <vector>
 
@@ -703,6 +704,154 @@ void nnsoftmax(Context& context, Allocator& allocator, int nout, Tensor* out, in
   (void)nout;
 }
 
+// ------------------------------------------------------------------------------------------ vl_nnlnorm
+// (x, g, b [, dzdy], 'epsilon', e, 'moments', m): the arguments of vl_nnbnorm, normalising the channels of each pixel
+
+void nnlnorm(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in) {
+  enum { optEpsilon, optMoments };
+  static OptionSpec const specs[] = {{"Epsilon", true, optEpsilon}, {"Moments", true, optMoments}, {NULL, false, 0}};
+  if (nin < 3) raise(VLE_IllegalArgument, "The arguments are less than three.");
+  const bool backMode = nin > 3 && in[3].kind != Arg::String;
+  int next = backMode ? 4 : 3;
+  double epsilon = 1e-4;
+  Arg const* momentsArg = NULL;
+  int opt;
+  Arg const* value = NULL;
+  while ((opt = nextOption(in, nin, specs, &next, &value)) >= 0) {
+    switch (opt) {
+      case optEpsilon:
+        if (!isPlainMatrix(*value) || value->tensor.getNumElements() != 1) raise(VLE_IllegalArgument, "EPSILON is not a plain scalar.");
+        epsilon = values(*value)[0];
+        break;
+      case optMoments: momentsArg = value; break;
+    }
+  }
+  Tensor data = dataTensor(in[0], "DATA", 4);
+  Tensor multipliers = dataTensor(in[1], "MULTIPLIERS", 1);
+  Tensor biases = dataTensor(in[2], "BIASES", 1);
+  Tensor derOutput, moments;
+  if (backMode) derOutput = dataTensor(in[3], "DEROUTPUT", 4);
+  if (momentsArg) moments = dataTensor(*momentsArg, "MOMENTS", 1);
+  if (!areCompatible(data, multipliers)) raise(VLE_IllegalArgument, "DATA and MULTIPLIERS do not have compatible formats.");
+  if (!areCompatible(data, biases)) raise(VLE_IllegalArgument, "DATA and BIASES do not have compatible formats.");
+  if (backMode && !areCompatible(data, derOutput)) raise(VLE_IllegalArgument, "DATA and DEROUTPUT do not have compatible formats.");
+  if (backMode && (data.getShape() != derOutput.getShape())) raise(VLE_IllegalArgument, "DATA and DEROUTPUT do not have the same size.");
+  if (momentsArg && !areCompatible(data, moments)) raise(VLE_IllegalArgument, "DATA and MOMENTS do not have compatible formats.");
+  if (multipliers.getNumElements() != data.getDepth()) raise(VLE_IllegalArgument, "The MULTIPLIERS size does not match the DATA depth.");
+  if (biases.getNumElements() != data.getDepth()) raise(VLE_IllegalArgument, "The BIASES size does not match the DATA depth.");
+  const std::size_t pixels = data.getHeight() * data.getWidth() * data.getSize();
+  if (momentsArg && moments.getNumElements() != 2 * pixels) raise(VLE_IllegalArgument, "The MOMENTS size does not match the DATA pixels.");
+  if (data.getDeviceType() != VLDT_GPU) raise(VLE_Unsupported, "vl_nnlnorm: DATA is on the CPU; this library implements the GPU (HIP, gfx950) device only");
+  if (data.getDataType() != VLDT_Float) raise(VLE_Unsupported, "vl_nnlnorm: only single precision is implemented on the HIP device");
+
+  if (data.getHeight() > (std::size_t)INT_MAX || data.getWidth() > (std::size_t)INT_MAX || data.getDepth() > (std::size_t)INT_MAX ||
+      data.getSize() > (std::size_t)INT_MAX)
+    raise(VLE_IllegalArgument, "vl_nnlnorm: an extent of DATA is larger than 2^31 - 1.");
+  if (!momentsArg && nout > (backMode ? 3 : 1)) {
+    std::size_t dims[4] = {data.getHeight(), data.getWidth(), data.getSize(), 2};
+    moments = newOutput(allocator, VLDT_GPU, VLDT_Float, TensorShape(dims, 4));
+  }
+  void* stream = context.getHipHelper().getStream();
+  const int H = (int)data.getHeight(), W = (int)data.getWidth(), C = (int)data.getDepth(), N = (int)data.getSize();
+  int rc;
+  if (!backMode) {
+    out[0] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[0].tensor.getShape());
+    rc = mcn_lnorm_forward(stream, MCN_FLOAT, out[0].getMemory(), (float*)moments.getMemory(), data.getMemory(), (float const*)multipliers.getMemory(),
+                           (float const*)biases.getMemory(), H, W, C, N, epsilon, momentsArg != NULL);
+    if (nout > 1) out[1] = moments;
+  } else {
+    const std::size_t bytes = mcn_lnorm_workspace_bytes(H, W, C, N);
+    void* ws = bytes ? context.getWorkspace(VLDT_GPU, bytes) : NULL;
+    if (bytes && !ws) failFromContext(context, context.getLastError());
+    out[0] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[0].tensor.getShape());
+    if (nout > 1) out[1] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[1].tensor.getShape());
+    if (nout > 2) out[2] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[2].tensor.getShape());
+    rc = mcn_lnorm_backward(stream, MCN_FLOAT, out[0].getMemory(), (float*)out[1].getMemory(), (float*)out[2].getMemory(), (float*)moments.getMemory(),
+                            data.getMemory(), (float const*)multipliers.getMemory(), derOutput.getMemory(), H, W, C, N, epsilon,
+                            momentsArg != NULL, ws, bytes);
+    if (nout > 3) out[3] = moments;
+  }
+  if (rc) raise(rc > 0 && rc <= (int)VLE_Interrupted ? (ErrorCode)rc : VLE_Unknown, mcn_last_error_message());
+}
+
+// ------------------------------------------------------------------------------------------ vl_nnfcloss
+// (x, f, b, c [, dzdy], 'instanceWeights', w, 'normalise', tf, 'logSums', s): vl_nnconv with filters of x's size, then
+// vl_nnloss 'softmaxlog', without the scores
+
+void nnfcloss(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in) {
+  enum { optInstanceWeights, optNormalise, optLogSums };
+  static OptionSpec const specs[] = {{"instanceWeights", true, optInstanceWeights}, {"normalise", true, optNormalise}, {"logSums", true, optLogSums}, {NULL, false, 0}};
+  if (nin < 4) raise(VLE_IllegalArgument, "There are less than four arguments.");
+  auto isEmpty = [](Arg const& a) { return a.kind == Arg::Array && a.tensor.getNumElements() == 0; };
+  auto scalar = [&](Arg const& a, char const* NAME) -> double {
+    if (!(isPlainMatrix(a) && a.tensor.getNumElements() == 1)) raise(VLE_IllegalArgument, std::string(NAME) + " is not a plain scalar.");
+    return values(a)[0];
+  };
+  int next = 4;
+  Arg const* dzdy = NULL;
+  if (nin > 4 && in[4].kind != Arg::String) {
+    if (!isEmpty(in[4])) dzdy = &in[4];
+    next = 5;
+  }
+  mcn_fcloss_geom g;
+  g.normalise = 1;
+  g.dataType = MCN_FLOAT;
+  Arg const *weights = NULL, *sums = NULL;
+  int opt;
+  Arg const* value = NULL;
+  while ((opt = nextOption(in, nin, specs, &next, &value)) >= 0) {
+    switch (opt) {
+      case optInstanceWeights: if (!isEmpty(*value)) weights = value; break;
+      case optNormalise: g.normalise = scalar(*value, "NORMALISE") != 0; break;
+      case optLogSums: if (!isEmpty(*value)) sums = value; break;
+    }
+  }
+  Tensor x = dataTensor(in[0], "X", 4);
+  Tensor f = dataTensor(in[1], "FILTERS", 4);
+  Tensor b, s;
+  if (!isEmpty(in[2])) b = dataTensor(in[2], "BIASES", 1);
+  if (sums) s = dataTensor(*sums, "LOGSUMS", 1);
+  if (!areCompatible(x, f)) raise(VLE_IllegalArgument, "X and FILTERS do not have compatible formats.");
+  if (b && !areCompatible(x, b)) raise(VLE_IllegalArgument, "X and BIASES do not have compatible formats.");
+  if (s && !areCompatible(x, s)) raise(VLE_IllegalArgument, "X and LOGSUMS do not have compatible formats.");
+  if (x.getHeight() != f.getHeight() || x.getWidth() != f.getWidth() || x.getDepth() != f.getDepth())
+    raise(VLE_IllegalArgument, "The FILTERS are not of the size of X.");
+  if (b && b.getNumElements() != f.getSize()) raise(VLE_IllegalArgument, "The number of elements of BIASES is not the same as the number of filters.");
+  if (s && s.getNumElements() != x.getSize()) raise(VLE_IllegalArgument, "The LOGSUMS size does not match the number of images.");
+  if (s && !dzdy) raise(VLE_IllegalArgument, "LOGSUMS are taken with DZDY only.");
+  const double derOutput = dzdy ? scalar(*dzdy, "DZDY") : 0;
+  if (x.getDeviceType() != VLDT_GPU) raise(VLE_Unsupported, "vl_nnfcloss: X is on the CPU; this library implements the GPU (HIP, gfx950) device only");
+  if (x.getDataType() != VLDT_Float) raise(VLE_Unsupported, "vl_nnfcloss: only single precision is implemented on the HIP device");
+  const std::size_t D = x.getHeight() * x.getWidth() * x.getDepth();
+  if (D > (std::size_t)INT_MAX || f.getSize() > (std::size_t)INT_MAX || x.getSize() > (std::size_t)INT_MAX)
+    raise(VLE_IllegalArgument, "vl_nnfcloss: more than 2^31 - 1 values per image, filters or images.");
+  g.D = (int)D; g.K = (int)f.getSize(); g.N = (int)x.getSize();
+  Tensor c = onDeviceAsSingle(context, allocator, in[3], "C");
+  Tensor w;
+  if (weights) w = onDeviceAsSingle(context, allocator, *weights, "INSTANCEWEIGHTS");
+  const std::size_t bytes = mcn_fcloss_workspace_bytes(&g, dzdy != NULL);
+  void* ws = bytes ? context.getWorkspace(VLDT_GPU, bytes) : NULL;
+  if (bytes && !ws) failFromContext(context, context.getLastError());
+  void* stream = context.getHipHelper().getStream();
+  int rc;
+  if (!dzdy) {
+    std::size_t one[2] = {1, 1}, images[2] = {1, x.getSize()};
+    out[0] = newOutput(allocator, VLDT_GPU, VLDT_Float, TensorShape(one, 2));
+    if (nout > 1) out[1] = newOutput(allocator, VLDT_GPU, VLDT_Float, TensorShape(images, 2));
+    rc = mcn_fcloss_forward(stream, &g, (float*)out[0].getMemory(), (float*)out[1].getMemory(), x.getMemory(), f.getMemory(),
+                            (float const*)b.getMemory(), (float const*)c.getMemory(), c.getNumElements(), (float const*)w.getMemory(),
+                            w.getNumElements(), ws, bytes);
+  } else {
+    out[0] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[0].tensor.getShape());
+    if (nout > 1) out[1] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[1].tensor.getShape());
+    if (nout > 2) out[2] = b ? newOutput(allocator, VLDT_GPU, VLDT_Float, in[2].tensor.getShape()) : emptyMatrix(VLDT_Float);
+    rc = mcn_fcloss_backward(stream, &g, out[0].getMemory(), out[1].getMemory(), (float*)out[2].getMemory(), (float const*)s.getMemory(),
+                             x.getMemory(), f.getMemory(), (float const*)b.getMemory(), (float const*)c.getMemory(), c.getNumElements(),
+                             (float const*)w.getMemory(), w.getNumElements(), derOutput, ws, bytes);
+  }
+  if (rc) raise(rc > 0 && rc <= (int)VLE_Interrupted ? (ErrorCode)rc : VLE_Unknown, mcn_last_error_message());
+}
+
 typedef void (*Body)(Context&, Allocator&, int, Tensor*, int, Arg const*);
 
 ErrorCode guarded(Body body, Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
@@ -743,6 +892,12 @@ ErrorCode vl_nnrelu(Context& context, Allocator& allocator, int nout, Tensor* ou
 }
 ErrorCode vl_nnloss(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in, std::string& message) {
   return guarded(nnloss, context, allocator, nout, out, nin, in, message);
+}
+ErrorCode vl_nnlnorm(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in, std::string& message) {
+  return guarded(nnlnorm, context, allocator, nout, out, nin, in, message);
+}
+ErrorCode vl_nnfcloss(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in, std::string& message) {
+  return guarded(nnfcloss, context, allocator, nout, out, nin, in, message);
 }
 
 } }  // namespace vl::frontend

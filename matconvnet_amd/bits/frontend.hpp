@@ -51,6 +51,8 @@ class Allocator {
 //   vl_nnloss : forward [y] (1 x 1 on the device)   backward [dzdx]
 //   vl_nnrelu : forward [y]             backward [dzdx]
 //   vl_nnsoftmax: forward [y]           backward [dzdx]
+//   vl_nnlnorm: forward [y, moments]    backward [dzdx, dzdg, dzdb, moments]
+//   vl_nnfcloss: forward [y, logSums]   backward [dzdx, dzdf, dzdb]
 ErrorCode vl_nnconv(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
                     std::string& message);
 ErrorCode vl_nnconvt(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
@@ -72,6 +74,15 @@ ErrorCode vl_nnsoftmax(Context& context, Allocator& allocator, int nout, Tensor*
 // weights: on the device (single) or host arrays (copied over).  dzdy: a host scalar, or empty for the forward mode.
 ErrorCode vl_nnloss(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
                     std::string& message);
+// vl_nnlnorm(x, g, b [, dzdy], 'epsilon', e, 'moments', m): layer normalisation, with vl_nnbnorm's arguments (no counterpart in the
+// reference).  Single precision, on the device; moments: H x W x N x 2, all means, then all deviations.
+ErrorCode vl_nnlnorm(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
+                     std::string& message);
+// vl_nnfcloss(x, f, b, c [, dzdy], 'instanceWeights', w, 'normalise', tf, 'logSums', s): vl_nnconv with filters of x's size followed by
+// vl_nnloss 'softmaxlog', without the scores (no counterpart in the reference).  x, f, b: single, on the device, b may be empty; c
+// and the weights as for vl_nnloss.  logSums: the forward call's second result, which saves the backward call a third of its work.
+ErrorCode vl_nnfcloss(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
+                      std::string& message);
 
 } }  // namespace vl::frontend
 #endif

@@ -699,29 +699,54 @@ def loss_backward(x, c, dzdy, g, instance_weights=None):
 def data_type(*tensors):
     """MCN_FLOAT or MCN_BFLOAT16: the data type of all the given tensors (None is passed over)."""
     torch = _torch()
-    kinds = {t.dtype for t in tensors if t is not None}
-    if len(kinds) != 1:
-        raise TypeError("tensors of different data types: %s" % sorted(str(k) for k in kinds))
-    kind = kinds.pop()
-    if kind not in (torch.float32, torch.bfloat16):
-        raise TypeError("neither single precision nor bfloat16: %s" % kind)
-    return BFLOAT16 if kind == torch.bfloat16 else FLOAT
+    kind = None
+    for t in tensors:
+        if t is not None and t.dtype != kind:
+            if kind is not None:
+                raise TypeError("tensors of different data types: %s, %s" % (kind, t.dtype))
+            kind = t.dtype
+    if kind == torch.float32:
+        return FLOAT
+    if kind == torch.bfloat16:
+        return BFLOAT16
+    raise TypeError("neither single precision nor bfloat16: %s" % kind)
 
 
 def _device(names, *tensors):
-    """Contiguous tensors on the device, or an error that names the one that is not."""
-    for name, t in zip(names.split(), tensors):
-        if t is not None and not (t.is_cuda and t.is_contiguous()):
-            raise ValueError("%s is not a contiguous tensor on the device" % name)
+    """Contiguous tensors on the current device (whose stream the calls take), or an error that names the one that is not."""
+    here = None
+    for i, t in enumerate(tensors):
+        if t is None:
+            continue
+        if not (t.is_cuda and t.is_contiguous()):
+            raise ValueError("%s is not a contiguous tensor on the device" % names.split()[i])
+        if here is None:
+            here = _torch().cuda.current_device()
+        if t.get_device() != here:
+            raise ValueError("%s is on device %d, not on the current one" % (names.split()[i], t.get_device()))
 
 
 def _single(names, *tensors):
     """... in single precision"""
     single = _torch().float32
-    for name, t in zip(names.split(), tensors):
+    for i, t in enumerate(tensors):
         if t is not None and t.dtype != single:
-            raise TypeError("%s is not single precision: %s" % (name, t.dtype))
+            raise TypeError("%s is not single precision: %s" % (names.split()[i], t.dtype))
     _device(names, *tensors)
+
+
+def _singles(x, *shape):
+    """A buffer of single-precision values on x's device"""
+    return x.new_empty(shape, dtype=_torch().float32)
+
+
+def _scratch(ws, x, nbytes):
+    """(address, bytes, what holds the memory) of the caller's Workspace, or of memory for this one call, of the current stream's pool (of
+    the graph's where one is captured): calls on two streams, or in two graphs, share none."""
+    if ws is not None:
+        return ws.get(nbytes) + (ws,)
+    buf = x.new_empty(nbytes, dtype=_torch().uint8) if nbytes else None
+    return ptr(buf), nbytes, buf
 
 
 def convert(x, dtype):
@@ -744,14 +769,13 @@ def lnorm_forward(x, g, b, eps=1e-5, moments=None):
     if given and moments.numel() != 2 * H * W * N:
         raise ValueError("moments does not have two values per pixel")
     y = _torch().empty_like(x)
-    mom = moments if given else empty((H, W, N, 2))
+    mom = moments if given else _singles(x, 2, N, W, H)
     check(lib().mcn_lnorm_forward(stream(), data_type(x), ptr(y), ptr(mom), ptr(x), ptr(g), ptr(b), H, W, Cc, N, eps, int(given)))
     return y, mom
 
 
 def lnorm_backward(x, g, dy, eps=1e-5, moments=None, want=(True, True, True), ws=None):
     """(dzdx, dzdg, dzdb) of layer normalisation; those not wanted are None.  moments: as lnorm_forward left them, or None."""
-    ws = ws or _ws
     H, W, Cc, N = _hwcn(x)
     _single("g moments", g, moments)
     _device("x dy", x, dy)
@@ -762,9 +786,9 @@ def lnorm_backward(x, g, dy, eps=1e-5, moments=None, want=(True, True, True), ws
     if moments is not None and moments.numel() != 2 * H * W * N:
         raise ValueError("moments does not have two values per pixel")
     dx = _torch().empty_like(x) if want[0] else None
-    dg = empty((Cc,)) if want[1] else None
-    db = empty((Cc,)) if want[2] else None
-    wp, wn = ws.get(lib().mcn_lnorm_workspace_bytes(H, W, Cc, N))
+    dg = _singles(x, Cc) if want[1] else None
+    db = _singles(x, Cc) if want[2] else None
+    wp, wn, held = _scratch(ws, x, lib().mcn_lnorm_workspace_bytes(H, W, Cc, N))
     check(lib().mcn_lnorm_backward(stream(), data_type(x, dy), ptr(dx), ptr(dg), ptr(db), ptr(moments), ptr(x), ptr(g), ptr(dy), H, W, Cc, N,
                                    eps, int(moments is not None), wp, wn))
     return dx, dg, db
@@ -791,11 +815,10 @@ def _fcloss_check(x, f, b, c, instance_weights, log_sums):
 def fcloss_forward(x, f, b, c, instance_weights=None, normalise=True, ws=None):
     """Softmax cross entropy of the scores x.f + b against the labels c (1..K as floats, 0: does not count), without a tensor of
     scores (include/mcn_hip.h: mcn_fcloss_forward): (y, log_sums).  x, f: float32 or bfloat16, b, c: float32."""
-    ws = ws or _ws
     _fcloss_check(x, f, b, c, instance_weights, None)
     g = fcloss_geom(x, f, normalise)
-    y, log_sums = empty((1,)), empty((g.N,))
-    wp, wn = ws.get(lib().mcn_fcloss_workspace_bytes(C.byref(g), 0))
+    y, log_sums = _singles(x, 1), _singles(x, g.N)
+    wp, wn, held = _scratch(ws, x, lib().mcn_fcloss_workspace_bytes(C.byref(g), 0))
     check(lib().mcn_fcloss_forward(stream(), C.byref(g), ptr(y), ptr(log_sums), ptr(x), ptr(f), ptr(b), ptr(c), c.numel(), ptr(instance_weights),
                                    0 if instance_weights is None else instance_weights.numel(), wp, wn))
     return y, log_sums
@@ -803,14 +826,13 @@ def fcloss_forward(x, f, b, c, instance_weights=None, normalise=True, ws=None):
 
 def fcloss_backward(x, f, b, c, dzdy=1.0, instance_weights=None, normalise=True, log_sums=None, want=(True, True, True), ws=None):
     """(dzdx, dzdf, dzdb) of fcloss_forward; those not wanted are None.  log_sums: as fcloss_forward left them, or None."""
-    ws = ws or _ws
     _fcloss_check(x, f, b, c, instance_weights, log_sums)
     g = fcloss_geom(x, f, normalise)
     torch = _torch()
     dx = torch.empty_like(x) if want[0] else None
     df = torch.empty_like(f) if want[1] else None
-    db = empty((g.K,)) if want[2] else None
-    wp, wn = ws.get(lib().mcn_fcloss_workspace_bytes(C.byref(g), 1))
+    db = _singles(x, g.K) if want[2] else None
+    wp, wn, held = _scratch(ws, x, lib().mcn_fcloss_workspace_bytes(C.byref(g), 1))
     check(lib().mcn_fcloss_backward(stream(), C.byref(g), ptr(dx), ptr(df), ptr(db), ptr(log_sums), ptr(x), ptr(f), ptr(b), ptr(c), c.numel(),
                                     ptr(instance_weights), 0 if instance_weights is None else instance_weights.numel(), float(dzdy), wp, wn))
     return dx, df, db
@@ -826,11 +848,10 @@ def _banks(x):
 
 def orthogonalise(x, steps=5, ws=None):
     """Filter banks (count, K, ...) in float32, each orthogonalised by Newton-Schulz products (include/mcn_hip.h: mcn_orthogonalise)."""
-    ws = ws or _ws
     _single("x", x)
     count, K, D = _banks(x)
     y = _torch().empty_like(x)
-    wp, wn = ws.get(lib().mcn_orthogonalise_workspace_bytes(K, D, count))
+    wp, wn, held = _scratch(ws, x, lib().mcn_orthogonalise_workspace_bytes(K, D, count))
     check(lib().mcn_orthogonalise(stream(), ptr(y), ptr(x), K, D, count, int(steps), wp, wn))
     return y
 

@@ -6,7 +6,7 @@
 // once in the backward pass.  The derivatives of g and b are sums over all pixels: every workgroup walks over many pixels with its
 // share of the sums in registers and leaves one partial sum per channel, which a second launch adds up in a fixed order.
 //
-// Two layouts.  "Rows": H = W = 1, a pixel's channels are neighbours; T lanes (16, 64, 256 or 1024) share a row.  "Planes": channels are a
+// Two layouts.  "Rows": H = W = 1, a pixel's channels are neighbours; T lanes (16 to 1024) share a row.  "Planes": channels are a
 // plane apart; lanes are pixels and the wavefronts of a workgroup share the channels.  Pixels with more channels than a workgroup
 // holds in registers are walked three times (lnorm_long_*).
 #include "mcn_internal.hpp"

@@ -143,7 +143,7 @@ struct OrthoEnd {
 // ---------------------------------------------------------------------------------------------- narrow matrices
 
 // Matrices whose shorter side is at most 64 and whose longer one at most 576 (what fits the local memory as pairs): a workgroup each
-// goes through all steps in one launch.  (3 banks of 64 filters of 576 values: 106 us through the launches above, NARROW here.)  X lies
+// goes through all steps in one launch.  (3 banks of 64 filters of 576 values: 106 us through the launches above, 54 here.)  X lies
 // in LDS as 64 rows; the reads of one product run along its rows, of the other across them: of every four 64-byte granules
 // (32 values' h or l) of a row the order is turned by r % 4, of their 16-byte chunks by r / 4 % 4, which spreads sixteen rows' equal
 // chunks, and four rows' equal granules, over all banks.  A, then B lie behind it, rows of 256 bytes, chunks turned by r % 16.

@@ -6,6 +6,8 @@
     y[, moments]             = vl_nnbnorm(x, g, b, 'epsilon', e[, 'moments', m])
     dzdx, dzdg, dzdb[, mom]  = vl_nnbnorm(x, g, b, dzdy, ...)
     y / dzdx                 = vl_nnpool(x, pool[, dzdy], 'stride', s, 'pad', p, 'method', 'max'|'avg')
+    y[, mom] / dzdx, ...     = vl_nnlnorm(x, g, b[, dzdy], 'epsilon', e, 'moments', m)
+    y[, sums] / dzdx, ...    = vl_nnfcloss(x, f, b, c[, dzdy], 'instanceWeights', w, 'normalise', tf, 'logSums', s)
 
 Arguments follow the MEX drivers (matlab/src/vl_nnconv.cu, vl_nnbnorm.cu, vl_nnpool.cu): data arguments are
 torch CUDA tensors standing for MATLAB arrays -- a MATLAB array of size H x W x C x N is a contiguous
@@ -224,6 +226,24 @@ def vl_nnloss(*args):
     """vl_nnloss(x, c [, dzdy], 'loss', name, 'instanceWeights', w, 'normalise', tf, 'threshold', t, 'topK', k)
     (matlab/vl_nnloss.m): the loss as a 1 x 1 device array, or dzdx when dzdy is given (a number)."""
     return _call("vl_nnloss", 1, list(args))[0]
+
+
+def vl_nnlnorm(*args, nout=None):
+    """vl_nnlnorm(x, g, b [, dzdy], 'epsilon', e, 'moments', m): layer normalisation with vl_nnbnorm's arguments; y[, moments], or
+    dzdx, dzdg, dzdb[, moments] with dzdy."""
+    back = len(args) > 3 and not isinstance(args[3], str)
+    n = nout if nout is not None else (3 if back else 1)
+    r = _call("vl_nnlnorm", n, list(args))
+    return r[0] if n == 1 else tuple(r[:n])
+
+
+def vl_nnfcloss(*args, nout=None):
+    """vl_nnfcloss(x, f, b, c [, dzdy], 'instanceWeights', w, 'normalise', tf, 'logSums', s): a fully connected layer and its loss
+    'softmaxlog' without the scores; y[, logSums], or dzdx, dzdf, dzdb with dzdy (a number)."""
+    back = len(args) > 4 and not isinstance(args[4], str) and 0 not in np.shape(args[4])
+    n = nout if nout is not None else (3 if back else 1)
+    r = _call("vl_nnfcloss", n, list(args))
+    return r[0] if n == 1 else tuple(r[:n])
 
 
 def vl_taccum(*args):

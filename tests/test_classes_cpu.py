@@ -3,6 +3,7 @@ conversion.  All of it is decided on the host, before anything is launched."""
 import ctypes as C
 
 import pytest
+import torch
 
 from matconvnet_amd import capi
 
@@ -134,3 +135,53 @@ def test_binding_refuses_what_the_library_cannot_see():
         capi.orthogonalise(x)
     with pytest.raises(TypeError):
         capi.orthogonalise(x.double())
+
+
+def z(*mshape):
+    """CPU float tensor standing for a MATLAB array of size mshape."""
+    return torch.zeros(tuple(reversed(mshape)), dtype=torch.float32)
+
+
+LNORM_ERRORS = [
+    ((z(2, 3, 8, 4), z(8)), "The arguments are less than three."),
+    ((z(2, 3, 8, 4), z(7), z(8)), "The MULTIPLIERS size does not match the DATA depth."),
+    ((z(2, 3, 8, 4), z(8), z(9)), "The BIASES size does not match the DATA depth."),
+    ((z(2, 3, 8, 4), z(8), z(8), z(2, 3, 8, 3)), "DATA and DEROUTPUT do not have the same size."),
+    ((z(2, 3, 8, 4), z(8), z(8), "moments", z(8, 2)), "The MOMENTS size does not match the DATA pixels."),
+    ((z(2, 3, 8, 4), z(8), z(8), "epsilon", [1.0, 2.0]), "EPSILON is not a plain scalar."),
+    ((z(2, 3, 8, 4), z(8), z(8), "nosuchoption"), "Unknown option 'nosuchoption'."),
+    ((z(2, 3, 8, 4), z(8).double(), z(8)), "DATA and MULTIPLIERS do not have compatible formats."),
+    ((z(2, 3, 8, 4), z(8), z(8), "moments", z(2, 3, 4, 2)), "vl_nnlnorm: DATA is on the CPU; this library implements the GPU (HIP, gfx950) device only"),
+]
+FCLOSS_ERRORS = [
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(10)), "There are less than four arguments."),
+    ((z(2, 3, 8, 4), z(3, 2, 8, 10), z(10), z(4)), "The FILTERS are not of the size of X."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(9), z(4)), "The number of elements of BIASES is not the same as the number of filters."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(10), z(4), "logSums", z(4)), "LOGSUMS are taken with DZDY only."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(10), z(4), 1.0, "logSums", z(5)), "The LOGSUMS size does not match the number of images."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(10), z(4), [1.0, 2.0]), "DZDY is not a plain scalar."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(10), z(4), "normalise", [1.0, 2.0]), "NORMALISE is not a plain scalar."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(10), z(4), "topK", 2.0), "Unknown option 'topK'."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10).double(), z(10), z(4)), "X and FILTERS do not have compatible formats."),
+    ((z(2, 3, 8, 4), z(2, 3, 8, 10), z(), z(4)), "vl_nnfcloss: X is on the CPU; this library implements the GPU (HIP, gfx950) device only"),
+]
+
+
+@pytest.mark.parametrize("function,args,message", [("vl_nnlnorm", *e) for e in LNORM_ERRORS] + [("vl_nnfcloss", *e) for e in FCLOSS_ERRORS])
+def test_front_end(function, args, message):
+    from matconvnet_amd import vlapi
+    with pytest.raises(vlapi.VlError) as e:
+        getattr(vlapi, function)(*args)
+    assert e.value.message == message
+
+
+def test_a_tensor_of_another_device(monkeypatch):
+    class Fake:
+        is_cuda, dtype = True, torch.float32
+        is_contiguous = staticmethod(lambda: True)
+        get_device = staticmethod(lambda: 1)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="x is on device 1"):
+        capi._single("b x", None, Fake())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    capi._single("b x", None, Fake())
