@@ -487,8 +487,8 @@ struct ProductPlan {
 // 64 / 128 / 256: 650 / 1040 / 1240 TFLOP/s with the chip full; pairs: 850 / 1140 / 1260.  P f of 2048 x 1024 over 16000 classes, pairs,
 // in us: 891, 288, 225 by tiles of 256 in 1, 4, 8 slices, 412, 196, 244 by tiles of 128, 234, 338, 497 by tiles of 64; chosen: 128 in 4.)
 struct StageCost { double alone, shared, ends; };
-constexpr StageCost kStageCost[2][3] = {{{1.5, 1.6, 8.0}, {0.62, 0.50, 3.0}, {0.29, 0.20, 1.0}},     // kBf16: 256, 128, 64
-                                        {{2.3, 2.5, 8.0}, {0.86, 0.70, 3.0}, {0.30, 0.24, 1.0}}};    // kPairs
+constexpr StageCost kStageCost[2][3] = {{{1.5, 1.6, 8.0}, {0.48, 0.50, 3.0}, {0.29, 0.20, 1.0}},     // kBf16: 256, 128, 64
+                                        {{2.3, 2.5, 8.0}, {0.65, 0.70, 3.0}, {0.30, 0.24, 1.0}}};    // kPairs
 constexpr double kJoin = 4.0;
 constexpr int kMostSlices = 32;
 inline ProductPlan plan_product(int type, long long M, long long N, long long depth, int count = 1, bool triangle = false) {
@@ -561,7 +561,12 @@ int product(hipStream_t s, const char* who, const char* name, const Matrix& A, c
             const Scratch& scratch, const E& e, int count = 1, bool triangle = false) {
   switch (p.tile) {
     case kTile256: return run_product<ProductShape<TYPE, 256, 256, 4, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-    case kTile128: return run_product<ProductShape<TYPE, 128, 128, 2, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+    case kTile128:
+      // (a workgroup that has its CU to itself takes eight wavefronts and four stages: 256 tiles by 64 stages of pairs 50 us instead of 62, 32
+      // tiles 35 instead of 52; where two share a CU, 512 tiles, it is 99 us against 96, of 16 stages 33 against 31)
+      if (p.tiles * p.slices <= device_compute_units())
+        return run_product<ProductShape<TYPE, 128, 128, 4, 2, 4>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+      return run_product<ProductShape<TYPE, 128, 128, 2, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
     default: return run_product<ProductShape<TYPE, 64, 64, 2, 2, 4>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
   }
 }
