@@ -5,7 +5,7 @@
 // [0.68, 1.21] after five steps, and none ever passes 1.22.  So X, A and B (its eigenvalues lie in [0.6, 3.4445]) stay below 3.5 in magnitude,
 // and the operands of the products are pairs of half-precision values (product.hpp) at a scale that is always the same, 2^14
 // (3.4445 * 2^14 < 65504).
-// A step is three products: A and A^2 are symmetric, of them only the tiles on and below the diagonal are made and written twice;
+// A step is three products, in three launches or two (ClosingEnd), for small matrices all steps in one (ortho_narrow): A and A^2 are symmetric, of them only the tiles on and below the diagonal are made and written twice;
 // 3 m^2 n + m^3 operations for an m x n matrix, m <= n.  All of a call's matrices (of one size) go through one launch per product.
 #include "product.hpp"
 
@@ -175,6 +175,69 @@ __device__ __forceinline__ floatx16p multiply_pairs(const uintx4p (&a)[2], const
   c = multiply<kPairs>(b[1], a[0], c);
   return multiply<kPairs>(b[0], a[0], c);
 }
+
+// ---------------------------------------------------------------------------------------------- A and B at once
+
+// Where one tile holds all of A = X X' (m <= 128) the workgroup that finishes it goes on to B = a I + b A + c A^2: A as pairs in LDS, rows of
+// 4 BM bytes with their 16-byte chunks turned by r % 16, read along its rows for both operands (it is symmetric).  One launch of three
+// less per step, which is what small matrices wait for: 64 x 2000 111 -> 86 us, 120 x 120 93 -> 86.  (Not where the tile of 128's long
+// reduction takes longer than three tiles of 64 and a launch: 128 x 4000 185 us by it, 142 without.)
+struct ClosingEnd {
+  unsigned short* out;      // B as pairs
+  long long pitch, size;
+  int m;
+  template <class S>
+  __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int, int, int which, int lane, int wm, int wn, char* lds) const {
+    static_assert(S::BM == S::BN && S::BM * S::BM * 4 <= S::ldsBytes, "A lies in LDS");
+    const int half = lane >> 5, l32 = lane & 31, m0 = 32 * wm * S::TM + l32, n0 = 32 * wn * S::TN + 4 * half;
+    const auto at = [&](int r, int c, int part) { return lds + r * (S::BM * 4) + (((((c >> 5) << 3) + (part << 2) + ((c & 31) >> 3)) ^ (r & 15)) << 4) + (c & 7) * 2; };
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = m0 + 32 * i, c = n0 + 32 * j + 8 * q;
+          float v[4];   // (what stands behind the last row or column of X may belong to other rows)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = r < m && c + e < m ? acc[i][j][4 * q + e] * kUnscale : 0.f;
+          put4(at(r, c, 0), at(r, c, 1), v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = 0.f;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S::BM / 16; ++s) {
+      uintx4p a[S::TM][2], b[S::TN][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i) a[i][q] = *(const uintx4p*)at(m0 + 32 * i, 16 * s + 8 * half, q);
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) b[j][q] = *(const uintx4p*)at(32 * (wn * S::TN + j) + l32, 16 * s + 8 * half, q);
+      }
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc[i][j] = multiply_pairs(a[i], b[j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = m0 + 32 * i, c = n0 + 32 * j + 8 * q;
+          if (r >= m || c / 32 * 64 >= pitch) continue;
+          float v[4];
+          get4(at(r, c, 0), at(r, c, 1), v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * (kC * kUnscale) + kB * v[e] + (r == c + e ? kA * kScale : 0.f);
+          unsigned short* o = out + which * size + r * pitch + (c / 32) * 64 + c % 32;
+          put4((char*)o, (char*)(o + 32), v);
+        }
+  }
+};
 
 // m rows (the shorter side), n columns.  FORM: how the matrix lies in memory, 0: rows of n values that can be read 16 bytes at a time,
 // 1: rows of n values, 2 (tall): columns of m values.
@@ -394,6 +457,7 @@ struct OrthoPlan {
   int normParts;
   long long pitch, mPitch;
   ProductPlan gram, square, update;   // A = X X', B = a I + b A + c A A, X <- B X
+  bool closes;                    // the first two in one launch
   size_t x[2], a, b, parts, sums, counters, total;
 };
 
@@ -401,6 +465,13 @@ OrthoPlan ortho_plan(int K, int D, int count) {
   OrthoPlan p;
   p.m = std::min(K, D);
   p.gram = plan_product(kPairs, p.m, p.m, std::max(K, D), count, true);
+  p.closes = false;
+  if (p.m <= 128 && !tunable("ortho_no_narrow", 0)) {
+    // (a tile of all of A against smaller ones and a launch more, which costs some 5 us)
+    const ProductPlan whole = plan_product(kPairs, p.m, p.m, std::max(K, D), count, true, p.m <= 64 ? 64 : 128);
+    p.closes = p.m <= kTileSize[whole.tile] && whole.tile != kTile256 && whole.cost < p.gram.cost + 5.0;
+    if (p.closes) p.gram = whole;
+  }
   p.square = plan_product(kPairs, p.m, p.m, p.m, count, true);
   p.update = plan_product(kPairs, K, D, p.m, count);
   p.normParts = (int)std::max<size_t>(1, std::min<size_t>(kNormParts, (size_t)K * D / 2048));
@@ -430,6 +501,14 @@ int ortho_check(const char* who, int K, int D, int count, int steps) {
   return MCN_SUCCESS;
 }
 
+template <bool ACROSS>
+int close_gram(hipStream_t s, const char* who, const Matrix& X, const OrthoPlan& p, const Scratch& scratch, const ClosingEnd& e, int count) {
+  if (p.gram.tile == kTile64)
+    return run_product<Tile64<kPairs>, ACROSS, ACROSS>(s, who, "ortho_gram", X, X, p.m, p.m, count, true, p.gram, scratch, e);
+  if (p.gram.alone()) return run_product<Tile128Alone<kPairs>, ACROSS, ACROSS>(s, who, "ortho_gram", X, X, p.m, p.m, count, true, p.gram, scratch, e);
+  return run_product<Tile128<kPairs>, ACROSS, ACROSS>(s, who, "ortho_gram", X, X, p.m, p.m, count, true, p.gram, scratch, e);
+}
+
 int orthogonalise(hipStream_t s, const char* who, const OrthoPlan& p, float* y, const float* x, int K, int D, int count, int steps, char* ws) {
   double* parts = (double*)(ws + p.parts);
   {
@@ -449,18 +528,23 @@ int orthogonalise(hipStream_t s, const char* who, const OrthoPlan& p, float* y, 
   const Matrix B = {ws + p.b, p.mPitch, p.m * p.mPitch, p.m};
   for (int step = 0; step < steps && !rc; ++step) {
     const Matrix X = {ws + p.x[step & 1], p.pitch, K * p.pitch, K};
-    OrthoEnd e = {(unsigned short*)(ws + p.a), nullptr, nullptr, p.mPitch, p.m * p.mPitch, p.m, p.m, 0.f, kUnscale, 0.f, 1};
-    rc = tall ? product<kPairs, true, true>(s, who, "ortho_gram", X, X, p.m, p.m, p.gram, scratch, e, count, true)
-              : product<kPairs, false, false>(s, who, "ortho_gram", X, X, p.m, p.m, p.gram, scratch, e, count, true);
+    if (p.closes) {
+      const ClosingEnd closing = {(unsigned short*)(ws + p.b), p.mPitch, p.m * p.mPitch, p.m};
+      rc = tall ? close_gram<true>(s, who, X, p, scratch, closing, count) : close_gram<false>(s, who, X, p, scratch, closing, count);
+    } else {
+      OrthoEnd e = {(unsigned short*)(ws + p.a), nullptr, nullptr, p.mPitch, p.m * p.mPitch, p.m, p.m, 0.f, kUnscale, 0.f, 1};
+      rc = tall ? product<kPairs, true, true>(s, who, "ortho_gram", X, X, p.m, p.m, p.gram, scratch, e, count, true)
+                : product<kPairs, false, false>(s, who, "ortho_gram", X, X, p.m, p.m, p.gram, scratch, e, count, true);
+      if (rc) break;
+      e.out = (unsigned short*)(ws + p.b);
+      e.c = (const unsigned short*)A.base;
+      e.add = kB;
+      e.times = kC * kUnscale;
+      e.identity = kA * kScale;
+      rc = product<kPairs, false, false>(s, who, "ortho_square", A, A, p.m, p.m, p.square, scratch, e, count, true);
+    }
     if (rc) break;
-    e.out = (unsigned short*)(ws + p.b);
-    e.c = (const unsigned short*)A.base;
-    e.add = kB;
-    e.times = kC * kUnscale;
-    e.identity = kA * kScale;
-    rc = product<kPairs, false, false>(s, who, "ortho_square", A, A, p.m, p.m, p.square, scratch, e, count, true);
-    if (rc) break;
-    e = {(unsigned short*)(ws + p.x[~step & 1]), step == steps - 1 ? y : nullptr, nullptr, p.pitch, K * p.pitch, K, D, 0.f, kUnscale, 0.f, 0};
+    const OrthoEnd e = {(unsigned short*)(ws + p.x[~step & 1]), step == steps - 1 ? y : nullptr, nullptr, p.pitch, K * p.pitch, K, D, 0.f, kUnscale, 0.f, 0};
     rc = tall ? product<kPairs, false, false>(s, who, "ortho_update", X, B, K, D, p.update, scratch, e, count)
               : product<kPairs, false, true>(s, who, "ortho_update", B, X, K, D, p.update, scratch, e, count);
   }

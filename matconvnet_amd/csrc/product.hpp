@@ -471,8 +471,10 @@ constexpr int kTileSize[3] = {256, 128, 64};
 struct ProductPlan {
   int tile, slices, perSlice, stages;
   long long tiles;
+  double cost;   // as the model below has it
   size_t partBytes() const { return slices > 1 ? (size_t)tiles * slices * kTileSize[tile] * kTileSize[tile] * 4 : 0; }
   size_t counters() const { return slices > 1 ? (size_t)tiles : 0; }
+  bool alone() const { return tiles * slices <= device_compute_units(); }   // a workgroup to a CU
   // the same cut for fewer rows or columns
   ProductPlan of(long long M, long long N) const {
     ProductPlan p = *this;
@@ -491,14 +493,14 @@ constexpr StageCost kStageCost[2][3] = {{{1.5, 1.6, 8.0}, {0.48, 0.50, 3.0}, {0.
                                         {{2.3, 2.5, 8.0}, {0.65, 0.70, 3.0}, {0.30, 0.24, 1.0}}};    // kPairs
 constexpr double kJoin = 4.0;
 constexpr int kMostSlices = 32;
-inline ProductPlan plan_product(int type, long long M, long long N, long long depth, int count = 1, bool triangle = false) {
+inline ProductPlan plan_product(int type, long long M, long long N, long long depth, int count = 1, bool triangle = false, int smallest = 0) {
   const int cus = std::max(1, device_compute_units());
   const int forced = tunable("product_tile", 0), cut = tunable("product_slices", 0);
   const int stages = (int)((depth + stage_depth(type) - 1) / stage_depth(type));
   ProductPlan best = {};
   double least = 1e300;
   for (int tile = 0; tile < 3; ++tile) {
-    if (forced && forced != kTileSize[tile]) continue;
+    if (forced ? forced != kTileSize[tile] : kTileSize[tile] < smallest) continue;
     const long long rows = (M + kTileSize[tile] - 1) / kTileSize[tile], columns = (N + kTileSize[tile] - 1) / kTileSize[tile];
     const long long tiles = count * (triangle ? rows * (rows + 1) / 2 : rows * columns);
     const StageCost& c = kStageCost[type][tile];
@@ -512,7 +514,7 @@ inline ProductPlan plan_product(int type, long long M, long long N, long long de
                           (slices > 1 ? kJoin + slices * part * (2.0 * tiles / 5.0e6 + 1.0 / 1.0e5) : 0.0);
       if (cost < least) {
         least = cost;
-        best = {tile, slices, perSlice, stages, tiles};
+        best = {tile, slices, perSlice, stages, tiles, cost};
       }
     }
   }
@@ -556,19 +558,20 @@ int run_product(hipStream_t s, const char* who, const char* name, const Matrix& 
   return check_launch(who);
 }
 
+template <int TYPE> using Tile256 = ProductShape<TYPE, 256, 256, 4, 2, 2>;
+template <int TYPE> using Tile128 = ProductShape<TYPE, 128, 128, 2, 2, 2>;
+// (a workgroup that has its CU to itself takes eight wavefronts and four stages: 256 tiles by 64 stages of pairs 50 us instead of 62, 32
+// tiles 35 instead of 52; where two share a CU, 512 tiles, it is 99 us against 96, of 16 stages 33 against 31)
+template <int TYPE> using Tile128Alone = ProductShape<TYPE, 128, 128, 4, 2, 4>;
+template <int TYPE> using Tile64 = ProductShape<TYPE, 64, 64, 2, 2, 4>;
+
 template <int TYPE, bool A_ACROSS, bool B_ACROSS, class E>
 int product(hipStream_t s, const char* who, const char* name, const Matrix& A, const Matrix& B, long long M, long long N, const ProductPlan& p,
             const Scratch& scratch, const E& e, int count = 1, bool triangle = false) {
-  switch (p.tile) {
-    case kTile256: return run_product<ProductShape<TYPE, 256, 256, 4, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-    case kTile128:
-      // (a workgroup that has its CU to itself takes eight wavefronts and four stages: 256 tiles by 64 stages of pairs 50 us instead of 62, 32
-      // tiles 35 instead of 52; where two share a CU, 512 tiles, it is 99 us against 96, of 16 stages 33 against 31)
-      if (p.tiles * p.slices <= device_compute_units())
-        return run_product<ProductShape<TYPE, 128, 128, 4, 2, 4>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-      return run_product<ProductShape<TYPE, 128, 128, 2, 2, 2>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-    default: return run_product<ProductShape<TYPE, 64, 64, 2, 2, 4>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-  }
+  if (p.tile == kTile256) return run_product<Tile256<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+  if (p.tile == kTile64) return run_product<Tile64<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+  if (p.alone()) return run_product<Tile128Alone<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+  return run_product<Tile128<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
 }
 
 }  // namespace mcn

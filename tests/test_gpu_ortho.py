@@ -62,6 +62,20 @@ def test_random_matrices(capi, count, K, D):
     check(capi, torch.randn((count, K, D), generator=r, device="cuda") * 1e-3)
 
 
+@pytest.mark.parametrize("count,K,D", [(1, 64, 2000), (1, 2001, 63), (3, 9, 900), (2, 33, 1023), (1, 120, 120), (2, 99, 130), (130, 90, 66), (300, 70, 71)])
+def test_one_tile_of_products(capi, count, K, D):
+    """Shapes whose X X' is one tile, also with its reduction cut into slices and with more matrices than the chip has units."""
+    r = torch.Generator(device="cuda")
+    r.manual_seed(K + D)
+    g = torch.randn((count, K, D), generator=r, device="cuda")
+    y = capi.orthogonalise(g)
+    assert bool(torch.isfinite(y).all())
+    for k in sorted({0, count // 2, count - 1}):
+        want, off = reference(g[k], 5)
+        assert float(torch.linalg.norm(y[k].double() - want)) <= off
+    assert torch.equal(capi.orthogonalise(g), y)
+
+
 @pytest.mark.parametrize("K,D", [(64, 200), (200, 64), (130, 130)])
 def test_few_strong_directions(capi, K, D):
     r = torch.Generator(device="cuda")
