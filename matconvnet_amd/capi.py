@@ -282,7 +282,9 @@ def ptr(t):
 
 
 def stream():
-    return C.c_void_p(_torch().cuda.current_stream().cuda_stream)
+    # (the handle alone: the stream object that torch.cuda.current_stream() makes takes 3 us, as long as a launch)
+    torch = _torch()
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 class Workspace:

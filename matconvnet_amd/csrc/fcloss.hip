@@ -178,10 +178,8 @@ __global__ __launch_bounds__(256) void fc_pack(PackJob j) {
   }
 }
 
-// (K D / 1024 workgroups: at most 2^34)
 __global__ __launch_bounds__(256) void fc_zero(void* __restrict__ p, size_t n, int is16) {
-  const size_t first = (size_t)blockIdx.x * 1024 + threadIdx.x;
-  for (size_t i = first; i < std::min(first + 1024, n); i += 256) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
     if (is16) ((unsigned short*)p)[i] = 0;
     else ((float*)p)[i] = 0.f;
   }
@@ -410,7 +408,7 @@ struct ProbabilitiesEnd {
   }
 };
 
-// out[m][n] = sum[m][n] + acc * factor * 1/scale of an operand * the instance's weight
+// out[m][n] = sum[m][n] + acc / the operands' scales * factor * the instance's weight
 struct StoreEnd {
   void* out;
   int bf16Out;
@@ -422,7 +420,9 @@ struct StoreEnd {
   int nWeights;
   template <class S>
   __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
-    const float u = (magnitude ? pair_unscale(*magnitude) : 1.f);
+    // (P as pairs is 2^14 too large; taken off together with the other operand's scale, before the factor, so that nothing leaves the range on
+    // the way.  Both are powers of two.)
+    const float u = magnitude ? pair_unscale(*magnitude) * (1.f / kProbability) : 1.f;
     const bool wide = (Ncols & 3) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)sum & 15) == 0;
     constexpr int J = turned_blocks<S, 4>();
     const RowTurn<J * 128> turn(lds, wn * S::WM + wm);
@@ -647,7 +647,8 @@ int check(const char* who, const mcn_fcloss_geom* g, size_t nLabels, const float
   if (!g) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null geometry", who);
   if (g->D < 0 || g->K < 0 || g->N < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative tensor extent", who);
   if (g->dataType != MCN_FLOAT && g->dataType != MCN_BFLOAT16) return fail(MCN_ILLEGAL_ARGUMENT, "%s: unknown data type %d", who, g->dataType);
-  if (g->D > (1 << 20) || g->K > (1 << 24)) return fail(MCN_UNSUPPORTED, "%s: more than 2^20 features or 2^24 classes", who);
+  if (g->D > (1 << 20) || g->K > (1 << 24) || g->N > (1 << 30))
+    return fail(MCN_UNSUPPORTED, "%s: more than 2^20 features, 2^24 classes or 2^30 images", who);
   if (g->N > 0 && (g->D == 0 || g->K == 0)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: instances without features or classes", who);
   if (nLabels != (size_t)g->N) return fail(MCN_ILLEGAL_ARGUMENT, "%s: C does not have one label per image", who);
   if (weights && g->N > 0 && (nWeights == 0 || (size_t)g->N % nWeights != 0))
@@ -769,7 +770,6 @@ int backward(const Call& c, void* derInput, void* derFilters, float* derBiases, 
   const Plan& p = c.p;
   const int N = c.g->N, D = c.g->D;
   const Matrix Xw = {c.ws + p.xw, p.xPitch, 0, N};
-  const float times = TYPE == kPairs ? factor / kProbability : factor;
   for (int k = 0; k < p.pieces; ++k) {
     const int first = k * p.piece, count = c.classes(k), columns = (count + 63) / 64 * 64;
     pack_piece(c, k, k == 0 && firstThere);
@@ -788,7 +788,7 @@ int backward(const Call& c, void* derInput, void* derFilters, float* derBiases, 
       // (the pieces add up in single precision: in derInput itself, or beside it)
       float* sum = TYPE == kPairs ? (float*)derInput : (float*)(c.ws + p.sum);
       const bool last = k == p.pieces - 1;
-      const StoreEnd d = {TYPE == kPairs || last ? derInput : sum, TYPE == kBf16 && last, k > 0 ? sum : nullptr, N, D, times,
+      const StoreEnd d = {TYPE == kPairs || last ? derInput : sum, TYPE == kBf16 && last, k > 0 ? sum : nullptr, N, D, factor,
                           TYPE == kPairs ? &c.magnitudes()->filters : nullptr, c.labels, c.weights, c.nWeights};
       ProductPlan q = p.dx;
       q.stages = div_up(count, stage_depth(TYPE));
@@ -796,7 +796,7 @@ int backward(const Call& c, void* derInput, void* derFilters, float* derBiases, 
       if (rc) return rc;
     }
     if (derFilters) {
-      const StoreEnd d = {(void*)c.piece_of(derFilters, first), TYPE == kBf16, nullptr, count, D, times,
+      const StoreEnd d = {(void*)c.piece_of(derFilters, first), TYPE == kBf16, nullptr, count, D, factor,
                           TYPE == kPairs ? &c.magnitudes()->features : nullptr, nullptr, nullptr, 1};
       rc = product<TYPE, true, true>(c.s, c.who, "fc_derivative_f", P, Xw, count, D, p.df.of(count, D), c.scratch(), d);
       if (rc) return rc;
@@ -817,7 +817,7 @@ using namespace mcn;
 extern "C" {
 
 size_t mcn_fcloss_workspace_bytes(const mcn_fcloss_geom* g, int backward) {
-  if (!g || g->D <= 0 || g->K <= 0 || g->N <= 0 || g->D > (1 << 20) || g->K > (1 << 24)) return 0;
+  if (!g || g->D <= 0 || g->K <= 0 || g->N <= 0 || g->D > (1 << 20) || g->K > (1 << 24) || g->N > (1 << 30)) return 0;
   if (g->dataType != MCN_FLOAT && g->dataType != MCN_BFLOAT16) return 0;
   // (the largest of the ways the tensors can be aligned)
   const void* odd = (const void*)2;
@@ -857,7 +857,7 @@ int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, void* der
   if (g->N == 0) {   // sums over no images
     const size_t n = (size_t)g->K * g->D;
     if (derFilters && n)
-      hipLaunchKernelGGL(fc_zero, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, as_stream(stream), derFilters, n, g->dataType == MCN_BFLOAT16);
+      hipLaunchKernelGGL(fc_zero, dim3((unsigned)std::min<size_t>(4096, (n + 1023) / 1024)), dim3(256), 0, as_stream(stream), derFilters, n, g->dataType == MCN_BFLOAT16);
     if (derBiases && g->K)
       hipLaunchKernelGGL(fc_zero, dim3((unsigned)((g->K + 1023) / 1024)), dim3(256), 0, as_stream(stream), derBiases, (size_t)g->K, 0);
     return check_launch(who);

@@ -589,8 +589,10 @@ int mcn_orthogonalise(mcn_stream_t stream, float* y, const float* x, int K, int 
   const int m = std::min(K, D), n = std::max(K, D);
   if (m <= kNarrowRows && n <= kNarrowColumns && !tunable("ortho_no_narrow", 0)) {
     const int lds = kNarrowRows * ((n + 63) / 64 * 256) + kSquareBytes;
-    const auto kernel = K > D ? ortho_narrow<2> : n % 4 == 0 && aligned16(x) && aligned16(y) ? ortho_narrow<0> : ortho_narrow<1>;
-    rc = allow_lds(who, (const void*)kernel, kNarrowRows * (kNarrowColumns * 4) + kSquareBytes);
+    static std::atomic<unsigned long long> raised[3];
+    const int form = K > D ? 2 : n % 4 == 0 && aligned16(x) && aligned16(y) ? 0 : 1;
+    const auto kernel = form == 2 ? ortho_narrow<2> : form == 1 ? ortho_narrow<1> : ortho_narrow<0>;
+    rc = allow_lds(who, (const void*)kernel, kNarrowRows * (kNarrowColumns * 4) + kSquareBytes, raised[form]);
     if (rc) return rc;
     KernelTimer timer("ortho_narrow", s);
     hipLaunchKernelGGL(kernel, dim3((unsigned)count), dim3(kNarrowThreads), lds, s, y, x, m, n, steps);

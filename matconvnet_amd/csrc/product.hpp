@@ -21,9 +21,7 @@
 #include "mcn_internal.hpp"
 
 #include <algorithm>
-#include <mutex>
-#include <set>
-#include <utility>
+#include <atomic>
 
 namespace mcn {
 
@@ -521,20 +519,18 @@ inline ProductPlan plan_product(int type, long long M, long long N, long long de
   return best;
 }
 
-// A kernel with more than 64 KiB of local memory has to be told so once per device.
-inline int allow_lds(const char* who, const void* kernel, int bytes) {
+// A kernel with more than 64 KiB of local memory has to be told so once per device (`raised`: the devices where that is done, a bit each).
+inline int allow_lds(const char* who, const void* kernel, int bytes, std::atomic<unsigned long long>& raised) {
   if (bytes <= 65536) return MCN_SUCCESS;
-  static std::mutex mutex;
-  static std::set<std::pair<const void*, int>> raised;
   const int dev = current_device();
   if (dev < 0) return fail(MCN_DEVICE_ERROR, "%s: no device", who);
-  std::lock_guard<std::mutex> lock(mutex);
-  if (raised.count({kernel, dev})) return MCN_SUCCESS;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (raised.load(std::memory_order_relaxed) & bit) return MCN_SUCCESS;
   if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
     (void)hipGetLastError();
     return fail(MCN_DEVICE_ERROR, "%s: local memory", who);
   }
-  raised.insert({kernel, dev});
+  raised.fetch_or(bit, std::memory_order_relaxed);
   return MCN_SUCCESS;
 }
 
@@ -547,10 +543,11 @@ struct Scratch {
 template <class S, bool A_ACROSS, bool B_ACROSS, class E>
 int run_product(hipStream_t s, const char* who, const char* name, const Matrix& A, const Matrix& B, long long M, long long N, int count, bool triangle,
                 const ProductPlan& p, const Scratch& scratch, const E& e) {
-  if (p.tiles * p.slices >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
+  if (p.tiles * p.slices >= (1ll << 32) / S::threads) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
   const TileGrid g = {div_up(M, S::BM), div_up(N, S::BN), count, triangle};
   const auto kernel = product_kernel<S, A_ACROSS, B_ACROSS, E>;
-  const int rc = allow_lds(who, (const void*)kernel, S::ldsBytes);
+  static std::atomic<unsigned long long> raised;
+  const int rc = allow_lds(who, (const void*)kernel, S::ldsBytes, raised);
   if (rc) return rc;
   KernelTimer timer(name, s);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tiles * p.slices)), dim3(S::threads), S::ldsBytes, s, A, B, g, p.stages,

@@ -73,6 +73,7 @@ def test_fcloss(backward):
     refused(fc(backward, D=0), ill, "without features or classes")
     refused(fc(backward, K=0), ill, "without features or classes")
     refused(fc(backward, D=(1 << 20) + 1), capi.UNSUPPORTED, "2^20")
+    refused(fc(backward, N=(1 << 30) + 1, labels=(1 << 30) + 1), capi.UNSUPPORTED, "2^30")
     refused(fc(backward, K=(1 << 24) + 1), capi.UNSUPPORTED, "2^24")
     for name in ("x", "f", "c"):
         refused(fc(backward, **{name: None}), ill, "null tensor")

@@ -179,6 +179,24 @@ def test_magnitudes_far_apart(capi):
     check(capi, torch.zeros_like(x), f, b, c, None)
 
 
+@pytest.mark.parametrize("power", [-120, -40, 60, 118])
+def test_powers_of_two(capi, power):
+    """Filters by 2^p and features by 2^-p: the same scores, so dzdx by 2^p and dzdf by 2^-p.  Bit for bit where the scaling of the inputs is
+    exact; at 2^-120 and 2^-118 it is not (an entry below 2^-6 or 2^-8 times that is a subnormal, rounded to a multiple of 2^-149), and what
+    is compared are the formulas of the rounded inputs."""
+    x, f, b, c, w = make(200, 150, 40, torch.float32, seed=9)
+    up, down = 2.0 ** power, 2.0 ** -power
+    check(capi, x * down, f * up, b, c, w)
+    if not (torch.equal(x * down * up, x) and torch.equal(f * up * down, f)):
+        return
+    y, sums = capi.fcloss_forward(x, f, b, c, instance_weights=w)
+    dx, df, db = capi.fcloss_backward(x, f, b, c, instance_weights=w, log_sums=sums)
+    y2, sums2 = capi.fcloss_forward(x * down, f * up, b, c, instance_weights=w)
+    dx2, df2, db2 = capi.fcloss_backward(x * down, f * up, b, c, instance_weights=w, log_sums=sums2)
+    assert torch.equal(y2, y) and torch.equal(sums2, sums) and torch.equal(db2, db)
+    assert torch.equal(dx2, dx * up) and torch.equal(df2, df * down)
+
+
 def test_labels_of_any_kind(capi):
     """Labels out of range go as in vl_nnloss: behind the last class to it, below 1 (but not 0) to the first."""
     x, f, b, c, _ = make(40, 30, 6, torch.float32, 9, skipped=False, weights=False)
