@@ -754,7 +754,7 @@ int forward(const Call& c, float* y, float* logSums) {
   float* const terms = (float*)(c.ws + p.terms);
   {
     KernelTimer timer("fc_log_sums", c.s);
-    hipLaunchKernelGGL(few ? fc_log_sums<4> : fc_log_sums<1>, dim3((unsigned)div_up(N, few ? 1 : 4)), dim3(256), 0, c.s, joined ? y : nullptr, logSums, terms,
+    hipLaunchKernelGGL(few ? fc_log_sums<4> : fc_log_sums<1>, dim3((unsigned)std::min(1 << 20, div_up(N, few ? 1 : 4))), dim3(256), 0, c.s, joined ? y : nullptr, logSums, terms,
                        (unsigned*)(c.ws + p.counters) + p.nCounters - 1, (const float2*)(c.ws + p.parts), (const float*)(c.ws + p.own), c.labels, c.weights,
                        c.nWeights, N, p.tiles, divide);
   }

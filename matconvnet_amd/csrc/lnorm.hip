@@ -36,6 +36,11 @@ struct LnP {
   int given;           // moments are an input
 };
 
+// One dimension of a grid holds less than 2^32 threads: more workgroups than kGridRow stand in rows of as many.
+constexpr size_t kGridRow = 1 << 20;
+__device__ __forceinline__ size_t block_of_grid() { return (size_t)blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 grid_of(size_t blocks) { return dim3((unsigned)std::min(blocks, kGridRow), (unsigned)((blocks + kGridRow - 1) / kGridRow)); }
+
 // A barrier for what lies in LDS: __syncthreads() also waits for every load and store that is on its way, the next row's and the last one's
 // output among them (8192 rows of 4096 bfloat16 values, backward: 57 us with it, 50 without).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -145,7 +150,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void lnorm_rows_forward(V* __res
                                                                         const float* __restrict__ g, const float* __restrict__ b, LnP p) {
   constexpr int kThreads = T > 256 ? T : 256;
   __shared__ float2 slots[32];
-  const size_t row = (size_t)blockIdx.x * (kThreads / T) + threadIdx.x / T;
+  const size_t row = block_of_grid() * (kThreads / T) + threadIdx.x / T;
   const bool live = row < p.items;   // (whole groups; they stay for the barriers)
   const int t = threadIdx.x % T;
   float v[NCH * VEC];
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(64 * kPlaneWaves) void lnorm_planes_forward(V* __re
                                                                          const float* __restrict__ g, const float* __restrict__ b, LnP p) {
   __shared__ float2 slots[2 * kPlaneWaves * PIX];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const size_t item = (size_t)blockIdx.x * PIX + lane % PIX;
+  const size_t item = block_of_grid() * PIX + lane % PIX;
   const bool live = item < p.items;
   const size_t base = pixel_base(live ? item : 0, p);
   float v[K];
@@ -622,7 +627,7 @@ void launch_rows(hipStream_t s, const LnArgs& a, bool backward) {
     hipLaunchKernelGGL((lnorm_rows_backward<V, VEC, T, NCH>), dim3((unsigned)a.groups), dim3(1024), 0, s, (V*)a.out, a.partials, a.moments,
                        (const V*)a.x, a.g, (const V*)a.dy, a.p);
   else
-    hipLaunchKernelGGL((lnorm_rows_forward<V, VEC, T, NCH>), dim3((unsigned)((a.p.items * T + (T > 256 ? T : 256) - 1) / (T > 256 ? T : 256))),
+    hipLaunchKernelGGL((lnorm_rows_forward<V, VEC, T, NCH>), grid_of((a.p.items * T + (T > 256 ? T : 256) - 1) / (T > 256 ? T : 256)),
                        dim3(T > 256 ? T : 256), 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, a.p);
 }
 
@@ -663,7 +668,7 @@ void launch_planes(hipStream_t s, const LnArgs& a, bool backward) {
     hipLaunchKernelGGL((lnorm_planes_backward<V, PIX, K>), dim3((unsigned)a.groups), block, 0, s, (V*)a.out, a.partials, a.moments, (const V*)a.x, a.g,
                        (const V*)a.dy, a.p);
   else
-    hipLaunchKernelGGL((lnorm_planes_forward<V, PIX, K>), dim3((unsigned)((a.p.items + PIX - 1) / PIX)), block, 0, s, (V*)a.out, a.moments, (const V*)a.x,
+    hipLaunchKernelGGL((lnorm_planes_forward<V, PIX, K>), grid_of((a.p.items + PIX - 1) / PIX), block, 0, s, (V*)a.out, a.moments, (const V*)a.x,
                        a.g, a.b, a.p);
 }
 

@@ -230,3 +230,16 @@ def test_convert(capi):
         h = capi.convert(x, torch.bfloat16)
         assert torch.equal(h, x.to(torch.bfloat16)) and torch.equal(capi.convert(h, torch.float32), h.float())
         assert torch.equal(capi.convert(h[1:], torch.float32), h[1:].float()) if n > 1 else True
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 2, (1 << 28) + 3), (2, 2, 2, (1 << 26) + 1)])
+def test_more_threads_than_a_dimension_of_a_grid_has(capi, shape):
+    """2^28 pixels of two channels, sixteen threads to a pixel."""
+    H, W, C, N = shape
+    x = torch.empty((N, C, W, H), dtype=torch.bfloat16, device="cuda").normal_()
+    g, b = torch.tensor([0.5, 2.0], device="cuda"), torch.tensor([1.0, -1.0], device="cuda")
+    y, mom = capi.lnorm_forward(x, g, b)
+    at = torch.cat([torch.arange(1000), torch.arange(N - 1000, N), torch.randint(0, N, (100000,))]).cuda()
+    want = Want(x[at], g, b, x[at], 1e-5)
+    near(y[at], want.back(want.y), want.back(want.y_off), "bf16")
+    near(mom[0, at].reshape(-1, 1), want.mu, want.mu_off, "mu")
