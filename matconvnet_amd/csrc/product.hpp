@@ -309,7 +309,7 @@ __device__ __forceinline__ void store8_pairs(unsigned short* row, int c, const f
   at[4] = l;
 }
 
-// A reduction cut into slices: every workgroup of a tile leaves its part in memory, the one that comes last adds them up in the order of the
+// A reduction cut into slices (of the tiles from `full` on): every workgroup of a tile leaves its part in memory, the one that comes last adds them up in the order of the
 // slices (its own among them: the same bits whichever is last) and goes on to finish the tile.  `counters`: one per tile, zero
 // before and after.  The XCDs' L2s are not coherent: the parts are written and read by relaxed atomic accesses at the scope of the
 // device, which go past them, and are counted once they have arrived.  (Plain accesses, and a count that releases and acquires, write
@@ -318,6 +318,7 @@ struct Slices {
   float* parts;
   unsigned* counters;
   int slices, perSlice;   // (slices == 1: neither pointer is used)
+  int full;               // tiles before the first that is cut
 };
 template <class S>
 __device__ __forceinline__ bool join_slices(const Slices& j, int tile, int slice, floatx16p (&acc)[S::TM][S::TN], char* lds) {
@@ -435,8 +436,9 @@ constexpr int kTileRows = 4;
 template <class S, bool A_ACROSS, bool B_ACROSS, class E>
 __global__ __launch_bounds__(S::threads, 2) void product_kernel(Matrix A, Matrix B, TileGrid g, int stages, Slices j, E e) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int id = xcd_contiguous_id((int)blockIdx.x, (int)gridDim.x);
-  const int tile = id / j.slices, slice = id - tile * j.slices;
+  const bool whole = (int)blockIdx.x < j.full;
+  const int id = whole ? xcd_contiguous_id((int)blockIdx.x, j.full) : xcd_contiguous_id((int)blockIdx.x - j.full, (int)gridDim.x - j.full);
+  const int cut = whole ? 0 : id / j.slices, slice = whole ? 0 : id - cut * j.slices, tile = whole ? id : j.full + cut;
   const int per = g.triangle ? g.tilesM * (g.tilesM + 1) / 2 : g.tilesM * g.tilesN;
   const int which = tile / per, t = tile - which * per;
   int tm, tn;
@@ -452,10 +454,10 @@ __global__ __launch_bounds__(S::threads, 2) void product_kernel(Matrix A, Matrix
     tm = first + within % rows;
     tn = within / rows;
   }
-  const int s0 = slice * j.perSlice;
+  const int s0 = slice * j.perSlice, mine = whole ? stages : max(0, min(j.perSlice, stages - s0));
   floatx16p acc[S::TM][S::TN];
-  product_tile<S, A_ACROSS, B_ACROSS>(A.of(which), B.of(which), (long long)tm * S::BM, (long long)tn * S::BN, s0, max(0, min(j.perSlice, stages - s0)), lds, acc);
-  if (!join_slices<S>(j, tile, slice, acc, lds)) return;
+  product_tile<S, A_ACROSS, B_ACROSS>(A.of(which), B.of(which), (long long)tm * S::BM, (long long)tn * S::BN, s0, mine, lds, acc);
+  if (!whole && !join_slices<S>(j, cut, slice, acc, lds)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   e.template finish<S>(acc, tm, tn, which, lane, wave % S::WM, wave / S::WM, lds);
 }
@@ -465,18 +467,22 @@ __global__ __launch_bounds__(S::threads, 2) void product_kernel(Matrix A, Matrix
 enum { kTile256, kTile128, kTile64 };
 constexpr int kTileSize[3] = {256, 128, 64};
 
-// How a product is cut: the tile, and how many workgroups share a tile's reduction.
+// How a product is cut: the tile, how many tiles are made whole (as many rounds of the chip as there are full ones), and how many workgroups
+// share the reduction of each of the others.
 struct ProductPlan {
   int tile, slices, perSlice, stages;
-  long long tiles;
+  long long tiles, full;
   double cost;   // as the model below has it
-  size_t partBytes() const { return slices > 1 ? (size_t)tiles * slices * kTileSize[tile] * kTileSize[tile] * 4 : 0; }
-  size_t counters() const { return slices > 1 ? (size_t)tiles : 0; }
-  bool alone() const { return tiles * slices <= device_compute_units(); }   // a workgroup to a CU
+  long long rest() const { return tiles - full; }
+  long long groups() const { return full + rest() * slices; }
+  size_t partBytes() const { return slices > 1 ? (size_t)rest() * slices * kTileSize[tile] * kTileSize[tile] * 4 : 0; }
+  size_t counters() const { return slices > 1 ? (size_t)rest() : 0; }
+  bool alone() const { return groups() <= device_compute_units(); }   // a workgroup to a CU
   // the same cut for fewer rows or columns
   ProductPlan of(long long M, long long N) const {
     ProductPlan p = *this;
     p.tiles = (M + kTileSize[tile] - 1) / kTileSize[tile] * ((N + kTileSize[tile] - 1) / kTileSize[tile]);
+    p.full = std::min(full, p.tiles);
     return p;
   }
 };
@@ -486,9 +492,12 @@ struct ProductPlan {
 // its end cost; a join costs kJoin, its parts' way to memory and back (all together at 5 TB/s, a tile's at 0.1).  (bfloat16, tiles of
 // 64 / 128 / 256: 650 / 1040 / 1240 TFLOP/s with the chip full; pairs: 850 / 1140 / 1260.  P f of 2048 x 1024 over 16000 classes, pairs,
 // in us: 891, 288, 225 by tiles of 256 in 1, 4, 8 slices, 412, 196, 244 by tiles of 128, 234, 338, 497 by tiles of 64; chosen: 128 in 4.)
+// What is left over behind whole rounds of the chip (one workgroup of 256 to a CU, two of the smaller ones) is cut finer: 528 tiles of
+// 128 by 128 stages of pairs 266 -> 210 us.
 struct StageCost { double alone, shared, ends; };
 constexpr StageCost kStageCost[2][3] = {{{1.5, 1.6, 8.0}, {0.48, 0.50, 3.0}, {0.29, 0.20, 1.0}},     // kBf16: 256, 128, 64
                                         {{2.3, 2.5, 8.0}, {0.65, 0.70, 3.0}, {0.30, 0.24, 1.0}}};    // kPairs
+constexpr int kResident[3] = {1, 2, 2};
 constexpr double kJoin = 4.0;
 constexpr int kMostSlices = 32;
 inline ProductPlan plan_product(int type, long long M, long long N, long long depth, int count = 1, bool triangle = false, int smallest = 0) {
@@ -503,16 +512,20 @@ inline ProductPlan plan_product(int type, long long M, long long N, long long de
     const long long tiles = count * (triangle ? rows * (rows + 1) / 2 : rows * columns);
     const StageCost& c = kStageCost[type][tile];
     const double part = 4.0 * kTileSize[tile] * kTileSize[tile];
+    const long long round = (long long)cus * kResident[tile];
+    const long long full = cut ? 0 : tiles / round * round, rest = tiles - full;
+    const double before = full / round * (stages * kResident[tile] * c.shared + c.ends);
     for (int slices = 1; slices <= kMostSlices && slices <= std::max(1, stages); ++slices) {
       if (cut && slices != div_up(std::max(1, stages), div_up(std::max(1, stages), cut))) continue;
       const int perSlice = std::max(1, div_up(stages, slices));
-      if (slices > 1 && ((slices - 1) * perSlice >= stages || (!cut && tiles * slices > 4ll * cus))) continue;   // (no empty slice; parts stay small)
-      const double waves = (double)((tiles * slices + cus - 1) / cus);
-      const double cost = perSlice * std::max(c.alone, waves * c.shared) + c.ends * std::max(1.0, waves / 2) +
-                          (slices > 1 ? kJoin + slices * part * (2.0 * tiles / 5.0e6 + 1.0 / 1.0e5) : 0.0);
+      if (slices > 1 && ((slices - 1) * perSlice >= stages || (!cut && rest * slices > 4ll * cus))) continue;   // (no empty slice; parts stay small)
+      const double waves = (double)((rest * slices + cus - 1) / cus);
+      const double cost = rest == 0 ? before
+                                    : before + perSlice * std::max(c.alone, waves * c.shared) + c.ends * std::max(1.0, waves / 2) +
+                                          (slices > 1 ? kJoin + slices * part * (2.0 * rest / 5.0e6 + 1.0 / 1.0e5) : 0.0);
       if (cost < least) {
         least = cost;
-        best = {tile, slices, perSlice, stages, tiles, cost};
+        best = {tile, slices, perSlice, stages, tiles, full, cost};
       }
     }
   }
@@ -543,15 +556,15 @@ struct Scratch {
 template <class S, bool A_ACROSS, bool B_ACROSS, class E>
 int run_product(hipStream_t s, const char* who, const char* name, const Matrix& A, const Matrix& B, long long M, long long N, int count, bool triangle,
                 const ProductPlan& p, const Scratch& scratch, const E& e) {
-  if (p.tiles * p.slices >= (1ll << 32) / S::threads) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
+  if (p.groups() >= (1ll << 32) / S::threads) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
   const TileGrid g = {div_up(M, S::BM), div_up(N, S::BN), count, triangle};
   const auto kernel = product_kernel<S, A_ACROSS, B_ACROSS, E>;
   static std::atomic<unsigned long long> raised;
   const int rc = allow_lds(who, (const void*)kernel, S::ldsBytes, raised);
   if (rc) return rc;
   KernelTimer timer(name, s);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(p.tiles * p.slices)), dim3(S::threads), S::ldsBytes, s, A, B, g, p.stages,
-                     Slices{scratch.parts, scratch.counters, p.slices, p.perSlice}, e);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)p.groups()), dim3(S::threads), S::ldsBytes, s, A, B, g, p.stages,
+                     Slices{scratch.parts, scratch.counters, p.slices, p.perSlice, (int)p.full}, e);
   return check_launch(who);
 }
 
