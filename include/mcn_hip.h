@@ -526,7 +526,8 @@ MCN_API int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput
    backward: derInput (shape of x), derFilters (shape of filters), derBiases (K), all fully overwritten, any may be NULL; logSums as the
    forward call left them, or NULL (made again, a third more work); derOutput the scalar derivative of y.
    Single precision: products on pairs of half-precision values, as exact as single-precision ones; P = softmax - 1 at the label is held
-   to 2^-39.  bfloat16: products of the bfloat16 values in single precision, P times the image's weight rounded to bfloat16.
+   to 2^-39.  bfloat16: products of the bfloat16 values in single precision; P is rounded to bfloat16, and so are, for derFilters, the
+   features times their image's weight.
    workspace: mcn_fcloss_workspace_bytes(g, 0 forward / 1 backward). */
 typedef struct mcn_fcloss_geom {
   int D, K, N;

@@ -64,7 +64,7 @@ __device__ __forceinline__ unsigned group_most(unsigned m, unsigned* lds) {   //
 // Workgroups [0, filterGroups): the filters; the rest: a wavefront per instance.
 __global__ __launch_bounds__(256) void fc_magnitudes(Magnitudes* __restrict__ out, unsigned* __restrict__ rows, const float* __restrict__ f, size_t n,
                                                      int filterGroups, int vec, const float* __restrict__ x, int D, int N,
-                                                     const float* __restrict__ labels, const float* __restrict__ weights, int nWeights, int wide) {
+                                                     const float* __restrict__ labels, const float* __restrict__ weights, int nWeights) {
   __shared__ unsigned lds[4];
   unsigned most = 0;
   if ((int)blockIdx.x < filterGroups) {
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void fc_magnitudes(Magnitudes* __restrict__ ou
     unsigned m = 0;
     for (int c = 8 * lane; c < D; c += 512) {
       float v[8];
-      load8(v, x + (size_t)row * D, c, D, wide);
+      load8(v, x + (size_t)row * D, c, D);
 #pragma unroll
       for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
     }
@@ -105,11 +105,13 @@ __global__ __launch_bounds__(256) void fc_magnitudes(Magnitudes* __restrict__ ou
 // Rows brought into the form the products read: pairs by a magnitude, or bfloat16 at a pitch of whole stages.
 enum { kFilters, kFeatures, kWeighted };   // by the tensor's magnitude; each row by its own; times the instance's weight (zeros for instances
                                            // that do not count, whatever they hold), by the tensor's
+// (In bfloat16 the weighted features are rounded, for dzdf alone.  Weights in P would round what both derivatives are made of by as much:
+// without them the label's -1, most of P, is exact.)
 struct PackPart {
   const void* x;
   unsigned short* out;
   long long pitch;
-  int rows, form, wide;                    // wide: rows can be read 16 bytes at a time
+  int rows, form;
   unsigned firstGroup;
 };
 struct PackJob {
@@ -161,13 +163,13 @@ __global__ __launch_bounds__(256) void fc_pack(PackJob j) {
         if (c == 0) j.unscale[row] = pair_unscale(j.rowMagnitudes[row]);
       }
       if (w != 0.f) {
-        load8(v, (const float*)p.x + (size_t)row * j.D, c, j.D, p.wide);
+        load8(v, (const float*)p.x + (size_t)row * j.D, c, j.D);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = v[k] * w * scale;
       }
       store8_pairs(p.out + (size_t)row * p.pitch, c, v);
     } else {
-      if (w != 0.f) load8(v, (const unsigned short*)p.x + (size_t)row * j.D, c, j.D, p.wide);
+      if (w != 0.f) load8(v, (const unsigned short*)p.x + (size_t)row * j.D, c, j.D);
       uintx4p h = {0, 0, 0, 0};
       if (w != 0.f) {
 #pragma unroll
@@ -575,8 +577,7 @@ struct Plan {
   ProductPlan scores, dx, df;      // of a whole piece; the last one, if smaller, is cut as they are
   size_t x, xUnscale, xw, f, magnitudes, rowMagnitudes, counters, parts, own, terms, logSums, p, sum, columns, products, total;
   int nCounters, tileRows;         // (counters: the last is fc_log_sums')
-  // whether rows of D values can be read 16 bytes at a time; workgroups that pack rows
-  int wide(const void* t, const mcn_fcloss_geom* g) const { return g->D % (type == kPairs ? 4 : 8) == 0 && aligned16(t); }
+  // workgroups that pack rows
   unsigned pack_groups(int rows, long long pitch) const {
     return (unsigned)(((size_t)rows * (pitch / (type == kPairs ? 16 : 8)) + 256 * kPackSteps - 1) / (256 * kPackSteps));
   }
@@ -677,7 +678,6 @@ void launch_pack(const Call& c, PackJob& j) {
   unsigned groups = 0;
   for (int k = 0; k < j.nParts; ++k) {
     j.parts[k].firstGroup = groups;
-    j.parts[k].wide = c.p.wide(j.parts[k].x, c.g);
     groups += c.p.pack_groups(j.parts[k].rows, j.parts[k].pitch);
   }
   if (groups == 0) {               // (the counters alone)
@@ -706,11 +706,11 @@ int prepare(const Call& c, bool weighted) {
     KernelTimer timer("fc_magnitudes", c.s);
     hipLaunchKernelGGL(fc_magnitudes, dim3((unsigned)(j.filterGroups + j.featureGroups)), dim3(256), 0, c.s, j.magnitudes, (unsigned*)(c.ws + p.rowMagnitudes),
                        (const float*)c.filters, n, j.filterGroups, (int)aligned16(c.filters), (const float*)c.x, c.g->D, c.g->N, c.labels, c.weights,
-                       c.nWeights, p.wide(c.x, c.g));
+                       c.nWeights);
   }
-  if (!p.fInPlace) j.parts[j.nParts++] = {c.filters, (unsigned short*)(c.ws + p.f), p.fPitch, c.classes(0), kFilters, 0, 0};
-  if (!p.xInPlace) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.x), p.xPitch, c.g->N, kFeatures, 0, 0};
-  if (weighted) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.xw), p.xPitch, c.g->N, kWeighted, 0, 0};
+  if (!p.fInPlace) j.parts[j.nParts++] = {c.filters, (unsigned short*)(c.ws + p.f), p.fPitch, c.classes(0), kFilters, 0};
+  if (!p.xInPlace) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.x), p.xPitch, c.g->N, kFeatures, 0};
+  if (weighted) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.xw), p.xPitch, c.g->N, kWeighted, 0};
   launch_pack(c, j);
   return check_launch(c.who);
 }
@@ -721,7 +721,7 @@ void pack_piece(const Call& c, int piece, bool there) {
   PackJob j = {};
   j.D = c.g->D;
   j.magnitudes = c.magnitudes();
-  j.parts[j.nParts++] = {c.piece_of(c.filters, piece * c.p.piece), (unsigned short*)(c.ws + c.p.f), c.p.fPitch, c.classes(piece), kFilters, 0, 0};
+  j.parts[j.nParts++] = {c.piece_of(c.filters, piece * c.p.piece), (unsigned short*)(c.ws + c.p.f), c.p.fPitch, c.classes(piece), kFilters, 0};
   launch_pack(c, j);
 }
 

@@ -54,7 +54,7 @@ __device__ __forceinline__ double norm_factor(double square, double scale) { ret
 
 // X = G/|G| as pairs, a thread per eight values; the zero matrix stays zero
 __global__ __launch_bounds__(256) void ortho_pack(unsigned short* __restrict__ out, const float* __restrict__ x, const double* __restrict__ parts,
-                                                  int used, int rows, int cols, long long pitch, int wide) {
+                                                  int used, int rows, int cols, long long pitch) {
   const int matrix = blockIdx.y, per = (int)(pitch / 16);
   const double factor = norm_factor(norm_square(parts, matrix, used), (double)kScale);
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void ortho_pack(unsigned short* __restrict__ o
   const int row = (int)(i / per), c = (int)(i - (size_t)row * per) * 8;
   const float* from = x + ((size_t)matrix * rows + row) * cols;
   float v[8];
-  load8(v, from, c, cols, wide);
+  load8(v, from, c, cols);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = (float)((double)v[k] * factor);
   store8_pairs(out + ((size_t)matrix * rows + row) * pitch, c, v);
@@ -519,7 +519,7 @@ int orthogonalise(hipStream_t s, const char* who, const OrthoPlan& p, float* y, 
   {
     KernelTimer timer("ortho_pack", s);
     hipLaunchKernelGGL(ortho_pack, dim3((unsigned)((K * (p.pitch / 16) + 255) / 256), (unsigned)count), dim3(256), 0, s, (unsigned short*)(ws + p.x[0]), x,
-                       parts, p.normParts, K, D, p.pitch, (int)(D % 4 == 0 && aligned16(x)));
+                       parts, p.normParts, K, D, p.pitch);
   }
   int rc = check_launch(who);
   const bool tall = K > D;
