@@ -523,6 +523,7 @@ MCN_API int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput
    logSums).  Biases of -infinity take classes out.
      y[0]      sum over the images of weight * (log sum exp scores - score of the label), over N if normalise
      logSums   (N values, may be NULL) log sum exp of the scores, for the backward call
+   Outputs overlap no input.
    backward: derInput (shape of x), derFilters (shape of filters), derBiases (K), all fully overwritten, any may be NULL; logSums as the
    forward call left them, or NULL (made again, a third more work); derOutput the scalar derivative of y.
    Single precision: products on pairs of half-precision values, as exact as single-precision ones; P = softmax - 1 at the label is held

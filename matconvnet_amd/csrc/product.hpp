@@ -277,7 +277,7 @@ __device__ __forceinline__ unsigned split_pair(float v) {
 __device__ __forceinline__ float half_bits(unsigned short b) { return (float)__builtin_bit_cast(_Float16, b); }
 
 // eight neighbours (from a multiple of eight on) of a row of D values; zeros behind its end.  Rows may start anywhere: 16-byte loads ask for
-// no alignment here (rows of odd lengths by single values: 21841 x 1001 bfloat16 values packed in 37 us, 20 now)
+// no alignment here (rows of odd lengths by single values: 21841 x 1001 bfloat16 values packed in 37 us, 22 so)
 typedef unsigned uintx4loose __attribute__((ext_vector_type(4), aligned(2)));
 typedef float floatx4loose __attribute__((ext_vector_type(4), aligned(4)));
 template <class V>
