@@ -151,6 +151,14 @@ Tensor newOutput(Allocator& allocator, DeviceType device, DataType type, TensorS
   return Tensor(shape, type, device, memory, bytes);
 }
 
+// Device memory of one call: of the allocator's, like its outputs, so that calls on two streams (or in two graphs) share none.
+void* callWorkspace(Allocator& allocator, std::size_t bytes) {
+  if (bytes == 0) return NULL;
+  void* memory = allocator.allocate(VLDT_GPU, bytes);
+  if (!memory) raise(VLE_OutOfGPUMemeory, "Could not allocate a workspace.");
+  return memory;
+}
+
 void failFromContext(Context& context, ErrorCode e) {
   if (e != VLE_Success) raise(e, context.getLastErrorMessage());
 }
@@ -761,8 +769,7 @@ void nnlnorm(Context& context, Allocator& allocator, int nout, Tensor* out, int 
     if (nout > 1) out[1] = moments;
   } else {
     const std::size_t bytes = mcn_lnorm_workspace_bytes(H, W, C, N);
-    void* ws = bytes ? context.getWorkspace(VLDT_GPU, bytes) : NULL;
-    if (bytes && !ws) failFromContext(context, context.getLastError());
+    void* ws = callWorkspace(allocator, bytes);
     out[0] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[0].tensor.getShape());
     if (nout > 1) out[1] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[1].tensor.getShape());
     if (nout > 2) out[2] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[2].tensor.getShape());
@@ -830,8 +837,7 @@ void nnfcloss(Context& context, Allocator& allocator, int nout, Tensor* out, int
   Tensor w;
   if (weights) w = onDeviceAsSingle(context, allocator, *weights, "INSTANCEWEIGHTS");
   const std::size_t bytes = mcn_fcloss_workspace_bytes(&g, dzdy != NULL);
-  void* ws = bytes ? context.getWorkspace(VLDT_GPU, bytes) : NULL;
-  if (bytes && !ws) failFromContext(context, context.getLastError());
+  void* ws = callWorkspace(allocator, bytes);
   void* stream = context.getHipHelper().getStream();
   int rc;
   if (!dzdy) {

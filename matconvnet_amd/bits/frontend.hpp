@@ -34,7 +34,8 @@ struct Arg {
   static Arg numeric(std::vector<double> const& values);
 };
 
-// Who provides memory for outputs (MATLAB's allocator in the MEX drivers).  Returning NULL = out of memory.
+// Who provides memory for outputs (MATLAB's allocator in the MEX drivers), and for what vl_nnlnorm and vl_nnfcloss keep on the device
+// during a call, which may go back when the call returns, to be used again behind it on its stream.  Returning NULL = out of memory.
 class Allocator {
  public:
   virtual ~Allocator() {}

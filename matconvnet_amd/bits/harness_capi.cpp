@@ -46,9 +46,10 @@ void fromTensor(Tensor const& t, vlh_arg* a) {
   a->text = NULL;
 }
 
-// one context per front-end function, like the static vl::MexContext of each MEX file
+// one context per front-end function, like the static vl::MexContext of each MEX file; vl_nnlnorm and vl_nnfcloss, which keep nothing in it,
+// have one per call
 Context& contextOf(int which) {
-  static Context contexts[10];
+  static Context contexts[8];
   return contexts[which];
 }
 
@@ -105,7 +106,8 @@ int vlh_call(const char* function, int nout, vlh_arg* out, int nin, const vlh_ar
     if (in[i].kind == 1) args.push_back(frontend::Arg::string(in[i].text ? in[i].text : ""));
     else args.push_back(frontend::Arg::array(toTensor(in[i])));
   }
-  Context& context = contextOf(which);
+  Context own;
+  Context& context = which < 8 ? contextOf(which) : own;
   context.getHipHelper().setStream(stream);
   CallbackAllocator allocator(alloc, user);
   Tensor results[4];

@@ -186,3 +186,35 @@ def test_a_tensor_of_another_device(monkeypatch):
         capi._single("b x", None, Fake())
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
     capi._single("b x", None, Fake())
+
+
+@pytest.mark.parametrize("function", ["vl_nnlnorm", "vl_nnfcloss", "vl_nnfcloss back"])
+def test_front_end_workspaces_are_of_one_call(function):
+    """Calls on two streams may share no memory: what a call keeps on the device comes from its allocator, as its outputs do.  (Addresses
+    that stand for device pointers; the allocator hands out the workspace and then has no more, so nothing is launched.)"""
+    from matconvnet_amd import vlapi
+    fc = "fcloss" in function
+
+    def array(*mshape):
+        a = vlapi.Arg(kind=0, data=4096, device=1, dtype=1, ndims=len(mshape))
+        for i, d in enumerate(mshape):
+            a.dims[i] = d
+        return a
+
+    one = C.c_double(1.0)
+    number = vlapi.Arg(kind=0, data=C.addressof(one), device=0, dtype=2, ndims=2)
+    number.dims[0] = number.dims[1] = 1
+    args = [array(2, 3, 8, 4), array(2, 3, 8, 10), array(10), array(4)] if fc else [array(2, 3, 8, 4), array(8), array(8), array(2, 3, 8, 4)]
+    if function.endswith("back"):
+        args.append(number)
+    g = capi.FcLossGeom(48, 10, 4, 1, 0)
+    need = capi.lib().mcn_fcloss_workspace_bytes(C.byref(g), int(len(args) == 5)) if fc else capi.lib().mcn_lnorm_workspace_bytes(2, 3, 8, 4)
+    asked = []
+
+    def alloc(user, device, nbytes):
+        asked.append((device, nbytes))
+        return 8192 if len(asked) == 1 else None
+
+    rc = vlapi.lib().vlh_call(function.split()[0].encode(), 3, (vlapi.Arg * 4)(), len(args), (vlapi.Arg * len(args))(*args), vlapi.ALLOC_FN(alloc), None, None)
+    assert rc != 0 and asked[0] == (1, need) and len(asked) == 2, asked
+    assert vlapi.lib().vlh_last_message().decode() == "Could not allocate an output array."

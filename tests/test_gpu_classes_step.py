@@ -218,3 +218,56 @@ def test_front_end_refuses(vl):
     assert e.value.message == "mcn_fcloss_forward: C does not have one label per image"
     with pytest.raises(vl.VlError):
         vl.vl_nnfcloss(d(1, 1, 8, 4).double(), d(1, 1, 8, 10).double(), d(10).double(), d(4))
+
+
+def front_step(vl, x, p, c, w, m):
+    """The same step through the front-end, up to the bank's derivative."""
+    y, moments = vl.vl_nnlnorm(x, p["g"], p["b"], "epsilon", EPS, nout=2)
+    loss, sums = vl.vl_nnfcloss(y, p["f"], p["fb"], c, "instanceWeights", w, nout=2)
+    dy, df, dfb = vl.vl_nnfcloss(y, p["f"], p["fb"], c, 1.0, "instanceWeights", w, "logSums", sums)
+    dx, dg, db = vl.vl_nnlnorm(x, p["g"], p["b"], dy, "epsilon", EPS, "moments", moments)
+    return dict(loss=loss, dx=dx, dg=dg, db=db, df=df, dfb=dfb)
+
+
+def test_front_end_on_two_streams_at_once(vl):
+    """As test_two_streams_at_once, through the front-end."""
+    jobs = [make(64, 128, 500, seed=1), make(40, 200, 300, seed=2)]
+    want = [front_step(vl, *j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(front_step(vl, *j))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for name in b:
+                assert torch.equal(a[name], b[name]), name
+
+
+def test_front_end_captured(vl):
+    """The front-end's calls in two graphs (each with memory of its own), replayed in turn with other inputs, against eager calls."""
+    jobs = [make(48, 96, 300, seed=1), make(20, 150, 70, seed=2)]
+    held = []
+    for j in jobs:
+        front_step(vl, *j)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = front_step(vl, *j)
+        held.append((graph, out))
+    for seed in (3, 4, 5):
+        for j, shape, (graph, out) in zip(jobs, ((48, 96, 300), (20, 150, 70)), held):
+            x, p, c, w, m = make(*shape, seed=seed)
+            for a, b in ((j[0], x), (j[2], c), (j[3], w)):
+                a.copy_(b)
+            for k in p:
+                j[1][k].copy_(p[k])
+        for graph, _ in held:
+            graph.replay()
+        torch.cuda.synchronize()
+        for j, (_, out) in zip(jobs, held):
+            want = front_step(vl, *j)
+            for name in want:
+                assert torch.equal(want[name], out[name]), (seed, name)
