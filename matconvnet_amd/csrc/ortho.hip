@@ -9,6 +9,8 @@
 // 3 m^2 n + m^3 operations for an m x n matrix, m <= n.  All of a call's matrices (of one size) go through one launch per product.
 #include "product.hpp"
 
+#include <climits>
+
 namespace mcn {
 namespace {
 
@@ -22,8 +24,11 @@ constexpr int kNormParts = 256;   // workgroups per matrix that sum squares, at 
 __global__ __launch_bounds__(256) void ortho_squares(double* __restrict__ parts, const float* __restrict__ x, size_t size, unsigned* __restrict__ counters,
                                                      int nCounters) {
   __shared__ double lds[4];
-  // (the products' counters are cleared on the way)
-  for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < nCounters; i += gridDim.x * gridDim.y * 256) counters[i] = 0;
+  // (the products' counters are cleared on the way, by the first matrix's workgroups: over all of them, up to 65535 matrices, the threads do
+  // not fit an int)
+  static_assert(kNormParts * 256ll <= INT_MAX / 2, "a thread's number among those of one matrix, and one stride behind it");
+  if (blockIdx.y == 0)
+    for (int i = (int)(blockIdx.x * 256 + threadIdx.x); i < nCounters; i += (int)(gridDim.x * 256)) counters[i] = 0;
   const float* v = x + (size_t)blockIdx.y * size;
   double s[4] = {};
   const size_t step = (size_t)gridDim.x * 256;
