@@ -64,8 +64,8 @@ Tunable g_tunables[] = {
     {"conv_no_uniform_tap", 0},        // 1: disable the uniform-tap variant of the pixel-major kernel (and the kernels with split operands)
     {"fcloss_piece_kib", 0},           // > 0: so many KiB for a piece of the classes instead of 256 MiB
     {"ortho_no_narrow", 0},            // 1: narrow matrices through the launches of the others too
-    {"product_tile", 0},               // 64, 128, 256: force the tile of the products of fcloss.hip and ortho.hip; 0 = choose
-    {"product_slices", 0},             // > 0: cut their reductions among so many workgroups (as far as there are stages)
+    {"product_tile", 0},               // 64, 128, 256: force the tile of the products of fcloss.hip and ortho.hip; anything else = choose
+    {"product_slices", 0},             // > 0: cut their reductions among so many workgroups (32 at most, and as far as there are stages)
     {"conv_wgrad_no_wide_rows", 0},    // 1: no 192-row filter-gradient tiles
 };
 }  // namespace

@@ -509,7 +509,9 @@ constexpr double kJoin = 4.0;
 constexpr int kMostSlices = 32;
 inline ProductPlan plan_product(int type, long long M, long long N, long long depth, int count = 1, bool triangle = false, int smallest = 0) {
   const int cus = std::max(1, device_compute_units());
-  const int forced = tunable("product_tile", 0), cut = tunable("product_slices", 0);
+  // (an unknown tile is none; a forced cut is held to what the loop below reaches)
+  const int asked = tunable("product_tile", 0), forced = asked == 64 || asked == 128 || asked == 256 ? asked : 0;
+  const int cut = std::max(0, std::min(tunable("product_slices", 0), kMostSlices));
   const int stages = (int)((depth + stage_depth(type) - 1) / stage_depth(type));
   ProductPlan best = {};
   double least = 1e300;

@@ -218,3 +218,19 @@ def test_front_end_workspaces_are_of_one_call(function):
     rc = vlapi.lib().vlh_call(function.split()[0].encode(), 3, (vlapi.Arg * 4)(), len(args), (vlapi.Arg * len(args))(*args), vlapi.ALLOC_FN(alloc), None, None)
     assert rc != 0 and asked[0] == (1, need) and len(asked) == 2, asked
     assert vlapi.lib().vlh_last_message().decode() == "Could not allocate an output array."
+
+
+@pytest.mark.parametrize("name,value,same", [("product_slices", 64, 32), ("product_slices", 1 << 30, 32), ("product_slices", -3, 0), ("product_tile", 100, 0), ("product_tile", -64, 0)])
+def test_every_product_has_a_plan(name, value, same):
+    """Cuts finer than are made, and tiles that there are not, are taken as the nearest that there is: the same plan, so the same workspace."""
+    L = capi.lib()
+    g = capi.FcLossGeom(8192, 1000, 300, 1, 1)   # (128 stages)
+
+    def sizes(v):
+        capi.set_tunable(name, v)
+        return [L.mcn_fcloss_workspace_bytes(C.byref(g), b) for b in (0, 1)] + [L.mcn_orthogonalise_workspace_bytes(500, 9000, 2)]
+
+    try:
+        assert sizes(value) == sizes(same)
+    finally:
+        capi.set_tunable(name, 0)

@@ -353,3 +353,15 @@ def test_every_cut_of_the_products(capi, dtype, tile, slices):
     finally:
         capi.set_tunable("product_tile", 0)
         capi.set_tunable("product_slices", 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name,value", [("product_slices", 64), ("product_tile", 100)])
+def test_cuts_and_tiles_that_there_are_not(capi, dtype, name, value):
+    """More slices than are made, of reductions with more stages than that, and an unknown tile."""
+    try:
+        capi.set_tunable(name, value)
+        check(capi, *make(2600, 300, 70, dtype, 16))
+        check(capi, *make(60, 70, 3000, dtype, 17))
+    finally:
+        capi.set_tunable(name, 0)
