@@ -496,6 +496,7 @@ MCN_API int mcn_softmax_backward(mcn_stream_t stream, float* derInput, const flo
  * connected layer and its loss as one operator, orthogonalised updates.  Where a call takes a data type, x, y and their
  * derivatives (and the filters and theirs) are of it; moments, multipliers, biases, labels and weights are single
  * precision.  Pointers of bfloat16 tensors are 2-byte aligned at least, of single-precision ones 4-byte.
+ * Workspaces are 16-byte aligned (mcn_lnorm_backward's 4-byte), or the call is refused.
  * A workspace serves one call at a time: calls that may run at once (on two streams, in two graphs) have one each.
  * ---------------------------------------------------------------------------------------------- */
 enum { MCN_FLOAT = 0, MCN_BFLOAT16 = 1 };

@@ -853,6 +853,7 @@ int mcn_fcloss_forward(mcn_stream_t stream, const mcn_fcloss_geom* g, float* y, 
   const Call c = {as_stream(stream), who, g, x, filters, biases, labels, instanceWeights, (int)nWeights, (char*)workspace, make_plan(g, x, filters, false)};
   if (!workspace || workspaceBytes < c.p.total)
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, c.p.total);
+  if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
   rc = prepare(c, false);
   if (rc) return rc;
   float* sums = logSums ? logSums : (float*)(c.ws + c.p.logSums);
@@ -878,6 +879,7 @@ int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, void* der
   const Call c = {as_stream(stream), who, g, x, filters, biases, labels, instanceWeights, (int)nWeights, (char*)workspace, make_plan(g, x, filters, true)};
   if (!workspace || workspaceBytes < c.p.total)
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, c.p.total);
+  if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
   rc = prepare(c, derFilters != nullptr);
   if (rc) return rc;
   const float factor = (float)(g->normalise ? derOutput / g->N : derOutput);

@@ -776,6 +776,7 @@ int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput, float*
   const size_t need = mcn_lnorm_workspace_bytes(H, W, C, N);
   if (!workspace || workspaceBytes < need)
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, need);
+  if ((uintptr_t)workspace & 3) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 4-byte aligned", who);
   a.out = derInput; a.moments = moments; a.x = x; a.g = multipliers; a.dy = derOutput;
   a.partials = sums ? (float*)workspace : nullptr;
   const bool regs = in_registers(C, a.p.HW);

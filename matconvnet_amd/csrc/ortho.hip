@@ -584,6 +584,7 @@ int mcn_orthogonalise(mcn_stream_t stream, float* y, const float* x, int K, int 
   const OrthoPlan p = ortho_plan(K, D, count);
   if (!workspace || workspaceBytes < p.total)
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, p.total);
+  if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
   hipStream_t s = as_stream(stream);
   if (steps == 0) {
     double* parts = (double*)((char*)workspace + p.parts);

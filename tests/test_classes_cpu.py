@@ -234,3 +234,13 @@ def test_every_product_has_a_plan(name, value, same):
         assert sizes(value) == sizes(same)
     finally:
         capi.set_tunable(name, 0)
+
+
+def test_workspaces_are_aligned():
+    off = lambda n: C.c_void_p(4096 + n)
+    for n in (1, 4, 8):
+        for backward in (0, 1):
+            refused(fc(backward, ws=off(n)), capi.ILLEGAL_ARGUMENT, "not 16-byte aligned")
+        refused(ortho(ws=off(n)), capi.ILLEGAL_ARGUMENT, "not 16-byte aligned")
+    for n in (1, 2):
+        refused(lnorm_backward(ws=off(n)), capi.ILLEGAL_ARGUMENT, "not 4-byte aligned")
