@@ -484,27 +484,50 @@ __device__ __forceinline__ void long_sum(float& a, float& b, float2* slots) {
   __syncthreads();
 }
 
+// Sums of two terms over a thread's channels c0, c0 + cs, ...: kLongStep of them at a time (their loads go out together), single precision
+// among these, in double one step behind the other, so that the sums are off by no more than those of few channels are (a thread of
+// "planes" has a quarter of all channels: added one by one in single precision, 20000 values of 0.1 had a mean off by 4e-5 of itself).
+constexpr int kLongStep = 16;
+template <class F>
+__device__ __forceinline__ void walk_channels(int c0, int cs, int C, float& a, float& b, F term) {
+  double sa = 0.0, sb = 0.0;
+  for (long long first = c0; first < C; first += (long long)kLongStep * cs) {
+    float pa = 0.f, pb = 0.f;
+#pragma unroll
+    for (int k = 0; k < kLongStep; ++k) {
+      const long long c = first + (long long)k * cs;
+      const float2 t = term(c < C ? (int)c : c0);
+      pa += c < C ? t.x : 0.f;
+      pb += c < C ? t.y : 0.f;
+    }
+    sa += (double)pa;
+    sb += (double)pb;
+  }
+  a = (float)sa;
+  b = (float)sb;
+}
+
 template <class V, bool ROWS, bool BACKWARD>
 __global__ __launch_bounds__(256) void lnorm_long(V* __restrict__ out, float* __restrict__ moments, const V* __restrict__ x,
                                                   const float* __restrict__ g, const float* __restrict__ b, const V* __restrict__ dy, LnP p) {
   __shared__ float2 slots[256];
-  const size_t item = ROWS ? (size_t)blockIdx.x : (size_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const size_t item = ROWS ? block_of_grid() : block_of_grid() * 64 + (threadIdx.x & 63);
   const bool live = item < p.items;
-  const size_t base = ROWS ? item * p.C : pixel_base(live ? item : 0, p), step = ROWS ? 1 : p.HW;
+  const size_t base = ROWS ? (live ? item : 0) * p.C : pixel_base(live ? item : 0, p), step = ROWS ? 1 : p.HW;
   const int c0 = ROWS ? threadIdx.x : threadIdx.x >> 6, cs = ROWS ? 256 : 4;
   float mu, sigma, none = 0.f;
   if (p.given) {
     mu = moments[live ? item : 0];
     sigma = moments[p.items + (live ? item : 0)];
   } else {
-    float s = 0.f, q = 0.f;
-    for (int c = c0; c < p.C; c += cs) s += to_float(x[base + c * step]);
+    float s, q;
+    walk_channels(c0, cs, p.C, s, none, [&](int c) { return make_float2(to_float(x[base + c * step]), 0.f); });
     long_sum<ROWS>(s, none, slots);
     mu = s / p.C;
-    for (int c = c0; c < p.C; c += cs) {
+    walk_channels(c0, cs, p.C, q, none, [&](int c) {
       const float d = to_float(x[base + c * step]) - mu;
-      q += d * d;
-    }
+      return make_float2(d * d, 0.f);
+    });
     long_sum<ROWS>(q, none, slots);
     sigma = sqrtf(q / p.C + p.epsilon);
     if (moments && live && c0 == 0) {
@@ -520,12 +543,11 @@ __global__ __launch_bounds__(256) void lnorm_long(V* __restrict__ out, float* __
     return;
   }
   if (!out) return;   // (only the moments were wanted)
-  float s1 = 0.f, s2 = 0.f;
-  for (int c = c0; c < p.C; c += cs) {
+  float s1, s2;
+  walk_channels(c0, cs, p.C, s1, s2, [&](int c) {
     const float a = to_float(dy[base + c * step]) * (g ? g[c] : 1.f);
-    s1 += a;
-    s2 += a * ((to_float(x[base + c * step]) - mu) * inv);
-  }
+    return make_float2(a, a * ((to_float(x[base + c * step]) - mu) * inv));
+  });
   long_sum<ROWS>(s1, s2, slots);
   s1 /= p.C;
   s2 /= p.C;
@@ -536,17 +558,16 @@ __global__ __launch_bounds__(256) void lnorm_long(V* __restrict__ out, float* __
     }
 }
 
-// Partial sums of dzdg and dzdb from stored moments.  Rows: a thread per channel, blockIdx.y a run of pixels.  Planes: a workgroup per
-// channel and run of pixels.
+// Partial sums of dzdg and dzdb from stored moments.  Rows: a thread per channel; planes: a workgroup per channel; blockIdx.z a run of pixels.
 template <class V, bool ROWS>
 __global__ __launch_bounds__(256) void lnorm_long_sums(float* __restrict__ partials, const float* __restrict__ moments, const V* __restrict__ x,
                                                        const V* __restrict__ dy, LnP p, size_t run) {
-  const size_t first = (size_t)blockIdx.y * run, last = std::min(first + run, p.items);
+  const size_t first = (size_t)blockIdx.z * run, last = std::min(first + run, p.items);
   float a = 0.f, b = 0.f;
-  int c;
+  size_t c;
   if (ROWS) {
-    c = (int)blockIdx.x * 256 + threadIdx.x;
-    if (c >= p.C) return;
+    c = block_of_grid() * 256 + threadIdx.x;
+    if (c >= (size_t)p.C) return;
     for (size_t i = first; i < last; ++i) {
       const float d = to_float(dy[i * p.C + c]);
       a += d * ((to_float(x[i * p.C + c]) - moments[i]) / moments[p.items + i]);
@@ -554,9 +575,10 @@ __global__ __launch_bounds__(256) void lnorm_long_sums(float* __restrict__ parti
     }
   } else {
     __shared__ float2 slots[16];
-    c = (int)blockIdx.x;
+    c = block_of_grid();
+    if (c >= (size_t)p.C) return;   // (whole workgroups)
     for (size_t i = first + threadIdx.x; i < last; i += 256) {
-      const size_t at = pixel_base(i, p) + (size_t)c * p.HW;
+      const size_t at = pixel_base(i, p) + c * p.HW;
       const float d = to_float(dy[at]);
       a += d * ((to_float(x[at]) - moments[i]) / moments[p.items + i]);
       b += d;
@@ -564,7 +586,7 @@ __global__ __launch_bounds__(256) void lnorm_long_sums(float* __restrict__ parti
     group_sum<256>(a, b, slots);
     if (threadIdx.x) return;
   }
-  float* out = partials + (size_t)blockIdx.y * 2 * p.C;
+  float* out = partials + (size_t)blockIdx.z * 2 * p.C;
   out[c] = a;
   out[p.C + c] = b;
 }
@@ -700,7 +722,7 @@ int launch(hipStream_t s, const char* who, LnArgs& a, bool backward, float* dg, 
       else hipLaunchKernelGGL((lnorm_long<V, false, true>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
       if (a.partials) {
         const size_t run = (a.p.items + a.groups - 1) / a.groups;
-        const dim3 sums((unsigned)(rows ? div_up(a.p.C, 256) : a.p.C), (unsigned)a.groups);
+        const dim3 sums((unsigned)(rows ? div_up(a.p.C, 256) : a.p.C), 1, (unsigned)a.groups);
         if (rows) hipLaunchKernelGGL((lnorm_long_sums<V, true>), sums, block, 0, s, a.partials, a.moments, (const V*)a.x, (const V*)a.dy, a.p, run);
         else hipLaunchKernelGGL((lnorm_long_sums<V, false>), sums, block, 0, s, a.partials, a.moments, (const V*)a.x, (const V*)a.dy, a.p, run);
       }

@@ -243,3 +243,26 @@ def test_more_threads_than_a_dimension_of_a_grid_has(capi, shape):
     want = Want(x[at], g, b, x[at], 1e-5)
     near(y[at], want.back(want.y), want.back(want.y_off), "bf16")
     near(mom[0, at].reshape(-1, 1), want.mu, want.mu_off, "mu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2, 1, 20000, 3), (7, 7, 2048, 2), (1, 3, 16385, 1), (1, 1, 20000, 3)])
+def test_sums_of_many_channels(capi, shape, dtype):
+    """More channels than registers hold: sums of equal values, whose roundings all go one way.  The bounds above, which count C/256 + 64 additions."""
+    H, W, C, N = shape
+    x, g, b, dy = make(shape, dtype, 7)
+    flat = torch.linspace(0.1, 0.9, N * W * H, device="cuda").view(N, 1, W, H)
+    x = (x * 0 + flat).to(dtype)
+    w = Want(x, g, b, dy, 1e-5)
+    tag = " bf16" if dtype == torch.bfloat16 else ""
+    y, mom = capi.lnorm_forward(x, g, b, 1e-5)
+    near(mom[0].reshape(-1, 1), w.mu, w.mu_off, "mu")
+    near(mom[1].reshape(-1, 1), w.sigma, w.sigma_off, "sigma")
+    near(y, w.back(w.y), w.back(w.y_off), "y" + tag)
+    dy = (dy * 0 + flat).to(dtype)
+    w = Want(x, g, b, dy, 1e-5)
+    for moments in (mom, None):
+        dx, dg, db = capi.lnorm_backward(x, g, dy, 1e-5, moments=moments)
+        near(dx, w.back(w.dx), w.back(w.dx_off), "dx" + tag)
+        near(dg, w.dg, w.dg_off, "dg")
+        near(db, w.db, w.db_off, "db")
