@@ -713,7 +713,7 @@ int launch(hipStream_t s, const char* who, LnArgs& a, bool backward, float* dg, 
     }
   } else {
     KernelTimer timer(backward ? "lnorm_backward" : "lnorm_forward", s);
-    const dim3 grid((unsigned)(rows ? a.p.items : (a.p.items + 63) / 64)), block(256);
+    const dim3 grid = grid_of(rows ? a.p.items : (a.p.items + 63) / 64), block(256);
     if (!backward) {
       if (rows) hipLaunchKernelGGL((lnorm_long<V, true, false>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
       else hipLaunchKernelGGL((lnorm_long<V, false, false>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
@@ -722,7 +722,8 @@ int launch(hipStream_t s, const char* who, LnArgs& a, bool backward, float* dg, 
       else hipLaunchKernelGGL((lnorm_long<V, false, true>), grid, block, 0, s, (V*)a.out, a.moments, (const V*)a.x, a.g, a.b, (const V*)a.dy, a.p);
       if (a.partials) {
         const size_t run = (a.p.items + a.groups - 1) / a.groups;
-        const dim3 sums((unsigned)(rows ? div_up(a.p.C, 256) : a.p.C), 1, (unsigned)a.groups);
+        dim3 sums = grid_of(rows ? div_up(a.p.C, 256) : a.p.C);
+        sums.z = (unsigned)a.groups;
         if (rows) hipLaunchKernelGGL((lnorm_long_sums<V, true>), sums, block, 0, s, a.partials, a.moments, (const V*)a.x, (const V*)a.dy, a.p, run);
         else hipLaunchKernelGGL((lnorm_long_sums<V, false>), sums, block, 0, s, a.partials, a.moments, (const V*)a.x, (const V*)a.dy, a.p, run);
       }

@@ -266,3 +266,18 @@ def test_sums_of_many_channels(capi, shape, dtype):
         near(dx, w.back(w.dx), w.back(w.dx_off), "dx" + tag)
         near(dg, w.dg, w.dg_off, "dg")
         near(db, w.db, w.db_off, "db")
+
+
+def test_as_many_channels_as_are_taken(capi):
+    """2^24 channels of two pixels: more workgroups for the sums over pixels than one dimension of a grid has threads for."""
+    shape = (2, 1, 1 << 24, 1)
+    x, g, b, dy = make(shape, torch.float32, 8)
+    y, mom = capi.lnorm_forward(x, g, b, 1e-5)
+    dx, dg, db = capi.lnorm_backward(x, g, dy, 1e-5, moments=mom)
+    w = Want(x, g, b, dy, 1e-5)
+    near(mom[0].reshape(-1, 1), w.mu, w.mu_off, "mu")
+    near(mom[1].reshape(-1, 1), w.sigma, w.sigma_off, "sigma")
+    near(y, w.back(w.y), w.back(w.y_off), "y")
+    near(dx, w.back(w.dx), w.back(w.dx_off), "dx")
+    near(dg, w.dg, w.dg_off, "dg")
+    near(db, w.db, w.db_off, "db")
