@@ -271,3 +271,40 @@ def test_front_end_captured(vl):
             want = front_step(vl, *j)
             for name in want:
                 assert torch.equal(want[name], out[name]), (seed, name)
+
+
+@pytest.mark.parametrize("N,C,K", [(32, 64, 100), (33, 257, 70), (7, 130, 1001)])
+def test_every_link_of_the_step(capi, N, C, K):
+    """Each call of a step against its formulas in double precision on what the call before it gave, with the bounds that its own tests
+    derive: nothing grows from link to link, so a result of 16 bits, or four Newton-Schulz steps instead of five, does not pass."""
+    import test_gpu_fcloss
+    import test_gpu_lnorm
+    import test_gpu_ortho
+    x, p, c, w, m = make(N, C, K)
+    y, moments = capi.lnorm_forward(x, p["g"], p["b"], EPS)
+    loss, sums = capi.fcloss_forward(y, p["f"], p["fb"], c, instance_weights=w)
+    dy, df, dfb = capi.fcloss_backward(y, p["f"], p["fb"], c, 1.0, instance_weights=w, log_sums=sums)
+    dx, dg, db = capi.lnorm_backward(x, p["g"], dy, EPS, moments=moments)
+    momentum = capi.taccum(MOMENTUM, m, 1.0, df.reshape(m.shape))
+    turned = capi.orthogonalise(momentum)
+    f = capi.taccum(1.0, p["f"], -RATE, turned.reshape(p["f"].shape))
+    for name, got in step(capi, x, p, c, w, m).items():   # (the step is these calls)
+        assert torch.equal(got, dict(loss=loss, dx=dx, dg=dg, db=db, df=df, dfb=dfb, f=f)[name]), name
+    norm = test_gpu_lnorm.Want(x, p["g"], p["b"], dy, EPS)
+    test_gpu_lnorm.near(y, norm.back(norm.y), norm.back(norm.y_off), "y")
+    for name, got in (("dx", dx), ("dg", dg), ("db", db)):
+        want, off = getattr(norm, name), getattr(norm, name + "_off")
+        test_gpu_lnorm.near(got, norm.back(want) if name == "dx" else want, norm.back(off) if name == "dx" else off, name)
+    head = test_gpu_fcloss.Want(y, p["f"], p["fb"], c, w)
+    for name, got in (("y", loss), ("dx", dy), ("df", df), ("db", dfb)):
+        test_gpu_fcloss.near(got, getattr(head, name).reshape(-1, 1) if name == "y" else getattr(head, name), getattr(head, name + "_off"), name)
+    # (the coefficients are held in single precision; a product, a sum: one rounding each)
+    want = MOMENTUM * m.double() + df.double().reshape(m.shape)
+    assert bool(((momentum.double() - want).abs() <= 2 * U * (MOMENTUM * m.double()).abs() + U * want.abs()).all())
+    want, off = test_gpu_ortho.reference(momentum[0], 5)
+    assert float(torch.linalg.norm(turned[0].double() - want)) <= off
+    want = p["f"].double() - RATE * turned.double().reshape(p["f"].shape)
+    assert bool(((f.double() - want).abs() <= 2 * U * (RATE * turned.double().reshape(p["f"].shape)).abs() + U * want.abs()).all())
+    # what would not pass: four steps
+    four, _ = test_gpu_ortho.reference(momentum[0], 4)
+    assert float(torch.linalg.norm(turned[0].double() - four)) > 10 * off
