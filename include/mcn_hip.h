@@ -527,9 +527,14 @@ MCN_API int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput
    Outputs overlap no input.
    backward: derInput (shape of x), derFilters (shape of filters), derBiases (K), all fully overwritten, any may be NULL; logSums as the
    forward call left them, or NULL (made again, a third more work); derOutput the scalar derivative of y.
-   Single precision: products on pairs of half-precision values, as exact as single-precision ones; P = softmax - 1 at the label is held
-   to 2^-39.  bfloat16: products of the bfloat16 values in single precision; P is rounded to bfloat16, and so are, for derFilters, the
-   features times their image's weight.
+   Single precision: products on pairs of half-precision values: a product of two values is off by 7e-8 of itself in the mean square, 2^-21
+   at most, and sums are in single precision.  An image's features share a scale, and so do a class's filter, a class's P (derFilters), an
+   image's P (derInput) and, for derFilters, a feature over the images: classes that are hardly ever likely, small features, small filters
+   and small images lose nothing.  Within an image's features, or a filter, what is below 2^-16 of the largest is held to 2^-39 of that:
+   scores lose where so small features meet filter values as much larger than their filter's others, derInput where a feature's value is
+   so small in all filters.
+   bfloat16: products of the bfloat16 values in single precision; P is rounded to bfloat16, and so are, for derFilters, the features times
+   their image's weight.
    workspace: mcn_fcloss_workspace_bytes(g, 0 forward / 1 backward). */
 typedef struct mcn_fcloss_geom {
   int D, K, N;

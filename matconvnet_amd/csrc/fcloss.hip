@@ -5,22 +5,24 @@
 //   dzdx = sum_k w P f, dzdf = sum_n w P x, dzdb = sum_n w P   (times the scalar derivative of y [/ N])
 //
 // Forward: every tile of scores leaves, per instance, its largest score and the sum of exponentials against it; a pass over those
-// (N x K / 256 pairs) gives the logarithms of the sums.  Backward: a piece of the classes at a time, the scores are made
-// again, P is written as 16-bit operands, and two products over it give the piece's dzdf and its share of dzdx.  The largest
-// buffer is the piece's P.  8 N D K operations in all, a quarter of them the scores made again: keeping N x K scores is
-// what this operator is there to avoid.
+// (8 bytes for 64 to 256 scores) gives the logarithms of the sums.  Backward: a piece of the classes at a time, the scores are made
+// again, P is written as operands, and two products over it give the piece's dzdf and its share of dzdx.  The largest buffers are the
+// piece's P and, where instances times classes are very many, the tiles' leavings over all classes.  8 N D K operations in all, a
+// quarter of them the scores made again: keeping N x K scores is what this operator is there to avoid.
+//
+// Single precision (pairs, product.hpp).  What shares a power of two as its scale decides what is lost, so each product has its own:
+//   scores  an instance's features, a class's filter: e_n and e_k, the exponents of their largest magnitudes;
+//   dzdf    (sum over n) a class's w P 2^e_n, a feature's x 2^-e_n over the instances: C_k and S_d, the exponents of the largest;
+//   dzdx    (sum over k) an instance's w P 2^e_k: R_n; the filters as in the scores.
+// So a class that is hardly ever likely, a feature that is small for all instances, a small filter or instance costs nobody anything.  P is
+// made in single precision first, with the magnitudes for R and C on the way (maxima by atomics: the order does not matter), and split by
+// them in a pass of its own (fc_split).
 #include "product.hpp"
 
 #include <algorithm>
 
 namespace mcn {
 namespace {
-
-struct FcP {
-  int D, K, N, type;           // type: kPairs (single precision) or kBf16
-  int nWeights;
-  float factor;                // of all derivatives: derOutput / N or derOutput
-};
 
 __device__ __forceinline__ float instance_weight(const float* labels, const float* weights, int nWeights, int n) {
   return labels[n] != 0.f ? (weights ? weights[n % nWeights] : 1.f) : 0.f;
@@ -35,80 +37,127 @@ __device__ __forceinline__ float wave_max(float v) {
 
 // ---------------------------------------------------------------------------------------------- operands
 
-// What a call's first launches leave: per workgroup of fc_magnitudes the largest magnitude of its filters, or of its instances' weighted
-// features, as the bits of floats (a NaN or an infinity wins, and pair_scale leaves such a tensor as it is); every instance's own;
-// and, from fc_pack, the two tensors'.
-constexpr int kFilterParts = 1024, kFeatureParts = 512;
-struct Magnitudes {
-  unsigned filters, features;                                     // (what the products' ends read)
-  unsigned filterParts[kFilterParts], featureParts[kFeatureParts];
-};
-constexpr int kMagnitudeStep = 256 * 4 * 8;   // values a workgroup takes at a time
-
-__device__ __forceinline__ unsigned magnitude4(uintx4p v) {
-  return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
-}
-__device__ __forceinline__ unsigned wave_most(unsigned m) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, kWave));
+__device__ __forceinline__ unsigned wave_most(unsigned m, int lanes) {   // over groups of `lanes` neighbours
+  for (int o = lanes / 2; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, kWave));
   return m;
 }
-__device__ __forceinline__ unsigned group_most(unsigned m, unsigned* lds) {   // of 256 threads
-  m = wave_most(m);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
-  __syncthreads();
-  return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+
+// Largest magnitudes, as the bits of floats
+__device__ __forceinline__ void raise(unsigned* at, unsigned bits) {
+  if (bits) __hip_atomic_fetch_max(at, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void clear_words(unsigned* words, size_t n) {   // by all workgroups of 256
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) words[i] = 0;
 }
 
-// Workgroups [0, filterGroups): the filters; the rest: a wavefront per instance.
-__global__ __launch_bounds__(256) void fc_magnitudes(Magnitudes* __restrict__ out, unsigned* __restrict__ rows, const float* __restrict__ f, size_t n,
-                                                     int filterGroups, int vec, const float* __restrict__ x, int D, int N,
-                                                     const float* __restrict__ labels, const float* __restrict__ weights, int nWeights) {
-  __shared__ unsigned lds[4];
-  unsigned most = 0;
-  if ((int)blockIdx.x < filterGroups) {
-    for (size_t first = (size_t)blockIdx.x * kMagnitudeStep; first < n; first += (size_t)filterGroups * kMagnitudeStep) {
-      if (vec && first + kMagnitudeStep <= n) {
-        const uintx4p* f4 = (const uintx4p*)(f + first) + threadIdx.x;
-        uintx4p v[8];
+// Single precision: rows as pairs, each by its own magnitude.  `lanes` neighbours share a row (one pack of eight values each where that is
+// enough); rows of up to kHeld packs a lane are read once.
+struct RowsPart {
+  const float* x;
+  unsigned short* out;
+  int* exponents;
+  int rows;
+  unsigned firstGroup, groups;
+};
+struct RowsJob {
+  RowsPart parts[2];
+  int nParts, D, lanes;
+  long long pitch;
+  unsigned* clear;             // counters and magnitudes, cleared on the way
+  size_t nClear;
+};
+constexpr int kHeld = 8;
+__global__ __launch_bounds__(256) void fc_pack_rows(RowsJob j) {
+  clear_words(j.clear, j.nClear);
+  if (j.nParts == 0) return;
+  const RowsPart p = j.parts[j.nParts > 1 && blockIdx.x >= j.parts[1].firstGroup ? 1 : 0];
+  const int t = (int)threadIdx.x % j.lanes, per = (int)(j.pitch / 16), rows = 256 / j.lanes;
+  for (long long first = (long long)(blockIdx.x - p.firstGroup) * rows; first < p.rows; first += (long long)p.groups * rows) {
+    const long long row = first + (int)threadIdx.x / j.lanes;
+    const bool live = row < p.rows;
+    const float* from = p.x + (size_t)(live ? row : 0) * j.D;
+    float v[kHeld][8];
+    unsigned most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = f4[256 * i];
+    for (int i = 0; i < kHeld; ++i) {
+      const int c = 8 * (t + j.lanes * i);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = max(most, magnitude4(v[i]));
-      } else {
-        for (size_t i = first + threadIdx.x; i < std::min(first + kMagnitudeStep, n); i += 256) most = max(most, __float_as_uint(f[i]) & 0x7fffffffu);
+      for (int k = 0; k < 8; ++k) v[i][k] = 0.f;
+      if (8 * j.lanes * i < j.D && live && c < j.D) load8(v[i], from, c, j.D);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(v[i][k]) & 0x7fffffffu);
+    for (int i = kHeld; j.lanes * i < per; ++i) {
+      const int c = 8 * (t + j.lanes * i);
+      float u[8];
+      if (live && c < j.D) {
+        load8(u, from, c, j.D);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(u[k]) & 0x7fffffffu);
       }
     }
-    most = group_most(most, lds);
-    if (threadIdx.x == 0) out->filterParts[blockIdx.x] = most;
-    return;
-  }
-  const int group = blockIdx.x - filterGroups, groups = gridDim.x - filterGroups, lane = threadIdx.x & 63;
-  for (int row = group * 4 + (int)(threadIdx.x >> 6); row < N; row += groups * 4) {
-    unsigned m = 0;
-    for (int c = 8 * lane; c < D; c += 512) {
-      float v[8];
-      load8(v, x + (size_t)row * D, c, D);
+    most = wave_most(most, j.lanes);
+    if (!live) continue;
+    const int e = exponent_of(most);
+    if (t == 0) p.exponents[row] = e;
+    unsigned short* const to = p.out + (size_t)row * j.pitch;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+    for (int i = 0; i < kHeld; ++i) {
+      const int pack = t + j.lanes * i;
+      if (j.lanes * i >= per || pack >= per) continue;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = ldexpf(v[i][k], kPairExponent - e);
+      store8_pairs(to, 8 * pack, v[i]);
     }
-    m = wave_most(m);
-    if (lane == 0) rows[row] = m;
-    const float w = instance_weight(labels, weights, nWeights, row);
-    if (w != 0.f) most = max(most, __float_as_uint(fabsf(__uint_as_float(m) * w)));
+    for (int i = kHeld; j.lanes * i < per; ++i) {
+      const int pack = t + j.lanes * i;
+      if (pack >= per) continue;
+      float u[8] = {};
+      if (8 * pack < j.D) load8(u, from, 8 * pack, j.D);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = ldexpf(u[k], kPairExponent - e);
+      store8_pairs(to, 8 * pack, u);
+    }
   }
-  most = group_most(most, lds);
-  if (threadIdx.x == 0) out->featureParts[group] = most;
 }
 
-// Rows brought into the form the products read: pairs by a magnitude, or bfloat16 at a pitch of whole stages.
-enum { kFilters, kFeatures, kWeighted };   // by the tensor's magnitude; each row by its own; times the instance's weight (zeros for instances
-                                           // that do not count, whatever they hold), by the tensor's
-// (In bfloat16 the weighted features are rounded, for dzdf alone.  Weights in P would round what both derivatives are made of by as much:
+// S_d: the largest magnitudes of x 2^-e_n over the instances that count.  A wavefront's lanes lie along 512 features, its rows one behind the
+// other.
+__global__ __launch_bounds__(1024) void fc_feature_magnitudes(unsigned* __restrict__ out, const float* __restrict__ x, const int* __restrict__ exponents,
+                                                             const float* __restrict__ labels, const float* __restrict__ weights, int nWeights, int D,
+                                                             int N, int rows) {
+  __shared__ unsigned joint[16][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)blockIdx.x * 512 + 8 * lane;
+  unsigned most[8] = {};
+  for (long long k = 0; k < rows; ++k) {
+    const long long n = ((long long)blockIdx.y * rows + k) * 16 + wave;
+    if (n >= N || instance_weight(labels, weights, nWeights, (int)n) == 0.f) continue;
+    const int e = exponents[n];
+    if (c >= D) continue;
+    float v[8];
+    load8(v, x + (size_t)n * D, c, D);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most[i] = max(most[i], __float_as_uint(ldexpf(fabsf(v[i]), -e)));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) joint[wave][8 * lane + i] = most[i];
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t >= 512 || (int)blockIdx.x * 512 + t >= D) return;
+  unsigned m = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) m = max(m, joint[w][t]);
+  raise(out + (size_t)blockIdx.x * 512 + t, m);
+}
+
+// bfloat16: rows at a pitch of whole stages, as they are or times the instance's weight (zeros for instances that do not count, whatever
+// they hold).  (The weighted features are rounded, for dzdf alone.  Weights in P would round what both derivatives are made of by as much:
 // without them the label's -1, most of P, is exact.)
+enum { kAsTheyAre, kWeighted };
 struct PackPart {
-  const void* x;
+  const unsigned short* x;
   unsigned short* out;
   long long pitch;
   int rows, form;
@@ -117,31 +166,22 @@ struct PackPart {
 struct PackJob {
   PackPart parts[3];
   int nParts, D;
-  Magnitudes* magnitudes;                  // pairs
-  int filterGroups, featureGroups;         // 0: `filters` and `features` are there already
-  const unsigned* rowMagnitudes;
-  float* unscale;                          // of the rows by their own magnitudes
   const float *labels, *weights;
   int nWeights;
-  unsigned* counters;                      // cleared on the way
-  int nCounters;
+  unsigned* clear;                         // counters, cleared on the way
+  size_t nClear;
 };
 constexpr int kPackSteps = 4;              // times eight values a thread
 
-template <int TYPE>
 __global__ __launch_bounds__(256) void fc_pack(PackJob j) {
-  __shared__ unsigned lds[4];
+  clear_words(j.clear, j.nClear);
   const int which = j.nParts > 2 && blockIdx.x >= j.parts[2].firstGroup ? 2 : j.nParts > 1 && blockIdx.x >= j.parts[1].firstGroup ? 1 : 0;
   const PackPart p = j.parts[which];
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < j.nCounters; i += 256) j.counters[i] = 0;
-  // (all of a thread's loads first, not each behind the store before it: 32000 x 1024 single-precision values 56 -> 52 us, 21841 x 1001 bfloat16
-  // ones 22 -> 20)
-  const int per = (int)(p.pitch / (TYPE == kPairs ? 16 : 8));
+  // (all of a thread's loads first, not each behind the store before it: 21841 x 1001 values 22 -> 20 us)
+  const int per = (int)(p.pitch / 8);
   const size_t all = (size_t)p.rows * per;
   int row[kPackSteps], c[kPackSteps];
   float w[kPackSteps], v[kPackSteps][8];
-  unsigned own[kPackSteps];
 #pragma unroll
   for (int step = 0; step < kPackSteps; ++step) {
     const size_t i = ((size_t)(blockIdx.x - p.firstGroup) * kPackSteps + step) * 256 + threadIdx.x;
@@ -149,45 +189,102 @@ __global__ __launch_bounds__(256) void fc_pack(PackJob j) {
     row[step] = live ? (int)(i / per) : -1;
     c[step] = live ? (int)(i - (size_t)row[step] * per) * 8 : 0;
     w[step] = !live ? 0.f : p.form == kWeighted ? instance_weight(j.labels, j.weights, j.nWeights, row[step]) : 1.f;
-    own[step] = TYPE == kPairs && p.form == kFeatures && live ? j.rowMagnitudes[row[step]] : 0u;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[step][k] = 0.f;
-    if (w[step] != 0.f) {
-      if (TYPE == kPairs) load8(v[step], (const float*)p.x + (size_t)row[step] * j.D, c[step], j.D);
-      else load8(v[step], (const unsigned short*)p.x + (size_t)row[step] * j.D, c[step], j.D);
-    }
-  }
-  float scale = 1.f;
-  if (TYPE == kPairs && p.form != kFeatures) {
-    unsigned m = 0;
-    const int parts = p.form == kFilters ? j.filterGroups : j.featureGroups;
-    const unsigned* from = p.form == kFilters ? j.magnitudes->filterParts : j.magnitudes->featureParts;
-    if (parts) {
-      for (int i = threadIdx.x; i < parts; i += 256) m = max(m, from[i]);
-      m = group_most(m, lds);
-      if (blockIdx.x == p.firstGroup && threadIdx.x == 0) (p.form == kFilters ? j.magnitudes->filters : j.magnitudes->features) = m;
-    } else {
-      m = j.magnitudes->filters;
-    }
-    scale = pair_scale(m);
+    if (w[step] != 0.f) load8(v[step], p.x + (size_t)row[step] * j.D, c[step], j.D);
   }
 #pragma unroll
   for (int step = 0; step < kPackSteps; ++step) {
     if (row[step] < 0) return;
-    unsigned short* const to = p.out + (size_t)row[step] * p.pitch;
-    if (TYPE == kPairs) {
-      if (p.form == kFeatures) {
-        scale = pair_scale(own[step]);
-        if (c[step] == 0) j.unscale[row[step]] = pair_unscale(own[step]);
+    uintx4p h;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = (unsigned)to_bf16(v[step][2 * k] * w[step]) | (unsigned)to_bf16(v[step][2 * k + 1] * w[step]) << 16;
+    *(uintx4p*)(p.out + (size_t)row[step] * p.pitch + c[step]) = h;
+  }
+}
+
+// Single precision: w P, as the scores' product left it, into the two derivatives' operands, and (the first piece) the features over their
+// instances' magnitudes and their own.  One of P's operands takes P's place: the 128 bytes of 32 values are 32 h and 32 l, and the four
+// threads that hold these values are neighbours of one wavefront, whose loads are all done before its first store.
+struct SplitGrid { int lanes, across, down; };   // threads to a row in a workgroup; workgroups to a row, and rows of these
+struct SplitJob {
+  SplitGrid grid, featureGrid;             // of P, of the features
+  float* p;
+  unsigned short *forFilters, *forInput;   // may be null; one of them is `p`
+  long long pitch;                         // of all three, in 16-bit values
+  int N, columns;                          // columns: whole blocks of 32
+  const int *instances, *classes;          // e_n, e_k
+  const unsigned *classMost, *instanceMost;   // whose exponents are C_k, R_n
+  unsigned featureGroup;                   // the first workgroup of the features
+  const float* x;
+  unsigned short* features;
+  long long xPitch;
+  int D;
+  const unsigned* featureMost;             // ... S_d
+  const float *labels, *weights;
+  int nWeights;
+};
+// A thread keeps its eight columns (`lanes` neighbours share a row) and goes over the rows STEPS at a time: their exponents are worked out
+// once, and STEPS rows are on their way together.
+template <int STEPS>
+__global__ __launch_bounds__(256) void fc_split(SplitJob j) {
+  const bool features = blockIdx.x >= j.featureGroup;
+  const SplitGrid g = features ? j.featureGrid : j.grid;
+  const int per = features ? (int)(j.xPitch / 16) : j.columns / 8, group = (int)(blockIdx.x - (features ? j.featureGroup : 0u));
+  const int c = 8 * (group % g.across * g.lanes + (int)threadIdx.x % g.lanes), rows = 256 / g.lanes;
+  if (c >= 8 * per) return;
+  int ck[8], ek[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    ck[k] = features ? (c + k < j.D ? kPairExponent - exponent_of(j.featureMost[c + k]) : 0) : j.forFilters ? kPairExponent - exponent_of(j.classMost[c + k]) : 0;
+    ek[k] = !features && j.forInput ? kPairExponent + j.classes[c + k] : 0;
+  }
+  for (long long first = (long long)(group / g.across) * rows * STEPS + (int)threadIdx.x / g.lanes; first < j.N; first += (long long)g.down * rows * STEPS) {
+    float v[STEPS][8];
+    int en[STEPS];
+    unsigned rn[STEPS];
+#pragma unroll
+    for (int step = 0; step < STEPS; ++step) {
+      const long long n = first + step * rows;
+      const bool live = n < j.N;
+      en[step] = live ? j.instances[n] : 0;
+      rn[step] = live && j.forInput && !features ? j.instanceMost[n] : 0u;
+      if (features) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[step][k] = 0.f;
+        if (live && c < j.D && instance_weight(j.labels, j.weights, j.nWeights, (int)n) != 0.f) load8(v[step], j.x + (size_t)n * j.D, c, j.D);
+      } else {
+        const uintx4p* from = (const uintx4p*)((const char*)j.p + ((size_t)(live ? n : first) * j.pitch + 2 * c) * 2);
+        const uintx4p a = from[0], b = from[1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[step][k] = __uint_as_float(a[k]);
+          v[step][4 + k] = __uint_as_float(b[k]);
+        }
       }
+    }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[step][k] = v[step][k] * w[step] * scale;
-      store8_pairs(to, c[step], v[step]);
-    } else {
-      uintx4p h;
+    for (int step = 0; step < STEPS; ++step) {
+      const long long n = first + step * rows;
+      if (n >= j.N) break;
+      float u[8];
+      if (features) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) h[k] = (unsigned)to_bf16(v[step][2 * k] * w[step]) | (unsigned)to_bf16(v[step][2 * k + 1] * w[step]) << 16;
-      *(uintx4p*)(to + c[step]) = h;
+        for (int k = 0; k < 8; ++k) u[k] = ldexpf(v[step][k], ck[k] - en[step]);
+        store8_pairs(j.features + (size_t)n * j.xPitch, c, u);
+        continue;
+      }
+      if (j.forFilters) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) u[k] = ldexpf(v[step][k], ck[k] + en[step]);
+        store8_pairs(j.forFilters + (size_t)n * j.pitch, c, u);
+      }
+      if (j.forInput) {
+        const int e = exponent_of(rn[step]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) u[k] = ldexpf(v[step][k], ek[k] - e);
+        store8_pairs(j.forInput + (size_t)n * j.pitch, c, u);
+      }
     }
   }
 }
@@ -201,22 +298,30 @@ __global__ __launch_bounds__(256) void fc_zero(void* __restrict__ p, size_t n, i
 
 // ---------------------------------------------------------------------------------------------- products
 
-// What the scores need: z = acc * unscale[m] * 1/scale(filters) + bias[n], -infinity behind the piece's last class
+// What the scores need: z = acc * 2^(e_n + e_k - 28) + bias[k], -infinity behind the piece's last class
 struct Scores {
-  const float *unscale, *bias;     // unscale: null for bfloat16
-  const unsigned* magnitude;       // of the filters
+  const int *instances, *classes;  // e_n and the piece's e_k (that of the filters' places up to whole tiles); bfloat16: null
+  const float* bias;
   int N, K, first;                 // instances, classes in this piece, the piece's first class
   template <class S>
   __device__ __forceinline__ void make(floatx16p (&acc)[S::TM][S::TN], int m0, int n0, int tileEnd) const {
-    if (unscale) {
-      const float f = pair_unscale(*magnitude);
+    if (S::type == kPairs) {
+      // (one exact step: the two scales one after the other could leave the range and come back)
+      int e[S::TM];
 #pragma unroll
-      for (int i = 0; i < S::TM; ++i) {
-        // (both are powers of two: one product, kept from infinity, where the sums are nothing but zeros or past the range)
-        const float u = fminf(unscale[min(m0 + 32 * i, N - 1)] * f, 3.0e38f);
+      for (int i = 0; i < S::TM; ++i) e[i] = instances[min(m0 + 32 * i, N - 1)] - 2 * kPairExponent;
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j) acc[i][j] *= u;
-      }
+      for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int4 k = *(const int4*)(classes + n0 + 32 * j + 8 * q);
+          const int ek[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+          for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][4 * q + r] = ldexpf(acc[i][j][4 * q + r], e[i] + ek[r]);
+          __builtin_amdgcn_sched_barrier(0);   // (not all blocks' exponents at once: there are no registers for them)
+        }
     }
     if (bias) {
 #pragma unroll
@@ -299,7 +404,14 @@ struct StatsEnd {
   }
 };
 
-constexpr float kProbability = 16384.f;   // P as pairs: in [-1, 1], by 2^14
+// One of two registers goes to the lane h away, the other stays.  (The empty assembly keeps the two apart: from a choice between two entries of
+// an array the compiler makes an index, and of that a comparison with every entry, 22 us for a tile of 256 x 256.)
+__device__ __forceinline__ void choose(bool upper, float& give, float& keep) {
+  float a = give, b = keep;
+  asm("" : "+v"(a), "+v"(b));
+  give = upper ? a : b;
+  keep = upper ? b : a;
+}
 
 // Sums over the 32 lanes of a half-wavefront of N values a lane (N a power of two, at most 32): lane l of the half ends up with the sum of
 // value l % N.  Every exchange halves what is left to add: 31 exchanges for 32 values, where adding each across takes 160.
@@ -309,8 +421,8 @@ __device__ __forceinline__ float lanes_fold(float (&v)[N], int lane) {
   for (int h = N / 2; h >= 1; h >>= 1) {
 #pragma unroll
     for (int k = 0; k < h; ++k) {
-      const bool upper = (lane & h) != 0;
-      const float give = upper ? v[k] : v[k + h], keep = upper ? v[k + h] : v[k];
+      float give = v[k], keep = v[k + h];
+      choose((lane & h) != 0, give, keep);
       v[k] = keep + __shfl_xor(give, h, kWave);
     }
   }
@@ -320,21 +432,42 @@ __device__ __forceinline__ float lanes_fold(float (&v)[N], int lane) {
   return s;
 }
 
-// Backward: P as the operand of two products (the instances' weights go into the other operand, or the result), and the columns' sums of
-// w P before it is rounded, one per tile.
+// The same for the largest
+template <int N>
+__device__ __forceinline__ float lanes_most(float (&v)[N], int lane) {
+#pragma unroll
+  for (int h = N / 2; h >= 1; h >>= 1) {
+#pragma unroll
+    for (int k = 0; k < h; ++k) {
+      float give = v[k], keep = v[k + h];
+      choose((lane & h) != 0, give, keep);
+      v[k] = fmaxf(keep, __shfl_xor(give, h, kWave));
+    }
+  }
+  float m = v[0];
+#pragma unroll
+  for (int o = N; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+  return m;
+}
+
+// Backward: P, and the columns' sums of w P, one per tile.  bfloat16: P as the operand of two products (the instances' weights go into the
+// other operand, or the result).  Single precision: w P itself, and the exponents that it is split by.
 struct ProbabilitiesEnd {
   Scores z;
-  unsigned short* out;
-  long long pitch;
+  void* out;
+  long long pitch;                 // in 16-bit values
   const float *labels, *weights, *logSums;
   int nWeights, classes;
   float* sums;                     // [tile rows][classes], times `factor`; may be null
   float factor;
+  unsigned *classMost, *instanceMost;   // the largest |w P| 2^e_n of a class, |w P| 2^e_k of an instance; null where nobody asks for them
   template <class S>
   __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
     const int m0 = tm * S::BM + 32 * wm * S::TM + (lane & 31), n0 = tn * S::BN + 32 * wn * S::TN + 4 * (lane >> 5);
     z.make<S>(acc, m0, n0, (tn + 1) * S::BN);
-    float* columns = (float*)(lds + S::ldsBytes - S::WM * S::BN * 4);  // [WM][BN]
+    constexpr bool pairs = S::type == kPairs;
+    unsigned* magnitudes = (unsigned*)(lds + S::ldsBytes - 2 * S::WM * S::BN * 4);  // [WM][BN]
+    float* columns = (float*)(lds + S::ldsBytes - S::WM * S::BN * 4);         // [WM][BN]
     float weight[S::TM];
 #pragma unroll
     for (int i = 0; i < S::TM; ++i) {
@@ -356,11 +489,58 @@ struct ProbabilitiesEnd {
           for (int r = 0; r < 16; ++r)
             if (c == 32 * j + 8 * (r / 4) + r % 4 && n0 + c < z.K) acc[i][j][r] -= 1.f;
       }
+      if (pairs && weights) {
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] *= w;
+      }
       if (__any(w == 0.f)) {       // (such an instance's scores may be anything)
 #pragma unroll
         for (int j = 0; j < S::TN; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[i][j][r] = w == 0.f ? 0.f : acc[i][j][r];
+      }
+    }
+    if (pairs && (classMost || instanceMost)) {
+      // (magnitudes that leave the range here do so in the derivatives)
+      int en[S::TM];
+      float most[S::TM];
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) {
+        en[i] = z.instances[min(m0 + 32 * i, z.N - 1)];
+        most[i] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j) {
+        float v[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int4 k = *(const int4*)(z.classes + n0 + 32 * j + 8 * q);
+          const int ek[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::TM; ++i) {
+              const float p = acc[i][j][4 * q + r];
+              m = fmaxf(m, fabsf(ldexpf(p, en[i])));
+              most[i] = fmaxf(most[i], fabsf(ldexpf(p, ek[r])));
+            }
+            v[4 * q + r] = m;
+          }
+        }
+        const unsigned m = __float_as_uint(lanes_most<16>(v, lane));
+        const int r = lane & 15;
+        if ((lane & 16) == 0) magnitudes[wm * S::BN + 32 * (wn * S::TN + j) + 8 * (r / 4) + 4 * (lane >> 5) + r % 4] = m;
+        __builtin_amdgcn_sched_barrier(0);   // (nor all blocks' exchanges: 1200 registers went to memory, 2.2 ms for 32000 classes instead of 1.7)
+      }
+      if (instanceMost) {
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i) {
+          const float m = fmaxf(most[i], __shfl_xor(most[i], 32, kWave));
+          if (lane < 32 && m0 + 32 * i < z.N) raise(instanceMost + m0 + 32 * i, __float_as_uint(m));
+        }
       }
     }
     if (sums) {
@@ -372,25 +552,36 @@ struct ProbabilitiesEnd {
         for (int r = 0; r < 16; ++r) {
           v[r] = 0.f;
 #pragma unroll
-          for (int i = 0; i < S::TM; ++i) v[r] += weight[i] * acc[i][j][r];
+          for (int i = 0; i < S::TM; ++i) v[r] += pairs ? acc[i][j][r] : weight[i] * acc[i][j][r];
         }
         const float s = lanes_fold<16>(v, lane);
         const int r = lane & 15;
         if ((lane & 16) == 0) columns[wm * S::BN + 32 * (wn * S::TN + j) + 8 * (r / 4) + 4 * (lane >> 5) + r % 4] = s;
       }
+    }
+    const bool raising = pairs && classMost;
+    if (sums || raising) {
       __syncthreads();
       for (int t = threadIdx.x; t < S::BN; t += S::threads) {
         const int n = tn * S::BN + t;
         if (n >= z.K) continue;
-        float s = columns[t];
+        if (sums) {
+          float s = columns[t];
 #pragma unroll
-        for (int w = 1; w < S::WM; ++w) s += columns[w * S::BN + t];
-        sums[(size_t)tm * classes + z.first + n] = s * factor;
+          for (int w = 1; w < S::WM; ++w) s += columns[w * S::BN + t];
+          sums[(size_t)tm * classes + z.first + n] = s * factor;
+        }
+        if (raising) {
+          unsigned m = magnitudes[t];
+#pragma unroll
+          for (int w = 1; w < S::WM; ++w) m = max(m, magnitudes[w * S::BN + t]);
+          raise(classMost + n, m);
+        }
       }
     }
-    constexpr int size = S::type == kPairs ? 4 : 2, J = turned_blocks<S, size>();
+    constexpr int size = pairs ? 4 : 2, J = turned_blocks<S, size>();
     const RowTurn<J * 32 * size> turn(lds, wn * S::WM + wm);
-    static_assert(S::WM * S::WN * RowTurn<J * 32 * size>::size + S::WM * S::BN * 4 <= S::ldsBytes, "beside the columns");
+    static_assert(S::WM * S::WN * RowTurn<J * 32 * size>::size + 2 * S::WM * S::BN * 4 <= S::ldsBytes, "beside the columns and the magnitudes");
     const int half = lane >> 5, l32 = lane & 31, first = tn * S::BN + 32 * wn * S::TN;
 #pragma unroll
     for (int i = 0; i < S::TM; ++i)
@@ -402,13 +593,10 @@ struct ProbabilitiesEnd {
           for (int q = 0; q < 4; ++q) {
             const floatx16p& a = acc[i][j0 + j];
             const int column = 8 * q + 4 * half;
-            unsigned h[4];
-            if (S::type == kPairs) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) h[r] = split_pair(a[4 * q + r] * kProbability);
-              *(uintx2p*)turn.at(l32, 128 * j + 2 * column) = (uintx2p){(h[0] & 0xffffu) | h[1] << 16, (h[2] & 0xffffu) | h[3] << 16};
-              *(uintx2p*)turn.at(l32, 128 * j + 64 + 2 * column) = (uintx2p){h[0] >> 16 | (h[1] & 0xffff0000u), h[2] >> 16 | (h[3] & 0xffff0000u)};
+            if (pairs) {
+              *(float4*)turn.at(l32, 128 * j + 4 * column) = make_float4(a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]);
             } else {
+              unsigned h[4];
 #pragma unroll
               for (int r = 0; r < 4; ++r) h[r] = to_bf16(a[4 * q + r]);
               *(uintx2p*)turn.at(l32, 64 * j + 2 * column) = (uintx2p){h[0] | h[1] << 16, h[2] | h[3] << 16};
@@ -416,7 +604,7 @@ struct ProbabilitiesEnd {
           }
         const int m1 = tm * S::BM + 32 * (wm * S::TM + i), start = (first + 32 * j0) * size;   // bytes from the row's first class
         turn.each(lane, [&](int row, int offset, uintx4p v) {
-          if (m1 + row < z.N && start + offset < 2 * pitch) *(uintx4p*)((char*)(out + (size_t)(m1 + row) * pitch) + start + offset) = v;
+          if (m1 + row < z.N && start + offset < 2 * pitch) *(uintx4p*)((char*)out + (size_t)(m1 + row) * pitch * 2 + start + offset) = v;
         });
       }
   }
@@ -429,14 +617,11 @@ struct StoreEnd {
   const float* sum;                   // what other pieces gave, may be null (and may be `out`)
   int M, Ncols;
   float factor;
-  const unsigned* magnitude;          // may be null
-  const float *labels, *weights;      // may be null: rows are instances
+  const unsigned *rowMost, *columnMost;   // pairs: the magnitudes whose exponents the rows and (may be null) the columns were scaled by
+  const float *labels, *weights;      // bfloat16, rows that are instances; or null
   int nWeights;
   template <class S>
   __device__ __forceinline__ void finish(floatx16p (&acc)[S::TM][S::TN], int tm, int tn, int, int lane, int wm, int wn, char* lds) const {
-    // (P as pairs is 2^14 too large; taken off together with the other operand's scale, before the factor, so that nothing leaves the range on
-    // the way.  Both are powers of two.)
-    const float u = magnitude ? pair_unscale(*magnitude) * (1.f / kProbability) : 1.f;
     const bool wide = (Ncols & 3) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)sum & 15) == 0;
     constexpr int J = turned_blocks<S, 4>();
     const RowTurn<J * 128> turn(lds, wn * S::WM + wm);
@@ -445,6 +630,7 @@ struct StoreEnd {
     for (int i = 0; i < S::TM; ++i) {
       const int m1 = tm * S::BM + 32 * (wm * S::TM + i);
       const float w = labels && m1 + l32 < M ? instance_weight(labels, weights, nWeights, m1 + l32) * factor : factor;
+      const int e = S::type == kPairs ? (m1 + l32 < M ? exponent_of(rowMost[m1 + l32]) : 0) - 2 * kPairExponent : 0;
 #pragma unroll
       for (int j0 = 0; j0 < S::TN; j0 += J) {
 #pragma unroll
@@ -452,8 +638,16 @@ struct StoreEnd {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const floatx16p& a = acc[i][j0 + j];
-            *(float4*)turn.at(l32, 128 * j + 32 * q + 16 * half) =
-                make_float4(a[4 * q] * u * w, a[4 * q + 1] * u * w, a[4 * q + 2] * u * w, a[4 * q + 3] * u * w);
+            float4 v = make_float4(a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]);
+            if (S::type == kPairs) {   // (one exact step, and before the factor: nothing leaves the range on the way)
+              int4 k = {};
+              if (columnMost) {
+                const uint4 c = *(const uint4*)(columnMost + tn * S::BN + 32 * (wn * S::TN + j0 + j) + 8 * q + 4 * half);
+                k = make_int4(exponent_of(c.x), exponent_of(c.y), exponent_of(c.z), exponent_of(c.w));
+              }
+              v = make_float4(ldexpf(v.x, e + k.x), ldexpf(v.y, e + k.y), ldexpf(v.z, e + k.z), ldexpf(v.w, e + k.w));
+            }
+            *(float4*)turn.at(l32, 128 * j + 32 * q + 16 * half) = make_float4(v.x * w, v.y * w, v.z * w, v.w * w);
           }
         const int n1 = tn * S::BN + 32 * (wn * S::TN + j0);
         if (wide) {
@@ -587,12 +781,12 @@ struct Plan {
   long long xPitch, fPitch, pPitch;
   int piece, pieces, tiles;        // classes per piece; tiles of scores over all classes
   ProductPlan scores, dx, df;      // of a whole piece; the last one, if smaller, is cut as they are
-  size_t x, xUnscale, xw, f, magnitudes, rowMagnitudes, counters, parts, own, terms, logSums, p, sum, columns, products, total;
+  size_t x, xExponents, xw, f, fExponents, cleared, parts, own, terms, logSums, p, p2, sum, columns, products, total;
   int nCounters, tileRows;         // (counters: the last is fc_log_sums')
-  // workgroups that pack rows
-  unsigned pack_groups(int rows, long long pitch) const {
-    return (unsigned)(((size_t)rows * (pitch / (type == kPairs ? 16 : 8)) + 256 * kPackSteps - 1) / (256 * kPackSteps));
-  }
+  // words that are cleared before they are used: counters; S_d; and, by piece, R_n and C_k
+  size_t featureMost, instanceMost, classMost, words;
+  // workgroups that pack eight values a thread, a few times
+  unsigned pack_groups(long long rows, long long packs) const { return (unsigned)((rows * packs + 256 * kPackSteps - 1) / (256 * kPackSteps)); }
 };
 
 // A piece's P, or packed filters: larger ones save passes over the sums of dzdx (128, 256, 512 MiB: 29.5, 29.5, 29.2 ms for 128000 classes in
@@ -605,14 +799,14 @@ size_t piece_bytes() {
 Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool backward) {
   Plan p;
   p.type = g->dataType == MCN_BFLOAT16 ? kBf16 : kPairs;
-  const bool whole = p.type == kBf16 && g->D % 64 == 0;
+  const bool whole = p.type == kBf16 && g->D % 64 == 0, pairs = p.type == kPairs;
   p.fInPlace = whole && aligned16(f);
   p.xInPlace = whole && aligned16(x);
   p.xPitch = row_halves(p.type, g->D);
   p.fPitch = p.fInPlace ? g->D : row_halves(p.type, g->D);
   // a piece: P (backward) and the packed filters stay within piece_bytes(), whole tiles
   const long long most = (g->K + 255ll) / 256 * 256;
-  const long long perClass = std::max<long long>(backward ? g->N * 2ll * (p.type == kPairs ? 2 : 1) : 0, p.fInPlace ? 0 : p.fPitch * 2);
+  const long long perClass = std::max<long long>(backward ? g->N * 2ll * (pairs ? 2 : 1) : 0, p.fInPlace ? 0 : p.fPitch * 2);
   long long piece = perClass ? std::max(256ll, (long long)piece_bytes() / perClass / 256 * 256) : most;
   if (piece < most) {              // equal pieces
     const long long n = (most + piece - 1) / piece;
@@ -632,25 +826,30 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  const auto whole_tiles = [](size_t n) { return (n + 255) / 256 * 256; };
   p.tileRows = div_up(g->N, kTileSize[p.scores.tile]);
   p.nCounters = 1 + (int)(backward ? std::max({p.scores.counters(), p.dx.counters(), p.df.counters()}) : p.scores.counters());
-  p.magnitudes = take(p.type == kPairs ? sizeof(Magnitudes) : 0);
-  p.rowMagnitudes = take(p.type == kPairs ? (size_t)g->N * 4 : 0);
-  p.counters = take(4 * (size_t)p.nCounters);
+  p.featureMost = whole_tiles((size_t)p.nCounters);
+  p.instanceMost = p.featureMost + (pairs && backward ? whole_tiles((size_t)g->D) : 0);
+  p.classMost = p.instanceMost + (pairs && backward ? whole_tiles((size_t)g->N) : 0);
+  p.words = p.classMost + (pairs && backward ? (size_t)p.piece : 0);
+  p.cleared = take(4 * p.words);
+  p.xExponents = take(pairs ? (size_t)g->N * 4 : 0);
+  p.fExponents = take(pairs ? whole_tiles((size_t)g->K) * 4 : 0);
   p.products = take(backward ? std::max({p.scores.partBytes(), p.dx.partBytes(), p.df.partBytes()}) : p.scores.partBytes());
   p.x = take(p.xInPlace ? 0 : (size_t)g->N * p.xPitch * 2);
-  p.xUnscale = take(p.type == kPairs ? (size_t)g->N * 4 : 0);
   p.f = take(p.fInPlace ? 0 : (size_t)std::min(p.piece, g->K) * p.fPitch * 2);
   p.parts = take((size_t)g->N * p.tiles * 8);
   p.own = take((size_t)g->N * 4);
   p.terms = take((size_t)g->N * 4);
   p.logSums = take((size_t)g->N * 4);
-  p.xw = p.p = p.sum = p.columns = 0;
+  p.xw = p.p = p.p2 = p.sum = p.columns = 0;
   if (backward) {
     p.xw = take((size_t)g->N * p.xPitch * 2);
     p.columns = take(p.tileRows > 1 ? (size_t)p.tileRows * g->K * 4 : 0);
     p.p = take((size_t)g->N * p.pPitch * 2);
-    p.sum = take(p.type == kBf16 && p.pieces > 1 ? (size_t)g->N * g->D * 4 : 0);
+    p.p2 = take(pairs ? (size_t)g->N * p.pPitch * 2 : 0);
+    p.sum = take(!pairs && p.pieces > 1 ? (size_t)g->N * g->D * 4 : 0);
   }
   p.total = at;
   return p;
@@ -678,69 +877,102 @@ struct Call {
   int nWeights;
   char* ws;
   Plan p;
-  Magnitudes* magnitudes() const { return (Magnitudes*)(ws + p.magnitudes); }
-  Scratch scratch() const { return {(float*)(ws + p.products), (unsigned*)(ws + p.counters)}; }
+  unsigned* words(size_t at) const { return (unsigned*)(ws + p.cleared) + at; }
+  Scratch scratch() const { return {(float*)(ws + p.products), words(0)}; }
+  int* instances() const { return (int*)(ws + p.xExponents); }
+  int* classExponents(int piece) const { return (int*)(ws + p.fExponents) + (size_t)piece * p.piece; }
   Matrix X() const { return {p.xInPlace ? x : ws + p.x, p.xPitch, 0, g->N}; }
   const char* piece_of(const void* t, int first) const { return (const char*)t + (size_t)first * g->D * (p.type == kPairs ? 4 : 2); }
   int classes(int piece) const { return std::min(p.piece, g->K - piece * p.piece); }
   Matrix F(int piece) const { return {p.fInPlace ? piece_of(filters, piece * p.piece) : ws + p.f, p.fPitch, 0, classes(piece)}; }
 };
 
-void launch_pack(const Call& c, PackJob& j) {
+// The filters of a piece and, before the first (`all`), the features (bfloat16: for dzdf the weighted ones too), where the products read them;
+// the words that the piece's products count and take maxima in are cleared, all of them before the first.
+void pack(const Call& c, int piece, bool all, bool weighted) {
+  const Plan& p = c.p;
+  const int D = c.g->D, N = c.g->N;
   unsigned groups = 0;
-  for (int k = 0; k < j.nParts; ++k) {
-    j.parts[k].firstGroup = groups;
-    groups += c.p.pack_groups(j.parts[k].rows, j.parts[k].pitch);
+  const auto at = [&](unsigned n) {
+    const unsigned first = groups;
+    groups += n;
+    return first;
+  };
+  const size_t from = all ? 0 : p.instanceMost;
+  unsigned* const clear = c.words(from);
+  const size_t nClear = p.words - from;
+  if (p.type == kPairs) {
+    RowsJob j = {};
+    j.D = D;
+    j.pitch = p.xPitch;
+    j.lanes = 1;
+    while (j.lanes < 64 && j.lanes < j.pitch / 16) j.lanes *= 2;
+    j.clear = clear; j.nClear = nClear;
+    const auto rows = [&](const void* x, size_t out, int* exponents, int n) {
+      const unsigned blocks = (unsigned)std::min<long long>(1 << 22, div_up(n, 256 / j.lanes));
+      j.parts[j.nParts++] = {(const float*)x, (unsigned short*)(c.ws + out), exponents, n, at(blocks), blocks};
+    };
+    rows(c.piece_of(c.filters, piece * p.piece), p.f, c.classExponents(piece), c.classes(piece));
+    if (all) rows(c.x, p.x, c.instances(), N);
+    KernelTimer timer("fc_pack", c.s);
+    hipLaunchKernelGGL(fc_pack_rows, dim3(groups), dim3(256), 0, c.s, j);
+    return;
   }
-  if (groups == 0) {               // (the counters alone)
-    j.parts[0] = {};
-    groups = 1;
+  PackJob j = {};
+  j.D = D;
+  j.labels = c.labels; j.weights = c.weights; j.nWeights = c.nWeights;
+  j.clear = clear; j.nClear = nClear;
+  const auto rows = [&](const void* x, size_t out, long long pitch, int n, int form) {
+    j.parts[j.nParts++] = {(const unsigned short*)x, (unsigned short*)(c.ws + out), pitch, n, form, at(p.pack_groups(n, pitch / 8))};
+  };
+  if (!p.fInPlace) rows(c.piece_of(c.filters, piece * p.piece), p.f, p.fPitch, c.classes(piece), kAsTheyAre);
+  if (all && !p.xInPlace) rows(c.x, p.x, p.xPitch, N, kAsTheyAre);
+  if (all && weighted) rows(c.x, p.xw, p.xPitch, N, kWeighted);
+  if (groups == 0) {
+    if (nClear == 0) return;       // (filters in place)
+    groups = 1;                    // (the counters alone)
   }
   KernelTimer timer("fc_pack", c.s);
-  if (c.p.type == kPairs) hipLaunchKernelGGL(fc_pack<kPairs>, dim3(groups), dim3(256), 0, c.s, j);
-  else hipLaunchKernelGGL(fc_pack<kBf16>, dim3(groups), dim3(256), 0, c.s, j);
-}
-
-// What comes before the products: magnitudes, the features (and, for dzdf, the weighted ones), the first piece of the filters, counters
-int prepare(const Call& c, bool weighted) {
-  const Plan& p = c.p;
-  PackJob j = {};
-  j.D = c.g->D;
-  j.labels = c.labels; j.weights = c.weights; j.nWeights = c.nWeights;
-  j.counters = (unsigned*)(c.ws + p.counters); j.nCounters = p.nCounters;
-  if (p.type == kPairs) {
-    const size_t n = (size_t)c.g->K * c.g->D;
-    j.magnitudes = c.magnitudes();
-    j.rowMagnitudes = (unsigned*)(c.ws + p.rowMagnitudes);
-    j.unscale = (float*)(c.ws + p.xUnscale);
-    j.filterGroups = (int)std::min<size_t>(kFilterParts, (n + kMagnitudeStep - 1) / kMagnitudeStep);
-    j.featureGroups = std::min(kFeatureParts, div_up(c.g->N, 4));
-    KernelTimer timer("fc_magnitudes", c.s);
-    hipLaunchKernelGGL(fc_magnitudes, dim3((unsigned)(j.filterGroups + j.featureGroups)), dim3(256), 0, c.s, j.magnitudes, (unsigned*)(c.ws + p.rowMagnitudes),
-                       (const float*)c.filters, n, j.filterGroups, (int)aligned16(c.filters), (const float*)c.x, c.g->D, c.g->N, c.labels, c.weights,
-                       c.nWeights);
-  }
-  if (!p.fInPlace) j.parts[j.nParts++] = {c.filters, (unsigned short*)(c.ws + p.f), p.fPitch, c.classes(0), kFilters, 0};
-  if (!p.xInPlace) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.x), p.xPitch, c.g->N, kFeatures, 0};
-  if (weighted) j.parts[j.nParts++] = {c.x, (unsigned short*)(c.ws + p.xw), p.xPitch, c.g->N, kWeighted, 0};
-  launch_pack(c, j);
-  return check_launch(c.who);
-}
-
-// the filters of a piece, where its products read them (`there`: prepare() has done it)
-void pack_piece(const Call& c, int piece, bool there) {
-  if (c.p.fInPlace || there) return;
-  PackJob j = {};
-  j.D = c.g->D;
-  j.magnitudes = c.magnitudes();
-  j.parts[j.nParts++] = {c.piece_of(c.filters, piece * c.p.piece), (unsigned short*)(c.ws + c.p.f), c.p.fPitch, c.classes(piece), kFilters, 0};
-  launch_pack(c, j);
+  hipLaunchKernelGGL(fc_pack, dim3(groups), dim3(256), 0, c.s, j);
 }
 
 template <int TYPE>
 Scores scores_of(const Call& c, int piece) {
-  return {TYPE == kPairs ? (const float*)(c.ws + c.p.xUnscale) : nullptr, c.biases, TYPE == kPairs ? &c.magnitudes()->filters : nullptr, c.g->N,
-          c.classes(piece), piece * c.p.piece};
+  return {TYPE == kPairs ? c.instances() : nullptr, TYPE == kPairs ? c.classExponents(piece) : nullptr, c.biases, c.g->N, c.classes(piece), piece * c.p.piece};
+}
+
+// Single precision: w P of a piece into the operands of the derivatives that are wanted, and before the first piece's the features into dzdf's
+void split(const Call& c, int piece, bool forInput, bool forFilters) {
+  const Plan& p = c.p;
+  SplitJob j = {};
+  j.p = (float*)(c.ws + p.p);
+  j.forInput = forInput ? (unsigned short*)(c.ws + p.p) : nullptr;
+  j.forFilters = !forFilters ? nullptr : (unsigned short*)(c.ws + (forInput ? p.p2 : p.p));
+  j.pitch = p.pPitch;
+  j.N = c.g->N; j.columns = (c.classes(piece) + 31) / 32 * 32;
+  j.instances = c.instances(); j.classes = c.classExponents(piece);
+  j.classMost = c.words(p.classMost); j.instanceMost = c.words(p.instanceMost);
+  j.x = (const float*)c.x; j.features = (unsigned short*)(c.ws + p.xw); j.xPitch = p.xPitch; j.D = c.g->D;
+  j.featureMost = c.words(p.featureMost);
+  j.labels = c.labels; j.weights = c.weights; j.nWeights = c.nWeights;
+  // (2048 x 32000 values: two rows at a time 247 us, four 190, eight 165, and by eight workgroups to a unit that go on down the rows 153, 5.1
+  // TB/s; few values: one, so that there are workgroups for all units)
+  const int steps = (long long)j.N * (j.columns + p.xPitch / 2) >= 4ll << 20 ? 8 : 1;
+  unsigned groups = 0;
+  const auto plan = [&](long long packs) {
+    SplitGrid g = {4, 0, 0};
+    while (g.lanes < 256 && g.lanes < packs) g.lanes *= 2;
+    g.across = div_up(packs, g.lanes);
+    g.down = (int)std::min<long long>(div_up(j.N, 256 / g.lanes * steps), std::max(1, 2048 / g.across));
+    groups += (unsigned)g.across * (unsigned)g.down;
+    return g;
+  };
+  j.grid = plan(j.columns / 8);
+  j.featureGroup = groups;
+  if (forFilters && piece == 0) j.featureGrid = plan(p.xPitch / 16);
+  KernelTimer timer("fc_split", c.s);
+  if (steps == 1) hipLaunchKernelGGL(fc_split<1>, dim3(groups), dim3(256), 0, c.s, j);
+  else hipLaunchKernelGGL(fc_split<8>, dim3(groups), dim3(256), 0, c.s, j);
 }
 
 // y may be null (the log sums alone)
@@ -749,7 +981,7 @@ int forward(const Call& c, float* y, float* logSums) {
   const Plan& p = c.p;
   const int N = c.g->N;
   for (int k = 0; k < p.pieces; ++k) {
-    pack_piece(c, k, k == 0);
+    if (k > 0) pack(c, k, false, false);
     StatsEnd e;
     e.z = scores_of<TYPE>(c, k);
     e.parts = (float2*)(c.ws + p.parts);
@@ -767,7 +999,7 @@ int forward(const Call& c, float* y, float* logSums) {
   {
     KernelTimer timer("fc_log_sums", c.s);
     hipLaunchKernelGGL(few ? fc_log_sums<4> : fc_log_sums<1>, dim3((unsigned)std::min(1 << 20, div_up(N, few ? 1 : 4))), dim3(256), 0, c.s, joined ? y : nullptr, logSums, terms,
-                       (unsigned*)(c.ws + p.counters) + p.nCounters - 1, (const float2*)(c.ws + p.parts), (const float*)(c.ws + p.own), c.labels, c.weights,
+                       c.words((size_t)p.nCounters - 1), (const float2*)(c.ws + p.parts), (const float*)(c.ws + p.own), c.labels, c.weights,
                        c.nWeights, N, p.tiles, divide);
   }
   if (y && !joined) {
@@ -781,36 +1013,46 @@ template <int TYPE>
 int backward(const Call& c, void* derInput, void* derFilters, float* derBiases, const float* logSums, float factor, bool firstThere) {
   const Plan& p = c.p;
   const int N = c.g->N, D = c.g->D;
+  const bool pairs = TYPE == kPairs;
   const Matrix Xw = {c.ws + p.xw, p.xPitch, 0, N};
+  if (pairs && derFilters) {
+    const int columns = div_up(D, 512), rows = std::max(1, div_up((long long)N * columns, 16 * 512));   // (some 512 workgroups)
+    KernelTimer timer("fc_feature_magnitudes", c.s);
+    hipLaunchKernelGGL(fc_feature_magnitudes, dim3((unsigned)columns, (unsigned)div_up(N, 16ll * rows)), dim3(1024), 0, c.s, c.words(p.featureMost),
+                       (const float*)c.x, c.instances(), c.labels, c.weights, c.nWeights, D, N, rows);
+  }
   for (int k = 0; k < p.pieces; ++k) {
     const int first = k * p.piece, count = c.classes(k), columns = (count + 63) / 64 * 64;
-    pack_piece(c, k, k == 0 && firstThere);
+    if (k > 0 || !firstThere) pack(c, k, false, false);
     ProbabilitiesEnd e;
     e.z = scores_of<TYPE>(c, k);
-    e.out = (unsigned short*)(c.ws + p.p);
+    e.out = c.ws + p.p;
     e.pitch = p.pPitch;
     e.labels = c.labels; e.weights = c.weights; e.logSums = logSums;
     e.nWeights = c.nWeights; e.classes = c.g->K;
     e.sums = !derBiases ? nullptr : p.tileRows > 1 ? (float*)(c.ws + p.columns) : derBiases;
     e.factor = factor;
+    e.classMost = pairs && derFilters ? c.words(p.classMost) : nullptr;
+    e.instanceMost = pairs && derInput ? c.words(p.instanceMost) : nullptr;
     int rc = product<TYPE, false, false>(c.s, c.who, "fc_probabilities", c.X(), c.F(k), N, columns, p.scores.of(N, columns), c.scratch(), e);
     if (rc) return rc;
+    if (pairs && (derInput || derFilters)) split(c, k, derInput != nullptr, derFilters != nullptr);
     const Matrix P = {c.ws + p.p, p.pPitch, 0, N};
     if (derInput) {
       // (the pieces add up in single precision: in derInput itself, or beside it)
-      float* sum = TYPE == kPairs ? (float*)derInput : (float*)(c.ws + p.sum);
+      float* sum = pairs ? (float*)derInput : (float*)(c.ws + p.sum);
       const bool last = k == p.pieces - 1;
-      const StoreEnd d = {TYPE == kPairs || last ? derInput : sum, TYPE == kBf16 && last, k > 0 ? sum : nullptr, N, D, factor,
-                          TYPE == kPairs ? &c.magnitudes()->filters : nullptr, c.labels, c.weights, c.nWeights};
+      const StoreEnd d = {pairs || last ? derInput : sum, !pairs && last, k > 0 ? sum : nullptr, N, D, factor, c.words(p.instanceMost), nullptr,
+                          pairs ? nullptr : c.labels, c.weights, c.nWeights};
       ProductPlan q = p.dx;
       q.stages = div_up(count, stage_depth(TYPE));
       rc = product<TYPE, false, true>(c.s, c.who, "fc_derivative_x", P, c.F(k), N, D, q, c.scratch(), d);
       if (rc) return rc;
     }
     if (derFilters) {
-      const StoreEnd d = {(void*)c.piece_of(derFilters, first), TYPE == kBf16, nullptr, count, D, factor,
-                          TYPE == kPairs ? &c.magnitudes()->features : nullptr, nullptr, nullptr, 1};
-      rc = product<TYPE, true, true>(c.s, c.who, "fc_derivative_f", P, Xw, count, D, p.df.of(count, D), c.scratch(), d);
+      const StoreEnd d = {(void*)c.piece_of(derFilters, first), !pairs, nullptr, count, D, factor, c.words(p.classMost), c.words(p.featureMost), nullptr, nullptr, 1};
+      const Matrix Pf = {c.ws + (pairs && derInput ? p.p2 : p.p), p.pPitch, 0, N};
+      rc = product<TYPE, true, true>(c.s, c.who, "fc_derivative_f", Pf, Xw, count, D, p.df.of(count, D), c.scratch(), d);
       if (rc) return rc;
     }
   }
@@ -854,8 +1096,7 @@ int mcn_fcloss_forward(mcn_stream_t stream, const mcn_fcloss_geom* g, float* y, 
   if (!workspace || workspaceBytes < c.p.total)
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, c.p.total);
   if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
-  rc = prepare(c, false);
-  if (rc) return rc;
+  pack(c, 0, true, false);
   float* sums = logSums ? logSums : (float*)(c.ws + c.p.logSums);
   return c.p.type == kPairs ? forward<kPairs>(c, y, sums) : forward<kBf16>(c, y, sums);
 }
@@ -880,8 +1121,7 @@ int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, void* der
   if (!workspace || workspaceBytes < c.p.total)
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, c.p.total);
   if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
-  rc = prepare(c, derFilters != nullptr);
-  if (rc) return rc;
+  pack(c, 0, true, derFilters != nullptr);
   const float factor = (float)(g->normalise ? derOutput / g->N : derOutput);
   const bool recompute = logSums == nullptr;
   if (recompute) {

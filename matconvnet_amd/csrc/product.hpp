@@ -5,11 +5,12 @@
 // index is the one that runs along a row: the row index is m or n) or ACROSS them (the reduction index counts the rows).
 //   kBf16   bfloat16 as it stands.
 //   kPairs  a single-precision value v as two half-precision ones, h = half(s v) and l = half(s v - h), s a power of two that puts the
-//           largest magnitude of the tensor (or row) into [2^14, 2^15).  h + l keeps 22 bits and the sign of l one more: v to 2^-24
-//           of itself down to 2^-29 of the largest magnitude, to 2^-40 of that magnitude below (l is subnormal there; the matrix
-//           instruction takes subnormals).  A product of two such values is the sum of three, hh + hl + lh; the dropped ll is
-//           at most 2^-24 and 1e-8 on average of it, a sixth of single precision's own rounding.  Three half-precision
-//           matrix instructions do what the six of a split into three bfloat16 do, which needs no scale.
+//           largest magnitude of what shares it into [2^14, 2^15).  h + l is v to 2^-23 of itself down to 2^-16 of that magnitude, and to
+//           2^-39 of that magnitude below (l is subnormal there; the matrix instruction takes subnormals): a bit is lost per power of
+//           two.  A product of two such values is the sum of three, hh + hl + lh; the dropped ll is at most 2^-22 of it.
+//           All told a product is off by 2^-21 of itself at most and 7e-8 in the mean square (a single-precision multiplication: 2^-24 and
+//           2.5e-8); sums are in single precision.  Three half-precision matrix instructions do what the six of a split into three
+//           bfloat16 do, which needs no scale.
 //           Of each 32 values of a row first the 32 h, then the 32 l: one row of a stage is 128 bytes in either type.
 //
 // One workgroup makes a BM x BN tile of D, a wavefront 32 TM x 32 TN of it by v_mfma_f32_32x32x16 with the operands exchanged, so that
@@ -257,17 +258,10 @@ __device__ __forceinline__ void product_tile(const Operand& A, const Operand& B,
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// The power of two s that puts a magnitude (its bits) into [2^14, 2^15), and 1 / s.  1 for zero and what is not finite.
-__device__ __forceinline__ float pair_scale(unsigned bits) {
-  const int e = (int)(bits >> 23 & 255);
-  if (bits == 0 || e == 255) return 1.f;
-  return __builtin_bit_cast(float, (unsigned)(127 + min(126, 14 - (e - 127))) << 23);
-}
-__device__ __forceinline__ float pair_unscale(unsigned bits) {
-  const int e = (int)(bits >> 23 & 255);
-  if (bits == 0 || e == 255) return 1.f;
-  return __builtin_bit_cast(float, (unsigned)(127 - min(126, 14 - (e - 127))) << 23);
-}
+// The exponent of a magnitude (its bits): 2^e <= magnitude < 2^(e + 1), subnormal ones included; -1 for zero and what is not finite.  A
+// value as pairs is brought up by kPairExponent - e.
+constexpr int kPairExponent = 14;
+__device__ __forceinline__ int exponent_of(unsigned bits) { return __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, bits)) - 1; }
 // v (already scaled) as its two halves, in the bits of an unsigned: h below, l above
 __device__ __forceinline__ unsigned split_pair(float v) {
   const _Float16 h = (_Float16)v;
