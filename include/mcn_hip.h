@@ -533,8 +533,12 @@ MCN_API int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput
    and small images lose nothing.  Within an image's features, or a filter, what is below 2^-16 of the largest is held to 2^-39 of that:
    scores lose where so small features meet filter values as much larger than their filter's others, derInput where a feature's value is
    so small in all filters.
+   P is the exponential of a score minus its log sum, off by some 2^-23 of their size, relative to itself.
    bfloat16: products of the bfloat16 values in single precision; P is rounded to bfloat16, and so are, for derFilters, the features times
    their image's weight.
+   What it costs against the two calls one after the other: in bfloat16 it reads the filters as they are; in single precision it splits
+   them first (three times their bytes), so over a bank too large for the caches a few images are faster by the two calls (128000 x 4096:
+   up to 64 images), and up to some 250 images over 1000 classes are as fast either way.
    workspace: mcn_fcloss_workspace_bytes(g, 0 forward / 1 backward). */
 typedef struct mcn_fcloss_geom {
   int D, K, N;
@@ -553,8 +557,10 @@ MCN_API int mcn_fcloss_backward(mcn_stream_t stream, const mcn_fcloss_geom* g, v
 /* `count` matrices of K x D single-precision values (filter banks: K filters of D = FH*FW*FC values each, as they lie in memory), one behind
    the other: each is divided by its Frobenius norm and taken `steps` times (5 is usual) through
      X <- a X + b (X X') X + c (X X')^2 X,  a = 3.4445, b = -4.7750, c = 2.0315,
-   which brings its singular values close to 1 (within [0.68, 1.21] for those above 1/200 of the norm).  The zero matrix stays zero.
-   Products on pairs of half-precision values, as exact as single-precision ones.  y does not overlap x. */
+   (coefficients: K. Jordan et al., "Muon: an optimizer for hidden layers in neural networks", 2024) which brings its singular values close
+   to 1 (within [0.68, 1.21] for those above 1/200 of the norm).  The zero matrix stays zero.  Products on pairs of half-precision values
+   (see above) at one scale: entries are held to 2^-23 of themselves or 2^-39 of the norm, whichever is more, so rows far smaller than the
+   matrix keep fewer digits.  y does not overlap x. */
 MCN_API size_t mcn_orthogonalise_workspace_bytes(int K, int D, int count);
 MCN_API int mcn_orthogonalise(mcn_stream_t stream, float* y, const float* x, int K, int D, int count, int steps, void* workspace,
                               size_t workspaceBytes);

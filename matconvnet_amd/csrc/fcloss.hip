@@ -350,7 +350,9 @@ struct Scores {
 template <class S>
 __device__ __forceinline__ bool has_column(int c) { return c >= 0 && c < 32 * S::TN && (c & 4) == 0; }
 
-// Forward: (largest score, sum of exponentials against it) per instance and tile, the score of the instance's class
+// Forward: (largest score, sum of exponentials against it) per instance and tile, the score of the instance's class.  (__expf, here and
+// for P, is off by 2^-24 of its argument's size, relative to its value; the roundings of the score and the log sum, whose difference
+// the argument is, make as much of it.)
 struct StatsEnd {
   Scores z;
   float2* parts;                   // [N][tiles]
@@ -789,7 +791,7 @@ struct Plan {
   unsigned pack_groups(long long rows, long long packs) const { return (unsigned)((rows * packs + 256 * kPackSteps - 1) / (256 * kPackSteps)); }
 };
 
-// A piece's P, or packed filters: larger ones save passes over the sums of dzdx (128, 256, 512 MiB: 29.5, 29.5, 29.2 ms for 128000 classes in
+// A piece's P (single precision: each of its two), or packed filters: larger ones save passes over the sums of dzdx (128, 256, 512 MiB: 29.5, 29.5, 29.2 ms for 128000 classes in
 // bfloat16, 1.76, 1.72, 1.72 ms for 32000 in single precision)
 size_t piece_bytes() {
   const int kib = tunable("fcloss_piece_kib", 0);

@@ -1,10 +1,11 @@
 // Orthogonalised updates: a matrix G of K filters x D values is replaced by (nearly) the closest one with orthonormal rows or columns, U V'
 // of its singular value decomposition U S V', by matrix products alone:
 //   X = G/|G|,  five times (or as asked)  X <- a X + (b A + c A^2) X,  A = X X'      (A = X'X and products from the right if K > D)
-// Every singular value s goes through p(s) = a s + b s^3 + c s^5; with a = 3.4445, b = -4.7750, c = 2.0315 values from 0.005 on end within
-// [0.68, 1.21] after five steps, and none ever passes 1.22.  So X, A and B (its eigenvalues lie in [0.6, 3.4445]) stay below 3.5 in magnitude,
+// Every singular value s goes through p(s) = a s + b s^3 + c s^5; with a = 3.4445, b = -4.7750, c = 2.0315 (K. Jordan et al., "Muon: an
+// optimizer for hidden layers in neural networks", 2024) values from 0.005 on end within [0.68, 1.21] after five steps, and none ever
+// passes 1.22.  So X, A and B (its eigenvalues lie in [0.6, 3.4445]) stay below 3.5 in magnitude,
 // and the operands of the products are pairs of half-precision values (product.hpp) at a scale that is always the same, 2^14
-// (3.4445 * 2^14 < 65504).
+// (3.4445 * 2^14 < 65504): an entry of X is held to 2^-23 of itself or, below 2^-16, to 2^-39.
 // A step is three products, in three launches or two (ClosingEnd), for small matrices all steps in one (ortho_narrow): A and A^2 are symmetric, of them only the tiles on and below the diagonal are made and written twice;
 // 3 m^2 n + m^3 operations for an m x n matrix, m <= n.  All of a call's matrices (of one size) go through one launch per product.
 #include "product.hpp"
