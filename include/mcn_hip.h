@@ -534,8 +534,8 @@ MCN_API int mcn_lnorm_backward(mcn_stream_t stream, int dataType, void* derInput
    scores lose where so small features meet filter values as much larger than their filter's others, derInput where a feature's value is
    so small in all filters.
    P is the exponential of a score minus its log sum, off by some 2^-23 of their size, relative to itself.
-   bfloat16: products of the bfloat16 values in single precision; P is rounded to bfloat16, and so are, for derFilters, the features times
-   their image's weight.
+   bfloat16: products of the bfloat16 values in single precision; P is rounded to bfloat16.  With instanceWeights derFilters takes
+   twice the products: the features times them are held as two bfloat16 values.
    What it costs against the two calls one after the other: in bfloat16 it reads the filters as they are; in single precision it splits
    them first (three times their bytes), so over a bank too large for the caches a few images are faster by the two calls (128000 x 4096:
    up to 64 images), and up to some 250 images over 1000 classes are as fast either way.

@@ -152,10 +152,11 @@ __global__ __launch_bounds__(1024) void fc_feature_magnitudes(unsigned* __restri
   raise(out + (size_t)blockIdx.x * 512 + t, m);
 }
 
-// bfloat16: rows at a pitch of whole stages, as they are or times the instance's weight (zeros for instances that do not count, whatever
-// they hold).  (The weighted features are rounded, for dzdf alone.  Weights in P would round what both derivatives are made of by as much:
-// without them the label's -1, most of P, is exact.)
-enum { kAsTheyAre, kWeighted };
+// bfloat16: rows at a pitch of whole stages: all of them; those of instances that count (zeros for the others, whatever they hold); or these
+// times the instances' weights, which as one bfloat16 value would round dzdf a third time, behind P and before the result, so as two, of each 64
+// rows (up to the next multiple: zeros) first the values, then what they miss.  (Weights in P would be rounded with it: without them the
+// label's -1, most of P, is exact.)
+enum { kAll, kCounting, kWeighted };
 struct PackPart {
   const unsigned short* x;
   unsigned short* out;
@@ -165,7 +166,7 @@ struct PackPart {
 };
 struct PackJob {
   PackPart parts[3];
-  int nParts, D;
+  int nParts, D, N;
   const float *labels, *weights;
   int nWeights;
   unsigned* clear;                         // counters, cleared on the way
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(256) void fc_pack(PackJob j) {
     const bool live = i < all;
     row[step] = live ? (int)(i / per) : -1;
     c[step] = live ? (int)(i - (size_t)row[step] * per) * 8 : 0;
-    w[step] = !live ? 0.f : p.form == kWeighted ? instance_weight(j.labels, j.weights, j.nWeights, row[step]) : 1.f;
+    w[step] = !live ? 0.f : p.form == kAll ? 1.f : row[step] < j.N ? instance_weight(j.labels, j.weights, j.nWeights, row[step]) : 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[step][k] = 0.f;
     if (w[step] != 0.f) load8(v[step], p.x + (size_t)row[step] * j.D, c[step], j.D);
@@ -196,10 +197,18 @@ __global__ __launch_bounds__(256) void fc_pack(PackJob j) {
 #pragma unroll
   for (int step = 0; step < kPackSteps; ++step) {
     if (row[step] < 0) return;
-    uintx4p h;
+    const float by = p.form == kWeighted ? w[step] : 1.f;
+    const size_t out = p.form == kWeighted ? (size_t)(row[step] / 64) * 128 + row[step] % 64 : (size_t)row[step];
+    uintx4p h, l;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = (unsigned)to_bf16(v[step][2 * k] * w[step]) | (unsigned)to_bf16(v[step][2 * k + 1] * w[step]) << 16;
-    *(uintx4p*)(p.out + (size_t)row[step] * p.pitch + c[step]) = h;
+    for (int k = 0; k < 4; ++k) {
+      const float u[2] = {v[step][2 * k] * by, v[step][2 * k + 1] * by};
+      const unsigned short a = to_bf16(u[0]), b = to_bf16(u[1]);
+      h[k] = (unsigned)a | (unsigned)b << 16;
+      l[k] = (unsigned)to_bf16(u[0] - from_bf16(a)) | (unsigned)to_bf16(u[1] - from_bf16(b)) << 16;
+    }
+    *(uintx4p*)(p.out + out * p.pitch + c[step]) = h;
+    if (p.form == kWeighted) *(uintx4p*)(p.out + (out + 64) * p.pitch + c[step]) = l;
   }
 }
 
@@ -783,6 +792,8 @@ struct Plan {
   long long xPitch, fPitch, pPitch;
   int piece, pieces, tiles;        // classes per piece; tiles of scores over all classes
   ProductPlan scores, dx, df;      // of a whole piece; the last one, if smaller, is cut as they are
+  ProductPlan dfWeighted;          // bfloat16: over weighted features in two parts
+  long long weightedRows;
   size_t x, xExponents, xw, f, fExponents, cleared, parts, own, terms, logSums, p, p2, sum, columns, products, total;
   int nCounters, tileRows;         // (counters: the last is fc_log_sums')
   // words that are cleared before they are used: counters; S_d; and, by piece, R_n and C_k
@@ -820,6 +831,8 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   p.scores = plan_product(p.type, g->N, classes, g->D);
   p.dx = plan_product(p.type, g->N, g->D, classes);
   p.df = plan_product(p.type, classes, g->D, g->N);
+  p.weightedRows = pairs ? 0 : (g->N + 63ll) / 64 * 128;
+  p.dfWeighted = pairs ? p.df : plan_product(p.type, classes, g->D, p.weightedRows);
   p.tiles = div_up(g->K, kTileSize[p.scores.tile]);
   p.pPitch = row_halves(p.type, std::min<long long>(p.piece, (g->K + 63) / 64 * 64));
   size_t at = 0;
@@ -830,7 +843,7 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   };
   const auto whole_tiles = [](size_t n) { return (n + 255) / 256 * 256; };
   p.tileRows = div_up(g->N, kTileSize[p.scores.tile]);
-  p.nCounters = 1 + (int)(backward ? std::max({p.scores.counters(), p.dx.counters(), p.df.counters()}) : p.scores.counters());
+  p.nCounters = 1 + (int)(backward ? std::max({p.scores.counters(), p.dx.counters(), p.df.counters(), p.dfWeighted.counters()}) : p.scores.counters());
   p.featureMost = whole_tiles((size_t)p.nCounters);
   p.instanceMost = p.featureMost + (pairs && backward ? whole_tiles((size_t)g->D) : 0);
   p.classMost = p.instanceMost + (pairs && backward ? whole_tiles((size_t)g->N) : 0);
@@ -838,7 +851,7 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   p.cleared = take(4 * p.words);
   p.xExponents = take(pairs ? (size_t)g->N * 4 : 0);
   p.fExponents = take(pairs ? whole_tiles((size_t)g->K) * 4 : 0);
-  p.products = take(backward ? std::max({p.scores.partBytes(), p.dx.partBytes(), p.df.partBytes()}) : p.scores.partBytes());
+  p.products = take(backward ? std::max({p.scores.partBytes(), p.dx.partBytes(), p.df.partBytes(), p.dfWeighted.partBytes()}) : p.scores.partBytes());
   p.x = take(p.xInPlace ? 0 : (size_t)g->N * p.xPitch * 2);
   p.f = take(p.fInPlace ? 0 : (size_t)std::min(p.piece, g->K) * p.fPitch * 2);
   p.parts = take((size_t)g->N * p.tiles * 8);
@@ -847,7 +860,7 @@ Plan make_plan(const mcn_fcloss_geom* g, const void* x, const void* f, bool back
   p.logSums = take((size_t)g->N * 4);
   p.xw = p.p = p.p2 = p.sum = p.columns = 0;
   if (backward) {
-    p.xw = take((size_t)g->N * p.xPitch * 2);
+    p.xw = take((size_t)(pairs ? g->N : p.weightedRows) * p.xPitch * 2);
     p.columns = take(p.tileRows > 1 ? (size_t)p.tileRows * g->K * 4 : 0);
     p.p = take((size_t)g->N * p.pPitch * 2);
     p.p2 = take(pairs ? (size_t)g->N * p.pPitch * 2 : 0);
@@ -889,9 +902,10 @@ struct Call {
   Matrix F(int piece) const { return {p.fInPlace ? piece_of(filters, piece * p.piece) : ws + p.f, p.fPitch, 0, classes(piece)}; }
 };
 
-// The filters of a piece and, before the first (`all`), the features (bfloat16: for dzdf the weighted ones too), where the products read them;
+// The filters of a piece and, before the first (`all`), the features, where the products read them (`derived`: in bfloat16 for dzdf too, without
+// weights the same where they have to be copied, what the scores of the others are made of being no matter behind the forward call);
 // the words that the piece's products count and take maxima in are cleared, all of them before the first.
-void pack(const Call& c, int piece, bool all, bool weighted) {
+void pack(const Call& c, int piece, bool all, bool derived) {
   const Plan& p = c.p;
   const int D = c.g->D, N = c.g->N;
   unsigned groups = 0;
@@ -921,15 +935,16 @@ void pack(const Call& c, int piece, bool all, bool weighted) {
     return;
   }
   PackJob j = {};
-  j.D = D;
+  j.D = D; j.N = N;
   j.labels = c.labels; j.weights = c.weights; j.nWeights = c.nWeights;
   j.clear = clear; j.nClear = nClear;
   const auto rows = [&](const void* x, size_t out, long long pitch, int n, int form) {
     j.parts[j.nParts++] = {(const unsigned short*)x, (unsigned short*)(c.ws + out), pitch, n, form, at(p.pack_groups(n, pitch / 8))};
   };
-  if (!p.fInPlace) rows(c.piece_of(c.filters, piece * p.piece), p.f, p.fPitch, c.classes(piece), kAsTheyAre);
-  if (all && !p.xInPlace) rows(c.x, p.x, p.xPitch, N, kAsTheyAre);
-  if (all && weighted) rows(c.x, p.xw, p.xPitch, N, kWeighted);
+  if (!p.fInPlace) rows(c.piece_of(c.filters, piece * p.piece), p.f, p.fPitch, c.classes(piece), kAll);
+  if (all && !p.xInPlace) rows(c.x, p.x, p.xPitch, N, derived && !c.weights ? kCounting : kAll);
+  if (all && derived && c.weights) rows(c.x, p.xw, p.xPitch, (int)(p.weightedRows / 2), kWeighted);
+  else if (all && derived && p.xInPlace) rows(c.x, p.xw, p.xPitch, N, kCounting);
   if (groups == 0) {
     if (nClear == 0) return;       // (filters in place)
     groups = 1;                    // (the counters alone)
@@ -1016,7 +1031,8 @@ int backward(const Call& c, void* derInput, void* derFilters, float* derBiases, 
   const Plan& p = c.p;
   const int N = c.g->N, D = c.g->D;
   const bool pairs = TYPE == kPairs;
-  const Matrix Xw = {c.ws + p.xw, p.xPitch, 0, N};
+  const bool weighted = !pairs && c.weights;
+  const Matrix Xf = weighted ? Matrix{c.ws + p.xw, p.xPitch, 0, p.weightedRows} : Matrix{c.ws + (pairs || p.xInPlace ? p.xw : p.x), p.xPitch, 0, N};
   if (pairs && derFilters) {
     const int columns = div_up(D, 512), rows = std::max(1, div_up((long long)N * columns, 16 * 512));   // (some 512 workgroups)
     KernelTimer timer("fc_feature_magnitudes", c.s);
@@ -1054,7 +1070,11 @@ int backward(const Call& c, void* derInput, void* derFilters, float* derBiases, 
     if (derFilters) {
       const StoreEnd d = {(void*)c.piece_of(derFilters, first), !pairs, nullptr, count, D, factor, c.words(p.classMost), c.words(p.featureMost), nullptr, nullptr, 1};
       const Matrix Pf = {c.ws + (pairs && derInput ? p.p2 : p.p), p.pPitch, 0, N};
-      rc = product<TYPE, true, true>(c.s, c.who, "fc_derivative_f", Pf, Xw, count, D, p.df.of(count, D), c.scratch(), d);
+      if constexpr (TYPE == kBf16)
+        rc = weighted ? product<TYPE, true, true, 2>(c.s, c.who, "fc_derivative_f", Pf, Xf, count, D, p.dfWeighted.of(count, D), c.scratch(), d)
+                      : product<TYPE, true, true>(c.s, c.who, "fc_derivative_f", Pf, Xf, count, D, p.df.of(count, D), c.scratch(), d);
+      else
+        rc = product<TYPE, true, true>(c.s, c.who, "fc_derivative_f", Pf, Xf, count, D, p.df.of(count, D), c.scratch(), d);
       if (rc) return rc;
     }
   }

@@ -108,8 +108,10 @@ __device__ __forceinline__ floatx16p multiply(uintx4p a, uintx4p b, floatx16p c)
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfx8, a), __builtin_bit_cast(bfx8, b), c, 0, 0, 0);
 }
 
-// One operand's loads.  A workgroup's wavefront w brings chunks [64 (w + i W), + 64) of a stage for every i.
-template <class S, bool ACROSS, int R>
+// One operand's loads.  A workgroup's wavefront w brings chunks [64 (w + i W), + 64) of a stage for every i.  REPEAT: how many stages of the
+// product each stage of the operand serves, one behind the other (against another operand whose values stand in two parts, a stage of the first
+// part and one of the second in turn).
+template <class S, bool ACROSS, int R, int REPEAT>
 struct Loader {
   typedef Stage<S::type, ACROSS, R> St;
   static constexpr int loads = St::chunks / S::threads;
@@ -118,11 +120,14 @@ struct Loader {
   const char* base;
   unsigned long long left;   // bytes from base to the end of the operand
   unsigned long long step;
+  int turn;                  // how often the stage that is due has been brought
   int more;                  // stages to come: the loads behind the last one go out all the same (their number is what is waited for) and
                              // find nothing
 
-  // first: first row (ALONG) or first value of m (ACROSS) of the tile; stage0: first stage
-  __device__ __forceinline__ void begin(const Operand& o, long long first, long long stage0, int stages, int tid) {
+  // first: first row (ALONG) or first value of m (ACROSS) of the tile; productStage: the product's first stage
+  __device__ __forceinline__ void begin(const Operand& o, long long first, long long productStage, int stages, int tid) {
+    const long long stage0 = productStage / REPEAT;
+    turn = (int)(productStage % REPEAT);
 #pragma unroll
     for (int i = 0; i < loads; ++i) {
       int row, chunk;
@@ -145,6 +150,8 @@ struct Loader {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (i * S::threads + wave * 64) * 16), 16, (int)offset[i], 0, 0, 0);
     if (i == loads - 1) {
       --more;
+      if (REPEAT > 1 && ++turn < REPEAT) return;
+      turn = 0;
       base += step;
       left = left > step ? left - step : 0;
     }
@@ -225,7 +232,7 @@ __device__ __forceinline__ void product_stage(const char* __restrict__ from, con
 
 // acc[i][j][r]: row m0 + 32 (wm TM + i) + lane % 32, column n0 + 32 (wn TN + j) + 8 (r / 4) + 4 (lane / 32) + r % 4.
 // lds: S::ldsBytes, free again behind the last barrier.
-template <class S, bool A_ACROSS, bool B_ACROSS>
+template <class S, bool A_ACROSS, bool B_ACROSS, int A_REPEAT>
 __device__ __forceinline__ void product_tile(const Operand& A, const Operand& B, long long m0, long long n0, long long stage0, int stages, char* lds,
                                              floatx16p (&acc)[S::TM][S::TN]) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -236,8 +243,8 @@ __device__ __forceinline__ void product_tile(const Operand& A, const Operand& B,
     for (int j = 0; j < S::TN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  Loader<S, A_ACROSS, S::BM> la;
-  Loader<S, B_ACROSS, S::BN> lb;
+  Loader<S, A_ACROSS, S::BM, A_REPEAT> la;
+  Loader<S, B_ACROSS, S::BN, 1> lb;
   la.begin(A, m0, stage0, stages, tid);
   lb.begin(B, n0, stage0, stages, tid);
 #pragma unroll
@@ -434,7 +441,7 @@ struct TileGrid {
 constexpr int kTileRows = 4;
 
 // What to do with a finished tile is E's: e.finish<S>(acc, tile row, tile column, which product, lane, wavefront along m, along n, LDS).
-template <class S, bool A_ACROSS, bool B_ACROSS, class E>
+template <class S, bool A_ACROSS, bool B_ACROSS, int A_REPEAT, class E>
 __global__ __launch_bounds__(S::threads, 2) void product_kernel(Matrix A, Matrix B, TileGrid g, int stages, Slices j, E e) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const bool whole = (int)blockIdx.x < j.full;
@@ -457,7 +464,7 @@ __global__ __launch_bounds__(S::threads, 2) void product_kernel(Matrix A, Matrix
   }
   const int s0 = slice * j.perSlice, mine = whole ? stages : max(0, min(j.perSlice, stages - s0));
   floatx16p acc[S::TM][S::TN];
-  product_tile<S, A_ACROSS, B_ACROSS>(A.of(which), B.of(which), (long long)tm * S::BM, (long long)tn * S::BN, s0, mine, lds, acc);
+  product_tile<S, A_ACROSS, B_ACROSS, A_REPEAT>(A.of(which), B.of(which), (long long)tm * S::BM, (long long)tn * S::BN, s0, mine, lds, acc);
   if (!whole && !join_slices<S>(j, cut, slice, acc, lds)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   e.template finish<S>(acc, tm, tn, which, lane, wave % S::WM, wave / S::WM, lds);
@@ -556,12 +563,12 @@ struct Scratch {
   unsigned* counters;
 };
 
-template <class S, bool A_ACROSS, bool B_ACROSS, class E>
+template <class S, bool A_ACROSS, bool B_ACROSS, int A_REPEAT = 1, class E>
 int run_product(hipStream_t s, const char* who, const char* name, const Matrix& A, const Matrix& B, long long M, long long N, int count, bool triangle,
                 const ProductPlan& p, const Scratch& scratch, const E& e) {
   if (p.groups() >= (1ll << 32) / S::threads) return fail(MCN_UNSUPPORTED, "%s: tensor too large", who);
   const TileGrid g = {div_up(M, S::BM), div_up(N, S::BN), count, triangle};
-  const auto kernel = product_kernel<S, A_ACROSS, B_ACROSS, E>;
+  const auto kernel = product_kernel<S, A_ACROSS, B_ACROSS, A_REPEAT, E>;
   static std::atomic<unsigned long long> raised;
   const int rc = allow_lds(who, (const void*)kernel, S::ldsBytes, raised);
   if (rc) return rc;
@@ -578,13 +585,13 @@ template <int TYPE> using Tile128 = ProductShape<TYPE, 128, 128, 2, 2, 2>;
 template <int TYPE> using Tile128Alone = ProductShape<TYPE, 128, 128, 4, 2, 4>;
 template <int TYPE> using Tile64 = ProductShape<TYPE, 64, 64, 2, 2, 4>;
 
-template <int TYPE, bool A_ACROSS, bool B_ACROSS, class E>
+template <int TYPE, bool A_ACROSS, bool B_ACROSS, int A_REPEAT = 1, class E>
 int product(hipStream_t s, const char* who, const char* name, const Matrix& A, const Matrix& B, long long M, long long N, const ProductPlan& p,
             const Scratch& scratch, const E& e, int count = 1, bool triangle = false) {
-  if (p.tile == kTile256) return run_product<Tile256<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-  if (p.tile == kTile64) return run_product<Tile64<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-  if (p.alone()) return run_product<Tile128Alone<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
-  return run_product<Tile128<TYPE>, A_ACROSS, B_ACROSS>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+  if (p.tile == kTile256) return run_product<Tile256<TYPE>, A_ACROSS, B_ACROSS, A_REPEAT>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+  if (p.tile == kTile64) return run_product<Tile64<TYPE>, A_ACROSS, B_ACROSS, A_REPEAT>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+  if (p.alone()) return run_product<Tile128Alone<TYPE>, A_ACROSS, B_ACROSS, A_REPEAT>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
+  return run_product<Tile128<TYPE>, A_ACROSS, B_ACROSS, A_REPEAT>(s, who, name, A, B, M, N, count, triangle, p, scratch, e);
 }
 
 }  // namespace mcn

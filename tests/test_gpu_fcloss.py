@@ -365,3 +365,25 @@ def test_cuts_and_tiles_that_there_are_not(capi, dtype, name, value):
         check(capi, *make(60, 70, 3000, dtype, 17))
     finally:
         capi.set_tunable(name, 0)
+
+
+@pytest.mark.parametrize("D,K,N", [(64, 64, 1), (65, 130, 2), (130, 10, 3), (192, 300, 1)])
+@pytest.mark.parametrize("normalise", [True, False])
+def test_weights_round_nothing_twice(capi, D, K, N, normalise):
+    """bfloat16 with weights: dzdf has one rounding of P to bfloat16 and one of its own: 2^-8 each.  (Want allows it a third, of the weighted
+    features, which are held to 2^-16.)"""
+    x, f, b, c, w = make(D, K, N, torch.bfloat16, 18, skipped=False)
+    want = Want(x, f, b, c, w, 0.7, normalise)
+    y, lse = capi.fcloss_forward(x, f, b, c, instance_weights=w, normalise=normalise)
+    xd, fd = x.double().reshape(N, D), f.double().reshape(K, D)
+    z = xd @ fd.t() + b.double()
+    p = torch.softmax(z, dim=1)
+    p[torch.arange(N, device="cuda"), (c - 1).long()] -= 1.0
+    wp = w.double()[:, None] * p * (0.7 / (N if normalise else 1))
+    # (P's own error in single precision, scores and log sums: less than 2^-14 of it here, where scores are at most 16 = 2^4: 2^4 x 64 u)
+    off = (2.0 ** -8 + 2.0 ** -14 + 2.0 ** -16 + (N + 16) * U) * (wp.abs().t() @ xd.abs())
+    for log_sums in (lse, None):
+        for parts in ((True, True, True), (False, True, False)):
+            df = capi.fcloss_backward(x, f, b, c, 0.7, instance_weights=w, normalise=normalise, log_sums=log_sums, want=parts)[1]
+            near(df, want.df, off + (2.0 ** -8) * (want.df.abs() + off), "dzdf")
+    assert float(z.abs().max()) <= 16
