@@ -416,7 +416,8 @@ struct StatsEnd {
 };
 
 // One of two registers goes to the lane h away, the other stays.  (The empty assembly keeps the two apart: from a choice between two entries of
-// an array the compiler makes an index, and of that a comparison with every entry, 22 us for a tile of 256 x 256.)
+// an array the compiler makes an index, and of that a comparison with every entry: P's kernel took 588 us for 32000 classes, 500 so, and 92 for
+// 21841 in bfloat16, 72 so.)
 __device__ __forceinline__ void choose(bool upper, float& give, float& keep) {
   float a = give, b = keep;
   asm("" : "+v"(a), "+v"(b));
