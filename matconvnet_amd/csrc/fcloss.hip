@@ -29,12 +29,6 @@ __device__ __forceinline__ float instance_weight(const float* labels, const floa
 }
 __device__ __forceinline__ int class_of(float label, int K) { return label >= 1.f ? min((int)fminf(label, 2147483520.f) - 1, K - 1) : 0; }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));
-  return v;
-}
-
 // ---------------------------------------------------------------------------------------------- operands
 
 __device__ __forceinline__ unsigned wave_most(unsigned m, int lanes) {   // over groups of `lanes` neighbours
@@ -803,8 +797,8 @@ struct Plan {
   unsigned pack_groups(long long rows, long long packs) const { return (unsigned)((rows * packs + 256 * kPackSteps - 1) / (256 * kPackSteps)); }
 };
 
-// A piece's P (single precision: each of its two), or packed filters: larger ones save passes over the sums of dzdx (128, 256, 512 MiB: 29.5, 29.5, 29.2 ms for 128000 classes in
-// bfloat16, 1.76, 1.72, 1.72 ms for 32000 in single precision)
+// A piece's P (single precision: each of its two), or packed filters: larger ones save passes over the sums of dzdx (128, 256, 512 MiB: 29.5,
+// 29.5, 29.2 ms for 128000 classes in bfloat16; in single precision, before P was split in a pass of its own, 1.76, 1.72, 1.72 ms for 32000)
 size_t piece_bytes() {
   const int kib = tunable("fcloss_piece_kib", 0);
   return kib > 0 ? (size_t)kib << 10 : (size_t)256 << 20;
@@ -903,9 +897,10 @@ struct Call {
   Matrix F(int piece) const { return {p.fInPlace ? piece_of(filters, piece * p.piece) : ws + p.f, p.fPitch, 0, classes(piece)}; }
 };
 
-// The filters of a piece and, before the first (`all`), the features, where the products read them (`derived`: in bfloat16 for dzdf too, without
-// weights the same where they have to be copied, what the scores of the others are made of being no matter behind the forward call);
-// the words that the piece's products count and take maxima in are cleared, all of them before the first.
+// The filters of a piece and, before the first (`all`), the features, where the products read them; the words that the piece's products count and
+// take maxima in are cleared, all of them before the first.  `derived`: bfloat16 features for dzdf too; without weights, where they are
+// copied anyway, one copy serves both (behind the forward call it does not matter what the scores of instances that do not count are
+// made of).
 void pack(const Call& c, int piece, bool all, bool derived) {
   const Plan& p = c.p;
   const int D = c.g->D, N = c.g->N;
