@@ -566,6 +566,96 @@ MCN_API int mcn_orthogonalise(mcn_stream_t stream, float* y, const float* x, int
                               size_t workspaceBytes);
 
 /* ------------------------------------------------------------------------------------------------
+ * operators with no counterpart in the reference, for training models in which positions see one another: heads normalised and rotated,
+ * attention over packed sequences, clipped gradients.  What is said above about data types, alignment and workspaces holds
+ * for them; workspaces are 16-byte aligned.  A position's channels are `heads` heads of D.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* Heads where they lie: channel d of head h at position n is data[n*position + h*head + d] (strides in values, not negative).  What
+   a call writes must not overlap itself; what it reads may (a stride of 0). */
+typedef struct mcn_heads {
+  void* data;
+  long long position, head;
+} mcn_heads;
+
+/* Normalisation of every head of queries and keys, and rotation by the position:
+     normalise != 0: u = multipliers .* x / sqrt(mean of the D squares + epsilon), else u = x
+     the two channels of pair j turn by angle_j = sum over the axes of positions[n][axis] * frequencies[axis][j]:
+       y_lo = u_lo cos - u_hi sin, y_hi = u_hi cos + u_lo sin
+   pair j is channels j and pairs + j, or with neighbours != 0 channels 2j and 2j + 1; channels from 2*pairs on are not turned, pairs = 0
+   turns none.  positions (N x axes, an image's row and column, a video's time, row and column...) and frequencies (axes x pairs: 0
+   where an axis does not turn a pair) are doubles on the device: angles are made in double.  multipliers (NULL: ones) are D single-precision
+   values for the queries, D for the keys.  D at most 512.  Either set may have no heads.  yq may be q, yk may be k.
+   backward: derQ, derK (NULL or of null data: not made) may be derOutputQ, derOutputK; derMultipliers (with normalise only; NULL: not
+   made) are fully overwritten, their sums taken in one order for one shape on one kind of device; without normalise q and k
+   are not read. */
+typedef struct mcn_hnorm_geom {
+  int D, heads, keyHeads, N;
+  int pairs, axes;
+  int neighbours, normalise;
+  int dataType;     /* of q, k, yq, yk and their derivatives */
+  double epsilon;
+} mcn_hnorm_geom;
+MCN_API int mcn_hnorm_forward(mcn_stream_t stream, const mcn_hnorm_geom* g, const mcn_heads* yq, const mcn_heads* yk, const mcn_heads* q,
+                              const mcn_heads* k, const float* multipliersQ, const float* multipliersK, const double* positions,
+                              const double* frequencies);
+MCN_API size_t mcn_hnorm_workspace_bytes(const mcn_hnorm_geom* g); /* of the backward call */
+MCN_API int mcn_hnorm_backward(mcn_stream_t stream, const mcn_hnorm_geom* g, const mcn_heads* derQ, const mcn_heads* derK,
+                               float* derMultipliersQ, float* derMultipliersK, const mcn_heads* q, const mcn_heads* k,
+                               const float* multipliersQ, const float* multipliersK, const double* positions, const double* frequencies,
+                               const mcn_heads* derOutputQ, const mcn_heads* derOutputK, void* workspace, size_t workspaceBytes);
+
+/* Attention of the positions of packed sequences: for every query i of a sequence and the keys j of the same sequence that it sees,
+     s_ij = scale * q_i . k_j,  logSums_i = log sum_j exp s_ij,  o_i = sum_j exp(s_ij - logSums_i) v_j
+   heads is a multiple of keyHeads: query head h goes with key head h / (heads / keyHeads).  Sequences lie one behind the other: sequence
+   i has the queries [queryStarts[i], queryStarts[i + 1]) of N and the keys [keyStarts[i], keyStarts[i + 1]) of M (device arrays of
+   sequences + 1 ascending numbers, both or neither; NULL: sequences of N / sequences queries and M / sequences keys each).  Either part may be
+   empty; starts outside of 0..N or 0..M are taken as the nearest of these.  causal != 0: the queries are the last positions of their
+   sequence, query i of n sees key j of m where j <= i + m - n.  A query that sees no key has o = 0, logSums = -infinity and gives no
+   derivative; keys that a query does not see have no part in it, whatever they hold.  Rows of no sequence are left as they were.
+   q, k, v, o and all derivatives are of dataType.  logSums is N x heads, a position's heads side by side.  scale 0: 1/sqrt(D).  D
+   at most 128.
+   backward: all that is asked for (derQ, derK, derV; NULL or of null data: not made) is fully overwritten for all positions of sequences; o and logSums
+   as the forward call left them.  Derivatives of heads that share keys are sums without atomics: the same bits every time.
+   bfloat16: products of the bfloat16 values in single precision; exp(s - logSums) and the scores' derivatives are rounded to bfloat16
+   for the products behind them.  Single precision: products and sums in single precision.
+   workspace: mcn_attention_workspace_bytes(g, 0 forward / 1 backward). */
+typedef struct mcn_attention_geom {
+  int D, heads, keyHeads;
+  int N, M;          /* queries and keys of all sequences */
+  int sequences;
+  int causal;
+  int dataType;
+  double scale;
+} mcn_attention_geom;
+MCN_API size_t mcn_attention_workspace_bytes(const mcn_attention_geom* g, int backward);
+MCN_API int mcn_attention_forward(mcn_stream_t stream, const mcn_attention_geom* g, const mcn_heads* o, float* logSums, const mcn_heads* q,
+                                  const mcn_heads* k, const mcn_heads* v, const int* queryStarts, const int* keyStarts, void* workspace,
+                                  size_t workspaceBytes);
+MCN_API int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, const mcn_heads* derQ, const mcn_heads* derK,
+                                   const mcn_heads* derV, const mcn_heads* o, const float* logSums, const mcn_heads* q, const mcn_heads* k,
+                                   const mcn_heads* v, const mcn_heads* derOutput, const int* queryStarts, const int* keyStarts,
+                                   void* workspace, size_t workspaceBytes);
+
+/* The norm of n gradients together, sqrt(sum of all squares) (device, one value), and the gradients clipped to it:
+     outs[i] = f * ders[i], f = maxNorm/norm where norm > maxNorm, 1 otherwise (also where the norm is no number)
+   ders, outs, counts, dataTypes are HOST arrays (device pointers, numbers of values, MCN_FLOAT or MCN_BFLOAT16 of each), read before
+   the call returns.  outs[i] may be ders[i] (and is not written then where f is 1); otherwise outputs overlap nothing.  norm may be NULL
+   in mcn_clip_gradients.  Squares are summed in double, in one order for one list. */
+MCN_API size_t mcn_clip_workspace_bytes(const size_t* counts, int n);
+MCN_API int mcn_gradient_norm(mcn_stream_t stream, float* norm, const void* const* ders, const size_t* counts, const int* dataTypes, int n,
+                              void* workspace, size_t workspaceBytes);
+MCN_API int mcn_clip_gradients(mcn_stream_t stream, void* const* outs, float* norm, const void* const* ders, const size_t* counts,
+                               const int* dataTypes, int n, double maxNorm, void* workspace, size_t workspaceBytes);
+/* mcn_sgd_momentum with derScale * der clipped as a whole to maxNorm: der is read once for the norm (device, may be NULL) and once by
+   the step, nothing is written in between.  All of the arena counts, parameters that are left alone too. */
+MCN_API size_t mcn_sgd_momentum_clipped_workspace_bytes(size_t chunks);
+MCN_API int mcn_sgd_momentum_clipped(mcn_stream_t stream, float* value, float* state, const float* der, size_t chunks,
+                                     const unsigned short* chunkParam, const double* rates, double learningRate, double weightDecay,
+                                     double momentum, double derScale, int nesterov, double maxNorm, float* norm, void* workspace,
+                                     size_t workspaceBytes);
+
+/* ------------------------------------------------------------------------------------------------
  * double precision -- the operators' VLDT_Double instantiation (bits/impl/dispatcher.hpp:60-98 switches on the
  * tensors' data type; bits/nnconv.cu:444-469, bits/nnbnorm.cu:388-442, bits/nnpooling.cu:270-282 instantiate
  * every product for float and double).  Same arguments and meaning as the single-precision calls above.  Pooling

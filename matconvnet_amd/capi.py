@@ -38,6 +38,18 @@ class FcLossGeom(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("D", "K", "N", "normalise", "dataType")]
 
 
+class Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("position", C.c_longlong), ("head", C.c_longlong)]
+
+
+class HnormGeom(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("D", "heads", "keyHeads", "N", "pairs", "axes", "neighbours", "normalise", "dataType")] + [("epsilon", C.c_double)]
+
+
+class AttentionGeom(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("D", "heads", "keyHeads", "N", "M", "sequences", "causal", "dataType")] + [("scale", C.c_double)]
+
+
 FLOAT, BFLOAT16 = 0, 1   # MCN_FLOAT, MCN_BFLOAT16
 
 LOSSES = ("classerror", "topkerror", "log", "softmaxlog", "mhinge", "mshinge", "binaryerror", "binarylog", "logistic",
@@ -132,6 +144,18 @@ PROTOTYPES = {
     "mcn_fcloss_backward": (_i, [_vp, C.POINTER(FcLossGeom), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _d, _vp, _sz]),
     "mcn_orthogonalise_workspace_bytes": (_sz, [_i, _i, _i]),
     "mcn_orthogonalise": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz]),
+    "mcn_hnorm_forward": (_i, [_vp, C.POINTER(HnormGeom)] + [C.POINTER(Heads)] * 4 + [_vp] * 4),
+    "mcn_hnorm_workspace_bytes": (_sz, [C.POINTER(HnormGeom)]),
+    "mcn_hnorm_backward": (_i, [_vp, C.POINTER(HnormGeom)] + [C.POINTER(Heads)] * 2 + [_vp] * 2 + [C.POINTER(Heads)] * 2 + [_vp] * 4 +
+                           [C.POINTER(Heads)] * 2 + [_vp, _sz]),
+    "mcn_attention_workspace_bytes": (_sz, [C.POINTER(AttentionGeom), _i]),
+    "mcn_attention_forward": (_i, [_vp, C.POINTER(AttentionGeom), C.POINTER(Heads), _vp] + [C.POINTER(Heads)] * 3 + [_vp, _vp, _vp, _sz]),
+    "mcn_attention_backward": (_i, [_vp, C.POINTER(AttentionGeom)] + [C.POINTER(Heads)] * 4 + [_vp] + [C.POINTER(Heads)] * 4 + [_vp, _vp, _vp, _sz]),
+    "mcn_clip_workspace_bytes": (_sz, [_vp, _i]),
+    "mcn_gradient_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _sz]),
+    "mcn_clip_gradients": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _d, _vp, _sz]),
+    "mcn_sgd_momentum_clipped_workspace_bytes": (_sz, [_sz]),
+    "mcn_sgd_momentum_clipped": (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _vp] + [_d] * 4 + [_i, _d, _vp, _vp, _sz]),
     "mcn_conv_forward_f64": (_i, [_vp, C.POINTER(ConvGeom), _vp, _d, _vp, _d, _vp, _vp]),
     "mcn_conv_backward_data_f64": (_i, [_vp, C.POINTER(ConvGeom), _vp, _vp, _vp]),
     "mcn_conv_backward_filter_f64": (_i, [_vp, C.POINTER(ConvGeom), _vp, _vp, _vp]),
@@ -858,6 +882,255 @@ def orthogonalise(x, steps=5, ws=None):
     return y
 
 
+def _heads(name, t, D=None):
+    """mcn_heads of a tensor (positions, heads, D) on the current device whose channels are neighbours; None stays none."""
+    if t is None:
+        return None
+    if t.dim() != 3 or (D is not None and t.shape[2] != D):
+        raise ValueError("%s is not a tensor (positions, heads, D) of the others' D" % name)
+    if not t.is_cuda:
+        raise ValueError("%s is not on the device" % name)
+    if t.get_device() != _torch().cuda.current_device():
+        raise ValueError("%s is on device %d, not on the current one" % (name, t.get_device()))
+    position, head, channel = t.stride()
+    if channel != 1 and t.shape[2] > 1:
+        raise ValueError("the channels of %s are not neighbours" % name)
+    return C.byref(Heads(t.data_ptr(), position, head))
+
+
+def _alike(x):
+    """A fresh contiguous tensor of x's shape and type"""
+    return _torch().empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def axis_frequencies(pairs, axes, base=10000.0):
+    """The usual frequencies of hnorm_forward as a float64 tensor (axes, sum(pairs)) on the device: pair j of all turns by position *
+    base^(-j / sum(pairs)); `pairs` holds how many pairs each axis turns, one run of them behind the other."""
+    torch = _torch()
+    pairs = [int(p) for p in pairs]
+    if len(pairs) != axes or min(pairs) < 0:
+        raise ValueError("pairs does not have one number per axis")
+    n = sum(pairs)
+    table = torch.zeros(axes, n, dtype=torch.float64)
+    f = float(base) ** (-torch.arange(n, dtype=torch.float64) / max(n, 1))
+    at = 0
+    for a, p in enumerate(pairs):
+        table[a, at:at + p] = f[at:at + p]
+        at += p
+    return table.cuda()
+
+
+def _hnorm_geom(q, k, gq, gk, positions, frequencies, epsilon, normalise, neighbours):
+    torch = _torch()
+    if q is None and k is None:
+        raise ValueError("neither queries nor keys")
+    x = q if q is not None else k
+    if x.dim() != 3:
+        raise ValueError("queries or keys are not a tensor (positions, heads, D)")
+    N, D = int(x.shape[0]), int(x.shape[2])
+    if q is not None and k is not None and (k.dim() != 3 or k.shape[0] != N or k.shape[2] != D):
+        raise ValueError("queries and keys do not have the same positions and channels")
+    _single("gq gk", gq, gk)
+    for name, g in (("gq", gq), ("gk", gk)):
+        if g is not None and not normalise:
+            raise ValueError("%s is taken with normalise only" % name)
+        if g is not None and g.numel() != D:
+            raise ValueError("%s does not have one value per channel" % name)
+    pairs = axes = 0
+    if (positions is None) != (frequencies is None):
+        raise ValueError("positions and frequencies are taken together")
+    if positions is not None:
+        _device("positions frequencies", positions, frequencies)
+        if positions.dtype != torch.float64 or frequencies.dtype != torch.float64:
+            raise TypeError("positions or frequencies are not double precision")
+        if frequencies.dim() != 2 or positions.dim() != 2 or positions.shape[0] != N or positions.shape[1] != frequencies.shape[0]:
+            raise ValueError("positions are not (positions, axes) or frequencies are not (axes, pairs)")
+        axes, pairs = int(frequencies.shape[0]), int(frequencies.shape[1])
+    return HnormGeom(D, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], N, pairs, axes, int(bool(neighbours)), int(bool(normalise)),
+                     data_type(q, k), float(epsilon))
+
+
+def _outs(names, out, *like):
+    """The caller's tensors to write, or fresh ones, each of the shape and type of `like`."""
+    if out is None:
+        return [None if x is None else _alike(x) for x in like]
+    out = list(out)
+    if len(out) != len(like):
+        raise ValueError("out does not have one tensor for each of %s" % names)
+    for name, y, x in zip(names.split(), out, like):
+        if y is not None and (x is None or y.shape != x.shape or y.dtype != x.dtype):
+            raise ValueError("%s is not of its input's shape and type" % name)
+    return [y if y is not None or x is None else _alike(x) for y, x in zip(out, like)]
+
+
+def hnorm_forward(q, k, gq=None, gk=None, positions=None, frequencies=None, epsilon=1e-6, normalise=True, neighbours=False, out=None):
+    """Heads of queries and keys normalised and rotated by their positions (include/mcn_hip.h: mcn_hnorm_forward): (yq, yk).  q (N, heads, D),
+    k (N, keyHeads, D): float32 or bfloat16, channels neighbours, any other strides (parts of a projection's output); either may be None.
+    gq, gk: D float32 values or None; positions (N, axes), frequencies (axes, pairs): float64, or both None.  out: the tensors to
+    write, which may be q and k."""
+    g = _hnorm_geom(q, k, gq, gk, positions, frequencies, epsilon, normalise, neighbours)
+    yq, yk = _outs("yq yk", out, q, k)
+    check(lib().mcn_hnorm_forward(stream(), C.byref(g), _heads("yq", yq), _heads("yk", yk), _heads("q", q, g.D), _heads("k", k, g.D), ptr(gq), ptr(gk),
+                                  ptr(positions), ptr(frequencies)))
+    return yq, yk
+
+
+def hnorm_backward(q, k, gq, gk, positions, frequencies, dyq, dyk, epsilon=1e-6, normalise=True, neighbours=False, want=(True, True, True, True),
+                   out=None, ws=None):
+    """(dq, dk, dgq, dgk) of hnorm_forward; those not wanted are None, and so are dgq, dgk without normalise.  out: the tensors dq
+    and dk are written to, which may be dyq and dyk."""
+    g = _hnorm_geom(q, k, gq, gk, positions, frequencies, epsilon, normalise, neighbours)
+    for name, d, x in (("dyq", dyq, q), ("dyk", dyk, k)):
+        if (d is None) != (x is None) or (d is not None and (d.shape != x.shape or d.dtype != x.dtype)):
+            raise ValueError("%s is not of its input's shape and type" % name)
+    if out is None:
+        out = [_alike(x) if w and x is not None else None for w, x in zip(want, (q, k))]
+    else:
+        out = _outs("dq dk", out, q, k)
+    dq, dk = [y if w else None for w, y in zip(want, out)]
+    dgq, dgk = [_singles(x, g.D) if w and normalise and x is not None else None for w, x in zip(want[2:], (q, k))]
+    x = q if q is not None else k
+    wp, wn, held = _scratch(ws, x, lib().mcn_hnorm_workspace_bytes(C.byref(g)) if dgq is not None or dgk is not None else 0)
+    check(lib().mcn_hnorm_backward(stream(), C.byref(g), _heads("dq", dq), _heads("dk", dk), ptr(dgq), ptr(dgk), _heads("q", q, g.D), _heads("k", k, g.D),
+                                   ptr(gq), ptr(gk), ptr(positions), ptr(frequencies), _heads("dyq", dyq), _heads("dyk", dyk), wp, wn))
+    return dq, dk, dgq, dgk
+
+
+def _attention_geom(q, k, v, sequences, q_starts, k_starts, causal, scale):
+    torch = _torch()
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise ValueError("%s is not a tensor (positions, heads, D)" % name)
+    if k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise ValueError("keys and values do not have the same shape, or not the queries' D")
+    if (q_starts is None) != (k_starts is None):
+        raise ValueError("q_starts and k_starts are taken together")
+    if q_starts is not None:
+        _device("q_starts k_starts", q_starts, k_starts)
+        for name, s in (("q_starts", q_starts), ("k_starts", k_starts)):
+            if s.dtype != torch.int32:
+                raise TypeError("%s is not of 32-bit integers" % name)
+        if q_starts.numel() != k_starts.numel() or q_starts.numel() < 1:
+            raise ValueError("q_starts and k_starts do not both have one number per sequence and one more")
+        if sequences not in (None, q_starts.numel() - 1):
+            raise ValueError("the starts are not those of %s sequences" % sequences)
+        sequences = q_starts.numel() - 1
+    else:
+        sequences = 1 if sequences is None else int(sequences)
+        if sequences < 1 or q.shape[0] % sequences or k.shape[0] % sequences:
+            raise ValueError("the positions are not %d sequences of one length" % sequences)
+    if scale is not None and not scale > 0:
+        raise ValueError("the scale is not positive")
+    return AttentionGeom(q.shape[2], q.shape[1], k.shape[1], q.shape[0], k.shape[0], sequences, int(bool(causal)), data_type(q, k, v),
+                         0.0 if scale is None else float(scale))
+
+
+def _rows(x, starts):
+    """A fresh tensor like x for rows that a call writes: all of them, or those of sequences (the others are zero then)"""
+    return _alike(x) if starts is None else _torch().zeros(x.shape, dtype=x.dtype, device=x.device)
+
+
+def attention_forward(q, k, v, q_starts=None, k_starts=None, sequences=None, causal=False, scale=None, out=None, ws=None):
+    """Softmax attention of packed sequences (include/mcn_hip.h: mcn_attention_forward): (y, log_sums).  q (N, heads, D), k and v
+    (M, keyHeads, D): float32 or bfloat16, channels neighbours, any other strides.  q_starts, k_starts: int32 on the device, sequences + 1
+    numbers each; without them `sequences` (one, if not given) of one length.  causal: the queries are the last positions of their
+    sequence.  log_sums (N, heads) in float32.  out: the tensor y is written to, whose rows of no sequence are left alone (a fresh one
+    holds zeros there)."""
+    g = _attention_geom(q, k, v, sequences, q_starts, k_starts, causal, scale)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+        raise ValueError("out is not of the queries' shape and type")
+    y = _rows(q, q_starts) if out is None else out
+    log_sums = _singles(q, g.N, g.heads) if q_starts is None else q.new_zeros((g.N, g.heads), dtype=_torch().float32)
+    wp, wn, held = _scratch(ws, q, lib().mcn_attention_workspace_bytes(C.byref(g), 0))
+    check(lib().mcn_attention_forward(stream(), C.byref(g), _heads("out", y), ptr(log_sums), _heads("q", q), _heads("k", k), _heads("v", v),
+                                      ptr(q_starts), ptr(k_starts), wp, wn))
+    return y, log_sums
+
+
+def attention_backward(q, k, v, y, log_sums, dy, q_starts=None, k_starts=None, sequences=None, causal=False, scale=None, want=(True, True, True),
+                       out=None, ws=None):
+    """(dq, dk, dv) of attention_forward from what it left in y and log_sums; those not wanted are None.  out: the tensors they are
+    written to, whose rows of no sequence are left alone (fresh ones hold zeros there)."""
+    g = _attention_geom(q, k, v, sequences, q_starts, k_starts, causal, scale)
+    for name, t in (("y", y), ("dy", dy)):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError("%s is not of the queries' shape and type" % name)
+    _single("log_sums", log_sums)
+    if log_sums.numel() != g.N * g.heads:
+        raise ValueError("log_sums does not have one value per query and head")
+    names, like, starts = ("dq", "dk", "dv"), (q, k, v), (q_starts, k_starts, k_starts)
+    if out is None:
+        out = (None, None, None)
+    for name, t, x in zip(names, out, like):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError("%s is not of its input's shape and type" % name)
+    d = [(t if t is not None else _rows(x, s)) if w else None for w, t, x, s in zip(want, out, like, starts)]
+    wp, wn, held = _scratch(ws, q, lib().mcn_attention_workspace_bytes(C.byref(g), 1))
+    check(lib().mcn_attention_backward(stream(), C.byref(g), _heads("dq", d[0]), _heads("dk", d[1]), _heads("dv", d[2]), _heads("y", y), ptr(log_sums),
+                                       _heads("q", q), _heads("k", k), _heads("v", v), _heads("dy", dy), ptr(q_starts), ptr(k_starts), wp, wn))
+    return tuple(d)
+
+
+class GradientList:
+    """Gradients that are clipped together, and where the clipped ones go (None: into their own places): contiguous float32 or bfloat16
+    tensors on one device, none of which overlaps another.  Holds the tensors; made once for those a program keeps."""
+
+    def __init__(self, ders, outs=None):
+        self.ders = list(ders)
+        self.outs = self.ders if outs is None else list(outs)
+        if len(self.outs) != len(self.ders):
+            raise ValueError("there is not one output per gradient")
+        self.device = None
+        for i, (g, y) in enumerate(zip(self.ders, self.outs)):
+            for t in (g, y):
+                if not (t.is_cuda and t.is_contiguous()):
+                    raise ValueError("gradient %d is not a contiguous tensor on the device" % i)
+                if self.device is None:
+                    self.device = t.get_device()
+                if t.get_device() != self.device:
+                    raise ValueError("gradient %d is on device %d, not on device %d" % (i, t.get_device(), self.device))
+            if g.shape != y.shape or g.dtype != y.dtype:
+                raise ValueError("output %d is not of its gradient's shape and type" % i)
+        n = len(self.ders)
+        spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i, side) for side, ts in enumerate((self.ders, self.outs))
+                 for i, t in enumerate(ts) if t.numel() and not (side and self.outs[i].data_ptr() == self.ders[i].data_ptr())]
+        spans.sort()
+        for a, b in zip(spans, spans[1:]):
+            if b[0] < a[1]:
+                raise ValueError("gradients or outputs %d and %d overlap" % (a[2], b[2]))
+        self.n = n
+        self.counts = (C.c_size_t * n)(*[g.numel() for g in self.ders])
+        self.types = (C.c_int * n)(*[data_type(g) for g in self.ders])
+        self.der_pointers = (C.c_void_p * n)(*[g.data_ptr() for g in self.ders])
+        self.out_pointers = (C.c_void_p * n)(*[y.data_ptr() for y in self.outs])
+        self.workspace_bytes = lib().mcn_clip_workspace_bytes(self.counts, n)
+
+    def _here(self):
+        torch = _torch()
+        if self.device is not None and self.device != torch.cuda.current_device():
+            raise ValueError("the gradients are on device %d, not on the current one" % self.device)
+        return torch.empty(1, dtype=torch.float32, device="cuda")
+
+
+def gradient_norm(gradients, ws=None):
+    """The norm of a GradientList's (or a list's) gradients together, a one-element device tensor (include/mcn_hip.h: mcn_gradient_norm)."""
+    g = gradients if isinstance(gradients, GradientList) else GradientList(gradients)
+    norm = g._here()
+    wp, wn, held = _scratch(ws, norm, g.workspace_bytes)
+    check(lib().mcn_gradient_norm(stream(), ptr(norm), g.der_pointers, g.counts, g.types, g.n, wp, wn))
+    return norm
+
+
+def clip_gradients(gradients, max_norm, ws=None):
+    """Clips a GradientList's (or, in place, a list's) gradients to a norm of max_norm together; the norm they had, a one-element device
+    tensor (include/mcn_hip.h: mcn_clip_gradients)."""
+    g = gradients if isinstance(gradients, GradientList) else GradientList(gradients)
+    norm = g._here()
+    wp, wn, held = _scratch(ws, norm, g.workspace_bytes)
+    check(lib().mcn_clip_gradients(stream(), g.out_pointers, ptr(norm), g.der_pointers, g.counts, g.types, g.n, float(max_norm), wp, wn))
+    return norm
+
+
 def relu_forward(x, leak=None):
     y = _torch().empty_like(x)
     if leak is None:
@@ -902,6 +1175,19 @@ def sgd_momentum(value, state, der, chunk_param, rates, learning_rate, weight_de
     check(lib().mcn_sgd_momentum(stream(), ptr(value), ptr(state), ptr(der), chunks, ptr(chunk_param), ptr(rates),
                                  float(learning_rate), float(weight_decay), float(momentum), float(der_scale),
                                  int(bool(nesterov))))
+
+
+def sgd_momentum_clipped(value, state, der, chunk_param, rates, learning_rate, weight_decay, momentum, max_norm, der_scale=1.0, nesterov=False, ws=None):
+    """sgd_momentum with the derivatives clipped to a norm of max_norm together, in the same pass (include/mcn_hip.h:
+    mcn_sgd_momentum_clipped); the norm they had, a one-element device tensor."""
+    chunks = chunk_param.numel()
+    assert value.numel() == state.numel() == der.numel() == chunks * SGD_CHUNK
+    _single("value state der", value, state, der)
+    norm = _singles(value, 1)
+    wp, wn, held = _scratch(ws, value, lib().mcn_sgd_momentum_clipped_workspace_bytes(chunks))
+    check(lib().mcn_sgd_momentum_clipped(stream(), ptr(value), ptr(state), ptr(der), chunks, ptr(chunk_param), ptr(rates), float(learning_rate),
+                                         float(weight_decay), float(momentum), float(der_scale), int(bool(nesterov)), float(max_norm), ptr(norm), wp, wn))
+    return norm
 
 
 def taccum(alpha, a, beta, b, out=None):

@@ -1,0 +1,1140 @@
+// Attention of the positions of packed sequences, heads in groups that share keys and values.
+//   s_ij = scale q_i . k_j,  L_i = log sum_j exp s_ij,  p_ij = exp(s_ij - L_i),  o_i = sum_j p_ij v_j
+//   backward: delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//             dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+// Bound by the matrix pipe where sequences are long (4 D operations a pair of positions forward, 10 D backward) and by reading k and v where
+// few queries meet many keys.  No tensor of scores: the softmax is taken along with the products, its largest score and its sum
+// running.
+//
+// Rows.  A key head's queries are the rows r = i G + g of one matrix, i the position, g the head of the group of G: one query a sequence
+// is a tile of G rows that reads its keys once, and dk, dv of a group are sums inside one workgroup.
+//
+// Products are v_mfma_f32_32x32x16_bf16, or 32x32x2_f32 in single precision, always with the operands such that a result's lane holds one
+// index of the side that stays (a query forward and for dq, a key for dk and dv) and sixteen of the 32 of the side that is walked:
+// 8 (r / 4) + 4 (lane / 32) + r % 4.  A row's maximum and sum then need one exchange between two lanes, and p or ds goes into the next
+// product straight from the registers: the order of a reduction is free, so the other operand is read from LDS in the same order.
+//
+// The walked side comes through LDS, brought there by the DMA a tile ahead, one barrier a tile.  Rows lie there 16 bytes by 16 bytes, exchanged
+// by the row so that neither reads along a row nor transposing reads across rows meet in a bank.
+#include "mcn_internal.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mcn {
+namespace {
+
+typedef unsigned short bf16;
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bfx8 __attribute__((ext_vector_type(8)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMostD = 128;
+constexpr unsigned kNowhere = 0xfffffff0u;   // an offset behind every buffer: reads zero
+
+__device__ __forceinline__ float bits_float(unsigned v) { return __builtin_bit_cast(float, v); }
+__device__ __forceinline__ unsigned float_bits(float v) { return __builtin_bit_cast(unsigned, v); }
+__device__ __forceinline__ unsigned short round_bf16(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) { return (unsigned)round_bf16(a) | (unsigned)round_bf16(b) << 16; }
+__device__ __forceinline__ float value_of(const float* p) { return *p; }
+__device__ __forceinline__ float value_of(const bf16* p) { return bits_float((unsigned)*p << 16); }
+__device__ __forceinline__ float power2(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ bool finite(float v) { return (float_bits(v) & 0x7f800000u) != 0x7f800000u; }
+
+// the other half's value of the 64 lanes (lane ^ 32)
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, kWave); }
+// whether both lanes of a row (or key) find it good
+__device__ __forceinline__ bool both_good(bool good) {
+  const unsigned long long m = __ballot(good);
+  return (m & m >> 32) >> (threadIdx.x & 31) & 1;
+}
+
+struct Tensor3 {            // heads where they lie, strides in bytes
+  char* data;
+  long long position, head;
+};
+
+struct AttentionP {
+  Tensor3 q, k, v, o, dO, dq, dk, dv;
+  float *logSums, *parts, *partSums;     // parts: a slice's o (normalised) and log sums
+  float *statL, *statD;                  // backward, [keyHeads][N G]: -L/scale, -delta
+  const int *qStarts, *kStarts;
+  int sequences, each, eachKeys;         // without starts: queries and keys of a sequence
+  int D, G, heads, keyHeads, N, M, causal;
+  int tiles, slices, vector;             // vector: outputs may be stored four values at a time
+  FastDiv byG, byTiles;                  // tiles of a sequence, without starts
+  float scale, c;                        // c = scale log2 e
+};
+
+template <class V> struct Matrix;
+template <> struct Matrix<bf16> {
+  static constexpr int perChunk = 8;
+  // 16 bytes a lane along the reduction: lane / 32 says which of two neighbouring runs of eight
+  __device__ static __forceinline__ floatx16 along(uintx4 a, uintx4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfx8, a), __builtin_bit_cast(bfx8, b), c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ float dot(uintx4 a, uintx4 b) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += bits_float(a[e] << 16) * bits_float(b[e] << 16) + bits_float(a[e] & 0xffff0000u) * bits_float(b[e] & 0xffff0000u);
+    return s;
+  }
+};
+template <> struct Matrix<float> {
+  static constexpr int perChunk = 4;
+  __device__ static __forceinline__ floatx16 along(uintx4 a, uintx4 b, floatx16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(bits_float(a[e]), bits_float(b[e]), c, 0, 0, 0);
+    return c;
+  }
+  __device__ static __forceinline__ float dot(uintx4 a, uintx4 b) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += bits_float(a[e]) * bits_float(b[e]);
+    return s;
+  }
+};
+
+// A tile in LDS: rows of DP values, chunk c (16 bytes) of a row at c ^ turn(row).  bfloat16: four rows that a transposing read takes lie in four
+// 64-byte runs of banks, and sixteen rows put a chunk in sixteen places; single precision: the latter.
+template <class V, int DP>
+struct Tile {
+  static constexpr int rowBytes = DP * (int)sizeof(V), chunks = rowBytes / 16, steps = chunks / 2, blocks = DP / 32;
+  __device__ static __forceinline__ int turn(int row) {
+    if (sizeof(V) == 4) return row & 15;
+    return chunks == 16 ? ((row & 3) << 2 | (row >> 2 & 3)) : ((row >> 1 & 1) << 2 | (row >> 2 & 3));
+  }
+  // chunks 2 s + lane / 32 of row first + lane % 32
+  __device__ static __forceinline__ uintx4 along(const char* lds, int first, int s, int lane) {
+    const int row = lane & 31;   // (first is a multiple of 32: the turn is the lane's own)
+    return *(const uintx4*)(lds + (first + row) * rowBytes + (((2 * s) ^ (turn(row) ^ (lane >> 5))) << 4));
+  }
+  // acc += (rows first .. first + 31 of the tile)' x p, the 32 columns from 32 b on: p in the order of a result's registers
+  __device__ static __forceinline__ floatx16 across(const char* lds, int first, int b, int lane, const uintx4 (&p)[sizeof(V) == 4 ? 4 : 2], floatx16 acc) {
+    if (sizeof(V) == 2) {
+      typedef __attribute__((address_space(3))) shortx4* lds_shorts;
+      const int quarter = (lane >> 5) * 4 + (lane >> 2 & 3), chunk = 4 * b + (lane >> 4 & 1) * 2 + (lane >> 1 & 1), within = (lane & 1) * 8;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int r0 = first + 16 * s + quarter, r1 = r0 + 8;
+        const uintx2 a0 = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_shorts)(lds + r0 * rowBytes + ((chunk ^ turn(quarter)) << 4) + within)));
+        const uintx2 a1 = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_shorts)(lds + r1 * rowBytes + ((chunk ^ turn(quarter + 8)) << 4) + within)));
+        acc = Matrix<bf16>::along((uintx4){a0.x, a0.y, a1.x, a1.y}, p[s], acc);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 8 * (r / 4) + 4 * (lane >> 5) + r % 4, column = 32 * b + (lane & 31);
+        const float a = *(const float*)(lds + (first + row) * rowBytes + ((column / 4 ^ turn(row)) << 4) + (column & 3) * 4);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, bits_float(p[r / 4 & 3][r % 4]), acc, 0, 0, 0);
+      }
+    }
+    return acc;
+  }
+  // a result's sixteen values as the operand of `across`
+  __device__ static __forceinline__ void operand(uintx4 (&p)[sizeof(V) == 4 ? 4 : 2], const float (&v)[16]) {
+    if (sizeof(V) == 2) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[s][e] = pack_bf16(v[8 * s + 2 * e], v[8 * s + 2 * e + 1]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r / 4 & (sizeof(V) == 4 ? 3 : 1)][r % 4] = float_bits(v[r]);
+    }
+  }
+};
+
+// Brings ROWS rows of a tile into LDS: wavefront w the 1024-byte pieces w, w + NW, ...  Offsets of rows come from `offset_of(row)`, in bytes
+// from the buffer's base, kNowhere for rows that are not there; columns behind D read as zero.
+template <class V, int DP, int ROWS, int NW, class Offset>
+__device__ __forceinline__ void bring(char* lds, const char* base, int D, int wave, int lane, Offset offset_of) {
+  typedef Tile<V, DP> T;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  constexpr int pieces = ROWS * T::rowBytes / 1024;
+  static_assert(pieces % NW == 0, "whole pieces");
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kNowhere, 0x00020000);
+#pragma unroll
+  for (int i = 0; i < pieces / NW; ++i) {
+    const int slot = (i * NW + wave) * 64 + lane, row = slot / T::chunks, chunk = (slot % T::chunks) ^ T::turn(row);
+    const unsigned at = offset_of(row);
+    const unsigned offset = at == kNowhere || chunk * Matrix<V>::perChunk >= D ? kNowhere : at + chunk * 16u;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (i * NW + wave) * 1024), 16, (int)offset, 0, 0, 0);
+  }
+}
+
+// 16 bytes of a row in global memory, zero where there is none
+template <class V>
+__device__ __forceinline__ uintx4 chunk_of(const char* row, int chunk, int D, bool live) {
+  uintx4 v = {0u, 0u, 0u, 0u};
+  if (live && chunk * Matrix<V>::perChunk < D) v = *(const uintx4*)(row + chunk * 16);
+  return v;
+}
+
+// Four neighbouring values of a row out
+template <class V>
+__device__ __forceinline__ void store4(char* row, int d, int D, int vector, float a, float b, float c, float e) {
+  if (vector) {
+    if (d >= D) return;
+    if (sizeof(V) == 2) *(uintx2*)(row + 2 * d) = (uintx2){pack_bf16(a, b), pack_bf16(c, e)};
+    else *(uintx4*)(row + 4 * d) = (uintx4){float_bits(a), float_bits(b), float_bits(c), float_bits(e)};
+    return;
+  }
+  const float v[4] = {a, b, c, e};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (d + k >= D) return;
+    if (sizeof(V) == 2) ((bf16*)row)[d + k] = round_bf16(v[k]);
+    else ((float*)row)[d + k] = v[k];
+  }
+}
+
+// ------------------------------------------------------------------------------------------ which sequence
+
+struct Span {
+  int q0, n, k0, m;   // the sequence's queries and keys
+  int first;          // first row (or key) of the tile, -1: nothing to do
+};
+
+__device__ __forceinline__ int clamped(int v, int most) { return v < 0 ? 0 : v > most ? most : v; }
+
+// Tile `tile` of SIZE rows (KEYS: keys).  With starts, sequence s has the tiles from before(s)/SIZE + s on, before(s) the rows ahead of it:
+// no tile holds two sequences, and floor(b/SIZE) + 1 numbers are enough for any sequence, so the tiles of all are known without
+// looking at the starts on the host.  The sequence of a tile is found 64 candidates at a time, all loads of a step at once.  HEAVY_FIRST:
+// a sequence's tiles in the order of falling work (causal).
+template <int SIZE, bool KEYS, bool LAST_FIRST>
+__device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
+  Span s;
+  int t;
+  if (!p.qStarts) {
+    int seq;
+    p.byTiles.divmod(tile, &seq, &t);
+    s.q0 = seq * p.each; s.n = p.each;
+    s.k0 = seq * p.eachKeys; s.m = p.eachKeys;
+    if (seq >= p.sequences) s.n = s.m = 0;
+  } else {
+    const auto before = [&](int i) { return (KEYS ? clamped(p.kStarts[i], p.M) : clamped(p.qStarts[i], p.N) * p.G) / SIZE + i; };
+    int lo = 0, n = p.sequences;
+    while (n > 1) {
+      const int step = (n + 63) / 64, i = lo + lane * step;
+      const unsigned long long below = __ballot(lane * step < n && before(i) <= tile);
+      const int found = below ? 63 - __builtin_clzll(below) : 0;
+      lo += found * step;
+      n = std::min(step, n - found * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    t = tile - before(lo);
+    s.q0 = clamped(p.qStarts[lo], p.N);
+    s.n = clamped(p.qStarts[lo + 1], p.N) - s.q0;
+    s.k0 = clamped(p.kStarts[lo], p.M);
+    s.m = clamped(p.kStarts[lo + 1], p.M) - s.k0;
+    if (s.n < 0) s.n = 0;
+    if (s.m < 0) s.m = 0;
+  }
+  const int rows = KEYS ? s.m : s.n * p.G, tiles = (rows + SIZE - 1) / SIZE;
+  s.first = t < 0 || t >= tiles ? -1 : (LAST_FIRST && p.causal ? tiles - 1 - t : t) * SIZE;
+  return s;
+}
+
+// ------------------------------------------------------------------------------------------ forward
+
+constexpr int kAhead = 2;   // tiles in LDS at a time
+
+// One tile of KT keys: fragments of 32 queries (q) against it.  `next` is filled meanwhile.  (A function of its own with `restrict` pointers:
+// that the loads fill none of what is read is what lets the reads go without waiting for them.)
+template <class V, int DP, int KT, class Bring>
+__device__ __forceinline__ void forward_tile(const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next, Bring bring_next,
+                                             const uintx4 (&q)[Tile<V, DP>::steps], floatx16 (&o)[DP / 32], float& most, float& sum, int j0, int limit,
+                                             bool edge, float c, int lane) {
+  typedef Tile<V, DP> T;
+  constexpr int KB = KT / 32;
+  bring_next(next);
+  floatx16 s[KB];
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < T::steps; ++k) s[b] = Matrix<V>::along(T::along(keys, 32 * b, k, lane), q[k], s[b]);
+  }
+  if (edge) {
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (j0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 >= limit) s[b][r] = -INFINITY;
+  }
+  float m = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
+  m = fmaxf(m, other_half(m));
+  // The reference of the exponentials is raised only when a score lies more than 2^8 above it: what is summed stays below 2^8 a key, and the
+  // outputs are scaled anew a few times in all instead of every tile.
+  const bool raise = m * c > most * c + 8.f || (most == -INFINITY && m > -INFINITY);
+  if (__any(raise)) {
+    const float to = raise ? m : most;
+    const float f = raise ? (most == -INFINITY ? 0.f : power2((most - to) * c)) : 1.f;
+    most = to;
+    sum *= f;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= f;
+  }
+  const float shift = most == -INFINITY ? 0.f : most * c;
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    float e[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) e[r] = power2(s[b][r] * c - shift);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum += e[r];
+    uintx4 operand[sizeof(V) == 4 ? 4 : 2];
+    T::operand(operand, e);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[d] = T::across(values, 32 * b, d, lane, operand, o[d]);
+  }
+}
+
+// NW wavefronts of 32 rows, tiles of KT keys
+template <class V, int DP, int NW, int KT>
+__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(AttentionP p) {
+  typedef Tile<V, DP> T;
+  constexpr int tileBytes = KT * T::rowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[kAhead * 2 * tileBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int head = id % p.keyHeads;
+  id /= p.keyHeads;
+  const int slice = id % p.slices;
+  const Span span = find<32 * NW, false, true>(p, id / p.slices, lane);
+  if (span.first < 0) return;
+  const int rows = span.n * p.G, off = span.m - span.n;
+  const int row = span.first + 32 * wave + (lane & 31);
+  const bool live = row < rows;
+  int i, g;
+  p.byG.divmod(live ? row : 0, &i, &g);
+  const int limit = !live ? 0 : p.causal ? std::max(0, std::min(span.m, i + off + 1)) : span.m;
+  // keys that some row of the workgroup sees
+  int end = span.m;
+  if (p.causal) end = std::max(0, std::min(end, p.byG.div(std::min(rows, span.first + 32 * NW) - 1) + off + 1));
+  int begin = 0;
+  if (p.slices > 1) {
+    const int share = ((end + p.slices - 1) / p.slices + KT - 1) / KT * KT;
+    begin = std::min(end, slice * share);
+    end = std::min(end, begin + share);
+  }
+  // ... that all rows of the wavefront see (those of its first row), and the last that some row sees
+  const int all = p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows - 1, span.first + 32 * wave)) + off + 1)) : span.m;
+  const int some = span.first + 32 * wave >= rows ? 0
+                   : p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows, span.first + 32 * wave + 32) - 1) + off + 1)) : span.m;
+
+  const long long position = span.q0 + i;
+  const int column = head * p.G + g;
+  uintx4 q[T::steps];
+  {
+    const char* at = p.q.data + position * p.q.position + column * p.q.head;
+#pragma unroll
+    for (int s = 0; s < T::steps; ++s) q[s] = chunk_of<V>(at, 2 * s + (lane >> 5), p.D, live);
+  }
+  const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
+  const char* values = p.v.data + (long long)span.k0 * p.v.position + head * p.v.head;
+  const unsigned kPitch = (unsigned)p.k.position, vPitch = (unsigned)p.v.position;
+  const auto bring_tile = [&](char* to, int j0) __attribute__((always_inline)) {
+    const int left = end - j0;
+    const char* kb = keys + (long long)j0 * p.k.position;
+    const char* vb = values + (long long)j0 * p.v.position;
+    bring<V, DP, KT, NW>(to, kb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * kPitch : kNowhere; });
+    bring<V, DP, KT, NW>(to + tileBytes, vb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * vPitch : kNowhere; });
+  };
+  floatx16 o[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float most = -INFINITY, sum = 0.f;
+  if (begin < end) bring_tile(lds, begin);
+  int turn = 0;
+  for (int j0 = begin; j0 < end; j0 += KT) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    char* from = lds + turn * 2 * tileBytes;
+    char* to = lds + (turn ^ 1) * 2 * tileBytes;
+    turn ^= 1;
+    const auto bring_next = [&](char* at) __attribute__((always_inline)) {
+      if (j0 + KT < end) bring_tile(at, j0 + KT);
+    };
+    if (j0 < some)
+      forward_tile<V, DP, KT>(from, from + tileBytes, to, bring_next, q, o, most, sum, j0, std::min(limit, end), j0 + KT > std::min(all, end), p.c, lane);
+    else bring_next(to);
+  }
+  sum += other_half(sum);
+  // A key that a row does not see has p = 0, but 0 times an infinity or a NaN of its values is NaN: a row that is not finite is added up
+  // key by key, over those it sees.
+  if (p.causal) {
+    bool good = true;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) good = good && finite(o[d][r]);
+    if (!both_good(good)) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+      const float shift = most == -INFINITY ? 0.f : most * p.c;
+      const char* at = p.q.data + position * p.q.position + column * p.q.head;
+#pragma unroll 1
+      for (int j = begin; j < std::min(limit, end); ++j) {
+        float s = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < p.D; ++d) s += value_of((const V*)at + d) * value_of((const V*)(keys + (long long)j * p.k.position) + d);
+        float e = power2(s * p.c - shift);
+        if (sizeof(V) == 2) e = bits_float((unsigned)round_bf16(e) << 16);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at2 = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+            if (at2 < p.D) o[d][r] += e * value_of((const V*)(values + (long long)j * p.v.position) + at2);
+          }
+      }
+    }
+  }
+  if (!live) return;
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  const float total = sum == 0.f ? -INFINITY : most * p.scale + logf(sum);
+  const long long index = position * p.heads + column;
+  if (p.slices == 1) {
+    if (lane < 32 && p.logSums) p.logSums[index] = total;
+    char* at = p.o.data + position * p.o.position + column * p.o.head;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        store4<V>(at, 32 * d + 8 * (r / 4) + 4 * (lane >> 5), p.D, p.vector, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
+  } else {
+    const long long part = (long long)slice * p.N * p.heads + index;
+    if (lane < 32) p.partSums[part] = total;
+    char* at = (char*)(p.parts + part * DP);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        store4<float>(at, 32 * d + 8 * (r / 4) + 4 * (lane >> 5), DP, 1, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
+  }
+}
+
+// The slices of a row put together: o = sum_s exp(L_s - L) o_s.  A wavefront per row and head; rows of no sequence are passed over.
+template <class V, int DP>
+__global__ __launch_bounds__(256) void attention_join(AttentionP p) {
+  const int lane = threadIdx.x & 63;
+  const long long index = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), all = (long long)p.N * p.heads;
+  if (index >= all) return;
+  const int position = (int)(index / p.heads), column = (int)(index % p.heads);
+  if (p.qStarts && (position < clamped(p.qStarts[0], p.N) || position >= clamped(p.qStarts[p.sequences], p.N))) return;
+  const float mine = lane < p.slices ? p.partSums[lane * all + index] : -INFINITY;
+  float most = mine;
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) most = fmaxf(most, __shfl_xor(most, k, kWave));
+  // (a NaN of one slice is a NaN of the row)
+  const float weight = most == -INFINITY && mine == mine ? 0.f : power2((mine - most) * kLog2e);
+  const float sum = wave_sum(weight);
+  constexpr int W = DP / 64;
+  float o[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) o[w] = 0.f;
+  for (int s = 0; s < p.slices; ++s) {
+    const float f = __shfl(weight, s, kWave);
+    if (f == 0.f) continue;
+    const float* at = p.parts + (s * all + index) * DP + lane;
+#pragma unroll
+    for (int w = 0; w < W; ++w) o[w] += f * at[64 * w];
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  if (lane == 0 && p.logSums) p.logSums[index] = sum == 0.f ? -INFINITY : most + logf(sum);
+  char* at = p.o.data + position * p.o.position + column * p.o.head;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const int d = lane + 64 * w;
+    if (d >= p.D) continue;
+    if (sizeof(V) == 2) ((bf16*)at)[d] = round_bf16(o[w] * inv);
+    else ((float*)at)[d] = o[w] * inv;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ dq, and delta for dk and dv
+
+template <class V, int DP, int KT, class Bring>
+__device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next, Bring bring_next,
+                                        const uintx4 (&q)[Tile<V, DP>::steps], const uintx4 (&dO)[Tile<V, DP>::steps], floatx16 (&dq)[DP / 32], float negL,
+                                        float negDelta, int j0, int limit, bool edge, float c, int lane) {
+  typedef Tile<V, DP> T;
+  bring_next(next);
+#pragma unroll
+  for (int b = 0; b < KT / 32; ++b) {
+    floatx16 s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = negL;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] = negDelta;
+#pragma unroll
+    for (int k = 0; k < T::steps; ++k) s = Matrix<V>::along(T::along(keys, 32 * b, k, lane), q[k], s);
+#pragma unroll
+    for (int k = 0; k < T::steps; ++k) dp = Matrix<V>::along(T::along(values, 32 * b, k, lane), dO[k], dp);
+    float e[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c) * dp[r];
+    if (edge) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (j0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 >= limit) e[r] = 0.f;
+    }
+    uintx4 operand[sizeof(V) == 4 ? 4 : 2];
+    T::operand(operand, e);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dq[d] = T::across(keys, 32 * b, d, lane, operand, dq[d]);
+  }
+}
+
+template <class V, int DP, int NW, int KT>
+__global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(AttentionP p) {
+  typedef Tile<V, DP> T;
+  constexpr int tileBytes = KT * T::rowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[kAhead * 2 * tileBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.x % p.keyHeads;
+  const Span span = find<32 * NW, false, true>(p, blockIdx.x / p.keyHeads, lane);
+  if (span.first < 0) return;
+  const int rows = span.n * p.G, off = span.m - span.n;
+  const int row = span.first + 32 * wave + (lane & 31);
+  const bool live = row < rows;
+  int i, g;
+  p.byG.divmod(live ? row : 0, &i, &g);
+  const int limit = !live ? 0 : p.causal ? std::max(0, std::min(span.m, i + off + 1)) : span.m;
+  int end = span.m;
+  if (p.causal) end = std::max(0, std::min(end, p.byG.div(std::min(rows, span.first + 32 * NW) - 1) + off + 1));
+  const int all = p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows - 1, span.first + 32 * wave)) + off + 1)) : span.m;
+  const int some = span.first + 32 * wave >= rows ? 0
+                   : p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows, span.first + 32 * wave + 32) - 1) + off + 1)) : span.m;
+  const long long position = span.q0 + i;
+  const int column = head * p.G + g;
+  uintx4 q[T::steps], dO[T::steps];
+  float negDelta = 0.f;
+  {
+    const char* at = p.q.data + position * p.q.position + column * p.q.head;
+    const char* dAt = p.dO.data + position * p.dO.position + column * p.dO.head;
+    const char* oAt = p.o.data + position * p.o.position + column * p.o.head;
+#pragma unroll
+    for (int s = 0; s < T::steps; ++s) dO[s] = chunk_of<V>(dAt, 2 * s + (lane >> 5), p.D, live);
+#pragma unroll
+    for (int s = 0; s < T::steps; ++s) negDelta -= Matrix<V>::dot(dO[s], chunk_of<V>(oAt, 2 * s + (lane >> 5), p.D, live));
+#pragma unroll
+    for (int s = 0; s < T::steps; ++s) q[s] = chunk_of<V>(at, 2 * s + (lane >> 5), p.D, live);
+  }
+  negDelta += other_half(negDelta);
+  float negL = 0.f;
+  if (live) {
+    negL = p.logSums[position * p.heads + column];
+    negL = negL == -INFINITY ? 0.f : -negL / p.scale;
+    if (lane < 32) {
+      const long long at = (long long)head * p.N * p.G + (long long)span.q0 * p.G + row;
+      p.statL[at] = negL;
+      p.statD[at] = negDelta;
+    }
+  }
+  if (!p.dq.data) return;
+  const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
+  const char* values = p.v.data + (long long)span.k0 * p.v.position + head * p.v.head;
+  const unsigned kPitch = (unsigned)p.k.position, vPitch = (unsigned)p.v.position;
+  const auto bring_tile = [&](char* to, int j0) __attribute__((always_inline)) {
+    const int left = end - j0;
+    const char* kb = keys + (long long)j0 * p.k.position;
+    const char* vb = values + (long long)j0 * p.v.position;
+    bring<V, DP, KT, NW>(to, kb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * kPitch : kNowhere; });
+    bring<V, DP, KT, NW>(to + tileBytes, vb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * vPitch : kNowhere; });
+  };
+  floatx16 dq[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+  if (end > 0) bring_tile(lds, 0);
+  int turn = 0;
+  for (int j0 = 0; j0 < end; j0 += KT) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    char* from = lds + turn * 2 * tileBytes;
+    char* to = lds + (turn ^ 1) * 2 * tileBytes;
+    turn ^= 1;
+    const auto bring_next = [&](char* at) __attribute__((always_inline)) {
+      if (j0 + KT < end) bring_tile(at, j0 + KT);
+    };
+    if (j0 < some) dq_tile<V, DP, KT>(from, from + tileBytes, to, bring_next, q, dO, dq, negL, negDelta, j0, limit, j0 + KT > std::min(all, end), p.c, lane);
+    else bring_next(to);
+  }
+  // (as in the forward pass: what is not finite is added up over the keys that a row sees)
+  if (p.causal) {
+    bool good = true;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) good = good && finite(dq[d][r]);
+    if (!both_good(good)) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+      const char* at = p.q.data + position * p.q.position + column * p.q.head;
+      const char* dAt = p.dO.data + position * p.dO.position + column * p.dO.head;
+#pragma unroll 1
+      for (int j = 0; j < limit; ++j) {
+        const V* kj = (const V*)(keys + (long long)j * p.k.position);
+        const V* vj = (const V*)(values + (long long)j * p.v.position);
+        float s = negL, dp = negDelta;
+#pragma unroll 1
+        for (int d = 0; d < p.D; ++d) {
+          s += value_of((const V*)at + d) * value_of(kj + d);
+          dp += value_of((const V*)dAt + d) * value_of(vj + d);
+        }
+        float e = power2(s * p.c) * dp;
+        if (sizeof(V) == 2) e = bits_float((unsigned)round_bf16(e) << 16);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at2 = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+            if (at2 < p.D) dq[d][r] += e * value_of(kj + at2);
+          }
+      }
+    }
+  }
+  if (!live) return;
+  char* at = p.dq.data + position * p.dq.position + column * p.dq.head;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      store4<V>(at, 32 * d + 8 * (r / 4) + 4 * (lane >> 5), p.D, p.vector, dq[d][r] * p.scale, dq[d][r + 1] * p.scale, dq[d][r + 2] * p.scale,
+                dq[d][r + 3] * p.scale);
+}
+
+// ------------------------------------------------------------------------------------------ dk, dv
+
+// One tile of RT rows against a wavefront's 32 keys
+template <class V, int DP, int RT, class Bring>
+__device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const char* __restrict__ ders, const float* __restrict__ statL,
+                                         const float* __restrict__ statD, char* __restrict__ next, Bring bring_next, const uintx4 (&k)[Tile<V, DP>::steps],
+                                         const uintx4 (&v)[Tile<V, DP>::steps], floatx16 (&dk)[DP / 32], floatx16 (&dv)[DP / 32], const FastDiv& byG, int r0,
+                                         int rows, int firstOf, bool edge, float c, int lane) {
+  typedef Tile<V, DP> T;
+  bring_next(next);
+#pragma unroll
+  for (int b = 0; b < RT / 32; ++b) {
+    floatx16 s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const float4 l = *(const float4*)(statL + 32 * b + 2 * r + 4 * (lane >> 5));
+      s[r] = l.x; s[r + 1] = l.y; s[r + 2] = l.z; s[r + 3] = l.w;
+    }
+#pragma unroll
+    for (int t = 0; t < T::steps; ++t) s = Matrix<V>::along(T::along(queries, 32 * b, t, lane), k[t], s);
+    float e[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c);
+    if (edge) {   // (firstOf: the first position that sees this lane's key)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+        if (row >= rows || byG.div(row) < firstOf) e[r] = 0.f;
+      }
+    }
+    uintx4 operand[sizeof(V) == 4 ? 4 : 2];
+    T::operand(operand, e);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dv[d] = T::across(ders, 32 * b, d, lane, operand, dv[d]);
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const float4 l = *(const float4*)(statD + 32 * b + 2 * r + 4 * (lane >> 5));
+      dp[r] = l.x; dp[r + 1] = l.y; dp[r + 2] = l.z; dp[r + 3] = l.w;
+    }
+#pragma unroll
+    for (int t = 0; t < T::steps; ++t) dp = Matrix<V>::along(T::along(ders, 32 * b, t, lane), v[t], dp);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) e[r] = edge && e[r] == 0.f ? 0.f : e[r] * dp[r];
+    T::operand(operand, e);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dk[d] = T::across(queries, 32 * b, d, lane, operand, dk[d]);
+  }
+}
+
+template <class V, int DP, int NW, int RT>
+__global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv(AttentionP p) {
+  typedef Tile<V, DP> T;
+  constexpr int tileBytes = RT * T::rowBytes, statBytes = RT * 4, bufferBytes = 2 * tileBytes + 2 * statBytes;
+  static_assert(RT <= 64, "one load brings the statistics of a tile");
+  __shared__ __attribute__((aligned(16))) char lds[kAhead * bufferBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.x % p.keyHeads;
+  const Span span = find<32 * NW, true, false>(p, blockIdx.x / p.keyHeads, lane);
+  if (span.first < 0) return;
+  const int rows = span.n * p.G, off = span.m - span.n;
+  const int key = span.first + 32 * wave + (lane & 31);
+  const bool live = key < span.m;
+  // the first position that sees the lane's key, the workgroup's first key, the wavefront's first and last one
+  const int firstOf = p.causal ? key - off : 0;
+  const int begin = p.causal ? std::min(rows, std::max(0, span.first - off) * p.G) / RT * RT : 0;
+  const int some = p.causal ? std::min(rows, std::max(0, span.first + 32 * wave - off) * p.G) : 0;
+  const int all = p.causal ? std::min(rows, std::max(0, span.first + 32 * wave + 31 - off) * p.G) : 0;
+
+  uintx4 k[T::steps], v[T::steps];
+  {
+    const char* at = p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head;
+    const char* vAt = p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head;
+#pragma unroll
+    for (int s = 0; s < T::steps; ++s) k[s] = chunk_of<V>(at, 2 * s + (lane >> 5), p.D, live);
+#pragma unroll
+    for (int s = 0; s < T::steps; ++s) v[s] = chunk_of<V>(vAt, 2 * s + (lane >> 5), p.D, live);
+  }
+  const char* queries = p.q.data + (long long)span.q0 * p.q.position + (long long)head * p.G * p.q.head;
+  const char* ders = p.dO.data + (long long)span.q0 * p.dO.position + (long long)head * p.G * p.dO.head;
+  const float* statL = p.statL + (long long)head * p.N * p.G + (long long)span.q0 * p.G;
+  const float* statD = p.statD + (long long)head * p.N * p.G + (long long)span.q0 * p.G;
+  const auto bring_tile = [&](char* to, int r0) __attribute__((always_inline)) {
+    const int i0 = p.byG.div(r0);
+    const char* qb = queries + (long long)i0 * p.q.position;
+    const char* db = ders + (long long)i0 * p.dO.position;
+    const auto offset = [&](int r, const Tensor3& t) __attribute__((always_inline)) {
+      int i, g;
+      p.byG.divmod(r0 + r, &i, &g);
+      return r0 + r < rows ? (unsigned)(i - i0) * (unsigned)t.position + (unsigned)g * (unsigned)t.head : kNowhere;
+    };
+    bring<V, DP, RT, NW>(to, qb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return offset(r, p.q); });
+    bring<V, DP, RT, NW>(to + tileBytes, db, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return offset(r, p.dO); });
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    if (wave < 2 && lane < RT) {
+      const float* from = (wave ? statD : statL) + r0;
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, std::min(rows - r0, RT) * 4, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + 2 * tileBytes + wave * statBytes), 4, lane * 4, 0, 0, 0);
+    }
+  };
+  floatx16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
+  if (begin < rows) bring_tile(lds, begin);
+  int turn = 0;
+  for (int r0 = begin; r0 < rows; r0 += RT) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    char* from = lds + turn * bufferBytes;
+    char* to = lds + (turn ^ 1) * bufferBytes;
+    turn ^= 1;
+    const auto bring_next = [&](char* at) __attribute__((always_inline)) {
+      if (r0 + RT < rows) bring_tile(at, r0 + RT);
+    };
+    if (r0 + RT > some)
+      dkv_tile<V, DP, RT>(from, from + tileBytes, (const float*)(from + 2 * tileBytes), (const float*)(from + 2 * tileBytes + statBytes), to, bring_next, k, v, dk,
+                          dv, p.byG, r0, rows, firstOf, r0 < all || r0 + RT > rows, p.c, lane);
+    else bring_next(to);
+  }
+  // (rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN)
+  if (p.causal) {
+    bool good = true;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) good = good && finite(dk[d][r]) && finite(dv[d][r]);
+    if (!both_good(good)) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
+      const V* kj = (const V*)(p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head);
+      const V* vj = (const V*)(p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head);
+#pragma unroll 1
+      for (int row = live ? std::max(0, firstOf) * p.G : rows; row < rows; ++row) {
+        int i, g;
+        p.byG.divmod(row, &i, &g);
+        const V* qi = (const V*)(queries + (long long)i * p.q.position + (long long)g * p.q.head);
+        const V* di = (const V*)(ders + (long long)i * p.dO.position + (long long)g * p.dO.head);
+        float s = statL[row], dp = statD[row];
+#pragma unroll 1
+        for (int d = 0; d < p.D; ++d) {
+          s += value_of(qi + d) * value_of(kj + d);
+          dp += value_of(di + d) * value_of(vj + d);
+        }
+        float e = power2(s * p.c), f = e * dp;
+        if (sizeof(V) == 2) {
+          e = bits_float((unsigned)round_bf16(e) << 16);
+          f = bits_float((unsigned)round_bf16(f) << 16);
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+            if (at < p.D) {
+              dv[d][r] += e * value_of(di + at);
+              dk[d][r] += f * value_of(qi + at);
+            }
+          }
+      }
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int at = 32 * d + 8 * (r / 4) + 4 * (lane >> 5);
+      if (p.dk.data)
+        store4<V>(p.dk.data + (long long)(span.k0 + key) * p.dk.position + head * p.dk.head, at, p.D, p.vector, dk[d][r] * p.scale, dk[d][r + 1] * p.scale,
+                  dk[d][r + 2] * p.scale, dk[d][r + 3] * p.scale);
+      if (p.dv.data)
+        store4<V>(p.dv.data + (long long)(span.k0 + key) * p.dv.position + head * p.dv.head, at, p.D, p.vector, dv[d][r], dv[d][r + 1], dv[d][r + 2],
+                  dv[d][r + 3]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ operands that do not start at 16 bytes
+
+struct PackP {
+  const char* from[5];
+  char* to[5];
+  long long position[5], head[5], items[5];   // (strides in bytes) heads of all positions
+  int heads[5];
+  int D, chunks;
+};
+
+// Heads of any D and strides, laid one behind the other, each a whole number of 16 bytes, zero behind D: a thread per 16 bytes
+template <class V>
+__global__ __launch_bounds__(256) void attention_pack(PackP p) {
+  constexpr int W = 16 / sizeof(V);
+  const int which = blockIdx.y;
+  const long long all = p.items[which] * p.chunks;
+  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < all; t += (long long)gridDim.x * 256) {
+    const long long item = t / p.chunks, position = item / p.heads[which];
+    const int chunk = (int)(t % p.chunks), head = (int)(item % p.heads[which]);
+    const V* from = (const V*)(p.from[which] + position * p.position[which] + head * p.head[which]) + chunk * W;
+    V v[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = chunk * W + e < p.D ? from[e] : V(0);
+    uintx4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      out[e] = sizeof(V) == 4 ? __builtin_bit_cast(unsigned, (float)v[e]) : (unsigned)v[2 * e % W] | (unsigned)v[(2 * e + 1) % W] << 16;
+    *(uintx4*)(p.to[which] + t * 16) = out;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+
+constexpr size_t kAlign = 256;
+size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+int check_heads(const char* who, const char* what, const mcn_heads* t, int heads, int positions, int D, int size, bool written) {
+  if (!t || !t->data) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null %s", who, what);
+  if ((uintptr_t)t->data % size) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %s is not aligned", who, what);
+  if (t->position < 0 || t->head < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative stride of %s", who, what);
+  if (t->position > (1ll << 31) || t->head > (1ll << 40)) return fail(MCN_UNSUPPORTED, "%s: stride of %s too large", who, what);
+  if (!written) return MCN_SUCCESS;
+  const bool inside = (positions <= 1 || t->position >= (long long)(heads - 1) * t->head + D) && (heads <= 1 || t->head >= D);
+  const bool outside = (heads <= 1 || t->head >= (long long)(positions - 1) * t->position + D) && (positions <= 1 || t->position >= D);
+  if (!inside && !outside) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the heads of %s overlap", who, what);
+  return MCN_SUCCESS;
+}
+
+int check_geom(const char* who, const mcn_attention_geom* g) {
+  if (!g) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null geometry", who);
+  if (g->dataType != MCN_FLOAT && g->dataType != MCN_BFLOAT16) return fail(MCN_ILLEGAL_ARGUMENT, "%s: unknown data type %d", who, g->dataType);
+  if (g->D < 0 || g->heads < 0 || g->keyHeads < 0 || g->N < 0 || g->M < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative extent", who);
+  if (g->D > kMostD) return fail(MCN_UNSUPPORTED, "%s: heads of more than %d channels", who, kMostD);
+  if (g->sequences < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative number of sequences", who);
+  if (g->heads && (g->keyHeads == 0 || g->heads % g->keyHeads)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %d heads over %d key heads", who, g->heads, g->keyHeads);
+  if (!(g->scale >= 0) || std::isinf(g->scale)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the scale is negative or no number", who);
+  // (rows of heads, and 256 positions behind the last one, are counted in 31 bits)
+  if (((long long)g->N + 256) * g->heads >= (1ll << 31) || (long long)g->M + 256 >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many positions", who);
+  return MCN_SUCCESS;
+}
+
+struct Operand {
+  const mcn_heads* t;
+  int positions, heads;
+  int together;   // heads that a tile in LDS holds rows of
+};
+
+// read as they lie: 16 bytes at a time, the rows of a tile within 32 bits of each other
+bool lies_well(const Operand& o, int D, int size) {
+  const int V = 16 / size;
+  const long long reach = 1ll << 30;   // bytes
+  return D % V == 0 && aligned16(o.t->data) && o.t->position % V == 0 && o.t->head % V == 0 && o.t->position * size <= reach / 64 &&
+         (o.together == 1 || o.t->head * size <= reach / (o.together - 1));
+}
+
+size_t packed_bytes(int positions, int heads, int D, int size) { return rounded((size_t)positions * heads * (((size_t)D * size + 15) / 16 * 16)); }
+
+struct Plan {
+  int DP, size, G, waves, slices, tiles, keyTiles;
+  size_t partsAt, sumsAt, statAt, packAt, bytes;
+};
+
+// How a forward call is cut.  Rows of a sequence on average up to 32: one wavefront a workgroup, and keys are cut into slices until there
+// are workgroups for the whole chip; otherwise four wavefronts.
+Plan plan_of(const mcn_attention_geom* g, int backward) {
+  Plan l = {};
+  l.size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
+  l.DP = g->D <= 64 ? 64 : 128;
+  l.G = g->keyHeads ? g->heads / g->keyHeads : 1;
+  const int sequences = std::max(1, g->sequences);
+  const long long rows = (long long)g->N * l.G;
+  l.waves = !backward && rows <= 32ll * sequences ? 1 : 4;
+  const int size = 32 * l.waves;
+  l.tiles = (int)(rows / size) + sequences;
+  l.keyTiles = g->M / 128 + sequences;
+  l.slices = 1;
+  if (!backward) {
+    const long long groups = (long long)(rows + size - 1) / size * g->keyHeads, want = 4ll * std::max(1, device_compute_units());
+    const int tile = l.size == 2 ? 64 : 32;
+    const long long most = std::max<long long>(1, g->M / sequences / (4 * tile));
+    l.slices = (int)std::max<long long>(1, std::min<long long>({64, most, want / std::max<long long>(1, groups)}));
+  }
+  size_t at = 0;
+  if (l.slices > 1) {
+    l.partsAt = at;
+    at += rounded((size_t)l.slices * g->N * g->heads * l.DP * sizeof(float));
+    l.sumsAt = at;
+    at += rounded((size_t)l.slices * g->N * g->heads * sizeof(float));
+  }
+  if (backward) {
+    l.statAt = at;
+    at += 2 * rounded((size_t)g->N * g->heads * sizeof(float));
+  }
+  l.packAt = at;
+  at += packed_bytes(g->N, g->heads, g->D, l.size) * (backward ? 3 : 1) + 2 * packed_bytes(g->M, g->keyHeads, g->D, l.size);
+  l.bytes = at;
+  return l;
+}
+
+Tensor3 in_bytes(const mcn_heads* t, int size) {
+  Tensor3 r = {};
+  if (t && t->data) r = {(char*)t->data, t->position * size, t->head * size};
+  return r;
+}
+
+bool stores_well(const mcn_heads* t) { return !t || !t->data || (((uintptr_t)t->data & 15) == 0 && t->position % 4 == 0 && t->head % 4 == 0); }
+
+template <class V>
+int pack(const char* who, hipStream_t s, const PackP& p, int n) {
+  if (!n) return MCN_SUCCESS;
+  long long most = 0;
+  for (int i = 0; i < n; ++i) most = std::max(most, p.items[i] * p.chunks);
+  KernelTimer timer("attention_pack", s);
+  hipLaunchKernelGGL(attention_pack<V>, dim3((unsigned)std::min<long long>((most + 255) / 256, 8192), (unsigned)n), dim3(256), 0, s, p);
+  return check_launch(who);
+}
+
+// The operands of a call where the kernels read them: as they lie, or packed into the workspace
+int place(const char* who, hipStream_t s, const mcn_attention_geom* g, const Plan& l, const Operand* operands, Tensor3** to, int n, char* workspace) {
+  PackP p = {};
+  p.D = g->D;
+  p.chunks = (g->D * l.size + 15) / 16;
+  size_t at = l.packAt;
+  int packs = 0;
+  for (int i = 0; i < n; ++i) {
+    const Operand& o = operands[i];
+    if (lies_well(o, g->D, l.size)) {
+      *to[i] = in_bytes(o.t, l.size);
+      continue;
+    }
+    p.from[packs] = (const char*)o.t->data;
+    p.to[packs] = workspace + at;
+    p.position[packs] = o.t->position * l.size;
+    p.head[packs] = o.t->head * l.size;
+    p.items[packs] = (long long)o.positions * o.heads;
+    p.heads[packs] = std::max(1, o.heads);
+    *to[i] = {workspace + at, (long long)p.chunks * 16 * o.heads, (long long)p.chunks * 16};
+    at += packed_bytes(o.positions, o.heads, g->D, l.size);
+    ++packs;
+  }
+  return g->dataType == MCN_BFLOAT16 ? pack<bf16>(who, s, p, packs) : pack<float>(who, s, p, packs);
+}
+
+void common(AttentionP* p, const mcn_attention_geom* g, const Plan& l, const int* qStarts, const int* kStarts) {
+  p->qStarts = qStarts;
+  p->kStarts = kStarts;
+  p->sequences = g->sequences;
+  p->each = g->sequences ? g->N / g->sequences : 0;
+  p->eachKeys = g->sequences ? g->M / g->sequences : 0;
+  p->D = g->D; p->G = l.G; p->heads = g->heads; p->keyHeads = g->keyHeads;
+  p->N = g->N; p->M = g->M; p->causal = g->causal != 0;
+  p->slices = l.slices;
+  p->byG = FastDiv(l.G);
+  const double scale = g->scale > 0 ? g->scale : 1.0 / std::sqrt((double)g->D);
+  p->scale = (float)scale;
+  p->c = (float)(scale * 1.4426950408889634);
+}
+
+// tiles of all sequences, of `size` rows or keys
+int tiles_of(AttentionP* p, int rowsEach, int size, long long rows) {
+  if (p->qStarts) return (int)(rows / size) + p->sequences;
+  const int each = std::max(1, div_up(rowsEach, size));
+  p->byTiles = FastDiv(each);
+  return each * p->sequences;
+}
+
+template <class V, int DP>
+int forward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
+  constexpr int KT = sizeof(V) == 2 ? 64 : 32;
+  const long long rows = (long long)p.N * p.G;
+  const long long blocks = (long long)tiles_of(&p, p.each * p.G, 32 * l.waves, rows) * p.keyHeads * p.slices;
+  if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+  {
+    KernelTimer timer("attention_forward", s);
+    if (l.waves == 1) hipLaunchKernelGGL((attention_forward<V, DP, 1, KT>), dim3((unsigned)blocks), dim3(64), 0, s, p);
+    else hipLaunchKernelGGL((attention_forward<V, DP, 4, KT>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+  }
+  int rc = check_launch(who);
+  if (rc || p.slices == 1) return rc;
+  KernelTimer timer("attention_join", s);
+  hipLaunchKernelGGL((attention_join<V, DP>), dim3((unsigned)div_up((long long)p.N * p.heads, 4)), dim3(256), 0, s, p);
+  return check_launch(who);
+}
+
+template <class V, int DP>
+int backward(const char* who, hipStream_t s, AttentionP& p) {
+  constexpr int KT = sizeof(V) == 2 ? 64 : 32;
+  if (p.N) {
+    const int tiles = tiles_of(&p, p.each * p.G, 128, (long long)p.N * p.G);
+    if ((long long)tiles * p.keyHeads >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+    KernelTimer timer("attention_dq", s);
+    hipLaunchKernelGGL((attention_dq<V, DP, 4, KT>), dim3((unsigned)(tiles * p.keyHeads)), dim3(256), 0, s, p);
+    const int rc = check_launch(who);
+    if (rc) return rc;
+  }
+  if (!p.M || (!p.dk.data && !p.dv.data)) return MCN_SUCCESS;
+  const int tiles = tiles_of(&p, p.eachKeys, 128, p.M);
+  if ((long long)tiles * p.keyHeads >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+  KernelTimer timer("attention_dkv", s);
+  hipLaunchKernelGGL((attention_dkv<V, DP, 4, 32>), dim3((unsigned)(tiles * p.keyHeads)), dim3(256), 0, s, p);
+  return check_launch(who);
+}
+
+int check_starts(const char* who, const mcn_attention_geom* g, const int* qStarts, const int* kStarts) {
+  if (!qStarts != !kStarts) return fail(MCN_ILLEGAL_ARGUMENT, "%s: starts of queries or of keys alone", who);
+  if (!qStarts && g->sequences && (g->N % g->sequences || g->M % g->sequences))
+    return fail(MCN_ILLEGAL_ARGUMENT, "%s: the positions are not %d sequences of one length", who, g->sequences);
+  return MCN_SUCCESS;
+}
+
+int check_workspace(const char* who, const void* workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, bytes, need);
+  if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
+  return MCN_SUCCESS;
+}
+
+}  // namespace
+}  // namespace mcn
+
+using namespace mcn;
+
+extern "C" {
+
+size_t mcn_attention_workspace_bytes(const mcn_attention_geom* g, int backward) {
+  if (!g || g->D <= 0 || g->heads <= 0 || g->keyHeads <= 0 || g->N < 0 || g->M < 0) return 0;
+  return plan_of(g, backward != 0).bytes;
+}
+
+int mcn_attention_forward(mcn_stream_t stream, const mcn_attention_geom* g, const mcn_heads* o, float* logSums, const mcn_heads* q, const mcn_heads* k,
+                          const mcn_heads* v, const int* queryStarts, const int* keyStarts, void* workspace, size_t workspaceBytes) {
+  const char* who = "mcn_attention_forward";
+  int rc = check_geom(who, g);
+  if (!rc) rc = check_starts(who, g, queryStarts, keyStarts);
+  if (rc || g->D == 0 || g->N == 0 || g->heads == 0 || g->sequences == 0) return rc;
+  const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
+  rc = check_heads(who, "queries", q, g->heads, g->N, g->D, size, false);
+  if (!rc && g->M) rc = check_heads(who, "keys", k, g->keyHeads, g->M, g->D, size, false);
+  if (!rc && g->M) rc = check_heads(who, "values", v, g->keyHeads, g->M, g->D, size, false);
+  if (!rc) rc = check_heads(who, "output", o, g->heads, g->N, g->D, size, true);
+  const Plan l = plan_of(g, 0);
+  if (!rc) rc = check_workspace(who, workspace, workspaceBytes, l.bytes);
+  if (rc) return rc;
+  AttentionP p = {};
+  common(&p, g, l, queryStarts, keyStarts);
+  hipStream_t s = as_stream(stream);
+  Operand operands[3] = {{q, g->N, g->heads, 1}, {k, g->M, g->keyHeads, 1}, {v, g->M, g->keyHeads, 1}};
+  Tensor3* to[3] = {&p.q, &p.k, &p.v};
+  rc = place(who, s, g, l, operands, to, g->M ? 3 : 1, (char*)workspace);
+  if (rc) return rc;
+  p.o = in_bytes(o, size);
+  p.vector = g->D % 4 == 0 && stores_well(o);
+  p.logSums = logSums;
+  p.parts = (float*)((char*)workspace + l.partsAt);
+  p.partSums = (float*)((char*)workspace + l.sumsAt);
+  if (g->dataType == MCN_BFLOAT16) return l.DP == 64 ? forward<bf16, 64>(who, s, p, l) : forward<bf16, 128>(who, s, p, l);
+  return l.DP == 64 ? forward<float, 64>(who, s, p, l) : forward<float, 128>(who, s, p, l);
+}
+
+int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, const mcn_heads* derQ, const mcn_heads* derK, const mcn_heads* derV,
+                           const mcn_heads* o, const float* logSums, const mcn_heads* q, const mcn_heads* k, const mcn_heads* v,
+                           const mcn_heads* derOutput, const int* queryStarts, const int* keyStarts, void* workspace, size_t workspaceBytes) {
+  const char* who = "mcn_attention_backward";
+  int rc = check_geom(who, g);
+  if (!rc) rc = check_starts(who, g, queryStarts, keyStarts);
+  const bool wantQ = derQ && derQ->data, wantK = derK && derK->data, wantV = derV && derV->data;
+  if (rc || g->D == 0 || g->heads == 0 || g->sequences == 0 || (g->N == 0 && g->M == 0) || (!wantQ && !wantK && !wantV)) return rc;
+  const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
+  if (g->N) {
+    rc = check_heads(who, "queries", q, g->heads, g->N, g->D, size, false);
+    if (!rc) rc = check_heads(who, "output", o, g->heads, g->N, g->D, size, false);
+    if (!rc) rc = check_heads(who, "output's derivative", derOutput, g->heads, g->N, g->D, size, false);
+    if (!rc && wantQ) rc = check_heads(who, "queries' derivative", derQ, g->heads, g->N, g->D, size, true);
+    if (!rc && !logSums) rc = fail(MCN_ILLEGAL_ARGUMENT, "%s: null log sums", who);
+  }
+  if (g->M) {
+    if (!rc) rc = check_heads(who, "keys", k, g->keyHeads, g->M, g->D, size, false);
+    if (!rc) rc = check_heads(who, "values", v, g->keyHeads, g->M, g->D, size, false);
+    if (!rc && wantK) rc = check_heads(who, "keys' derivative", derK, g->keyHeads, g->M, g->D, size, true);
+    if (!rc && wantV) rc = check_heads(who, "values' derivative", derV, g->keyHeads, g->M, g->D, size, true);
+  }
+  const Plan l = plan_of(g, 1);
+  if (!rc) rc = check_workspace(who, workspace, workspaceBytes, l.bytes);
+  if (rc) return rc;
+  AttentionP p = {};
+  common(&p, g, l, queryStarts, keyStarts);
+  hipStream_t s = as_stream(stream);
+  Operand operands[5];
+  Tensor3* to[5];
+  int n = 0;
+  const auto add = [&](const mcn_heads* t, int positions, int heads, int together, Tensor3* where) {
+    operands[n] = {t, positions, heads, together};
+    to[n++] = where;
+  };
+  if (g->N) {
+    add(q, g->N, g->heads, l.G, &p.q);
+    add(o, g->N, g->heads, 1, &p.o);
+    add(derOutput, g->N, g->heads, l.G, &p.dO);
+  }
+  if (g->M) {
+    add(k, g->M, g->keyHeads, 1, &p.k);
+    add(v, g->M, g->keyHeads, 1, &p.v);
+  }
+  rc = place(who, s, g, l, operands, to, n, (char*)workspace);
+  if (rc) return rc;
+  p.dq = in_bytes(derQ, size);
+  p.dk = in_bytes(derK, size);
+  p.dv = in_bytes(derV, size);
+  p.vector = g->D % 4 == 0 && stores_well(derQ) && stores_well(derK) && stores_well(derV);
+  p.logSums = const_cast<float*>(logSums);
+  p.statL = (float*)((char*)workspace + l.statAt);
+  p.statD = p.statL + rounded((size_t)g->N * g->heads * sizeof(float)) / sizeof(float);
+  if (g->dataType == MCN_BFLOAT16) return l.DP == 64 ? backward<bf16, 64>(who, s, p) : backward<bf16, 128>(who, s, p);
+  return l.DP == 64 ? backward<float, 64>(who, s, p) : backward<float, 128>(who, s, p);
+}
+
+}  // extern "C"

@@ -71,12 +71,15 @@ __global__ __launch_bounds__(256) void eltwise_kernel(float* __restrict__ y, con
 
 // SGD with momentum over an arena of parameters: one workgroup per chunk of 1024 elements, every chunk inside one
 // parameter, whose rates come from a table.  Each element goes through the roundings of the three scaled sums the
-// reference performs one parameter at a time.
+// reference performs one parameter at a time.  CLIPPED: the factor of the derivatives is read from the device, where the norm left it.
+template <bool CLIPPED>
 __global__ __launch_bounds__(256) void sgd_momentum_kernel(float* __restrict__ value, float* __restrict__ state,
                                                            const float* __restrict__ der,
                                                            const unsigned short* __restrict__ chunkParam,
                                                            const double* __restrict__ rates, double learningRate,
-                                                           double weightDecay, float momentum, float derScale, int nesterov) {
+                                                           double weightDecay, float momentum, float derScale, int nesterov,
+                                                           const float* __restrict__ derFactor) {
+  if (CLIPPED) derScale = *derFactor;
   const int p = chunkParam[blockIdx.x];
   const float lr = (float)(learningRate * rates[2 * p]), decay = (float)(weightDecay * rates[2 * p + 1]);
   if (!(lr > 0.f || decay > 0.f)) return;
@@ -101,6 +104,15 @@ __global__ __launch_bounds__(256) void sgd_momentum_kernel(float* __restrict__ v
   one(v.w, g.w, m.w, vo.w, mo.w);
   stream_store4((float4*)state + i, mo);
   stream_store4((float4*)value + i, vo);
+}
+
+int check_sgd(const char* who, const float* value, const float* state, const float* der, size_t chunks, const unsigned short* chunkParam,
+              const double* rates) {
+  if (!value || !state || !der || !chunkParam || !rates) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null argument", who);
+  if (!aligned16(value) || !aligned16(state) || !aligned16(der))
+    return fail(MCN_ILLEGAL_ARGUMENT, "%s: the arenas must be 16-byte aligned", who);
+  if (chunks >= (1ull << 31)) return fail(MCN_UNSUPPORTED, "%s: arena too large", who);
+  return MCN_SUCCESS;
 }
 
 template <int OP>
@@ -181,14 +193,30 @@ int mcn_sgd_momentum(mcn_stream_t stream, float* value, float* state, const floa
                      const unsigned short* chunkParam, const double* rates, double learningRate, double weightDecay,
                      double momentum, double derScale, int nesterov) {
   if (chunks == 0) return MCN_SUCCESS;
-  if (!value || !state || !der || !chunkParam || !rates) return fail(MCN_ILLEGAL_ARGUMENT, "mcn_sgd_momentum: null argument");
-  if (!aligned16(value) || !aligned16(state) || !aligned16(der))
-    return fail(MCN_ILLEGAL_ARGUMENT, "mcn_sgd_momentum: the arenas must be 16-byte aligned");
-  if (chunks >= (1ull << 31)) return fail(MCN_UNSUPPORTED, "mcn_sgd_momentum: arena too large");
+  int rc = check_sgd("mcn_sgd_momentum", value, state, der, chunks, chunkParam, rates);
+  if (rc) return rc;
   KernelTimer timer("sgd_momentum_kernel", as_stream(stream));
-  hipLaunchKernelGGL(sgd_momentum_kernel, dim3((unsigned)chunks), dim3(256), 0, as_stream(stream), value, state, der,
-                     chunkParam, rates, learningRate, weightDecay, (float)momentum, (float)derScale, nesterov ? 1 : 0);
+  hipLaunchKernelGGL(sgd_momentum_kernel<false>, dim3((unsigned)chunks), dim3(256), 0, as_stream(stream), value, state, der,
+                     chunkParam, rates, learningRate, weightDecay, (float)momentum, (float)derScale, nesterov ? 1 : 0, (const float*)nullptr);
   return check_launch("mcn_sgd_momentum");
+}
+size_t mcn_sgd_momentum_clipped_workspace_bytes(size_t chunks) { return clip_factor_workspace(chunks * MCN_SGD_CHUNK); }
+int mcn_sgd_momentum_clipped(mcn_stream_t stream, float* value, float* state, const float* der, size_t chunks,
+                             const unsigned short* chunkParam, const double* rates, double learningRate, double weightDecay,
+                             double momentum, double derScale, int nesterov, double maxNorm, float* norm, void* workspace,
+                             size_t workspaceBytes) {
+  const char* who = "mcn_sgd_momentum_clipped";
+  if (!(maxNorm >= 0)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the largest norm is negative", who);
+  int rc = chunks ? check_sgd(who, value, state, der, chunks, chunkParam, rates) : MCN_SUCCESS;
+  if (rc) return rc;
+  hipStream_t s = as_stream(stream);
+  float* factor;
+  rc = clip_factor(who, s, norm, &factor, der, chunks * MCN_SGD_CHUNK, derScale, maxNorm, workspace, workspaceBytes);
+  if (rc || chunks == 0) return rc;
+  KernelTimer timer("sgd_momentum_kernel", s);
+  hipLaunchKernelGGL(sgd_momentum_kernel<true>, dim3((unsigned)chunks), dim3(256), 0, s, value, state, der, chunkParam, rates, learningRate,
+                     weightDecay, (float)momentum, 0.f, nesterov ? 1 : 0, (const float*)factor);
+  return check_launch(who);
 }
 int mcn_convert(mcn_stream_t stream, void* dst, int dstType, const void* src, int srcType, size_t n) {
   if ((dstType != MCN_FLOAT && dstType != MCN_BFLOAT16) || (srcType != MCN_FLOAT && srcType != MCN_BFLOAT16))

@@ -42,6 +42,11 @@ class KernelTimer {
   hipStream_t stream;
 };
 
+// The factor that brings derScale * der under the norm `most`, times derScale, on the device (in the workspace); *norm (may be null) the norm.
+size_t clip_factor_workspace(size_t count);
+int clip_factor(const char* who, hipStream_t s, float* norm, float** factor, const float* der, size_t count, double derScale, double most, void* workspace,
+                size_t workspaceBytes);
+
 inline hipStream_t as_stream(mcn_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
