@@ -33,12 +33,16 @@ typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMostD = 128;
-constexpr unsigned kNowhere = 0xfffffff0u;   // an offset behind every buffer: reads zero
+constexpr unsigned kNowhere = 0x80000000u;   // an offset behind every buffer, and so is what is a tile's size further on: reads zero
 
 __device__ __forceinline__ float bits_float(unsigned v) { return __builtin_bit_cast(float, v); }
 __device__ __forceinline__ unsigned float_bits(float v) { return __builtin_bit_cast(unsigned, v); }
 __device__ __forceinline__ unsigned short round_bf16(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
-__device__ __forceinline__ unsigned pack_bf16(float a, float b) { return (unsigned)round_bf16(a) | (unsigned)round_bf16(b) << 16; }
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bfx2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2){a, b}, bfx2));
+}
 __device__ __forceinline__ float value_of(const float* p) { return *p; }
 __device__ __forceinline__ float value_of(const bf16* p) { return bits_float((unsigned)*p << 16); }
 __device__ __forceinline__ float power2(float v) { return __builtin_amdgcn_exp2f(v); }
@@ -60,7 +64,7 @@ struct Tensor3 {            // heads where they lie, strides in bytes
 struct AttentionP {
   Tensor3 q, k, v, o, dO, dq, dk, dv;
   float *logSums, *parts, *partSums;     // parts: a slice's o (normalised) and log sums
-  float *statL, *statD;                  // backward, [keyHeads][N G]: -L/scale, -delta
+  float *statL, *statD;                  // backward, [heads][N]: -L/scale, -delta
   const int *qStarts, *kStarts;
   int sequences, each, eachKeys;         // without starts: queries and keys of a sequence
   int D, G, heads, keyHeads, N, M, causal;
@@ -97,6 +101,14 @@ template <> struct Matrix<float> {
     return s;
   }
 };
+
+// Keeps what follows from the lane's number inside a loop's body: addresses made ahead of the loop take registers that the backward kernels do
+// not have (with 128 channels they were kept in memory, and every read of one waited for the tile that was on its way).
+template <class V, int DP>
+__device__ __forceinline__ int fresh(int lane) {
+  if (sizeof(V) == 2 && DP == 128) asm volatile("" : "+v"(lane));
+  return lane;
+}
 
 // A tile in LDS: rows of DP values, chunk c (16 bytes) of a row at c ^ turn(row).  bfloat16: four rows that a transposing read takes lie in four
 // 64-byte runs of banks, and sixteen rows put a chunk in sixteen places; single precision: the latter.
@@ -150,23 +162,37 @@ struct Tile {
   }
 };
 
-// Brings ROWS rows of a tile into LDS: wavefront w the 1024-byte pieces w, w + NW, ...  Offsets of rows come from `offset_of(row)`, in bytes
-// from the buffer's base, kNowhere for rows that are not there; columns behind D read as zero.
-template <class V, int DP, int ROWS, int NW, class Offset>
-__device__ __forceinline__ void bring(char* lds, const char* base, int D, int wave, int lane, Offset offset_of) {
+// Brings ROWS rows of a tile into LDS: wavefront w the 1024-byte pieces w, w + NW, ...  A lane's offsets are made once; where the rows of its
+// pieces are 16 apart (the turn's period) they follow from the first.  What is behind the rows that are left, or behind D, reads as zero.
+template <class V, int DP, int ROWS, int NW>
+struct Loader {
   typedef Tile<V, DP> T;
-  typedef __attribute__((address_space(3))) void* lds_ptr;
-  constexpr int pieces = ROWS * T::rowBytes / 1024;
-  static_assert(pieces % NW == 0, "whole pieces");
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)kNowhere, 0x00020000);
+  static constexpr int pieces = ROWS * T::rowBytes / 1024 / NW, rowsOfPiece = 1024 / T::rowBytes;
+  static constexpr bool periodic = NW * rowsOfPiece % 16 == 0;
+  static_assert(ROWS * T::rowBytes % (1024 * NW) == 0, "whole pieces");
+  unsigned offset[periodic ? 1 : pieces];
+  unsigned pitch, width;   // bytes from row to row, and of a row
+  __device__ __forceinline__ void begin(const Tensor3& t, int D, int wave, int lane) {
+    pitch = (unsigned)t.position;
+    width = (unsigned)(D * (int)sizeof(V) + 15) / 16 * 16;   // (rows that were packed are whole pieces of 16 bytes)
 #pragma unroll
-  for (int i = 0; i < pieces / NW; ++i) {
-    const int slot = (i * NW + wave) * 64 + lane, row = slot / T::chunks, chunk = (slot % T::chunks) ^ T::turn(row);
-    const unsigned at = offset_of(row);
-    const unsigned offset = at == kNowhere || chunk * Matrix<V>::perChunk >= D ? kNowhere : at + chunk * 16u;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (i * NW + wave) * 1024), 16, (int)offset, 0, 0, 0);
+    for (int i = 0; i < (periodic ? 1 : pieces); ++i) {
+      const int slot = (i * NW + wave) * 64 + lane, row = slot / T::chunks, chunk = (slot % T::chunks) ^ T::turn(row);
+      offset[i] = chunk * Matrix<V>::perChunk >= D ? kNowhere : row * pitch + chunk * 16u;
+    }
   }
-}
+  // from: the tile's first row; left: rows from there on (may be none)
+  __device__ __forceinline__ void bring(char* lds, const char* from, int left, int wave) const {
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    const unsigned records = left <= 0 ? 0u : (unsigned)(std::min(left, ROWS) - 1) * pitch + width;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (int)records, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < pieces; ++i) {
+      const unsigned at = periodic ? offset[0] + i * (NW * rowsOfPiece) * pitch : offset[i];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + (i * NW + wave) * 1024), 16, (int)at, 0, 0, 0);
+    }
+  }
+};
 
 // 16 bytes of a row in global memory, zero where there is none
 template <class V>
@@ -346,13 +372,16 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
   }
   const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
   const char* values = p.v.data + (long long)span.k0 * p.v.position + head * p.v.head;
-  const unsigned kPitch = (unsigned)p.k.position, vPitch = (unsigned)p.v.position;
-  const auto bring_tile = [&](char* to, int j0) __attribute__((always_inline)) {
-    const int left = end - j0;
-    const char* kb = keys + (long long)j0 * p.k.position;
-    const char* vb = values + (long long)j0 * p.v.position;
-    bring<V, DP, KT, NW>(to, kb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * kPitch : kNowhere; });
-    bring<V, DP, KT, NW>(to + tileBytes, vb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * vPitch : kNowhere; });
+  Loader<V, DP, KT, NW> loadK, loadV;
+  loadK.begin(p.k, p.D, wave, lane);
+  loadV.begin(p.v, p.D, wave, lane);
+  const char* nextK = keys + (long long)begin * p.k.position;   // the tile that is brought next
+  const char* nextV = values + (long long)begin * p.v.position;
+  const auto bring_tile = [&](char* to, int left) __attribute__((always_inline)) {
+    loadK.bring(to, nextK, left, wave);
+    loadV.bring(to + tileBytes, nextV, left, wave);
+    nextK += (long long)KT * p.k.position;
+    nextV += (long long)KT * p.v.position;
   };
   floatx16 o[DP / 32];
 #pragma unroll
@@ -360,7 +389,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float most = -INFINITY, sum = 0.f;
-  if (begin < end) bring_tile(lds, begin);
+  if (begin < end) bring_tile(lds, end - begin);
   int turn = 0;
   for (int j0 = begin; j0 < end; j0 += KT) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -368,7 +397,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
     char* to = lds + (turn ^ 1) * 2 * tileBytes;
     turn ^= 1;
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
-      if (j0 + KT < end) bring_tile(at, j0 + KT);
+      if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
     if (j0 < some)
       forward_tile<V, DP, KT>(from, from + tileBytes, to, bring_next, q, o, most, sum, j0, std::min(limit, end), j0 + KT > std::min(all, end), p.c, lane);
@@ -477,6 +506,7 @@ __device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const cha
                                         float negDelta, int j0, int limit, bool edge, float c, int lane) {
   typedef Tile<V, DP> T;
   bring_next(next);
+  lane = fresh<V, DP>(lane);
 #pragma unroll
   for (int b = 0; b < KT / 32; ++b) {
     floatx16 s, dp;
@@ -544,7 +574,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
     negL = p.logSums[position * p.heads + column];
     negL = negL == -INFINITY ? 0.f : -negL / p.scale;
     if (lane < 32) {
-      const long long at = (long long)head * p.N * p.G + (long long)span.q0 * p.G + row;
+      const long long at = (long long)column * p.N + position;
       p.statL[at] = negL;
       p.statD[at] = negDelta;
     }
@@ -552,20 +582,23 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
   if (!p.dq.data) return;
   const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
   const char* values = p.v.data + (long long)span.k0 * p.v.position + head * p.v.head;
-  const unsigned kPitch = (unsigned)p.k.position, vPitch = (unsigned)p.v.position;
-  const auto bring_tile = [&](char* to, int j0) __attribute__((always_inline)) {
-    const int left = end - j0;
-    const char* kb = keys + (long long)j0 * p.k.position;
-    const char* vb = values + (long long)j0 * p.v.position;
-    bring<V, DP, KT, NW>(to, kb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * kPitch : kNowhere; });
-    bring<V, DP, KT, NW>(to + tileBytes, vb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return r < left ? r * vPitch : kNowhere; });
+  Loader<V, DP, KT, NW> loadK, loadV;
+  loadK.begin(p.k, p.D, wave, lane);
+  loadV.begin(p.v, p.D, wave, lane);
+  const char* nextK = keys;   // the tile that is brought next
+  const char* nextV = values;
+  const auto bring_tile = [&](char* to, int left) __attribute__((always_inline)) {
+    loadK.bring(to, nextK, left, wave);
+    loadV.bring(to + tileBytes, nextV, left, wave);
+    nextK += (long long)KT * p.k.position;
+    nextV += (long long)KT * p.v.position;
   };
   floatx16 dq[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
-  if (end > 0) bring_tile(lds, 0);
+  if (end > 0) bring_tile(lds, end);
   int turn = 0;
   for (int j0 = 0; j0 < end; j0 += KT) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -573,7 +606,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
     char* to = lds + (turn ^ 1) * 2 * tileBytes;
     turn ^= 1;
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
-      if (j0 + KT < end) bring_tile(at, j0 + KT);
+      if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
     if (j0 < some) dq_tile<V, DP, KT>(from, from + tileBytes, to, bring_next, q, dO, dq, negL, negDelta, j0, limit, j0 + KT > std::min(all, end), p.c, lane);
     else bring_next(to);
@@ -626,14 +659,15 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
 
 // ------------------------------------------------------------------------------------------ dk, dv
 
-// One tile of RT rows against a wavefront's 32 keys
+// One tile of RT positions of a head against a wavefront's 32 keys
 template <class V, int DP, int RT, class Bring>
 __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const char* __restrict__ ders, const float* __restrict__ statL,
                                          const float* __restrict__ statD, char* __restrict__ next, Bring bring_next, const uintx4 (&k)[Tile<V, DP>::steps],
-                                         const uintx4 (&v)[Tile<V, DP>::steps], floatx16 (&dk)[DP / 32], floatx16 (&dv)[DP / 32], const FastDiv& byG, int r0,
-                                         int rows, int firstOf, bool edge, float c, int lane) {
+                                         const uintx4 (&v)[Tile<V, DP>::steps], floatx16 (&dk)[DP / 32], floatx16 (&dv)[DP / 32], int i0, int n, int firstOf,
+                                         bool edge, float c, int lane) {
   typedef Tile<V, DP> T;
   bring_next(next);
+  lane = fresh<V, DP>(lane);
 #pragma unroll
   for (int b = 0; b < RT / 32; ++b) {
     floatx16 s, dp;
@@ -650,8 +684,8 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
     if (edge) {   // (firstOf: the first position that sees this lane's key)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = r0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-        if (row >= rows || byG.div(row) < firstOf) e[r] = 0.f;
+        const int i = i0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+        if (i >= n || i < firstOf) e[r] = 0.f;
       }
     }
     uintx4 operand[sizeof(V) == 4 ? 4 : 2];
@@ -673,6 +707,7 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
   }
 }
 
+// NW wavefronts of 32 keys; they walk over the positions of one head of the group after the other
 template <class V, int DP, int NW, int RT>
 __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv(AttentionP p) {
   typedef Tile<V, DP> T;
@@ -683,14 +718,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
   const int head = blockIdx.x % p.keyHeads;
   const Span span = find<32 * NW, true, false>(p, blockIdx.x / p.keyHeads, lane);
   if (span.first < 0) return;
-  const int rows = span.n * p.G, off = span.m - span.n;
+  const int off = span.m - span.n;
   const int key = span.first + 32 * wave + (lane & 31);
   const bool live = key < span.m;
-  // the first position that sees the lane's key, the workgroup's first key, the wavefront's first and last one
+  // the first position that sees the lane's key, the workgroup's first key (from a tile's border on), the wavefront's first and its last one
   const int firstOf = p.causal ? key - off : 0;
-  const int begin = p.causal ? std::min(rows, std::max(0, span.first - off) * p.G) / RT * RT : 0;
-  const int some = p.causal ? std::min(rows, std::max(0, span.first + 32 * wave - off) * p.G) : 0;
-  const int all = p.causal ? std::min(rows, std::max(0, span.first + 32 * wave + 31 - off) * p.G) : 0;
+  const int begin = p.causal ? std::max(0, span.first - off) / RT * RT : 0;
+  const int some = p.causal ? span.first + 32 * wave - off : 0;
+  const int all = p.causal ? span.first + 32 * wave + 31 - off : 0;
 
   uintx4 k[T::steps], v[T::steps];
   {
@@ -703,24 +738,34 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
   }
   const char* queries = p.q.data + (long long)span.q0 * p.q.position + (long long)head * p.G * p.q.head;
   const char* ders = p.dO.data + (long long)span.q0 * p.dO.position + (long long)head * p.G * p.dO.head;
-  const float* statL = p.statL + (long long)head * p.N * p.G + (long long)span.q0 * p.G;
-  const float* statD = p.statD + (long long)head * p.N * p.G + (long long)span.q0 * p.G;
-  const auto bring_tile = [&](char* to, int r0) __attribute__((always_inline)) {
-    const int i0 = p.byG.div(r0);
-    const char* qb = queries + (long long)i0 * p.q.position;
-    const char* db = ders + (long long)i0 * p.dO.position;
-    const auto offset = [&](int r, const Tensor3& t) __attribute__((always_inline)) {
-      int i, g;
-      p.byG.divmod(r0 + r, &i, &g);
-      return r0 + r < rows ? (unsigned)(i - i0) * (unsigned)t.position + (unsigned)g * (unsigned)t.head : kNowhere;
-    };
-    bring<V, DP, RT, NW>(to, qb, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return offset(r, p.q); });
-    bring<V, DP, RT, NW>(to + tileBytes, db, p.D, wave, lane, [&](int r) __attribute__((always_inline)) { return offset(r, p.dO); });
+  const float* statL = p.statL + (long long)head * p.G * p.N + span.q0;
+  const float* statD = p.statD + (long long)head * p.G * p.N + span.q0;
+  Loader<V, DP, RT, NW> loadQ, loadD;
+  loadQ.begin(p.q, p.D, wave, lane);
+  loadD.begin(p.dO, p.D, wave, lane);
+  // the tile that is brought next: position nextI of the head whose first positions are at headQ, headD, headStat
+  const char *headQ = queries, *headD = ders;
+  const char *nextQ = queries + (long long)begin * p.q.position, *nextD = ders + (long long)begin * p.dO.position;
+  const float* headStat = wave ? statD : statL;   // (of the first two wavefronts)
+  int nextI = begin;
+  const auto bring_tile = [&](char* to) __attribute__((always_inline)) {
+    loadQ.bring(to, nextQ, span.n - nextI, wave);
+    loadD.bring(to + tileBytes, nextD, span.n - nextI, wave);
     typedef __attribute__((address_space(3))) void* lds_ptr;
     if (wave < 2 && lane < RT) {
-      const float* from = (wave ? statD : statL) + r0;
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, std::min(rows - r0, RT) * 4, 0x00020000);
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(headStat + nextI), 0, std::min(span.n - nextI, RT) * 4, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + 2 * tileBytes + wave * statBytes), 4, lane * 4, 0, 0, 0);
+    }
+    nextI += RT;
+    nextQ += (long long)RT * p.q.position;
+    nextD += (long long)RT * p.dO.position;
+    if (nextI >= span.n) {   // the next head
+      nextI = begin;
+      headQ += p.q.head;
+      headD += p.dO.head;
+      headStat += p.N;
+      nextQ = headQ + (long long)begin * p.q.position;
+      nextD = headD + (long long)begin * p.dO.position;
     }
   };
   floatx16 dk[DP / 32], dv[DP / 32];
@@ -728,20 +773,23 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
-  if (begin < rows) bring_tile(lds, begin);
-  int turn = 0;
-  for (int r0 = begin; r0 < rows; r0 += RT) {
+  const int each = begin < span.n ? (span.n - begin + RT - 1) / RT : 0, tiles = each * p.G;
+  if (tiles) bring_tile(lds);
+  int turn = 0, i0 = begin;
+  for (int t = 0; t < tiles; ++t) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     char* from = lds + turn * bufferBytes;
     char* to = lds + (turn ^ 1) * bufferBytes;
     turn ^= 1;
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
-      if (r0 + RT < rows) bring_tile(at, r0 + RT);
+      if (t + 1 < tiles) bring_tile(at);
     };
-    if (r0 + RT > some)
+    if (i0 + RT > some)
       dkv_tile<V, DP, RT>(from, from + tileBytes, (const float*)(from + 2 * tileBytes), (const float*)(from + 2 * tileBytes + statBytes), to, bring_next, k, v, dk,
-                          dv, p.byG, r0, rows, firstOf, r0 < all || r0 + RT > rows, p.c, lane);
+                          dv, i0, span.n, firstOf, i0 < all || i0 + RT > span.n, p.c, lane);
     else bring_next(to);
+    i0 += RT;
+    if (i0 >= span.n) i0 = begin;
   }
   // (rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN)
   if (p.causal) {
@@ -758,12 +806,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
       const V* kj = (const V*)(p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head);
       const V* vj = (const V*)(p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head);
 #pragma unroll 1
-      for (int row = live ? std::max(0, firstOf) * p.G : rows; row < rows; ++row) {
-        int i, g;
-        p.byG.divmod(row, &i, &g);
+      for (int t = 0; t < p.G * span.n; ++t) {
+        const int g = t / span.n, i = t % span.n;
+        if (!live || i < firstOf) continue;
         const V* qi = (const V*)(queries + (long long)i * p.q.position + (long long)g * p.q.head);
         const V* di = (const V*)(ders + (long long)i * p.dO.position + (long long)g * p.dO.head);
-        float s = statL[row], dp = statD[row];
+        float s = statL[(long long)g * p.N + i], dp = statD[(long long)g * p.N + i];
 #pragma unroll 1
         for (int d = 0; d < p.D; ++d) {
           s += value_of(qi + d) * value_of(kj + d);
@@ -866,15 +914,13 @@ int check_geom(const char* who, const mcn_attention_geom* g) {
 struct Operand {
   const mcn_heads* t;
   int positions, heads;
-  int together;   // heads that a tile in LDS holds rows of
 };
 
-// read as they lie: 16 bytes at a time, the rows of a tile within 32 bits of each other
+// read as they lie: 16 bytes at a time, rows one behind the other, those of a tile within 2^30 bytes
 bool lies_well(const Operand& o, int D, int size) {
   const int V = 16 / size;
-  const long long reach = 1ll << 30;   // bytes
-  return D % V == 0 && aligned16(o.t->data) && o.t->position % V == 0 && o.t->head % V == 0 && o.t->position * size <= reach / 64 &&
-         (o.together == 1 || o.t->head * size <= reach / (o.together - 1));
+  return D % V == 0 && aligned16(o.t->data) && o.t->position % V == 0 && o.t->head % V == 0 && o.t->position * size <= (1ll << 30) / 64 &&
+         (o.positions <= 1 || o.t->position >= D);
 }
 
 size_t packed_bytes(int positions, int heads, int D, int size) { return rounded((size_t)positions * heads * (((size_t)D * size + 15) / 16 * 16)); }
@@ -1067,7 +1113,7 @@ int mcn_attention_forward(mcn_stream_t stream, const mcn_attention_geom* g, cons
   AttentionP p = {};
   common(&p, g, l, queryStarts, keyStarts);
   hipStream_t s = as_stream(stream);
-  Operand operands[3] = {{q, g->N, g->heads, 1}, {k, g->M, g->keyHeads, 1}, {v, g->M, g->keyHeads, 1}};
+  Operand operands[3] = {{q, g->N, g->heads}, {k, g->M, g->keyHeads}, {v, g->M, g->keyHeads}};
   Tensor3* to[3] = {&p.q, &p.k, &p.v};
   rc = place(who, s, g, l, operands, to, g->M ? 3 : 1, (char*)workspace);
   if (rc) return rc;
@@ -1111,18 +1157,18 @@ int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, con
   Operand operands[5];
   Tensor3* to[5];
   int n = 0;
-  const auto add = [&](const mcn_heads* t, int positions, int heads, int together, Tensor3* where) {
-    operands[n] = {t, positions, heads, together};
+  const auto add = [&](const mcn_heads* t, int positions, int heads, Tensor3* where) {
+    operands[n] = {t, positions, heads};
     to[n++] = where;
   };
   if (g->N) {
-    add(q, g->N, g->heads, l.G, &p.q);
-    add(o, g->N, g->heads, 1, &p.o);
-    add(derOutput, g->N, g->heads, l.G, &p.dO);
+    add(q, g->N, g->heads, &p.q);
+    add(o, g->N, g->heads, &p.o);
+    add(derOutput, g->N, g->heads, &p.dO);
   }
   if (g->M) {
-    add(k, g->M, g->keyHeads, 1, &p.k);
-    add(v, g->M, g->keyHeads, 1, &p.v);
+    add(k, g->M, g->keyHeads, &p.k);
+    add(v, g->M, g->keyHeads, &p.v);
   }
   rc = place(who, s, g, l, operands, to, n, (char*)workspace);
   if (rc) return rc;
