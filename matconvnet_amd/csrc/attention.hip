@@ -69,7 +69,7 @@ struct AttentionP {
   int sequences, each, eachKeys;         // without starts: queries and keys of a sequence
   int D, G, heads, keyHeads, N, M, causal;
   int tiles, slices, vector;             // vector: outputs may be stored four values at a time
-  FastDiv byG, byTiles;                  // tiles of a sequence, without starts
+  FastDiv byG, byTiles, bySequences;     // (tiles of a sequence, sequences: without starts)
   float scale, c;                        // c = scale log2 e
 };
 
@@ -104,17 +104,18 @@ template <> struct Matrix<float> {
 
 // Keeps what follows from the lane's number inside a loop's body: addresses made ahead of the loop take registers that the backward kernels do
 // not have (with 128 channels they were kept in memory, and every read of one waited for the tile that was on its way).
-template <class V, int DP>
+template <class V, int DW>
 __device__ __forceinline__ int fresh(int lane) {
-  if (sizeof(V) == 2 && DP == 128) asm volatile("" : "+v"(lane));
+  if (sizeof(V) == 2 && DW == 128) asm volatile("" : "+v"(lane));
   return lane;
 }
 
-// A tile in LDS: rows of DP values, chunk c (16 bytes) of a row at c ^ turn(row).  bfloat16: four rows that a transposing read takes lie in four
+// A tile in LDS: rows of DP values, of which the products take DW; chunk c (16 bytes) of a row at c ^ turn(row).  bfloat16: four rows that a transposing read takes lie in four
 // 64-byte runs of banks, and sixteen rows put a chunk in sixteen places; single precision: the latter.
-template <class V, int DP>
+template <class V, int DW>
 struct Tile {
-  static constexpr int rowBytes = DP * (int)sizeof(V), chunks = rowBytes / 16, steps = chunks / 2, blocks = DP / 32;
+  static constexpr int DP = DW <= 64 ? 64 : 128;
+  static constexpr int rowBytes = DP * (int)sizeof(V), chunks = rowBytes / 16, steps = DW * (int)sizeof(V) / 32, blocks = DW / 32;
   __device__ static __forceinline__ int turn(int row) {
     if (sizeof(V) == 4) return row & 15;
     return chunks == 16 ? ((row & 3) << 2 | (row >> 2 & 3)) : ((row >> 1 & 1) << 2 | (row >> 2 & 3));
@@ -164,9 +165,9 @@ struct Tile {
 
 // Brings ROWS rows of a tile into LDS: wavefront w the 1024-byte pieces w, w + NW, ...  A lane's offsets are made once; where the rows of its
 // pieces are 16 apart (the turn's period) they follow from the first.  What is behind the rows that are left, or behind D, reads as zero.
-template <class V, int DP, int ROWS, int NW>
+template <class V, int DW, int ROWS, int NW>
 struct Loader {
-  typedef Tile<V, DP> T;
+  typedef Tile<V, DW> T;
   static constexpr int pieces = ROWS * T::rowBytes / 1024 / NW, rowsOfPiece = 1024 / T::rowBytes;
   static constexpr bool periodic = NW * rowsOfPiece % 16 == 0;
   static_assert(ROWS * T::rowBytes % (1024 * NW) == 0, "whole pieces");
@@ -229,23 +230,70 @@ struct Span {
 
 __device__ __forceinline__ int clamped(int v, int most) { return v < 0 ? 0 : v > most ? most : v; }
 
-// Tile `tile` of SIZE rows (KEYS: keys).  With starts, sequence s has the tiles from before(s)/SIZE + s on, before(s) the rows ahead of it:
-// no tile holds two sequences, and floor(b/SIZE) + 1 numbers are enough for any sequence, so the tiles of all are known without
-// looking at the starts on the host.  The sequence of a tile is found 64 candidates at a time, all loads of a step at once.  HEAVY_FIRST:
-// a sequence's tiles in the order of falling work (causal).
-template <int SIZE, bool KEYS, bool LAST_FIRST>
+__device__ __forceinline__ int wave_total(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+// Tile `tile` of SIZE rows (KEYS: keys) of all sequences'.  Causal tiles differ in their work (rows: the last of a sequence see the most keys;
+// keys: the first are seen by the most rows), so they are taken in the order of falling work, over all sequences: of the
+// `level`-th most first.  (13 sequences of up to 1100 positions, dk and dv: a sequence's tiles one after the other left a tail of a third.)
+// With starts on the device and more than 64 sequences, sequence s has the tiles from before(s)/SIZE + s on, before(s) the rows ahead
+// of it: no tile holds two sequences, floor(b/SIZE) + 1 numbers are enough for any, so the number of all tiles is known without the starts;
+// the sequence is found 64 candidates at a time, all loads of a step at once.
+template <int SIZE, bool KEYS>
 __device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
   Span s;
-  int t;
+  int t = -1, lo;
   if (!p.qStarts) {
     int seq;
-    p.byTiles.divmod(tile, &seq, &t);
+    const int tiles = p.byTiles.d;
+    if (p.causal) {
+      p.bySequences.divmod(tile, &t, &seq);
+      if (!KEYS) t = tiles - 1 - t;
+    } else {
+      p.byTiles.divmod(tile, &seq, &t);
+    }
     s.q0 = seq * p.each; s.n = p.each;
     s.k0 = seq * p.eachKeys; s.m = p.eachKeys;
-    if (seq >= p.sequences) s.n = s.m = 0;
+    const int rows = KEYS ? s.m : s.n * p.G;
+    s.first = t >= 0 && t * SIZE < rows ? t * SIZE : -1;
+    return s;
+  }
+  if (p.causal && p.sequences <= 64) {
+    int count = 0;   // tiles of sequence `lane`
+    if (lane < p.sequences) {
+      const int* at = KEYS ? p.kStarts : p.qStarts;
+      const int most = KEYS ? p.M : p.N;
+      count = std::max(0, clamped(at[lane + 1], most) - clamped(at[lane], most)) * (KEYS ? 1 : p.G);
+      count = (count + SIZE - 1) / SIZE;
+    }
+    int low = 1, high = count;   // level l: tiles with l - 1 lighter ones in their sequence; those of level `low` or above are more than `tile`
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) high = std::max(high, __shfl_xor(high, o, kWave));
+    ++high;
+    int above = 0;               // tiles of level `high` or above
+    if (wave_total(count) <= tile) low = 0;
+    else
+      while (high - low > 1) {
+        const int mid = (low + high) / 2, total = wave_total(std::max(0, count - mid + 1));
+        if (total > tile) low = mid;
+        else {
+          high = mid;
+          above = total;
+        }
+      }
+    const unsigned long long some = __ballot(count >= low && lane < p.sequences);
+    const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0));
+    const unsigned long long one = __ballot((some >> lane & 1) && rank == tile - above);
+    lo = one && low ? __builtin_ctzll(one) : 0;
+    const int tiles = __shfl(count, lo, kWave);
+    t = !low || !one ? -1 : KEYS ? tiles - low : low - 1;
   } else {
     const auto before = [&](int i) { return (KEYS ? clamped(p.kStarts[i], p.M) : clamped(p.qStarts[i], p.N) * p.G) / SIZE + i; };
-    int lo = 0, n = p.sequences;
+    int n = p.sequences;
+    lo = 0;
     while (n > 1) {
       const int step = (n + 63) / 64, i = lo + lane * step;
       const unsigned long long below = __ballot(lane * step < n && before(i) <= tile);
@@ -253,17 +301,17 @@ __device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
       lo += found * step;
       n = std::min(step, n - found * step);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
     t = tile - before(lo);
-    s.q0 = clamped(p.qStarts[lo], p.N);
-    s.n = clamped(p.qStarts[lo + 1], p.N) - s.q0;
-    s.k0 = clamped(p.kStarts[lo], p.M);
-    s.m = clamped(p.kStarts[lo + 1], p.M) - s.k0;
-    if (s.n < 0) s.n = 0;
-    if (s.m < 0) s.m = 0;
   }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  t = __builtin_amdgcn_readfirstlane(t);
+  s.q0 = clamped(p.qStarts[lo], p.N);
+  s.n = std::max(0, clamped(p.qStarts[lo + 1], p.N) - s.q0);
+  s.k0 = clamped(p.kStarts[lo], p.M);
+  s.m = std::max(0, clamped(p.kStarts[lo + 1], p.M) - s.k0);
   const int rows = KEYS ? s.m : s.n * p.G, tiles = (rows + SIZE - 1) / SIZE;
-  s.first = t < 0 || t >= tiles ? -1 : (LAST_FIRST && p.causal ? tiles - 1 - t : t) * SIZE;
+  if (p.causal && !KEYS && p.sequences > 64 && t >= 0) t = tiles - 1 - t;   // (within a sequence, at least)
+  s.first = t < 0 || t >= tiles ? -1 : t * SIZE;
   return s;
 }
 
@@ -271,14 +319,13 @@ __device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
 
 constexpr int kAhead = 2;   // tiles in LDS at a time
 
-// One tile of KT keys: fragments of 32 queries (q) against it.  `next` is filled meanwhile.  (A function of its own with `restrict` pointers:
+// KB blocks of 32 keys of a tile: fragments of 32 queries (q) against them.  `next` is filled meanwhile.  (A function of its own with `restrict` pointers:
 // that the loads fill none of what is read is what lets the reads go without waiting for them.)
-template <class V, int DP, int KT, class Bring>
+template <class V, int DW, int KB, class Bring>
 __device__ __forceinline__ void forward_tile(const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next, Bring bring_next,
-                                             const uintx4 (&q)[Tile<V, DP>::steps], floatx16 (&o)[DP / 32], float& most, float& sum, int j0, int limit,
+                                             const uintx4 (&q)[Tile<V, DW>::steps], floatx16 (&o)[DW / 32], float& most, float& sum, int j0, int limit,
                                              bool edge, float c, int lane) {
-  typedef Tile<V, DP> T;
-  constexpr int KB = KT / 32;
+  typedef Tile<V, DW> T;
   bring_next(next);
   floatx16 s[KB];
 #pragma unroll
@@ -310,7 +357,7 @@ __device__ __forceinline__ void forward_tile(const char* __restrict__ keys, cons
     most = to;
     sum *= f;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] *= f;
   }
@@ -325,32 +372,33 @@ __device__ __forceinline__ void forward_tile(const char* __restrict__ keys, cons
     uintx4 operand[sizeof(V) == 4 ? 4 : 2];
     T::operand(operand, e);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) o[d] = T::across(values, 32 * b, d, lane, operand, o[d]);
+    for (int d = 0; d < DW / 32; ++d) o[d] = T::across(values, 32 * b, d, lane, operand, o[d]);
   }
 }
 
-// NW wavefronts of 32 rows, tiles of KT keys
-template <class V, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(AttentionP p) {
-  typedef Tile<V, DP> T;
-  constexpr int tileBytes = KT * T::rowBytes;
+// NB blocks of 32 rows, tiles of KT keys; NS wavefronts share a block, each takes its blocks of 32 keys of every tile, and what they have is put
+// together through LDS.
+template <class V, int DW, int NB, int NS, int KT>
+__global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_forward(AttentionP p) {
+  typedef Tile<V, DW> T;
+  constexpr int NW = NB * NS, KB = KT / 32 / NS, tileBytes = KT * T::rowBytes;
   __shared__ __attribute__((aligned(16))) char lds[kAhead * 2 * tileBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = wave % NB, share0 = wave / NB * KB * 32;
   int id = blockIdx.x;
   const int head = id % p.keyHeads;
   id /= p.keyHeads;
   const int slice = id % p.slices;
-  const Span span = find<32 * NW, false, true>(p, id / p.slices, lane);
+  const Span span = find<32 * NB, false>(p, id / p.slices, lane);
   if (span.first < 0) return;
   const int rows = span.n * p.G, off = span.m - span.n;
-  const int row = span.first + 32 * wave + (lane & 31);
+  const int row = span.first + 32 * block + (lane & 31);
   const bool live = row < rows;
   int i, g;
   p.byG.divmod(live ? row : 0, &i, &g);
   const int limit = !live ? 0 : p.causal ? std::max(0, std::min(span.m, i + off + 1)) : span.m;
   // keys that some row of the workgroup sees
   int end = span.m;
-  if (p.causal) end = std::max(0, std::min(end, p.byG.div(std::min(rows, span.first + 32 * NW) - 1) + off + 1));
+  if (p.causal) end = std::max(0, std::min(end, p.byG.div(std::min(rows, span.first + 32 * NB) - 1) + off + 1));
   int begin = 0;
   if (p.slices > 1) {
     const int share = ((end + p.slices - 1) / p.slices + KT - 1) / KT * KT;
@@ -358,9 +406,9 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
     end = std::min(end, begin + share);
   }
   // ... that all rows of the wavefront see (those of its first row), and the last that some row sees
-  const int all = p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows - 1, span.first + 32 * wave)) + off + 1)) : span.m;
-  const int some = span.first + 32 * wave >= rows ? 0
-                   : p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows, span.first + 32 * wave + 32) - 1) + off + 1)) : span.m;
+  const int all = p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows - 1, span.first + 32 * block)) + off + 1)) : span.m;
+  const int some = span.first + 32 * block >= rows ? 0
+                   : p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows, span.first + 32 * block + 32) - 1) + off + 1)) : span.m;
 
   const long long position = span.q0 + i;
   const int column = head * p.G + g;
@@ -372,7 +420,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
   }
   const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
   const char* values = p.v.data + (long long)span.k0 * p.v.position + head * p.v.head;
-  Loader<V, DP, KT, NW> loadK, loadV;
+  Loader<V, DW, KT, NW> loadK, loadV;
   loadK.begin(p.k, p.D, wave, lane);
   loadV.begin(p.v, p.D, wave, lane);
   const char* nextK = keys + (long long)begin * p.k.position;   // the tile that is brought next
@@ -383,9 +431,9 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
     nextK += (long long)KT * p.k.position;
     nextV += (long long)KT * p.v.position;
   };
-  floatx16 o[DP / 32];
+  floatx16 o[DW / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+  for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float most = -INFINITY, sum = 0.f;
@@ -399,22 +447,48 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
       if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
-    if (j0 < some)
-      forward_tile<V, DP, KT>(from, from + tileBytes, to, bring_next, q, o, most, sum, j0, std::min(limit, end), j0 + KT > std::min(all, end), p.c, lane);
+    const int j = j0 + share0;
+    if (j < std::min(some, end))
+      forward_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, o, most, sum, j, std::min(limit, end),
+                              j + 32 * KB > std::min(all, end), p.c, lane);
     else bring_next(to);
   }
   sum += other_half(sum);
+  if (NS == 2) {
+    constexpr int values = DW / 32 * 16 + 2;
+    static_assert(NS == 1 || NB * values * 256 <= (int)sizeof(lds), "room");
+    float* room = (float*)lds + block * values * 64 + lane;
+    __syncthreads();
+    if (share0) {
+#pragma unroll
+      for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) room[(16 * d + r) * 64] = o[d][r];
+      room[(values - 2) * 64] = most;
+      room[(values - 1) * 64] = sum;
+    }
+    __syncthreads();
+    if (share0) return;
+    const float most1 = room[(values - 2) * 64], to = fmaxf(most, most1);
+    const float f = most == -INFINITY ? 0.f : power2((most - to) * p.c), f1 = most1 == -INFINITY ? 0.f : power2((most1 - to) * p.c);
+    sum = sum * f + room[(values - 1) * 64] * f1;
+    most = to;
+#pragma unroll
+    for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f + room[(16 * d + r) * 64] * f1;
+  }
   // A key that a row does not see has p = 0, but 0 times an infinity or a NaN of its values is NaN: a row that is not finite is added up
   // key by key, over those it sees.
   if (p.causal) {
     bool good = true;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) good = good && finite(o[d][r]);
     if (!both_good(good)) {
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
       const float shift = most == -INFINITY ? 0.f : most * p.c;
@@ -427,7 +501,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
         float e = power2(s * p.c - shift);
         if (sizeof(V) == 2) e = bits_float((unsigned)round_bf16(e) << 16);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int at2 = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
@@ -444,24 +518,24 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_forward(At
     if (lane < 32 && p.logSums) p.logSums[index] = total;
     char* at = p.o.data + position * p.o.position + column * p.o.head;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
         store4<V>(at, 32 * d + 8 * (r / 4) + 4 * (lane >> 5), p.D, p.vector, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
   } else {
     const long long part = (long long)slice * p.N * p.heads + index;
     if (lane < 32) p.partSums[part] = total;
-    char* at = (char*)(p.parts + part * DP);
+    char* at = (char*)(p.parts + part * DW);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
-        store4<float>(at, 32 * d + 8 * (r / 4) + 4 * (lane >> 5), DP, 1, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
+        store4<float>(at, 32 * d + 8 * (r / 4) + 4 * (lane >> 5), DW, 1, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
   }
 }
 
 // The slices of a row put together: o = sum_s exp(L_s - L) o_s.  A wavefront per row and head; rows of no sequence are passed over.
-template <class V, int DP>
+template <class V, int DW>
 __global__ __launch_bounds__(256) void attention_join(AttentionP p) {
   const int lane = threadIdx.x & 63;
   const long long index = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), all = (long long)p.N * p.heads;
@@ -475,16 +549,16 @@ __global__ __launch_bounds__(256) void attention_join(AttentionP p) {
   // (a NaN of one slice is a NaN of the row)
   const float weight = most == -INFINITY && mine == mine ? 0.f : power2((mine - most) * kLog2e);
   const float sum = wave_sum(weight);
-  constexpr int W = DP / 64;
+  constexpr int W = (DW + 63) / 64;
   float o[W];
 #pragma unroll
   for (int w = 0; w < W; ++w) o[w] = 0.f;
   for (int s = 0; s < p.slices; ++s) {
     const float f = __shfl(weight, s, kWave);
     if (f == 0.f) continue;
-    const float* at = p.parts + (s * all + index) * DP + lane;
+    const float* at = p.parts + (s * all + index) * DW + lane;
 #pragma unroll
-    for (int w = 0; w < W; ++w) o[w] += f * at[64 * w];
+    for (int w = 0; w < W; ++w) o[w] += f * (DW % 64 == 0 || lane + 64 * w < DW ? at[64 * w] : 0.f);
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   if (lane == 0 && p.logSums) p.logSums[index] = sum == 0.f ? -INFINITY : most + logf(sum);
@@ -500,15 +574,16 @@ __global__ __launch_bounds__(256) void attention_join(AttentionP p) {
 
 // ------------------------------------------------------------------------------------------ dq, and delta for dk and dv
 
-template <class V, int DP, int KT, class Bring>
+template <class V, int DW, int KB, class Bring>
 __device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next, Bring bring_next,
-                                        const uintx4 (&q)[Tile<V, DP>::steps], const uintx4 (&dO)[Tile<V, DP>::steps], floatx16 (&dq)[DP / 32], float negL,
-                                        float negDelta, int j0, int limit, bool edge, float c, int lane) {
-  typedef Tile<V, DP> T;
+                                        const uintx4 (&q)[Tile<V, DW>::steps], const uintx4 (&dO)[Tile<V, DW>::steps], floatx16 (&dq)[DW / 32], float negL,
+                                        float negDelta, int j0, int limit, int last, bool edge, float c, int lane) {
+  typedef Tile<V, DW> T;
   bring_next(next);
-  lane = fresh<V, DP>(lane);
+  lane = fresh<V, DW>(lane);
 #pragma unroll
-  for (int b = 0; b < KT / 32; ++b) {
+  for (int b = 0; b < KB; ++b) {
+    if (b && j0 + 32 * b >= last) break;
     floatx16 s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = negL;
@@ -529,30 +604,31 @@ __device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const cha
     uintx4 operand[sizeof(V) == 4 ? 4 : 2];
     T::operand(operand, e);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) dq[d] = T::across(keys, 32 * b, d, lane, operand, dq[d]);
+    for (int d = 0; d < DW / 32; ++d) dq[d] = T::across(keys, 32 * b, d, lane, operand, dq[d]);
   }
 }
 
-template <class V, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(AttentionP p) {
-  typedef Tile<V, DP> T;
-  constexpr int tileBytes = KT * T::rowBytes;
+// (NB, NS, KT: as in the forward pass)
+template <class V, int DW, int NB, int NS, int KT>
+__global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attention_dq(AttentionP p) {
+  typedef Tile<V, DW> T;
+  constexpr int NW = NB * NS, KB = KT / 32 / NS, tileBytes = KT * T::rowBytes;
   __shared__ __attribute__((aligned(16))) char lds[kAhead * 2 * tileBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = wave % NB, share0 = wave / NB * KB * 32;
   const int head = blockIdx.x % p.keyHeads;
-  const Span span = find<32 * NW, false, true>(p, blockIdx.x / p.keyHeads, lane);
+  const Span span = find<32 * NB, false>(p, blockIdx.x / p.keyHeads, lane);
   if (span.first < 0) return;
   const int rows = span.n * p.G, off = span.m - span.n;
-  const int row = span.first + 32 * wave + (lane & 31);
+  const int row = span.first + 32 * block + (lane & 31);
   const bool live = row < rows;
   int i, g;
   p.byG.divmod(live ? row : 0, &i, &g);
   const int limit = !live ? 0 : p.causal ? std::max(0, std::min(span.m, i + off + 1)) : span.m;
   int end = span.m;
-  if (p.causal) end = std::max(0, std::min(end, p.byG.div(std::min(rows, span.first + 32 * NW) - 1) + off + 1));
-  const int all = p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows - 1, span.first + 32 * wave)) + off + 1)) : span.m;
-  const int some = span.first + 32 * wave >= rows ? 0
-                   : p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows, span.first + 32 * wave + 32) - 1) + off + 1)) : span.m;
+  if (p.causal) end = std::max(0, std::min(end, p.byG.div(std::min(rows, span.first + 32 * NB) - 1) + off + 1));
+  const int all = p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows - 1, span.first + 32 * block)) + off + 1)) : span.m;
+  const int some = span.first + 32 * block >= rows ? 0
+                   : p.causal ? std::max(0, std::min(span.m, p.byG.div(std::min(rows, span.first + 32 * block + 32) - 1) + off + 1)) : span.m;
   const long long position = span.q0 + i;
   const int column = head * p.G + g;
   uintx4 q[T::steps], dO[T::steps];
@@ -573,7 +649,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
   if (live) {
     negL = p.logSums[position * p.heads + column];
     negL = negL == -INFINITY ? 0.f : -negL / p.scale;
-    if (lane < 32) {
+    if (lane < 32 && !share0) {
       const long long at = (long long)column * p.N + position;
       p.statL[at] = negL;
       p.statD[at] = negDelta;
@@ -582,7 +658,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
   if (!p.dq.data) return;
   const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
   const char* values = p.v.data + (long long)span.k0 * p.v.position + head * p.v.head;
-  Loader<V, DP, KT, NW> loadK, loadV;
+  Loader<V, DW, KT, NW> loadK, loadV;
   loadK.begin(p.k, p.D, wave, lane);
   loadV.begin(p.v, p.D, wave, lane);
   const char* nextK = keys;   // the tile that is brought next
@@ -593,9 +669,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
     nextK += (long long)KT * p.k.position;
     nextV += (long long)KT * p.v.position;
   };
-  floatx16 dq[DP / 32];
+  floatx16 dq[DW / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+  for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
   if (end > 0) bring_tile(lds, end);
@@ -608,19 +684,38 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
       if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
-    if (j0 < some) dq_tile<V, DP, KT>(from, from + tileBytes, to, bring_next, q, dO, dq, negL, negDelta, j0, limit, j0 + KT > std::min(all, end), p.c, lane);
+    const int j = j0 + share0;
+    if (j < std::min(some, end))
+      dq_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, dO, dq, negL, negDelta, j, limit,
+                         std::min(some, end), j + 32 * KB > std::min(all, end), p.c, lane);
     else bring_next(to);
+  }
+  if (NS == 2) {
+    float* room = (float*)lds + block * DW / 32 * 16 * 64 + lane;
+    __syncthreads();
+    if (share0) {
+#pragma unroll
+      for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) room[(16 * d + r) * 64] = dq[d][r];
+    }
+    __syncthreads();
+    if (share0) return;
+#pragma unroll
+    for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[d][r] += room[(16 * d + r) * 64];
   }
   // (as in the forward pass: what is not finite is added up over the keys that a row sees)
   if (p.causal) {
     bool good = true;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) good = good && finite(dq[d][r]);
     if (!both_good(good)) {
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
       const char* at = p.q.data + position * p.q.position + column * p.q.head;
@@ -638,7 +733,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
         float e = power2(s * p.c) * dp;
         if (sizeof(V) == 2) e = bits_float((unsigned)round_bf16(e) << 16);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int at2 = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
@@ -650,7 +745,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
   if (!live) return;
   char* at = p.dq.data + position * p.dq.position + column * p.dq.head;
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+  for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4)
       store4<V>(at, 32 * d + 8 * (r / 4) + 4 * (lane >> 5), p.D, p.vector, dq[d][r] * p.scale, dq[d][r + 1] * p.scale, dq[d][r + 2] * p.scale,
@@ -659,73 +754,72 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dq(
 
 // ------------------------------------------------------------------------------------------ dk, dv
 
-// One tile of RT positions of a head against a wavefront's 32 keys
-template <class V, int DP, int RT, class Bring>
+// 32 positions of a head against a wavefront's 32 keys
+template <class V, int DW, class Bring>
 __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const char* __restrict__ ders, const float* __restrict__ statL,
-                                         const float* __restrict__ statD, char* __restrict__ next, Bring bring_next, const uintx4 (&k)[Tile<V, DP>::steps],
-                                         const uintx4 (&v)[Tile<V, DP>::steps], floatx16 (&dk)[DP / 32], floatx16 (&dv)[DP / 32], int i0, int n, int firstOf,
+                                         const float* __restrict__ statD, char* __restrict__ next, Bring bring_next, const uintx4 (&k)[Tile<V, DW>::steps],
+                                         const uintx4 (&v)[Tile<V, DW>::steps], floatx16 (&dk)[DW / 32], floatx16 (&dv)[DW / 32], int i0, int n, int firstOf,
                                          bool edge, float c, int lane) {
-  typedef Tile<V, DP> T;
+  typedef Tile<V, DW> T;
   bring_next(next);
-  lane = fresh<V, DP>(lane);
+  lane = fresh<V, DW>(lane);
+  floatx16 s, dp;
 #pragma unroll
-  for (int b = 0; b < RT / 32; ++b) {
-    floatx16 s, dp;
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const float4 l = *(const float4*)(statL + 32 * b + 2 * r + 4 * (lane >> 5));
-      s[r] = l.x; s[r + 1] = l.y; s[r + 2] = l.z; s[r + 3] = l.w;
-    }
-#pragma unroll
-    for (int t = 0; t < T::steps; ++t) s = Matrix<V>::along(T::along(queries, 32 * b, t, lane), k[t], s);
-    float e[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c);
-    if (edge) {   // (firstOf: the first position that sees this lane's key)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = i0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-        if (i >= n || i < firstOf) e[r] = 0.f;
-      }
-    }
-    uintx4 operand[sizeof(V) == 4 ? 4 : 2];
-    T::operand(operand, e);
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) dv[d] = T::across(ders, 32 * b, d, lane, operand, dv[d]);
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const float4 l = *(const float4*)(statD + 32 * b + 2 * r + 4 * (lane >> 5));
-      dp[r] = l.x; dp[r + 1] = l.y; dp[r + 2] = l.z; dp[r + 3] = l.w;
-    }
-#pragma unroll
-    for (int t = 0; t < T::steps; ++t) dp = Matrix<V>::along(T::along(ders, 32 * b, t, lane), v[t], dp);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) e[r] = edge && e[r] == 0.f ? 0.f : e[r] * dp[r];
-    T::operand(operand, e);
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) dk[d] = T::across(queries, 32 * b, d, lane, operand, dk[d]);
+  for (int r = 0; r < 16; r += 4) {
+    const float4 l = *(const float4*)(statL + 2 * r + 4 * (lane >> 5));
+    s[r] = l.x; s[r + 1] = l.y; s[r + 2] = l.z; s[r + 3] = l.w;
   }
+#pragma unroll
+  for (int t = 0; t < T::steps; ++t) s = Matrix<V>::along(T::along(queries, 0, t, lane), k[t], s);
+  float e[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c);
+  if (edge) {   // (firstOf: the first position that sees this lane's key)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = i0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+      if (i >= n || i < firstOf) e[r] = 0.f;
+    }
+  }
+  uintx4 operand[sizeof(V) == 4 ? 4 : 2];
+  T::operand(operand, e);
+#pragma unroll
+  for (int d = 0; d < DW / 32; ++d) dv[d] = T::across(ders, 0, d, lane, operand, dv[d]);
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    const float4 l = *(const float4*)(statD + 2 * r + 4 * (lane >> 5));
+    dp[r] = l.x; dp[r + 1] = l.y; dp[r + 2] = l.z; dp[r + 3] = l.w;
+  }
+#pragma unroll
+  for (int t = 0; t < T::steps; ++t) dp = Matrix<V>::along(T::along(ders, 0, t, lane), v[t], dp);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) e[r] = edge && e[r] == 0.f ? 0.f : e[r] * dp[r];
+  T::operand(operand, e);
+#pragma unroll
+  for (int d = 0; d < DW / 32; ++d) dk[d] = T::across(queries, 0, d, lane, operand, dk[d]);
 }
 
-// NW wavefronts of 32 keys; they walk over the positions of one head of the group after the other
-template <class V, int DP, int NW, int RT>
-__global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv(AttentionP p) {
-  typedef Tile<V, DP> T;
+// NB blocks of 32 keys; they walk over the positions of one head of the group after the other.  NS wavefronts share a block, each takes its 32
+// positions of every tile, and their sums are added up through LDS.
+template <class V, int DW, int NB, int NS>
+__global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attention_dkv(AttentionP p) {
+  typedef Tile<V, DW> T;
+  constexpr int NW = NB * NS, RT = 32 * NS;
   constexpr int tileBytes = RT * T::rowBytes, statBytes = RT * 4, bufferBytes = 2 * tileBytes + 2 * statBytes;
   static_assert(RT <= 64, "one load brings the statistics of a tile");
   __shared__ __attribute__((aligned(16))) char lds[kAhead * bufferBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = wave % NB, share0 = wave / NB * 32;
   const int head = blockIdx.x % p.keyHeads;
-  const Span span = find<32 * NW, true, false>(p, blockIdx.x / p.keyHeads, lane);
+  const Span span = find<32 * NB, true>(p, blockIdx.x / p.keyHeads, lane);
   if (span.first < 0) return;
   const int off = span.m - span.n;
-  const int key = span.first + 32 * wave + (lane & 31);
+  const int key = span.first + 32 * block + (lane & 31);
   const bool live = key < span.m;
   // the first position that sees the lane's key, the workgroup's first key (from a tile's border on), the wavefront's first and its last one
   const int firstOf = p.causal ? key - off : 0;
   const int begin = p.causal ? std::max(0, span.first - off) / RT * RT : 0;
-  const int some = p.causal ? span.first + 32 * wave - off : 0;
-  const int all = p.causal ? span.first + 32 * wave + 31 - off : 0;
+  const int some = p.causal ? span.first + 32 * block - off : 0;
+  const int all = p.causal ? span.first + 32 * block + 31 - off : 0;
 
   uintx4 k[T::steps], v[T::steps];
   {
@@ -740,7 +834,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
   const char* ders = p.dO.data + (long long)span.q0 * p.dO.position + (long long)head * p.G * p.dO.head;
   const float* statL = p.statL + (long long)head * p.G * p.N + span.q0;
   const float* statD = p.statD + (long long)head * p.G * p.N + span.q0;
-  Loader<V, DP, RT, NW> loadQ, loadD;
+  Loader<V, DW, RT, NW> loadQ, loadD;
   loadQ.begin(p.q, p.D, wave, lane);
   loadD.begin(p.dO, p.D, wave, lane);
   // the tile that is brought next: position nextI of the head whose first positions are at headQ, headD, headStat
@@ -768,9 +862,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
       nextD = headD + (long long)begin * p.dO.position;
     }
   };
-  floatx16 dk[DP / 32], dv[DP / 32];
+  floatx16 dk[DW / 32], dv[DW / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+  for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
   const int each = begin < span.n ? (span.n - begin + RT - 1) / RT : 0, tiles = each * p.G;
@@ -784,23 +878,49 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
       if (t + 1 < tiles) bring_tile(at);
     };
-    if (i0 + RT > some)
-      dkv_tile<V, DP, RT>(from, from + tileBytes, (const float*)(from + 2 * tileBytes), (const float*)(from + 2 * tileBytes + statBytes), to, bring_next, k, v, dk,
-                          dv, i0, span.n, firstOf, i0 < all || i0 + RT > span.n, p.c, lane);
+    const int i = i0 + share0;
+    if (i + 32 > some && i < span.n)
+      dkv_tile<V, DW>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, (const float*)(from + 2 * tileBytes) + share0,
+                      (const float*)(from + 2 * tileBytes + statBytes) + share0, to, bring_next, k, v, dk, dv, i, span.n, firstOf, i < all || i + 32 > span.n, p.c,
+                      lane);
     else bring_next(to);
     i0 += RT;
     if (i0 >= span.n) i0 = begin;
+  }
+  if (NS == 2) {
+    constexpr int values = DW / 32 * 16;
+    static_assert(NS == 1 || NB * 2 * values * 256 <= (int)sizeof(lds), "room");
+    float* room = (float*)lds + block * 2 * values * 64 + lane;
+    __syncthreads();
+    if (share0) {
+#pragma unroll
+      for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          room[(16 * d + r) * 64] = dk[d][r];
+          room[(values + 16 * d + r) * 64] = dv[d][r];
+        }
+    }
+    __syncthreads();
+    if (share0) return;
+#pragma unroll
+    for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        dk[d][r] += room[(16 * d + r) * 64];
+        dv[d][r] += room[(values + 16 * d + r) * 64];
+      }
   }
   // (rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN)
   if (p.causal) {
     bool good = true;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) good = good && finite(dk[d][r]) && finite(dv[d][r]);
     if (!both_good(good)) {
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
       const V* kj = (const V*)(p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head);
@@ -823,7 +943,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
           f = bits_float((unsigned)round_bf16(f) << 16);
         }
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int at = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
@@ -837,7 +957,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(V) == 4 ? 1 : 2) void attention_dkv
   }
   if (!live) return;
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+  for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int at = 32 * d + 8 * (r / 4) + 4 * (lane >> 5);
@@ -926,26 +1046,32 @@ bool lies_well(const Operand& o, int D, int size) {
 size_t packed_bytes(int positions, int heads, int D, int size) { return rounded((size_t)positions * heads * (((size_t)D * size + 15) / 16 * 16)); }
 
 struct Plan {
-  int DP, size, G, waves, slices, tiles, keyTiles;
+  int DW, size, G, blocks, slices;
   size_t partsAt, sumsAt, statAt, packAt, bytes;
 };
+
+// Whether two wavefronts share a block of 32 rows or keys.  They make twice as many workgroups of half the length, which bring twice as many
+// tiles.  Rows: where the chip is not filled otherwise (one sequence of 4096, 4 heads of 128 over one, bfloat16: forward 53.8 -> 46.3 us, dq
+// 122 -> 74; 196 positions x 32 x 12 heads of 64, 768 workgroups: 18.8 -> 20.8 and 24.3 -> 29.5).  Keys: everywhere but in short sequences, whose
+// last tiles hold more that is not there (packed sequences of up to 1100, 32 heads over 8: 279 -> 251; 196 positions: 39.0 -> 42.9).
+bool split(const char* name, bool rule) {
+  const int forced = tunable(name, 0);
+  return forced ? forced == 2 : rule;
+}
 
 // How a forward call is cut.  Rows of a sequence on average up to 32: one wavefront a workgroup, and keys are cut into slices until there
 // are workgroups for the whole chip; otherwise four wavefronts.
 Plan plan_of(const mcn_attention_geom* g, int backward) {
   Plan l = {};
   l.size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
-  l.DP = g->D <= 64 ? 64 : 128;
+  l.DW = g->D <= 64 ? 64 : g->D <= 96 ? 96 : 128;
   l.G = g->keyHeads ? g->heads / g->keyHeads : 1;
   const int sequences = std::max(1, g->sequences);
   const long long rows = (long long)g->N * l.G;
-  l.waves = !backward && rows <= 32ll * sequences ? 1 : 4;
-  const int size = 32 * l.waves;
-  l.tiles = (int)(rows / size) + sequences;
-  l.keyTiles = g->M / 128 + sequences;
   l.slices = 1;
   if (!backward) {
-    const long long groups = (long long)(rows + size - 1) / size * g->keyHeads, want = 4ll * std::max(1, device_compute_units());
+    l.blocks = rows <= 32ll * sequences ? 1 : split("attention_forward_split", (rows / 128 + sequences) * g->keyHeads * 4 < 5ll * device_compute_units()) ? 2 : 4;
+    const long long groups = (long long)div_up(rows, 32 * l.blocks) * g->keyHeads, want = 4ll * std::max(1, device_compute_units());
     const int tile = l.size == 2 ? 64 : 32;
     const long long most = std::max<long long>(1, g->M / sequences / (4 * tile));
     l.slices = (int)std::max<long long>(1, std::min<long long>({64, most, want / std::max<long long>(1, groups)}));
@@ -953,7 +1079,7 @@ Plan plan_of(const mcn_attention_geom* g, int backward) {
   size_t at = 0;
   if (l.slices > 1) {
     l.partsAt = at;
-    at += rounded((size_t)l.slices * g->N * g->heads * l.DP * sizeof(float));
+    at += rounded((size_t)l.slices * g->N * g->heads * l.DW * sizeof(float));
     l.sumsAt = at;
     at += rounded((size_t)l.slices * g->N * g->heads * sizeof(float));
   }
@@ -1031,44 +1157,61 @@ int tiles_of(AttentionP* p, int rowsEach, int size, long long rows) {
   if (p->qStarts) return (int)(rows / size) + p->sequences;
   const int each = std::max(1, div_up(rowsEach, size));
   p->byTiles = FastDiv(each);
+  p->bySequences = FastDiv(p->sequences);
   return each * p->sequences;
 }
 
-template <class V, int DP>
+template <class V, int DW>
 int forward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   constexpr int KT = sizeof(V) == 2 ? 64 : 32;
   const long long rows = (long long)p.N * p.G;
-  const long long blocks = (long long)tiles_of(&p, p.each * p.G, 32 * l.waves, rows) * p.keyHeads * p.slices;
+  const long long blocks = (long long)tiles_of(&p, p.each * p.G, 32 * l.blocks, rows) * p.keyHeads * p.slices;
   if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+  const dim3 grid((unsigned)blocks);
   {
     KernelTimer timer("attention_forward", s);
-    if (l.waves == 1) hipLaunchKernelGGL((attention_forward<V, DP, 1, KT>), dim3((unsigned)blocks), dim3(64), 0, s, p);
-    else hipLaunchKernelGGL((attention_forward<V, DP, 4, KT>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    if (l.blocks == 1) hipLaunchKernelGGL((attention_forward<V, DW, 1, 1, KT>), grid, dim3(64), 0, s, p);
+    else if (l.blocks == 2) hipLaunchKernelGGL((attention_forward<V, DW, 2, 2, 64>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attention_forward<V, DW, 4, 1, KT>), grid, dim3(256), 0, s, p);
   }
   int rc = check_launch(who);
   if (rc || p.slices == 1) return rc;
   KernelTimer timer("attention_join", s);
-  hipLaunchKernelGGL((attention_join<V, DP>), dim3((unsigned)div_up((long long)p.N * p.heads, 4)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((attention_join<V, DW>), dim3((unsigned)div_up((long long)p.N * p.heads, 4)), dim3(256), 0, s, p);
   return check_launch(who);
 }
 
-template <class V, int DP>
+template <class V, int DW>
 int backward(const char* who, hipStream_t s, AttentionP& p) {
   constexpr int KT = sizeof(V) == 2 ? 64 : 32;
   if (p.N) {
-    const int tiles = tiles_of(&p, p.each * p.G, 128, (long long)p.N * p.G);
-    if ((long long)tiles * p.keyHeads >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+    const long long rows = (long long)p.N * p.G;
+    const bool two = split("attention_dq_split", (rows / 128 + p.sequences) * p.keyHeads < 2ll * device_compute_units());
+    const long long blocks = (long long)tiles_of(&p, p.each * p.G, two ? 64 : 128, rows) * p.keyHeads;
+    if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
     KernelTimer timer("attention_dq", s);
-    hipLaunchKernelGGL((attention_dq<V, DP, 4, KT>), dim3((unsigned)(tiles * p.keyHeads)), dim3(256), 0, s, p);
+    if (two) hipLaunchKernelGGL((attention_dq<V, DW, 2, 2, 64>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attention_dq<V, DW, 4, 1, KT>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     const int rc = check_launch(who);
     if (rc) return rc;
   }
   if (!p.M || (!p.dk.data && !p.dv.data)) return MCN_SUCCESS;
-  const int tiles = tiles_of(&p, p.eachKeys, 128, p.M);
-  if ((long long)tiles * p.keyHeads >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+  const bool two = split("attention_dkv_split", (p.M / 128 + p.sequences) * p.keyHeads < (p.N < 512ll * p.sequences ? 2ll : DW == 64 ? 6ll : 4ll) * device_compute_units());
+  const long long blocks = (long long)tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads;
+  if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
   KernelTimer timer("attention_dkv", s);
-  hipLaunchKernelGGL((attention_dkv<V, DP, 4, 32>), dim3((unsigned)(tiles * p.keyHeads)), dim3(256), 0, s, p);
+  if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((attention_dkv<V, DW, 4, 1>), dim3((unsigned)blocks), dim3(256), 0, s, p);
   return check_launch(who);
+}
+
+template <class V>
+int forward_of(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
+  return l.DW == 64 ? forward<V, 64>(who, s, p, l) : l.DW == 96 ? forward<V, 96>(who, s, p, l) : forward<V, 128>(who, s, p, l);
+}
+template <class V>
+int backward_of(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
+  return l.DW == 64 ? backward<V, 64>(who, s, p) : l.DW == 96 ? backward<V, 96>(who, s, p) : backward<V, 128>(who, s, p);
 }
 
 int check_starts(const char* who, const mcn_attention_geom* g, const int* qStarts, const int* kStarts) {
@@ -1122,8 +1265,7 @@ int mcn_attention_forward(mcn_stream_t stream, const mcn_attention_geom* g, cons
   p.logSums = logSums;
   p.parts = (float*)((char*)workspace + l.partsAt);
   p.partSums = (float*)((char*)workspace + l.sumsAt);
-  if (g->dataType == MCN_BFLOAT16) return l.DP == 64 ? forward<bf16, 64>(who, s, p, l) : forward<bf16, 128>(who, s, p, l);
-  return l.DP == 64 ? forward<float, 64>(who, s, p, l) : forward<float, 128>(who, s, p, l);
+  return g->dataType == MCN_BFLOAT16 ? forward_of<bf16>(who, s, p, l) : forward_of<float>(who, s, p, l);
 }
 
 int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, const mcn_heads* derQ, const mcn_heads* derK, const mcn_heads* derV,
@@ -1179,8 +1321,7 @@ int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, con
   p.logSums = const_cast<float*>(logSums);
   p.statL = (float*)((char*)workspace + l.statAt);
   p.statD = p.statL + rounded((size_t)g->N * g->heads * sizeof(float)) / sizeof(float);
-  if (g->dataType == MCN_BFLOAT16) return l.DP == 64 ? backward<bf16, 64>(who, s, p) : backward<bf16, 128>(who, s, p);
-  return l.DP == 64 ? backward<float, 64>(who, s, p) : backward<float, 128>(who, s, p);
+  return g->dataType == MCN_BFLOAT16 ? backward_of<bf16>(who, s, p, l) : backward_of<float>(who, s, p, l);
 }
 
 }  // extern "C"

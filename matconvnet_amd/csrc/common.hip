@@ -63,6 +63,9 @@ Tunable g_tunables[] = {
     {"conv_force_direct", 0},          // 1: always use the direct (non-MFMA) convolution kernels
     {"conv_no_uniform_tap", 0},        // 1: disable the uniform-tap variant of the pixel-major kernel (and the kernels with split operands)
     {"fcloss_piece_kib", 0},           // > 0: so many KiB for a piece of the classes instead of 256 MiB
+    {"attention_forward_split", 0},    // 1, 2: force so many wavefronts to a block of 32 rows; 0 = choose
+    {"attention_dq_split", 0},         // (likewise)
+    {"attention_dkv_split", 0},        // (likewise, of 32 keys)
     {"ortho_no_narrow", 0},            // 1: narrow matrices through the launches of the others too
     {"product_tile", 0},               // 64, 128, 256: force the tile of the products of fcloss.hip and ortho.hip; anything else = choose
     {"product_slices", 0},             // > 0: cut their reductions among so many workgroups (32 at most, and as far as there are stages)
