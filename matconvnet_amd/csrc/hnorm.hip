@@ -10,7 +10,8 @@
 // revolution in double: position 10^6 times frequency 1 keeps all of a single-precision sine.
 //
 // A lane holds VP pairs, 2 VP channels: the pairs' first channels and their second ones a run of pairs apart, or neighbours.  Channels of
-// no pair are held as pairs that are not turned.
+// no pair are held likewise and not turned.  Heads of any size and address are read four values at a time from wherever they start, what is
+// left over value by value.
 #include "mcn_internal.hpp"
 
 #include <algorithm>
@@ -42,26 +43,39 @@ struct HnormP {
   float* partials;     // backward: [workgroups][2][D], or null
   int D, N, pairs, axes, normalise;
   int slices, perSlice;   // of the two sets' heads one behind the other: a wavefront's share of a position
+  FastDiv bySlices;
   float epsilon;
 };
 
-// where VP pairs from the chunk's first one on lie: their first VP channels and the other VP
-template <int VP, bool NEIGHBOURS>
+// Where a chunk of VP pairs lies: its first channels from lo on and the others from hi on (neighbours: the first VP of its channels, and the
+// rest); nLo and nHi of them are there.  Chunks of pairs that turn come first, then those of channels of no pair.  WHOLE: nothing is left over in
+// either, and everything starts at a multiple of 16 bytes.
+template <int VP, bool NEIGHBOURS, bool WHOLE>
 struct Place {
-  int lo, hi;
-  bool turned, live, both;   // both: false where an odd channel is left (VP == 1)
+  int lo, hi, nLo, nHi, pair;
+  bool turned;
   __device__ __forceinline__ Place(int chunk, int D, int pairs) {
-    const int c = chunk * VP;
-    turned = c < pairs;
-    if (turned) {
-      lo = NEIGHBOURS ? 2 * c : c;
-      hi = NEIGHBOURS ? 2 * c + VP : c + pairs;
-    } else {
-      lo = 2 * c;   // = 2 pairs + 2 (c - pairs)
-      hi = lo + VP;
+    const int turning = (pairs + VP - 1) / VP;
+    turned = chunk < turning;
+    pair = chunk * VP;
+    int left;   // channels from lo on, neighbours and channels of no pair
+    if (turned && !NEIGHBOURS) {
+      lo = pair;
+      hi = pair + pairs;
+      nLo = nHi = WHOLE ? VP : std::min(VP, pairs - pair);
+      return;
     }
-    live = lo < D;
-    both = hi < D;
+    if (turned) {
+      lo = 2 * pair;
+      left = 2 * (pairs - pair);
+    } else {
+      lo = 2 * pairs + 2 * VP * (chunk - turning);
+      left = D - lo;
+    }
+    hi = lo + VP;
+    nLo = std::min(VP, left);
+    nHi = std::min(VP, left - VP);
+    if (WHOLE) nLo = nHi = left > 0 ? VP : 0;
   }
 };
 
@@ -73,12 +87,44 @@ template <class V, int VP>
 struct Raw {
   Pack<V, VP> lo, hi;
 };
-template <class V, int VP>
-__device__ __forceinline__ Raw<V, VP> fetch(const V* head, int lo, int hi, bool live, bool both) {
-  Raw<V, VP> r = {};
-  if (live) r.lo = *(const Pack<V, VP>*)(head + lo);
-  if (live && both) r.hi = *(const Pack<V, VP>*)(head + hi);
+// VP values that may start anywhere
+template <class V, int VP> struct Loose;
+template <> struct Loose<float, 4> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Loose<bf16, 4> { typedef unsigned short type __attribute__((ext_vector_type(4), aligned(2))); };
+template <class V, int VP, bool WHOLE>
+__device__ __forceinline__ Pack<V, VP> load_some(const V* at, int n) {
+  Pack<V, VP> r = {};
+  if constexpr (WHOLE) {
+    if (n > 0) r = *(const Pack<V, VP>*)at;
+  } else {
+    if (n == VP) {
+      const typename Loose<V, VP>::type v = *(const typename Loose<V, VP>::type*)at;
+#pragma unroll
+      for (int e = 0; e < VP; ++e) r.v[e] = v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VP - 1; ++e)
+        if (e < n) r.v[e] = at[e];
+    }
+  }
   return r;
+}
+template <class V, int VP, bool WHOLE>
+__device__ __forceinline__ void store_some(V* at, int n, const Pack<V, VP>& r) {
+  if constexpr (WHOLE) {
+    if (n > 0) *(Pack<V, VP>*)at = r;
+  } else {
+    if (n == VP) {
+      typename Loose<V, VP>::type v;
+#pragma unroll
+      for (int e = 0; e < VP; ++e) v[e] = r.v[e];
+      *(typename Loose<V, VP>::type*)at = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < VP - 1; ++e)
+        if (e < n) at[e] = r.v[e];
+    }
+  }
 }
 template <class V, int VP>
 __device__ __forceinline__ void unpack(float (&w)[2 * VP], const Raw<V, VP>& r) {
@@ -88,22 +134,32 @@ __device__ __forceinline__ void unpack(float (&w)[2 * VP], const Raw<V, VP>& r) 
     w[VP + e] = to_float(r.hi.v[e]);
   }
 }
-template <class V, int VP>
-__device__ __forceinline__ void store(V* head, int lo, int hi, bool both, const float (&w)[2 * VP]) {
+template <class V, int VP, bool WHOLE>
+__device__ __forceinline__ void store(V* head, int lo, int hi, int nLo, int nHi, const float (&w)[2 * VP]) {
   Raw<V, VP> r;
 #pragma unroll
   for (int e = 0; e < VP; ++e) {
     r.lo.v[e] = from_float<V>(w[e]);
     r.hi.v[e] = from_float<V>(w[VP + e]);
   }
-  *(Pack<V, VP>*)(head + lo) = r.lo;
-  if (both) *(Pack<V, VP>*)(head + hi) = r.hi;
+  store_some<V, VP, WHOLE>(head + lo, nLo, r.lo);
+  store_some<V, VP, WHOLE>(head + hi, nHi, r.hi);
 }
 
+// The sum over a group's lanes, in each of them: within 16 lanes by the vector instructions' own lane exchange (through LDS, as shuffles go, the
+// four exchanges of each of the backward pass's two sums are waited for: 16384 x 40 heads of 128, bfloat16: 140 us, 120 so)
+template <int CONTROL>
+__device__ __forceinline__ float exchanged(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
 template <int T>
 __device__ __forceinline__ float group_sum(float v) {
+  v += exchanged<0xB1>(v);                // lane ^ 1
+  v += exchanged<0x4E>(v);                // lane ^ 2
+  if (T >= 8) v += exchanged<0x141>(v);   // the other four of eight, mirrored
+  if (T >= 16) v += exchanged<0x140>(v);  // the other eight of sixteen, mirrored
 #pragma unroll
-  for (int o = T / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  for (int o = 16; o < T; o *= 2) v += __shfl_xor(v, o, kWave);
   return v;
 }
 
@@ -114,11 +170,21 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-__device__ __forceinline__ void angles(float (*lds)[kMostD / 2], const HnormP& p, int n, int lane) {
+constexpr int kAxes = 3;   // of so many axes and up to 64 pairs a lane keeps its pair's frequencies
+struct Turns {
+  double frequency[kAxes], position[kAxes];
+};
+__device__ __forceinline__ bool kept(const HnormP& p) { return p.axes <= kAxes && p.pairs <= 64; }
+__device__ __forceinline__ void angles(float (*lds)[kMostD / 2], const HnormP& p, const Turns& turns, int n, int lane) {
   wave_order();
   for (int j = lane; j < p.pairs; j += 64) {
     double angle = 0.0;
-    for (int a = 0; a < p.axes; ++a) angle += p.positions[(size_t)n * p.axes + a] * p.frequencies[(size_t)a * p.pairs + j];
+    if (kept(p)) {
+#pragma unroll
+      for (int a = 0; a < kAxes; ++a) angle += turns.position[a] * turns.frequency[a];
+    } else {
+      for (int a = 0; a < p.axes; ++a) angle += p.positions[(size_t)n * p.axes + a] * p.frequencies[(size_t)a * p.pairs + j];
+    }
     double r = angle * 0.15915494309189533577;   // revolutions
     r -= rint(r);
     float s, c;
@@ -129,136 +195,200 @@ __device__ __forceinline__ void angles(float (*lds)[kMostD / 2], const HnormP& p
   wave_order();
 }
 
-// T lanes to a head, NCH chunks of VP pairs a lane, HB heads on their way at a time
-template <class V, int VP, int T, int NCH, int HB, bool NEIGHBOURS, bool BACKWARD>
+// A wavefront's place in its work: kGroups * HB heads of a set from `first` on, of position n
+struct Cursor {
+  int unit, n, which, first, to;
+};
+
+// T lanes to a head, NCH chunks of VP pairs a lane, HB heads a lane at a time; the next HB are on their way meanwhile, the next position's
+// too (16384 x 40 heads of 128, bfloat16: forward and backward 109 and 183 us with a position's loads behind its angles, 72 and 120 so).
+template <class V, int VP, int T, int NCH, int HB, bool NEIGHBOURS, bool WHOLE, bool BACKWARD>
 __global__ __launch_bounds__(64 * kWaves) void hnorm_kernel(HnormP p) {
   constexpr int kGroups = 64 / T, W = 2 * VP;
   __shared__ float turn[kWaves][2][kMostD / 2];
   __shared__ float join[BACKWARD ? kWaves * 64 * W : 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = lane % T, group = lane / T;
-  float sums[2][NCH][W];
-  if (BACKWARD) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, t = lane % T, group = lane / T;
+  const int units = p.N * p.slices, step = gridDim.x * kWaves;
+  float g[2][NCH][W], sums[BACKWARD ? 2 : 1][NCH][W], cosine[NCH][VP], sine[NCH][VP];
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int i = 0; i < NCH; ++i)
-#pragma unroll
-        for (int e = 0; e < W; ++e) sums[w][i][e] = 0.f;
-  }
-  const long long units = (long long)p.N * p.slices, step = (long long)gridDim.x * kWaves;
-  for (long long unit = (long long)blockIdx.x * kWaves + wave; unit < units; unit += step) {
-    const int n = __builtin_amdgcn_readfirstlane((int)(unit / p.slices)), slice = __builtin_amdgcn_readfirstlane((int)(unit % p.slices));
-    angles(turn[wave], p, n, lane);
-    float cosine[NCH][VP], sine[NCH][VP];
+  for (int w = 0; w < 2; ++w)
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const Place<VP, NEIGHBOURS> at(i * T + t, p.D, p.pairs);
+      const Place<VP, NEIGHBOURS, WHOLE> at(i * T + t, p.D, p.pairs);
 #pragma unroll
       for (int e = 0; e < VP; ++e) {
-        const int j = at.turned ? (i * T + t) * VP + e : 0;
-        cosine[i][e] = turn[wave][0][j];
-        sine[i][e] = turn[wave][1][j];
+        g[w][i][e] = p.set[w].g && e < at.nLo ? p.set[w].g[at.lo + e] : 1.f;
+        g[w][i][VP + e] = p.set[w].g && e < at.nHi ? p.set[w].g[at.hi + e] : 1.f;
+        if (BACKWARD) sums[w][i][e] = sums[w][i][VP + e] = 0.f;
       }
     }
+
+  // the first heads at or behind a place
+  const auto settle = [&](Cursor& c) __attribute__((always_inline)) {
+    while (c.unit < units) {
+      int slice;
+      p.bySlices.divmod(c.unit, &c.n, &slice);
+      for (; c.which < 2; ++c.which, c.first = -1) {
+        const int before = c.which ? p.set[0].heads : 0;
+        c.to = std::min(p.set[c.which].heads, (slice + 1) * p.perSlice - before);
+        if (c.first < 0) c.first = std::max(0, slice * p.perSlice - before);
+        if (c.first < c.to) return;
+      }
+      c.unit += step;
+      c.which = 0;
+      c.first = -1;
+    }
+  };
+  typedef Raw<V, VP> Heads[HB][NCH];
+  const auto fetch_heads = [&](Heads& x, Heads& d, const Cursor& c) __attribute__((always_inline)) {
+    const HeadsP& set = p.set[c.which];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const HeadsP& set = p.set[which];
-      const int before = which ? p.set[0].heads : 0;
-      const int from = std::max(0, slice * p.perSlice - before), to = std::min(set.heads, (slice + 1) * p.perSlice - before);
-      if (from >= to) continue;
-      float g[NCH][W];
+    for (int b = 0; b < HB; ++b) {
+      const int h = c.first + b * kGroups + group;
+      const bool mine = h < c.to;
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const Place<VP, NEIGHBOURS> at(i * T + t, p.D, p.pairs);
-#pragma unroll
-        for (int e = 0; e < VP; ++e) {
-          g[i][e] = set.g && at.live ? set.g[at.lo + e] : 1.f;
-          g[i][VP + e] = set.g && at.live && at.both ? set.g[at.hi + e] : 1.f;
+        const Place<VP, NEIGHBOURS, WHOLE> at(i * T + t, p.D, p.pairs);
+        const int nLo = mine ? at.nLo : 0, nHi = mine ? at.nHi : 0;
+        if (!BACKWARD || p.normalise) {
+          const V* from = (const V*)set.x + c.n * set.xPos + h * set.xHead;
+          x[b][i].lo = load_some<V, VP, WHOLE>(from + at.lo, nLo);
+          x[b][i].hi = load_some<V, VP, WHOLE>(from + at.hi, nHi);
         }
-      }
-      for (int first = from; first < to; first += kGroups * HB) {
-        Raw<V, VP> x[HB][NCH], d[HB][BACKWARD ? NCH : 1];
-#pragma unroll
-        for (int b = 0; b < HB; ++b) {
-          const int h = first + b * kGroups + group;
-          const bool mine = h < to;
-#pragma unroll
-          for (int i = 0; i < NCH; ++i) {
-            const Place<VP, NEIGHBOURS> at(i * T + t, p.D, p.pairs);
-            x[b][i] = {};
-            if (!BACKWARD || p.normalise) x[b][i] = fetch<V, VP>((const V*)set.x + n * set.xPos + h * set.xHead, at.lo, at.hi, mine && at.live, at.both);
-            if (BACKWARD) d[b][i] = fetch<V, VP>((const V*)set.dy + n * set.dyPos + h * set.dyHead, at.lo, at.hi, mine && at.live, at.both);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < HB; ++b) {
-          const int h = first + b * kGroups + group;
-          const bool mine = h < to;
-          float w[NCH][W];
-          float squares = 0.f;
-#pragma unroll
-          for (int i = 0; i < NCH; ++i) {
-            unpack<V, VP>(w[i], x[b][i]);
-#pragma unroll
-            for (int e = 0; e < W; ++e) squares += w[i][e] * w[i][e];
-          }
-          float inv = 1.f;
-          if (p.normalise) inv = 1.f / sqrtf(group_sum<T>(squares) / (float)p.D + p.epsilon);
-          if (!BACKWARD) {
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-              const Place<VP, NEIGHBOURS> at(i * T + t, p.D, p.pairs);
-              if (p.normalise) {
-#pragma unroll
-                for (int e = 0; e < W; ++e) w[i][e] = w[i][e] * inv * g[i][e];
-              }
-#pragma unroll
-              for (int e = 0; e < VP; ++e) {
-                const int F = first_of<VP, NEIGHBOURS>(e), S = second_of<VP, NEIGHBOURS>(e);
-                const float lo = w[i][F], hi = w[i][S];
-                w[i][F] = at.turned ? lo * cosine[i][e] - hi * sine[i][e] : lo;
-                w[i][S] = at.turned ? hi * cosine[i][e] + lo * sine[i][e] : hi;
-              }
-              if (mine && at.live) store<V, VP>((V*)set.out + n * set.outPos + h * set.outHead, at.lo, at.hi, at.both, w[i]);
-            }
-          } else {
-            float du[NCH][W];
-            float product = 0.f;
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-              const Place<VP, NEIGHBOURS> at(i * T + t, p.D, p.pairs);
-              unpack<V, VP>(du[i], d[b][i]);
-#pragma unroll
-              for (int e = 0; e < VP; ++e) {
-                const int F = first_of<VP, NEIGHBOURS>(e), S = second_of<VP, NEIGHBOURS>(e);
-                const float lo = du[i][F], hi = du[i][S];
-                du[i][F] = at.turned ? lo * cosine[i][e] + hi * sine[i][e] : lo;
-                du[i][S] = at.turned ? hi * cosine[i][e] - lo * sine[i][e] : hi;
-              }
-              if (p.normalise) {
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                  w[i][e] *= inv;
-                  sums[which][i][e] += du[i][e] * w[i][e];   // (what is no channel, or no head, is zero)
-                  du[i][e] *= g[i][e];
-                  product += du[i][e] * w[i][e];
-                }
-              }
-            }
-            if (p.normalise) product = group_sum<T>(product) / (float)p.D;
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-              const Place<VP, NEIGHBOURS> at(i * T + t, p.D, p.pairs);
-              if (p.normalise) {
-#pragma unroll
-                for (int e = 0; e < W; ++e) du[i][e] = (du[i][e] - w[i][e] * product) * inv;
-              }
-              if (set.out && mine && at.live) store<V, VP>((V*)set.out + n * set.outPos + h * set.outHead, at.lo, at.hi, at.both, du[i]);
-            }
-          }
+        if (BACKWARD) {
+          const V* from = (const V*)set.dy + c.n * set.dyPos + h * set.dyHead;
+          d[b][i].lo = load_some<V, VP, WHOLE>(from + at.lo, nLo);
+          d[b][i].hi = load_some<V, VP, WHOLE>(from + at.hi, nHi);
         }
       }
     }
+  };
+  const auto work = [&](const HeadsP& set, const float (&g)[NCH][W], float (&sums)[NCH][W], const Heads& x, const Heads& d, const Cursor& c)
+                        __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+      const int h = c.first + b * kGroups + group;
+      const bool mine = h < c.to;
+      float w[NCH][W];
+      float squares = 0.f;
+      if (!BACKWARD || p.normalise) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          unpack<V, VP>(w[i], x[b][i]);
+#pragma unroll
+          for (int e = 0; e < W; ++e) squares += w[i][e] * w[i][e];
+        }
+      }
+      float inv = 1.f;
+      if (p.normalise) inv = 1.f / sqrtf(group_sum<T>(squares) / (float)p.D + p.epsilon);
+      if (!BACKWARD) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const Place<VP, NEIGHBOURS, WHOLE> at(i * T + t, p.D, p.pairs);
+          if (p.normalise) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) w[i][e] = w[i][e] * inv * g[i][e];
+          }
+#pragma unroll
+          for (int e = 0; e < VP; ++e) {
+            const int F = first_of<VP, NEIGHBOURS>(e), S = second_of<VP, NEIGHBOURS>(e);
+            const float lo = w[i][F], hi = w[i][S];
+            w[i][F] = at.turned ? lo * cosine[i][e] - hi * sine[i][e] : lo;
+            w[i][S] = at.turned ? hi * cosine[i][e] + lo * sine[i][e] : hi;
+          }
+          if (mine) store<V, VP, WHOLE>((V*)set.out + c.n * set.outPos + h * set.outHead, at.lo, at.hi, at.nLo, at.nHi, w[i]);
+        }
+      } else {
+        float du[NCH][W];
+        float product = 0.f;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const Place<VP, NEIGHBOURS, WHOLE> at(i * T + t, p.D, p.pairs);
+          unpack<V, VP>(du[i], d[b][i]);
+#pragma unroll
+          for (int e = 0; e < VP; ++e) {
+            const int F = first_of<VP, NEIGHBOURS>(e), S = second_of<VP, NEIGHBOURS>(e);
+            const float lo = du[i][F], hi = du[i][S];
+            du[i][F] = at.turned ? lo * cosine[i][e] + hi * sine[i][e] : lo;
+            du[i][S] = at.turned ? hi * cosine[i][e] - lo * sine[i][e] : hi;
+          }
+          if (p.normalise) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+              w[i][e] *= inv;
+              sums[i][e] += du[i][e] * w[i][e];   // (what is no channel, or no head, is zero)
+              du[i][e] *= g[i][e];
+              product += du[i][e] * w[i][e];
+            }
+          }
+        }
+        if (p.normalise) product = group_sum<T>(product) / (float)p.D;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const Place<VP, NEIGHBOURS, WHOLE> at(i * T + t, p.D, p.pairs);
+          if (p.normalise) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) du[i][e] = (du[i][e] - w[i][e] * product) * inv;
+          }
+          if (set.out && mine) store<V, VP, WHOLE>((V*)set.out + c.n * set.outPos + h * set.outHead, at.lo, at.hi, at.nLo, at.nHi, du[i]);
+        }
+      }
+    }
+  };
+
+  // (asked for ahead of the heads, so that they are waited for alone)
+  Turns turns;
+#pragma unroll
+  for (int a = 0; a < kAxes; ++a) turns.position[a] = turns.frequency[a] = 0.0;
+  const auto fetch_position = [&](const Cursor& c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < kAxes; ++a)
+      if (a < p.axes) turns.position[a] = p.positions[(size_t)c.n * p.axes + a];
+  };
+  const bool keeps = p.pairs && kept(p);
+  if (keeps) {
+#pragma unroll
+    for (int a = 0; a < kAxes; ++a)
+      if (a < p.axes && lane < p.pairs) turns.frequency[a] = p.frequencies[(size_t)a * p.pairs + lane];
+  }
+  Heads xa, da, xb, db;
+  Cursor here = {(int)blockIdx.x * kWaves + wave, 0, 0, -1, 0};
+  settle(here);
+  if (here.unit < units) {
+    if (keeps) fetch_position(here);
+    fetch_heads(xa, da, here);
+  }
+  int angled = -1;   // the position whose angles are at hand
+  const auto turn_over = [&](Heads& x, Heads& d, Heads& nextX, Heads& nextD) __attribute__((always_inline)) {
+    if (angled != here.n && p.pairs) {
+      angled = here.n;
+      angles(turn[wave], p, turns, here.n, lane);
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const Place<VP, NEIGHBOURS, WHOLE> at(i * T + t, p.D, p.pairs);
+#pragma unroll
+        for (int e = 0; e < VP; ++e) {
+          const int j = at.turned && at.pair + e < p.pairs ? at.pair + e : 0;
+          cosine[i][e] = turn[wave][0][j];
+          sine[i][e] = turn[wave][1][j];
+        }
+      }
+    }
+    Cursor next = here;
+    next.first += kGroups * HB;
+    settle(next);
+    if (next.unit < units) {
+      if (keeps && next.n != here.n) fetch_position(next);
+      fetch_heads(nextX, nextD, next);
+    }
+    if (here.which == 0) work(p.set[0], g[0], sums[0], x, d, here);
+    else work(p.set[1], g[1], sums[BACKWARD ? 1 : 0], x, d, here);
+    here = next;
+  };
+  while (here.unit < units) {
+    turn_over(xa, da, xb, db);
+    if (here.unit >= units) break;
+    turn_over(xb, db, xa, da);
   }
   if (!BACKWARD || !p.partials) return;
   // the workgroup's sums: groups and wavefronts added up in one order
@@ -272,12 +402,12 @@ __global__ __launch_bounds__(64 * kWaves) void hnorm_kernel(HnormP p) {
       __syncthreads();
       float* out = p.partials + ((size_t)blockIdx.x * 2 + which) * p.D;
       for (int k = threadIdx.x; k < T * W; k += 64 * kWaves) {
-        const Place<VP, NEIGHBOURS> at(i * T + k / W, p.D, p.pairs);
+        const Place<VP, NEIGHBOURS, WHOLE> at(i * T + k / W, p.D, p.pairs);
         const int e = k % W;
         float s = 0.f;
 #pragma unroll 8
         for (int j = 0; j < kWaves * kGroups; ++j) s += join[j * T * W + k];
-        if (at.live && (e < VP || at.both)) out[(e < VP ? at.lo : at.hi) + e % VP] = s;
+        if (e % VP < (e < VP ? at.nLo : at.nHi)) out[(e < VP ? at.lo : at.hi) + e % VP] = s;
       }
     }
 }
@@ -308,36 +438,40 @@ __global__ __launch_bounds__(256) void hnorm_join(float* __restrict__ dgq, float
 
 // ---------------------------------------------------------------------------------------------- host
 
-// workgroups of a backward pass: as many as run at once, each sums as it goes
-int backward_groups(long long units) { return (int)std::max<long long>(1, std::min<long long>(2ll * std::max(1, device_compute_units()), (units + kWaves - 1) / kWaves)); }
+// chunks of a head: of pairs that turn, and of channels of no pair
+int chunks_of(const HnormP& p, int VP) { return div_up(p.pairs, VP) + div_up(p.D - 2 * p.pairs, 2 * VP); }
 
-template <class V, int VP, int T, int NCH, bool NEIGHBOURS>
+// Workgroups: as many as run at once (forward 4 on a CU, backward 2), each walks over positions
+int groups_of(long long units, int perUnit) {
+  return (int)std::max<long long>(1, std::min<long long>((long long)perUnit * std::max(1, device_compute_units()), (units + kWaves - 1) / kWaves));
+}
+int backward_groups(long long units) { return groups_of(units, 3); }
+
+template <class V, int VP, int T, int NCH, bool NEIGHBOURS, bool WHOLE>
 void launch_kernel(hipStream_t s, const HnormP& p, bool backward, int groups) {
-  constexpr int forwardBatch = NCH == 1 ? 4 : 2, backwardBatch = NCH == 1 ? 2 : 1;
-  const long long units = (long long)p.N * p.slices;
+  constexpr int forwardBatch = NCH == 1 ? 2 : 1, backwardBatch = sizeof(V) == 2 && NCH == 1 ? 2 : 1;
   if (backward)
-    hipLaunchKernelGGL((hnorm_kernel<V, VP, T, NCH, backwardBatch, NEIGHBOURS, true>), dim3((unsigned)groups), dim3(64 * kWaves), 0, s, p);
+    hipLaunchKernelGGL((hnorm_kernel<V, VP, T, NCH, backwardBatch, NEIGHBOURS, WHOLE, true>), dim3((unsigned)groups), dim3(64 * kWaves), 0, s, p);
   else
-    hipLaunchKernelGGL((hnorm_kernel<V, VP, T, NCH, forwardBatch, NEIGHBOURS, false>), dim3((unsigned)std::min<long long>((units + kWaves - 1) / kWaves, 1 << 20)),
+    hipLaunchKernelGGL((hnorm_kernel<V, VP, T, NCH, forwardBatch, NEIGHBOURS, WHOLE, false>), dim3((unsigned)groups_of((long long)p.N * p.slices, 4)),
                        dim3(64 * kWaves), 0, s, p);
 }
 
 template <class V, bool NEIGHBOURS>
 void choose(hipStream_t s, const HnormP& p, bool wide, bool backward, int groups) {
-  constexpr int VP = 16 / sizeof(V);
+  constexpr int VP = 4;
+  const int chunks = chunks_of(p, VP);
   if (wide) {
-    const int chunks = div_up(p.D, 2 * VP);
-    if (chunks <= 4) launch_kernel<V, VP, 4, 1, NEIGHBOURS>(s, p, backward, groups);
-    else if (chunks <= 8) launch_kernel<V, VP, 8, 1, NEIGHBOURS>(s, p, backward, groups);
-    else if (chunks <= 16) launch_kernel<V, VP, 16, 1, NEIGHBOURS>(s, p, backward, groups);
-    else if (chunks <= 32) launch_kernel<V, VP, 32, 1, NEIGHBOURS>(s, p, backward, groups);
-    else launch_kernel<V, VP, 64, 1, NEIGHBOURS>(s, p, backward, groups);
+    if (chunks <= 4) launch_kernel<V, VP, 4, 1, NEIGHBOURS, true>(s, p, backward, groups);
+    else if (chunks <= 8) launch_kernel<V, VP, 8, 1, NEIGHBOURS, true>(s, p, backward, groups);
+    else if (chunks <= 16) launch_kernel<V, VP, 16, 1, NEIGHBOURS, true>(s, p, backward, groups);
+    else if (chunks <= 32) launch_kernel<V, VP, 32, 1, NEIGHBOURS, true>(s, p, backward, groups);
+    else launch_kernel<V, VP, 64, 1, NEIGHBOURS, true>(s, p, backward, groups);
   } else {
-    const int chunks = div_up(p.D, 2);
-    if (chunks <= 16) launch_kernel<V, 1, 16, 1, NEIGHBOURS>(s, p, backward, groups);
-    else if (chunks <= 64) launch_kernel<V, 1, 64, 1, NEIGHBOURS>(s, p, backward, groups);
-    else if (chunks <= 128) launch_kernel<V, 1, 64, 2, NEIGHBOURS>(s, p, backward, groups);
-    else launch_kernel<V, 1, 64, 4, NEIGHBOURS>(s, p, backward, groups);
+    if (chunks <= 8) launch_kernel<V, 4, 8, 1, NEIGHBOURS, false>(s, p, backward, groups);
+    else if (chunks <= 16) launch_kernel<V, 4, 16, 1, NEIGHBOURS, false>(s, p, backward, groups);
+    else if (chunks <= 64) launch_kernel<V, 4, 64, 1, NEIGHBOURS, false>(s, p, backward, groups);
+    else launch_kernel<V, 4, 64, 2, NEIGHBOURS, false>(s, p, backward, groups);
   }
 }
 
@@ -376,11 +510,12 @@ void share_out(HnormP* p, int lanes) {
   const int slices = (int)std::max<long long>(1, std::min<long long>(most, want / std::max(1, p->N)));
   p->perSlice = std::max(1, div_up(heads, slices));
   p->slices = std::max(1, div_up(heads, p->perSlice));
+  p->bySlices = FastDiv(p->slices);
 }
 
 int lanes_of(const HnormP& p, int VP, bool wide) {
-  const int chunks = div_up(p.D, wide ? 2 * VP : 2);
-  if (!wide) return chunks <= 16 ? 16 : 64;
+  const int chunks = chunks_of(p, wide ? VP : 4);
+  if (!wide) return chunks <= 8 ? 8 : chunks <= 16 ? 16 : 64;
   return chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : chunks <= 32 ? 32 : 64;
 }
 
@@ -391,7 +526,7 @@ struct Call {
 
 int run(const char* who, hipStream_t s, const mcn_hnorm_geom* g, const Call& c, const double* positions, const double* frequencies, bool backward,
         float* dgq, float* dgk, void* workspace, size_t workspaceBytes) {
-  const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4, VP = 16 / size;
+  const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4, VP = 4;
   HnormP p = {};
   p.D = g->D; p.N = g->N; p.axes = g->axes;
   p.pairs = positions ? g->pairs : 0;
