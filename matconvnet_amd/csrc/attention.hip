@@ -63,7 +63,8 @@ struct Tensor3 {            // heads where they lie, strides in bytes
 
 struct AttentionP {
   Tensor3 q, k, v, o, dO, dq, dk, dv;
-  float *logSums, *parts, *partSums;     // parts: a slice's o (normalised) and log sums
+  float *logSums, *parts, *partSums;     // parts: a slice's o (normalised) and log sums; backward, of groupParts: [M][keyHeads][2][DW] of dk and dv
+  int groupParts, headsOfPart;           // dk, dv: the group's heads in so many workgroups
   float *statL, *statD;                  // backward, [heads][N]: -L/scale, -delta
   const int *qStarts, *kStarts;
   int sequences, each, eachKeys;         // without starts: queries and keys of a sequence
@@ -809,8 +810,11 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
   static_assert(RT <= 64, "one load brings the statistics of a tile");
   __shared__ __attribute__((aligned(16))) char lds[kAhead * bufferBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = wave % NB, share0 = wave / NB * 32;
-  const int head = blockIdx.x % p.keyHeads;
-  const Span span = find<32 * NB, true>(p, blockIdx.x / p.keyHeads, lane);
+  int id = blockIdx.x;
+  const int head = id % p.keyHeads;
+  id /= p.keyHeads;
+  const int part = id % p.groupParts, firstHead = part * p.headsOfPart, heads = std::min(p.headsOfPart, p.G - firstHead);
+  const Span span = find<32 * NB, true>(p, id / p.groupParts, lane);
   if (span.first < 0) return;
   const int off = span.m - span.n;
   const int key = span.first + 32 * block + (lane & 31);
@@ -830,10 +834,10 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
 #pragma unroll
     for (int s = 0; s < T::steps; ++s) v[s] = chunk_of<V>(vAt, 2 * s + (lane >> 5), p.D, live);
   }
-  const char* queries = p.q.data + (long long)span.q0 * p.q.position + (long long)head * p.G * p.q.head;
-  const char* ders = p.dO.data + (long long)span.q0 * p.dO.position + (long long)head * p.G * p.dO.head;
-  const float* statL = p.statL + (long long)head * p.G * p.N + span.q0;
-  const float* statD = p.statD + (long long)head * p.G * p.N + span.q0;
+  const char* queries = p.q.data + (long long)span.q0 * p.q.position + ((long long)head * p.G + firstHead) * p.q.head;
+  const char* ders = p.dO.data + (long long)span.q0 * p.dO.position + ((long long)head * p.G + firstHead) * p.dO.head;
+  const float* statL = p.statL + ((long long)head * p.G + firstHead) * p.N + span.q0;
+  const float* statD = p.statD + ((long long)head * p.G + firstHead) * p.N + span.q0;
   Loader<V, DW, RT, NW> loadQ, loadD;
   loadQ.begin(p.q, p.D, wave, lane);
   loadD.begin(p.dO, p.D, wave, lane);
@@ -867,7 +871,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
   for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
-  const int each = begin < span.n ? (span.n - begin + RT - 1) / RT : 0, tiles = each * p.G;
+  const int each = begin < span.n ? (span.n - begin + RT - 1) / RT : 0, tiles = each * heads;
   if (tiles) bring_tile(lds);
   int turn = 0, i0 = begin;
   for (int t = 0; t < tiles; ++t) {
@@ -926,7 +930,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       const V* kj = (const V*)(p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head);
       const V* vj = (const V*)(p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head);
 #pragma unroll 1
-      for (int t = 0; t < p.G * span.n; ++t) {
+      for (int t = 0; t < heads * span.n; ++t) {
         const int g = t / span.n, i = t % span.n;
         if (!live || i < firstOf) continue;
         const V* qi = (const V*)(queries + (long long)i * p.q.position + (long long)g * p.q.head);
@@ -956,6 +960,18 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     }
   }
   if (!live) return;
+  if (p.groupParts > 1) {
+    char* at = (char*)(p.parts + (((long long)part * p.M + span.k0 + key) * p.keyHeads + head) * 2 * DW);
+#pragma unroll
+    for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int first = 32 * d + 8 * (r / 4) + 4 * (lane >> 5);
+        store4<float>(at, first, DW, 1, dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]);
+        store4<float>(at + DW * 4, first, DW, 1, dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]);
+      }
+    return;
+  }
 #pragma unroll
   for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
@@ -968,6 +984,30 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
         store4<V>(p.dv.data + (long long)(span.k0 + key) * p.dv.position + head * p.dv.head, at, p.D, p.vector, dv[d][r], dv[d][r + 1], dv[d][r + 2],
                   dv[d][r + 3]);
     }
+}
+
+// dk and dv of a group whose heads were in several workgroups: the parts added up in their order.  A thread per key, head and four channels.
+template <class V, int DW>
+__global__ __launch_bounds__(256) void attention_dkv_join(AttentionP p) {
+  constexpr int kFours = 2 * DW / 4;
+  const long long index = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)p.M * p.keyHeads;
+  const long long item = index / kFours;
+  if (item >= all) return;
+  const int four = (int)(index % kFours), key = (int)(item / p.keyHeads), head = (int)(item % p.keyHeads);
+  if (p.kStarts && (key < clamped(p.kStarts[0], p.M) || key >= clamped(p.kStarts[p.sequences], p.M))) return;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int part = 0; part < p.groupParts; ++part) {
+    const float4 v = *(const float4*)(p.parts + (part * all + item) * 2 * DW + 4 * four);
+    sum.x += v.x;
+    sum.y += v.y;
+    sum.z += v.z;
+    sum.w += v.w;
+  }
+  const bool isK = four < kFours / 2;
+  const Tensor3& out = isK ? p.dk : p.dv;
+  if (!out.data) return;
+  const float f = isK ? p.scale : 1.f;
+  store4<V>(out.data + key * out.position + head * out.head, 4 * (four % (kFours / 2)), p.D, p.vector, sum.x * f, sum.y * f, sum.z * f, sum.w * f);
 }
 
 // ------------------------------------------------------------------------------------------ operands that do not start at 16 bytes
@@ -1047,6 +1087,7 @@ size_t packed_bytes(int positions, int heads, int D, int size) { return rounded(
 
 struct Plan {
   int DW, size, G, blocks, slices;
+  int dqBlocks, dkvBlocks, groupParts, headsOfPart;   // backward
   size_t partsAt, sumsAt, statAt, packAt, bytes;
 };
 
@@ -1076,7 +1117,24 @@ Plan plan_of(const mcn_attention_geom* g, int backward) {
     const long long most = std::max<long long>(1, g->M / sequences / (4 * tile));
     l.slices = (int)std::max<long long>(1, std::min<long long>({64, most, want / std::max<long long>(1, groups)}));
   }
+  l.groupParts = 1;
+  l.headsOfPart = l.G;
+  if (backward) {
+    const long long cus = std::max(1, device_compute_units());
+    l.dqBlocks = split("attention_dq_split", (rows / 128 + sequences) * g->keyHeads < 2 * cus) ? 2 : 4;
+    l.dkvBlocks = split("attention_dkv_split", (g->M / 128 + sequences) * (long long)g->keyHeads < (g->N < 512ll * sequences ? 2 : l.DW == 64 ? 6 : 4) * cus) ? 2 : 4;
+    // The heads of a group in several workgroups, where there are not two rounds of them otherwise (GROUP_PARTS)
+    const long long groups = std::max(1ll, ((long long)g->M / (32 * l.dkvBlocks) + sequences) * g->keyHeads), want = (l.size == 2 ? 4 : 2) * cus;
+    const int forced = tunable("attention_group_parts", 0);
+    const int parts = forced ? std::min(forced, l.G) : (int)std::max<long long>(1, std::min<long long>(l.G, (want + groups - 1) / groups));
+    l.headsOfPart = div_up(l.G, parts);
+    l.groupParts = div_up(l.G, l.headsOfPart);
+  }
   size_t at = 0;
+  if (l.groupParts > 1) {
+    l.partsAt = at;
+    at += rounded((size_t)l.groupParts * g->M * g->keyHeads * 2 * l.DW * sizeof(float));
+  }
   if (l.slices > 1) {
     l.partsAt = at;
     at += rounded((size_t)l.slices * g->N * g->heads * l.DW * sizeof(float));
@@ -1146,6 +1204,8 @@ void common(AttentionP* p, const mcn_attention_geom* g, const Plan& l, const int
   p->D = g->D; p->G = l.G; p->heads = g->heads; p->keyHeads = g->keyHeads;
   p->N = g->N; p->M = g->M; p->causal = g->causal != 0;
   p->slices = l.slices;
+  p->groupParts = l.groupParts;
+  p->headsOfPart = l.headsOfPart;
   p->byG = FastDiv(l.G);
   const double scale = g->scale > 0 ? g->scale : 1.0 / std::sqrt((double)g->D);
   p->scale = (float)scale;
@@ -1182,11 +1242,11 @@ int forward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
 }
 
 template <class V, int DW>
-int backward(const char* who, hipStream_t s, AttentionP& p) {
+int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   constexpr int KT = sizeof(V) == 2 ? 64 : 32;
   if (p.N) {
     const long long rows = (long long)p.N * p.G;
-    const bool two = split("attention_dq_split", (rows / 128 + p.sequences) * p.keyHeads < 2ll * device_compute_units());
+    const bool two = l.dqBlocks == 2;
     const long long blocks = (long long)tiles_of(&p, p.each * p.G, two ? 64 : 128, rows) * p.keyHeads;
     if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
     KernelTimer timer("attention_dq", s);
@@ -1196,12 +1256,20 @@ int backward(const char* who, hipStream_t s, AttentionP& p) {
     if (rc) return rc;
   }
   if (!p.M || (!p.dk.data && !p.dv.data)) return MCN_SUCCESS;
-  const bool two = split("attention_dkv_split", (p.M / 128 + p.sequences) * p.keyHeads < (p.N < 512ll * p.sequences ? 2ll : DW == 64 ? 6ll : 4ll) * device_compute_units());
-  const long long blocks = (long long)tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads;
+  const bool two = l.dkvBlocks == 2;
+  const long long blocks = (long long)tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads * p.groupParts;
   if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
-  KernelTimer timer("attention_dkv", s);
-  if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((attention_dkv<V, DW, 4, 1>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+  {
+    KernelTimer timer("attention_dkv", s);
+    if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attention_dkv<V, DW, 4, 1>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+  }
+  int rc = check_launch(who);
+  if (rc || p.groupParts == 1) return rc;
+  const long long threads = (long long)p.M * p.keyHeads * (2 * DW / 4);
+  if (threads >= (1ll << 39)) return fail(MCN_UNSUPPORTED, "%s: too many keys", who);
+  KernelTimer timer("attention_dkv_join", s);
+  hipLaunchKernelGGL((attention_dkv_join<V, DW>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
   return check_launch(who);
 }
 
@@ -1211,7 +1279,7 @@ int forward_of(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
 }
 template <class V>
 int backward_of(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
-  return l.DW == 64 ? backward<V, 64>(who, s, p) : l.DW == 96 ? backward<V, 96>(who, s, p) : backward<V, 128>(who, s, p);
+  return l.DW == 64 ? backward<V, 64>(who, s, p, l) : l.DW == 96 ? backward<V, 96>(who, s, p, l) : backward<V, 128>(who, s, p, l);
 }
 
 int check_starts(const char* who, const mcn_attention_geom* g, const int* qStarts, const int* kStarts) {
@@ -1319,6 +1387,7 @@ int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, con
   p.dv = in_bytes(derV, size);
   p.vector = g->D % 4 == 0 && stores_well(derQ) && stores_well(derK) && stores_well(derV);
   p.logSums = const_cast<float*>(logSums);
+  p.parts = (float*)((char*)workspace + l.partsAt);
   p.statL = (float*)((char*)workspace + l.statAt);
   p.statD = p.statL + rounded((size_t)g->N * g->heads * sizeof(float)) / sizeof(float);
   return g->dataType == MCN_BFLOAT16 ? backward_of<bf16>(who, s, p, l) : backward_of<float>(who, s, p, l);

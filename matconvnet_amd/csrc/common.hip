@@ -66,6 +66,7 @@ Tunable g_tunables[] = {
     {"attention_forward_split", 0},    // 1, 2: force so many wavefronts to a block of 32 rows; 0 = choose
     {"attention_dq_split", 0},         // (likewise)
     {"attention_dkv_split", 0},        // (likewise, of 32 keys)
+    {"attention_group_parts", 0},      // > 0: dk and dv with the heads of a group in so many workgroups
     {"ortho_no_narrow", 0},            // 1: narrow matrices through the launches of the others too
     {"product_tile", 0},               // 64, 128, 256: force the tile of the products of fcloss.hip and ortho.hip; anything else = choose
     {"product_slices", 0},             // > 0: cut their reductions among so many workgroups (32 at most, and as far as there are stages)
