@@ -126,20 +126,22 @@ struct Tile {
     const int row = lane & 31;   // (first is a multiple of 32: the turn is the lane's own)
     return *(const uintx4*)(lds + (first + row) * rowBytes + (((2 * s) ^ (turn(row) ^ (lane >> 5))) << 4));
   }
+  // (bfloat16) rows first .. first + 15 as the other operand of `across`, the 32 columns from 32 b on
+  __device__ static __forceinline__ uintx4 turned(const char* lds, int first, int b, int lane) {
+    typedef __attribute__((address_space(3))) shortx4* lds_shorts;
+    const int quarter = (lane >> 5) * 4 + (lane >> 2 & 3), chunk = 4 * b + (lane >> 4 & 1) * 2 + (lane >> 1 & 1), within = (lane & 1) * 8;
+    const int r0 = first + quarter, r1 = r0 + 8;
+    const uintx2 a0 = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_shorts)(lds + r0 * rowBytes + ((chunk ^ turn(quarter)) << 4) + within)));
+    const uintx2 a1 = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_shorts)(lds + r1 * rowBytes + ((chunk ^ turn(quarter + 8)) << 4) + within)));
+    return (uintx4){a0.x, a0.y, a1.x, a1.y};
+  }
   // acc += (rows first .. first + 31 of the tile)' x p, the 32 columns from 32 b on: p in the order of a result's registers
   __device__ static __forceinline__ floatx16 across(const char* lds, int first, int b, int lane, const uintx4 (&p)[sizeof(V) == 4 ? 4 : 2], floatx16 acc) {
     if (sizeof(V) == 2) {
-      typedef __attribute__((address_space(3))) shortx4* lds_shorts;
-      const int quarter = (lane >> 5) * 4 + (lane >> 2 & 3), chunk = 4 * b + (lane >> 4 & 1) * 2 + (lane >> 1 & 1), within = (lane & 1) * 8;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int r0 = first + 16 * s + quarter, r1 = r0 + 8;
-        const uintx2 a0 = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_shorts)(lds + r0 * rowBytes + ((chunk ^ turn(quarter)) << 4) + within)));
-        const uintx2 a1 = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_shorts)(lds + r1 * rowBytes + ((chunk ^ turn(quarter + 8)) << 4) + within)));
-        acc = Matrix<bf16>::along((uintx4){a0.x, a0.y, a1.x, a1.y}, p[s], acc);
-      }
+      for (int s = 0; s < 2; ++s) acc = Matrix<bf16>::along(turned(lds, first + 16 * s, b, lane), p[s], acc);
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -195,6 +197,22 @@ struct Loader {
     }
   }
 };
+
+// N matrix instructions, step i of them on what read(i) brought from LDS DEPTH steps before: left to itself the compiler reads one step ahead, and
+// every instruction waits for most of a read's latency.  Vector instructions may move among the steps.
+template <int DEPTH, int N, class Read, class Step>
+__device__ __forceinline__ void steps_ahead(Read read, Step step) {
+  uintx4 a[DEPTH];
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) a[i] = read(i);
+  __builtin_amdgcn_sched_barrier(6);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    step(i, a[i % DEPTH]);
+    if (i + DEPTH < N) a[i % DEPTH] = read(i + DEPTH);
+    __builtin_amdgcn_sched_barrier(6);
+  }
+}
 
 // 16 bytes of a row in global memory, zero where there is none
 template <class V>
@@ -330,50 +348,81 @@ __device__ __forceinline__ void forward_tile(const char* __restrict__ keys, cons
   bring_next(next);
   floatx16 s[KB];
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
+  for (int b = 0; b < KB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+  // masks, the running maximum; then exponentials
+  const auto largest = [&]() __attribute__((always_inline)) {
+    if (edge) {
 #pragma unroll
-    for (int k = 0; k < T::steps; ++k) s[b] = Matrix<V>::along(T::along(keys, 32 * b, k, lane), q[k], s[b]);
-  }
-  if (edge) {
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (j0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 >= limit) s[b][r] = -INFINITY;
+    }
+    float m = -INFINITY;
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (j0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 >= limit) s[b][r] = -INFINITY;
-  }
-  float m = -INFINITY;
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
+    m = fmaxf(m, other_half(m));
+    // The reference of the exponentials is raised only when a score lies more than 2^8 above it: what is summed stays below 2^8 a key, and the
+    // outputs are scaled anew a few times in all instead of every tile.
+    const bool raise = m * c > most * c + 8.f || (most == -INFINITY && m > -INFINITY);
+    if (__any(raise)) {
+      const float to = raise ? m : most;
+      const float f = raise ? (most == -INFINITY ? 0.f : power2((most - to) * c)) : 1.f;
+      most = to;
+      sum *= f;
 #pragma unroll
-  for (int b = 0; b < KB; ++b)
+      for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
-  m = fmaxf(m, other_half(m));
-  // The reference of the exponentials is raised only when a score lies more than 2^8 above it: what is summed stays below 2^8 a key, and the
-  // outputs are scaled anew a few times in all instead of every tile.
-  const bool raise = m * c > most * c + 8.f || (most == -INFINITY && m > -INFINITY);
-  if (__any(raise)) {
-    const float to = raise ? m : most;
-    const float f = raise ? (most == -INFINITY ? 0.f : power2((most - to) * c)) : 1.f;
-    most = to;
-    sum *= f;
-#pragma unroll
-    for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] *= f;
-  }
-  const float shift = most == -INFINITY ? 0.f : most * c;
-#pragma unroll
-  for (int b = 0; b < KB; ++b) {
+        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+    }
+  };
+  uintx4 operand[KB][sizeof(V) == 4 ? 4 : 2];
+  const auto exponentials = [&](int b) __attribute__((always_inline)) {
+    const float shift = most == -INFINITY ? 0.f : most * c;
     float e[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) e[r] = power2(s[b][r] * c - shift);
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum += e[r];
-    uintx4 operand[sizeof(V) == 4 ? 4 : 2];
-    T::operand(operand, e);
+    T::operand(operand[b], e);
+  };
+  if constexpr (sizeof(V) == 2) {
+    constexpr int S = T::steps, P = DW / 32 * 2;   // steps of a block of 32 keys: scores, outputs
+    steps_ahead<S, KB * (S + P)>(
+        [&](int i) __attribute__((always_inline)) {
+          if (i < KB * S) return T::along(keys, 32 * (i / S), i % S, lane);
+          i -= KB * S;
+          return T::turned(values, 32 * (i / P) + 16 * (i % 2), i % P / 2, lane);
+        },
+        [&](int i, uintx4 a) __attribute__((always_inline)) {
+          if (i < KB * S) {
+            s[i / S] = Matrix<V>::along(a, q[i % S], s[i / S]);
+            return;
+          }
+          i -= KB * S;
+          if (i == 0) {
+            largest();
 #pragma unroll
-    for (int d = 0; d < DW / 32; ++d) o[d] = T::across(values, 32 * b, d, lane, operand, o[d]);
+            for (int b = 0; b < KB; ++b) exponentials(b);
+          }
+          o[i % P / 2] = Matrix<V>::along(a, operand[i / P][i % 2], o[i % P / 2]);
+        });
+  } else {
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int k = 0; k < T::steps; ++k) s[b] = Matrix<V>::along(T::along(keys, 32 * b, k, lane), q[k], s[b]);
+    largest();
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      exponentials(b);
+#pragma unroll
+      for (int d = 0; d < DW / 32; ++d) o[d] = T::across(values, 32 * b, d, lane, operand[b], o[d]);
+    }
   }
 }
 
@@ -590,22 +639,43 @@ __device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const cha
     for (int r = 0; r < 16; ++r) s[r] = negL;
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = negDelta;
-#pragma unroll
-    for (int k = 0; k < T::steps; ++k) s = Matrix<V>::along(T::along(keys, 32 * b, k, lane), q[k], s);
-#pragma unroll
-    for (int k = 0; k < T::steps; ++k) dp = Matrix<V>::along(T::along(values, 32 * b, k, lane), dO[k], dp);
-    float e[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c) * dp[r];
-    if (edge) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (j0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 >= limit) e[r] = 0.f;
-    }
     uintx4 operand[sizeof(V) == 4 ? 4 : 2];
-    T::operand(operand, e);
+    const auto scores = [&]() __attribute__((always_inline)) {
+      float e[16];
 #pragma unroll
-    for (int d = 0; d < DW / 32; ++d) dq[d] = T::across(keys, 32 * b, d, lane, operand, dq[d]);
+      for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c) * dp[r];
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (j0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 >= limit) e[r] = 0.f;
+      }
+      T::operand(operand, e);
+    };
+    if constexpr (sizeof(V) == 2) {
+      constexpr int S = T::steps, P = DW / 32 * 2;
+      steps_ahead<3, 2 * S + P>(
+          [&](int i) __attribute__((always_inline)) {
+            if (i < S) return T::along(keys, 32 * b, i, lane);
+            if (i < 2 * S) return T::along(values, 32 * b, i - S, lane);
+            return T::turned(keys, 32 * b + 16 * (i % 2), (i - 2 * S) / 2, lane);
+          },
+          [&](int i, uintx4 a) __attribute__((always_inline)) {
+            if (i < S) s = Matrix<V>::along(a, q[i], s);
+            else if (i < 2 * S) dp = Matrix<V>::along(a, dO[i - S], dp);
+            else {
+              if (i == 2 * S) scores();
+              dq[(i - 2 * S) / 2] = Matrix<V>::along(a, operand[i % 2], dq[(i - 2 * S) / 2]);
+            }
+          });
+    } else {
+#pragma unroll
+      for (int k = 0; k < T::steps; ++k) s = Matrix<V>::along(T::along(keys, 32 * b, k, lane), q[k], s);
+#pragma unroll
+      for (int k = 0; k < T::steps; ++k) dp = Matrix<V>::along(T::along(values, 32 * b, k, lane), dO[k], dp);
+      scores();
+#pragma unroll
+      for (int d = 0; d < DW / 32; ++d) dq[d] = T::across(keys, 32 * b, d, lane, operand, dq[d]);
+    }
   }
 }
 
@@ -765,50 +835,57 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
   bring_next(next);
   lane = fresh<V, DW>(lane);
   floatx16 s, dp;
+  float e[16];
+  uintx4 operand[sizeof(V) == 4 ? 4 : 2];
+  const auto start = [&](floatx16& v, const float* stat) __attribute__((always_inline)) {
 #pragma unroll
-  for (int r = 0; r < 16; r += 4) {
-    const float4 l = *(const float4*)(statL + 2 * r + 4 * (lane >> 5));
-    s[r] = l.x; s[r + 1] = l.y; s[r + 2] = l.z; s[r + 3] = l.w;
-  }
+    for (int r = 0; r < 16; r += 4) {
+      const float4 l = *(const float4*)(stat + 2 * r + 4 * (lane >> 5));
+      v[r] = l.x; v[r + 1] = l.y; v[r + 2] = l.z; v[r + 3] = l.w;
+    }
+  };
+  const auto masked = [&]() __attribute__((always_inline)) {   // (firstOf: the first position that sees this lane's key)
+    if (!edge) return;
+    const int here = i0 + 4 * (lane >> 5), low = firstOf - here, high = n - here;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (8 * (r / 4) + r % 4 < low || 8 * (r / 4) + r % 4 >= high) e[r] = 0.f;
+  };
+  const auto probabilities = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c);
+    masked();
+    T::operand(operand, e);
+  };
+  const auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) e[r] *= dp[r];
+    masked();
+    T::operand(operand, e);
+  };
+  start(s, statL);
 #pragma unroll
   for (int t = 0; t < T::steps; ++t) s = Matrix<V>::along(T::along(queries, 0, t, lane), k[t], s);
-  float e[16];
-#pragma unroll
-  for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c);
-  if (edge) {   // (firstOf: the first position that sees this lane's key)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int i = i0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-      if (i >= n || i < firstOf) e[r] = 0.f;
-    }
-  }
-  uintx4 operand[sizeof(V) == 4 ? 4 : 2];
-  T::operand(operand, e);
+  probabilities();
 #pragma unroll
   for (int d = 0; d < DW / 32; ++d) dv[d] = T::across(ders, 0, d, lane, operand, dv[d]);
-#pragma unroll
-  for (int r = 0; r < 16; r += 4) {
-    const float4 l = *(const float4*)(statD + 2 * r + 4 * (lane >> 5));
-    dp[r] = l.x; dp[r + 1] = l.y; dp[r + 2] = l.z; dp[r + 3] = l.w;
-  }
+  start(dp, statD);
 #pragma unroll
   for (int t = 0; t < T::steps; ++t) dp = Matrix<V>::along(T::along(ders, 0, t, lane), v[t], dp);
-#pragma unroll
-  for (int r = 0; r < 16; ++r) e[r] = edge && e[r] == 0.f ? 0.f : e[r] * dp[r];
-  T::operand(operand, e);
+  scores();
 #pragma unroll
   for (int d = 0; d < DW / 32; ++d) dk[d] = T::across(queries, 0, d, lane, operand, dk[d]);
 }
 
 // NB blocks of 32 keys; they walk over the positions of one head of the group after the other.  NS wavefronts share a block, each takes its 32
 // positions of every tile, and their sums are added up through LDS.
-template <class V, int DW, int NB, int NS>
+template <class V, int DW, int NB, int NS, int AHEAD>
 __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attention_dkv(AttentionP p) {
   typedef Tile<V, DW> T;
   constexpr int NW = NB * NS, RT = 32 * NS;
   constexpr int tileBytes = RT * T::rowBytes, statBytes = RT * 4, bufferBytes = 2 * tileBytes + 2 * statBytes;
   static_assert(RT <= 64, "one load brings the statistics of a tile");
-  __shared__ __attribute__((aligned(16))) char lds[kAhead * bufferBytes];
+  __shared__ __attribute__((aligned(16))) char lds[AHEAD * bufferBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = wave % NB, share0 = wave / NB * 32;
   int id = blockIdx.x;
   const int head = id % p.keyHeads;
@@ -843,9 +920,10 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
   loadD.begin(p.dO, p.D, wave, lane);
   // the tile that is brought next: position nextI of the head whose first positions are at headQ, headD, headStat
   const char *headQ = queries, *headD = ders;
-  const char *nextQ = queries + (long long)begin * p.q.position, *nextD = ders + (long long)begin * p.dO.position;
+  const int each = begin < span.n ? (span.n - begin + RT - 1) / RT : 0, tiles = each * heads, last = begin + (each - 1) * RT;
+  const char *nextQ = queries + (long long)last * p.q.position, *nextD = ders + (long long)last * p.dO.position;
   const float* headStat = wave ? statD : statL;   // (of the first two wavefronts)
-  int nextI = begin;
+  int nextI = last;
   const auto bring_tile = [&](char* to) __attribute__((always_inline)) {
     loadQ.bring(to, nextQ, span.n - nextI, wave);
     loadD.bring(to + tileBytes, nextD, span.n - nextI, wave);
@@ -854,16 +932,16 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(headStat + nextI), 0, std::min(span.n - nextI, RT) * 4, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + 2 * tileBytes + wave * statBytes), 4, lane * 4, 0, 0, 0);
     }
-    nextI += RT;
-    nextQ += (long long)RT * p.q.position;
-    nextD += (long long)RT * p.dO.position;
-    if (nextI >= span.n) {   // the next head
-      nextI = begin;
+    nextI -= RT;
+    nextQ -= (long long)RT * p.q.position;
+    nextD -= (long long)RT * p.dO.position;
+    if (nextI < begin) {   // the next head
+      nextI = last;
       headQ += p.q.head;
       headD += p.dO.head;
       headStat += p.N;
-      nextQ = headQ + (long long)begin * p.q.position;
-      nextD = headD + (long long)begin * p.dO.position;
+      nextQ = headQ + (long long)last * p.q.position;
+      nextD = headD + (long long)last * p.dO.position;
     }
   };
   floatx16 dk[DW / 32], dv[DW / 32];
@@ -871,16 +949,18 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
   for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
-  const int each = begin < span.n ? (span.n - begin + RT - 1) / RT : 0, tiles = each * heads;
   if (tiles) bring_tile(lds);
-  int turn = 0, i0 = begin;
+  if (AHEAD == 3 && tiles > 1) bring_tile(lds + bufferBytes);
+  int at0 = 0, i0 = last;   // where the tile that is due lies
   for (int t = 0; t < tiles; ++t) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    char* from = lds + turn * bufferBytes;
-    char* to = lds + (turn ^ 1) * bufferBytes;
-    turn ^= 1;
+    // (three buffers: the tile behind this one may be on its way still, 2 pieces a wavefront of each tensor)
+    if (AHEAD == 3 && t + 1 < tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * Loader<V, DW, RT, NW>::pieces) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    char* from = lds + at0;
+    char* to = lds + (at0 == 0 ? (AHEAD - 1) * bufferBytes : at0 - bufferBytes);   // the one of the tile before
+    at0 = at0 == (AHEAD - 1) * bufferBytes ? 0 : at0 + bufferBytes;
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
-      if (t + 1 < tiles) bring_tile(at);
+      if (t + AHEAD - 1 < tiles) bring_tile(at);
     };
     const int i = i0 + share0;
     if (i + 32 > some && i < span.n)
@@ -888,8 +968,8 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
                       (const float*)(from + 2 * tileBytes + statBytes) + share0, to, bring_next, k, v, dk, dv, i, span.n, firstOf, i < all || i + 32 > span.n, p.c,
                       lane);
     else bring_next(to);
-    i0 += RT;
-    if (i0 >= span.n) i0 = begin;
+    i0 -= RT;
+    if (i0 < begin) i0 = last;
   }
   if (NS == 2) {
     constexpr int values = DW / 32 * 16;
@@ -1257,12 +1337,13 @@ int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   }
   if (!p.M || (!p.dk.data && !p.dv.data)) return MCN_SUCCESS;
   const bool two = l.dkvBlocks == 2;
+  constexpr int AHEADX = 2;
   const long long blocks = (long long)tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads * p.groupParts;
   if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
   {
     KernelTimer timer("attention_dkv", s);
-    if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((attention_dkv<V, DW, 4, 1>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attention_dkv<V, DW, 4, 1, AHEADX>), dim3((unsigned)blocks), dim3(256), 0, s, p);
   }
   int rc = check_launch(who);
   if (rc || p.groupParts == 1) return rc;
