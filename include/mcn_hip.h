@@ -612,7 +612,8 @@ MCN_API int mcn_hnorm_backward(mcn_stream_t stream, const mcn_hnorm_geom* g, con
    sequences + 1 ascending numbers, both or neither; NULL: sequences of N / sequences queries and M / sequences keys each).  Either part may be
    empty; starts outside of 0..N or 0..M are taken as the nearest of these.  causal != 0: the queries are the last positions of their
    sequence, query i of n sees key j of m where j <= i + m - n.  A query that sees no key has o = 0, logSums = -infinity and gives no
-   derivative; keys that a query does not see have no part in it, whatever they hold.  Rows of no sequence are left as they were.
+   derivative; keys that a query does not see have no part in it, whatever they hold.  Rows of no sequence (before the first one's, behind
+   the last one's) are left as they were, or with clear != 0 set to zero.
    q, k, v, o and all derivatives are of dataType.  logSums is N x heads, a position's heads side by side.  scale 0: 1/sqrt(D).  D
    at most 128.
    backward: all that is asked for (derQ, derK, derV; NULL or of null data: not made) is fully overwritten for all positions of sequences; o and logSums
@@ -625,6 +626,7 @@ typedef struct mcn_attention_geom {
   int N, M;          /* queries and keys of all sequences */
   int sequences;
   int causal;
+  int clear;
   int dataType;
   double scale;
 } mcn_attention_geom;

@@ -47,7 +47,7 @@ class HnormGeom(C.Structure):
 
 
 class AttentionGeom(C.Structure):
-    _fields_ = [(n, C.c_int) for n in ("D", "heads", "keyHeads", "N", "M", "sequences", "causal", "dataType")] + [("scale", C.c_double)]
+    _fields_ = [(n, C.c_int) for n in ("D", "heads", "keyHeads", "N", "M", "sequences", "causal", "clear", "dataType")] + [("scale", C.c_double)]
 
 
 FLOAT, BFLOAT16 = 0, 1   # MCN_FLOAT, MCN_BFLOAT16
@@ -1021,26 +1021,22 @@ def _attention_geom(q, k, v, sequences, q_starts, k_starts, causal, scale):
             raise ValueError("the positions are not %d sequences of one length" % sequences)
     if scale is not None and not scale > 0:
         raise ValueError("the scale is not positive")
-    return AttentionGeom(q.shape[2], q.shape[1], k.shape[1], q.shape[0], k.shape[0], sequences, int(bool(causal)), data_type(q, k, v),
+    return AttentionGeom(q.shape[2], q.shape[1], k.shape[1], q.shape[0], k.shape[0], sequences, int(bool(causal)), 0, data_type(q, k, v),
                          0.0 if scale is None else float(scale))
-
-
-def _rows(x, starts):
-    """A fresh tensor like x for rows that a call writes: all of them, or those of sequences (the others are zero then)"""
-    return _alike(x) if starts is None else _torch().zeros(x.shape, dtype=x.dtype, device=x.device)
 
 
 def attention_forward(q, k, v, q_starts=None, k_starts=None, sequences=None, causal=False, scale=None, out=None, ws=None):
     """Softmax attention of packed sequences (include/mcn_hip.h: mcn_attention_forward): (y, log_sums).  q (N, heads, D), k and v
     (M, keyHeads, D): float32 or bfloat16, channels neighbours, any other strides.  q_starts, k_starts: int32 on the device, sequences + 1
     numbers each; without them `sequences` (one, if not given) of one length.  causal: the queries are the last positions of their
-    sequence.  log_sums (N, heads) in float32.  out: the tensor y is written to, whose rows of no sequence are left alone (a fresh one
-    holds zeros there)."""
+    sequence.  log_sums (N, heads) in float32.  out: the tensor y is written to, whose rows of no sequence are left alone (and log_sums holds
+    nothing in particular there; without out both hold zeros)."""
     g = _attention_geom(q, k, v, sequences, q_starts, k_starts, causal, scale)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise ValueError("out is not of the queries' shape and type")
-    y = _rows(q, q_starts) if out is None else out
-    log_sums = _singles(q, g.N, g.heads) if q_starts is None else q.new_zeros((g.N, g.heads), dtype=_torch().float32)
+    g.clear = int(out is None)
+    y = _alike(q) if out is None else out
+    log_sums = _singles(q, g.N, g.heads)
     wp, wn, held = _scratch(ws, q, lib().mcn_attention_workspace_bytes(C.byref(g), 0))
     check(lib().mcn_attention_forward(stream(), C.byref(g), _heads("out", y), ptr(log_sums), _heads("q", q), _heads("k", k), _heads("v", v),
                                       ptr(q_starts), ptr(k_starts), wp, wn))
@@ -1058,13 +1054,9 @@ def attention_backward(q, k, v, y, log_sums, dy, q_starts=None, k_starts=None, s
     _single("log_sums", log_sums)
     if log_sums.numel() != g.N * g.heads:
         raise ValueError("log_sums does not have one value per query and head")
-    names, like, starts = ("dq", "dk", "dv"), (q, k, v), (q_starts, k_starts, k_starts)
-    if out is None:
-        out = (None, None, None)
-    for name, t, x in zip(names, out, like):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError("%s is not of its input's shape and type" % name)
-    d = [(t if t is not None else _rows(x, s)) if w else None for w, t, x, s in zip(want, out, like, starts)]
+    g.clear = int(out is None)
+    d = [t if w else None for w, t in zip(want, _outs("dq dk dv", out, q, k, v))] if out is not None else [
+        _alike(x) if w else None for w, x in zip(want, (q, k, v))]
     wp, wn, held = _scratch(ws, q, lib().mcn_attention_workspace_bytes(C.byref(g), 1))
     check(lib().mcn_attention_backward(stream(), C.byref(g), _heads("dq", d[0]), _heads("dk", d[1]), _heads("dv", d[2]), _heads("y", y), ptr(log_sums),
                                        _heads("q", q), _heads("k", k), _heads("v", v), _heads("dy", dy), ptr(q_starts), ptr(k_starts), wp, wn))

@@ -1121,6 +1121,31 @@ __global__ __launch_bounds__(256) void attention_pack(PackP p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------ rows of no sequence
+
+struct ClearP {
+  char* data[4];
+  long long position[4], head[4];   // strides in bytes
+  const int* starts[4];
+  int positions[4], heads[4], width[4], size[4];   // (width: values of a head)
+  int n, sequences;
+};
+
+// Zeros for the rows before the first sequence's and behind the last one's
+__global__ __launch_bounds__(256) void attention_clear(ClearP p) {
+  for (int t = 0; t < p.n; ++t) {
+    const int first = clamped(p.starts[t][0], p.positions[t]), last = std::max(first, clamped(p.starts[t][p.sequences], p.positions[t]));
+    const long long rows = first + p.positions[t] - last, each = (long long)p.heads[t] * p.width[t];
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * each; i += (long long)gridDim.x * 256) {
+      const long long r = i / each;
+      const int within = (int)(i % each), head = within / p.width[t], d = within % p.width[t];
+      char* at = p.data[t] + (r < first ? r : last + r - first) * p.position[t] + head * p.head[t];
+      if (p.size[t] == 4) ((unsigned*)at)[d] = 0u;
+      else ((unsigned short*)at)[d] = 0;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- host
 
 constexpr size_t kAlign = 256;
@@ -1363,6 +1388,29 @@ int backward_of(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   return l.DW == 64 ? backward<V, 64>(who, s, p, l) : l.DW == 96 ? backward<V, 96>(who, s, p, l) : backward<V, 128>(who, s, p, l);
 }
 
+struct Clear {
+  ClearP p = {};
+  void add(const Tensor3& t, const int* starts, int positions, int heads, int width, int size) {
+    if (!t.data) return;
+    const int i = p.n++;
+    p.data[i] = t.data;
+    p.position[i] = t.position;
+    p.head[i] = t.head;
+    p.starts[i] = starts;
+    p.positions[i] = positions;
+    p.heads[i] = heads;
+    p.width[i] = width;
+    p.size[i] = size;
+  }
+  int run(const char* who, hipStream_t s, const mcn_attention_geom* g) {
+    if (!p.n) return MCN_SUCCESS;
+    p.sequences = g->sequences;
+    KernelTimer timer("attention_clear", s);
+    hipLaunchKernelGGL(attention_clear, dim3(256), dim3(256), 0, s, p);
+    return check_launch(who);
+  }
+};
+
 int check_starts(const char* who, const mcn_attention_geom* g, const int* qStarts, const int* kStarts) {
   if (!qStarts != !kStarts) return fail(MCN_ILLEGAL_ARGUMENT, "%s: starts of queries or of keys alone", who);
   if (!qStarts && g->sequences && (g->N % g->sequences || g->M % g->sequences))
@@ -1393,7 +1441,7 @@ int mcn_attention_forward(mcn_stream_t stream, const mcn_attention_geom* g, cons
   const char* who = "mcn_attention_forward";
   int rc = check_geom(who, g);
   if (!rc) rc = check_starts(who, g, queryStarts, keyStarts);
-  if (rc || g->D == 0 || g->N == 0 || g->heads == 0 || g->sequences == 0) return rc;
+  if (rc || g->D == 0 || g->N == 0 || g->heads == 0 || (g->sequences == 0 && !(g->clear && queryStarts))) return rc;
   const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
   rc = check_heads(who, "queries", q, g->heads, g->N, g->D, size, false);
   if (!rc && g->M) rc = check_heads(who, "keys", k, g->keyHeads, g->M, g->D, size, false);
@@ -1412,8 +1460,16 @@ int mcn_attention_forward(mcn_stream_t stream, const mcn_attention_geom* g, cons
   p.o = in_bytes(o, size);
   p.vector = g->D % 4 == 0 && stores_well(o);
   p.logSums = logSums;
+  if (g->clear && queryStarts) {
+    Clear clear;
+    clear.add(p.o, queryStarts, g->N, g->heads, g->D, size);
+    clear.add({(char*)logSums, 4ll * g->heads, 4}, queryStarts, g->N, g->heads, 1, 4);
+    rc = clear.run(who, s, g);
+    if (rc) return rc;
+  }
   p.parts = (float*)((char*)workspace + l.partsAt);
   p.partSums = (float*)((char*)workspace + l.sumsAt);
+  if (g->sequences == 0) return MCN_SUCCESS;
   return g->dataType == MCN_BFLOAT16 ? forward_of<bf16>(who, s, p, l) : forward_of<float>(who, s, p, l);
 }
 
@@ -1424,7 +1480,7 @@ int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, con
   int rc = check_geom(who, g);
   if (!rc) rc = check_starts(who, g, queryStarts, keyStarts);
   const bool wantQ = derQ && derQ->data, wantK = derK && derK->data, wantV = derV && derV->data;
-  if (rc || g->D == 0 || g->heads == 0 || g->sequences == 0 || (g->N == 0 && g->M == 0) || (!wantQ && !wantK && !wantV)) return rc;
+  if (rc || g->D == 0 || g->heads == 0 || (g->sequences == 0 && !(g->clear && queryStarts)) || (g->N == 0 && g->M == 0) || (!wantQ && !wantK && !wantV)) return rc;
   const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
   if (g->N) {
     rc = check_heads(who, "queries", q, g->heads, g->N, g->D, size, false);
@@ -1466,11 +1522,20 @@ int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, con
   p.dq = in_bytes(derQ, size);
   p.dk = in_bytes(derK, size);
   p.dv = in_bytes(derV, size);
+  if (g->clear && queryStarts) {
+    Clear clear;
+    if (g->N) clear.add(p.dq, queryStarts, g->N, g->heads, g->D, size);
+    if (g->M) clear.add(p.dk, keyStarts, g->M, g->keyHeads, g->D, size);
+    if (g->M) clear.add(p.dv, keyStarts, g->M, g->keyHeads, g->D, size);
+    rc = clear.run(who, s, g);
+    if (rc) return rc;
+  }
   p.vector = g->D % 4 == 0 && stores_well(derQ) && stores_well(derK) && stores_well(derV);
   p.logSums = const_cast<float*>(logSums);
   p.parts = (float*)((char*)workspace + l.partsAt);
   p.statL = (float*)((char*)workspace + l.statAt);
   p.statD = p.statL + rounded((size_t)g->N * g->heads * sizeof(float)) / sizeof(float);
+  if (g->sequences == 0) return MCN_SUCCESS;
   return g->dataType == MCN_BFLOAT16 ? backward_of<bf16>(who, s, p, l) : backward_of<float>(who, s, p, l);
 }
 
