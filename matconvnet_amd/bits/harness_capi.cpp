@@ -262,6 +262,7 @@ int vlh_resnet50_loss_derivative(void* net, double derOutput) { return (int)((ha
 int vlh_resnet50_losses(void* net, double values[3]) {
   return (int)((harness::ResNet50*)net)->losses(values, values + 1, values + 2);
 }
+int vlh_resnet50_set_clip(void* net, double maxNorm) { return (int)((harness::ResNet50*)net)->setClip(maxNorm); }
 int vlh_resnet50_sgd_step(void* net, double learningRate, double momentum, double weightDecay) {
   return (int)((harness::ResNet50*)net)->sgdStep(learningRate, momentum, weightDecay);
 }

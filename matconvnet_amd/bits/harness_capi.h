@@ -97,6 +97,8 @@ VLH_API int vlh_resnet50_backward(void* net);
 /* SGD with momentum and weight decay on all parameters (one worker) and the moving average of the batch moments, as
    examples/cnn_train_dag.m:316-364 with the rates of cnn_imagenet_init_resnet.m:178-195; buffers "momentum.<parameter>"
    and "running.<moments>" hold the solver state */
+/* maxNorm > 0: that update clips the derivatives of all parameters together to this norm; buffer "gradientNorm" holds the norm they had */
+VLH_API int vlh_resnet50_set_clip(void* net, double maxNorm);
 VLH_API int vlh_resnet50_sgd_step(void* net, double learningRate, double momentum, double weightDecay);
 /* the loss layers at the end of the network (cnn_imagenet_init_resnet.m:128-139) on buffers "prediction" and "labels"
    (N class numbers 1..classes as floats, 0 = skip): _loss_derivative writes "dprediction" for vlh_resnet50_backward

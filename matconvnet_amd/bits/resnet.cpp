@@ -37,7 +37,8 @@ double conv_flops(int outH, int outW, int fh, int fw, int cin, int cout) {
 
 ResNet50::ResNet50(int N, double epsilon, int imageSize, int classes)
     : N(N), S(imageSize), classes(classes), epsilon(epsilon), fused(true), testMode(false), error(VLE_Success), flops(0), values(NULL),
-      ders(NULL), state(NULL), batchMoments(NULL), runningMoments(NULL), chunkParam(NULL), rates(NULL), chunks(0),
+      ders(NULL), state(NULL), batchMoments(NULL), runningMoments(NULL), chunkParam(NULL), rates(NULL),
+      clip(0), clipWorkspace(NULL), clipBytes(0), chunks(0),
       momentsCount(0), parameterCount(0), deferred(false), partialArena(NULL), sumJobsDevice(NULL), stemPartialBytes(0),
       fcPartialBytes(0), sumJobCount(0), sumBlocks(0), packed(false), packedArena(NULL), packedJobs(NULL), stemBytes(0),
       fcForwardBytes(0), fcBackwardBytes(0), fcBackwardOffset(0), packedJobCount(0), packedBlocks(0), graph(NULL),
@@ -86,6 +87,7 @@ ResNet50::ResNet50(int N, double epsilon, int imageSize, int classes)
 
   make("avg", TensorShape(1, 1, C, N)); make("davg", TensorShape(1, 1, C, N));
   make("prediction", TensorShape(1, 1, classes, N)); make("dprediction", TensorShape(1, 1, classes, N));
+  make("gradientNorm", TensorShape(1, 1, 1, 1));
   make("labels", TensorShape(1, 1, 1, N)); make("loss.terms", TensorShape(1, 1, 1, N)); make("loss.values", TensorShape(4, 1, 1, 1));
   flops += conv_flops(1, 1, 1, 1, C, classes);
   if (error == VLE_Success) buildArenas();
@@ -204,11 +206,35 @@ void ResNet50::view(std::string const& name, TensorShape const& shape, float* me
   slots.push_back(s);
 }
 
+ErrorCode ResNet50::setClip(double maxNorm) {
+  if (error != VLE_Success) return error;
+  if (!(maxNorm >= 0)) {
+    message = "the largest norm of the gradients is negative";
+    return VLE_IllegalArgument;
+  }
+  if (maxNorm > 0 && !clipWorkspace) {
+    clipBytes = mcn_sgd_momentum_clipped_workspace_bytes(chunks);
+    if (hipMalloc(&clipWorkspace, clipBytes) != hipSuccess) {
+      (void)hipGetLastError();
+      clipWorkspace = NULL;
+      message = "cannot allocate the clipping's workspace";
+      return VLE_OutOfGPUMemeory;
+    }
+  }
+  clip = maxNorm;
+  return VLE_Success;
+}
+
 ErrorCode ResNet50::sgdStep(double learningRate, double momentum, double weightDecay) {
   if (error != VLE_Success) return error;
   void* st = context.getHipHelper().getStream();
   // gradient-trained parameters: the default solver of examples/cnn_train_dag.m:340-364, one worker
-  ABI("sgd", mcn_sgd_momentum(st, values, state, ders, chunks, chunkParam, rates, learningRate, weightDecay, momentum, 1.0, 0));
+  if (clip > 0) {
+    ABI("sgd", mcn_sgd_momentum_clipped(st, values, state, ders, chunks, chunkParam, rates, learningRate, weightDecay, momentum, 1.0, 0, clip,
+                                        (float*)slot("gradientNorm").getMemory(), clipWorkspace, clipBytes));
+  } else {
+    ABI("sgd", mcn_sgd_momentum(st, values, state, ders, chunks, chunkParam, rates, learningRate, weightDecay, momentum, 1.0, 0));
+  }
   // moments: trainMethod 'average' (:331-335) with the rate cnn_imagenet_init_resnet.m:190-195 sets, fan-out 1
   const double rate = 0.3;
   ABI("moments", mcn_taccum(st, runningMoments, (float)(1.0 - rate), runningMoments, (float)rate, batchMoments, momentsCount));
@@ -479,7 +505,7 @@ ResNet50::~ResNet50() {
   for (std::size_t i = 0; i < slots.size(); ++i)
     if (slots[i].owned && slots[i].tensor.getMemory()) (void)hipFree(slots[i].tensor.getMemory());
   void* arenas[] = {values, ders, state, batchMoments, runningMoments, chunkParam, rates, packedArena, packedJobs,
-                    partialArena, sumJobsDevice};
+                    partialArena, sumJobsDevice, clipWorkspace};
   for (void* a : arenas)
     if (a) (void)hipFree(a);
 }

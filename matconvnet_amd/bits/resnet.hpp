@@ -68,6 +68,9 @@ class ResNet50 {
   // losses() returns that loss and the top-1 / top-5 error rates of the batch (it waits for the stream).
   ErrorCode lossDerivative(double derOutput = 1.0);
   ErrorCode losses(double* objective, double* top1Error, double* top5Error);
+  // maxNorm > 0: sgdStep() clips the derivatives of all parameters, taken together, to that norm (it is no part of the reference's solver);
+  // the norm they had is in buffer "gradientNorm" then.  0 (the default): never.
+  ErrorCode setClip(double maxNorm);
   // one update of all parameters from the derivatives backward() left (numWorkers = 1), and of the moving averages of
   // the moments from those forward() left
   ErrorCode sgdStep(double learningRate, double momentum, double weightDecay);
@@ -106,6 +109,9 @@ class ResNet50 {
   float *values, *ders, *state, *batchMoments, *runningMoments;
   unsigned short* chunkParam;   // device
   double* rates;                // device
+  double clip;
+  void* clipWorkspace;
+  std::size_t clipBytes;
   std::size_t chunks, momentsCount, parameterCount;
   bool deferred;
   void *partialArena, *sumJobsDevice;   // partial banks of the stem and the classifier; device table of all summing jobs

@@ -97,6 +97,7 @@ def lib():
         L.vlh_resnet50_init.argtypes = [C.c_void_p, C.c_ulonglong]
         L.vlh_resnet50_forward.argtypes = [C.c_void_p]
         L.vlh_resnet50_backward.argtypes = [C.c_void_p]
+        L.vlh_resnet50_set_clip.argtypes = [C.c_void_p, C.c_double]
         L.vlh_resnet50_sgd_step.argtypes = [C.c_void_p, C.c_double, C.c_double, C.c_double]
         L.vlh_resnet50_loss_derivative.argtypes = [C.c_void_p, C.c_double]
         L.vlh_resnet50_losses.argtypes = [C.c_void_p, C.POINTER(C.c_double)]
@@ -371,6 +372,10 @@ class ResNet50(_NamedBuffers):
 
     def backward(self):
         self._check(self.L.vlh_resnet50_backward(self.h))
+
+    def set_clip(self, max_norm):
+        """sgd_step clips the derivatives of all parameters together to this norm (0: never); buffer "gradientNorm" holds what it was."""
+        self._check(self.L.vlh_resnet50_set_clip(self.h, float(max_norm)))
 
     def sgd_step(self, learning_rate, momentum=0.9, weight_decay=1e-4):
         self._check(self.L.vlh_resnet50_sgd_step(self.h, learning_rate, momentum, weight_decay))
