@@ -612,8 +612,8 @@ MCN_API int mcn_hnorm_backward(mcn_stream_t stream, const mcn_hnorm_geom* g, con
    sequences + 1 ascending numbers, both or neither; NULL: sequences of N / sequences queries and M / sequences keys each).  Either part may be
    empty; starts outside of 0..N or 0..M are taken as the nearest of these.  causal != 0: the queries are the last positions of their
    sequence, query i of n sees key j of m where j <= i + m - n.  A query that sees no key has o = 0, logSums = -infinity and gives no
-   derivative; keys that a query does not see have no part in it, whatever they hold.  Rows of no sequence (before the first one's, behind
-   the last one's) are left as they were, or with clear != 0 set to zero.
+   derivative.  Keys that a query does not see have no part in it, whatever they hold (and queries none in the derivatives of keys they do not
+   see); where what it does see makes it not finite in one channel, others may be not finite as well.  Rows of no sequence (before the first one's, behind the last one's) are left as they were, or with clear != 0 set to zero.
    q, k, v, o and all derivatives are of dataType.  logSums is N x heads, a position's heads side by side.  scale 0: 1/sqrt(D).  D
    at most 128.
    backward: all that is asked for (derQ, derK, derV; NULL or of null data: not made) is fully overwritten for all positions of sequences; o and logSums

@@ -222,6 +222,51 @@ __device__ __forceinline__ uintx4 chunk_of(const char* row, int chunk, int D, bo
   return v;
 }
 
+// The sums of a row of D values times a weight onto a result's lane: the columns that the lane holds
+template <class V, int DW>
+__device__ __forceinline__ void add_row(floatx16 (&acc)[DW / 32], const char* row, float weight, int D, int lane) {
+#pragma unroll
+  for (int d = 0; d < DW / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int at = 32 * d + 2 * r + 4 * (lane >> 5);
+      if (at >= D) continue;   // (rows are whole pieces of 16 bytes)
+      if (sizeof(V) == 2) {
+        const uintx2 v = *(const uintx2*)(row + 2 * at);
+        acc[d][r] += weight * bits_float(v.x << 16);
+        acc[d][r + 1] += weight * bits_float(v.x & 0xffff0000u);
+        acc[d][r + 2] += weight * bits_float(v.y << 16);
+        acc[d][r + 3] += weight * bits_float(v.y & 0xffff0000u);
+      } else {
+        const uintx4 v = *(const uintx4*)(row + 4 * at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[d][r + e] += weight * bits_float(v[e]);
+      }
+      if (r % 8 == 4) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// All finite, in both lanes of a row (or key)
+template <int N>
+__device__ __forceinline__ bool all_finite(const floatx16 (&v)[N]) {
+  bool good = true;
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) good = good && finite(v[d][r]);
+  return both_good(good);
+}
+// The product of two rows in global memory, by a lane and its other half.  (From memory again, and two loads at a time: what the slow sums
+// behind a loop keep in registers the loop does not have.)
+template <class V, int DW>
+__device__ __forceinline__ float row_product(const char* a, const char* b, int D, int lane) {
+  float s = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < Tile<V, DW>::steps; ++k) s += Matrix<V>::dot(chunk_of<V>(a, 2 * k + (lane >> 5), D, true), chunk_of<V>(b, 2 * k + (lane >> 5), D, true));
+  return s + other_half(s);
+}
+template <class V>
+__device__ __forceinline__ float as_operand(float v) { return sizeof(V) == 2 ? bits_float((unsigned)round_bf16(v) << 16) : v; }
+
 // Four neighbouring values of a row out
 template <class V>
 __device__ __forceinline__ void store4(char* row, int d, int D, int vector, float a, float b, float c, float e) {
@@ -489,6 +534,7 @@ __global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_
   float most = -INFINITY, sum = 0.f;
   if (begin < end) bring_tile(lds, end - begin);
   int turn = 0;
+  bool edges = false, before = true;   // tiles that not all rows see have begun; whether the row was finite then
   for (int j0 = begin; j0 < end; j0 += KT) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     char* from = lds + turn * 2 * tileBytes;
@@ -498,6 +544,10 @@ __global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_
       if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
     const int j = j0 + share0;
+    if (p.causal && !edges && j + 32 * KB > std::min(all, end)) {
+      edges = true;
+      before = all_finite(o);
+    }
     if (j < std::min(some, end))
       forward_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, o, most, sum, j, std::min(limit, end),
                               j + 32 * KB > std::min(all, end), p.c, lane);
@@ -528,35 +578,23 @@ __global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f + room[(16 * d + r) * 64] * f1;
   }
-  // A key that a row does not see has p = 0, but 0 times an infinity or a NaN of its values is NaN: a row that is not finite is added up
-  // key by key, over those it sees.
+  // A key that a row does not see has p = 0, but 0 times an infinity or a NaN of its values is NaN: a row that the tiles which not all rows see
+  // have made not finite is added up key by key, over those it sees; the others keep what they have.
   if (p.causal) {
-    bool good = true;
-#pragma unroll
-    for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) good = good && finite(o[d][r]);
-    if (!both_good(good)) {
-#pragma unroll
-      for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-      const float shift = most == -INFINITY ? 0.f : most * p.c;
-      const char* at = p.q.data + position * p.q.position + column * p.q.head;
-#pragma unroll 1
-      for (int j = begin; j < std::min(limit, end); ++j) {
-        float s = 0.f;
-#pragma unroll 1
-        for (int d = 0; d < p.D; ++d) s += value_of((const V*)at + d) * value_of((const V*)(keys + (long long)j * p.k.position) + d);
-        float e = power2(s * p.c - shift);
-        if (sizeof(V) == 2) e = bits_float((unsigned)round_bf16(e) << 16);
+    const bool good = !before || all_finite(o);
+    if (__any(!good)) {
+      if (!good) {
 #pragma unroll
         for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int at2 = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-            if (at2 < p.D) o[d][r] += e * value_of((const V*)(values + (long long)j * p.v.position) + at2);
-          }
+          for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+      }
+      const float shift = most == -INFINITY ? 0.f : most * p.c;
+      const char* query = p.q.data + position * p.q.position + column * p.q.head;
+#pragma unroll 1
+      for (int j = begin; j < std::min(some, end); ++j) {
+        const float e = power2(row_product<V, DW>(query, keys + (long long)j * p.k.position, p.D, lane) * p.c - shift);
+        if (!good && j < limit) add_row<V, DW>(o, values + (long long)j * p.v.position, as_operand<V>(e), p.D, lane);
       }
     }
   }
@@ -747,6 +785,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
   if (end > 0) bring_tile(lds, end);
   int turn = 0;
+  bool edges = false, before = true;
   for (int j0 = 0; j0 < end; j0 += KT) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     char* from = lds + turn * 2 * tileBytes;
@@ -756,6 +795,10 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
     const int j = j0 + share0;
+    if (p.causal && !edges && j + 32 * KB > std::min(all, end)) {
+      edges = true;
+      before = all_finite(dq);
+    }
     if (j < std::min(some, end))
       dq_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, dO, dq, negL, negDelta, j, limit,
                          std::min(some, end), j + 32 * KB > std::min(all, end), p.c, lane);
@@ -779,37 +822,22 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
   }
   // (as in the forward pass: what is not finite is added up over the keys that a row sees)
   if (p.causal) {
-    bool good = true;
-#pragma unroll
-    for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) good = good && finite(dq[d][r]);
-    if (!both_good(good)) {
-#pragma unroll
-      for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
-      const char* at = p.q.data + position * p.q.position + column * p.q.head;
-      const char* dAt = p.dO.data + position * p.dO.position + column * p.dO.head;
-#pragma unroll 1
-      for (int j = 0; j < limit; ++j) {
-        const V* kj = (const V*)(keys + (long long)j * p.k.position);
-        const V* vj = (const V*)(values + (long long)j * p.v.position);
-        float s = negL, dp = negDelta;
-#pragma unroll 1
-        for (int d = 0; d < p.D; ++d) {
-          s += value_of((const V*)at + d) * value_of(kj + d);
-          dp += value_of((const V*)dAt + d) * value_of(vj + d);
-        }
-        float e = power2(s * p.c) * dp;
-        if (sizeof(V) == 2) e = bits_float((unsigned)round_bf16(e) << 16);
+    const bool good = !before || all_finite(dq);
+    if (__any(!good)) {
+      if (!good) {
 #pragma unroll
         for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int at2 = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-            if (at2 < p.D) dq[d][r] += e * value_of(kj + at2);
-          }
+          for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+      }
+      const char* query = p.q.data + position * p.q.position + column * p.q.head;
+      const char* der = p.dO.data + position * p.dO.position + column * p.dO.head;
+#pragma unroll 1
+      for (int j = 0; j < std::min(some, end); ++j) {
+        const char* key = keys + (long long)j * p.k.position;
+        const float e = power2((negL + row_product<V, DW>(query, key, p.D, lane)) * p.c) *
+                        (negDelta + row_product<V, DW>(der, values + (long long)j * p.v.position, p.D, lane));
+        if (!good && j < limit) add_row<V, DW>(dq, key, as_operand<V>(e), p.D, lane);
       }
     }
   }
@@ -951,6 +979,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
   if (tiles) bring_tile(lds);
   if (AHEAD == 3 && tiles > 1) bring_tile(lds + bufferBytes);
+  bool edges = false, before = true;
   int at0 = 0, i0 = last;   // where the tile that is due lies
   for (int t = 0; t < tiles; ++t) {
     // (three buffers: the tile behind this one may be on its way still, 2 pieces a wavefront of each tensor)
@@ -963,6 +992,10 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       if (t + AHEAD - 1 < tiles) bring_tile(at);
     };
     const int i = i0 + share0;
+    if (p.causal && !edges && i < all) {
+      edges = true;
+      before = all_finite(dk) && all_finite(dv);
+    }
     if (i + 32 > some && i < span.n)
       dkv_tile<V, DW>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, (const float*)(from + 2 * tileBytes) + share0,
                       (const float*)(from + 2 * tileBytes + statBytes) + share0, to, bring_next, k, v, dk, dv, i, span.n, firstOf, i < all || i + 32 > span.n, p.c,
@@ -997,46 +1030,28 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
   }
   // (rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN)
   if (p.causal) {
-    bool good = true;
-#pragma unroll
-    for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) good = good && finite(dk[d][r]) && finite(dv[d][r]);
-    if (!both_good(good)) {
-#pragma unroll
-      for (int d = 0; d < DW / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
-      const V* kj = (const V*)(p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head);
-      const V* vj = (const V*)(p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head);
-#pragma unroll 1
-      for (int t = 0; t < heads * span.n; ++t) {
-        const int g = t / span.n, i = t % span.n;
-        if (!live || i < firstOf) continue;
-        const V* qi = (const V*)(queries + (long long)i * p.q.position + (long long)g * p.q.head);
-        const V* di = (const V*)(ders + (long long)i * p.dO.position + (long long)g * p.dO.head);
-        float s = statL[(long long)g * p.N + i], dp = statD[(long long)g * p.N + i];
-#pragma unroll 1
-        for (int d = 0; d < p.D; ++d) {
-          s += value_of(qi + d) * value_of(kj + d);
-          dp += value_of(di + d) * value_of(vj + d);
-        }
-        float e = power2(s * p.c), f = e * dp;
-        if (sizeof(V) == 2) {
-          e = bits_float((unsigned)round_bf16(e) << 16);
-          f = bits_float((unsigned)round_bf16(f) << 16);
-        }
+    const bool good = !before || (all_finite(dk) && all_finite(dv));
+    if (__any(!good)) {
+      if (!good) {
 #pragma unroll
         for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int at = 32 * d + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-            if (at < p.D) {
-              dv[d][r] += e * value_of(di + at);
-              dk[d][r] += f * value_of(qi + at);
-            }
-          }
+          for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
       }
+      const char* keyRow = p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head;
+      const char* valueRow = p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head;
+#pragma unroll 1
+      for (int h = 0; h < heads; ++h)
+#pragma unroll 1
+        for (int i = std::max(0, some); i < span.n; ++i) {
+          const char* query = queries + (long long)i * p.q.position + h * p.q.head;
+          const char* der = ders + (long long)i * p.dO.position + h * p.dO.head;
+          const float e = power2((statL[(long long)h * p.N + i] + row_product<V, DW>(keyRow, query, p.D, lane)) * p.c);
+          const float f = e * (statD[(long long)h * p.N + i] + row_product<V, DW>(valueRow, der, p.D, lane));
+          if (good || i < firstOf) continue;
+          add_row<V, DW>(dv, der, as_operand<V>(e), p.D, lane);
+          add_row<V, DW>(dk, query, as_operand<V>(f), p.D, lane);
+        }
     }
   }
   if (!live) return;
@@ -1169,6 +1184,7 @@ int check_geom(const char* who, const mcn_attention_geom* g) {
   if (g->D < 0 || g->heads < 0 || g->keyHeads < 0 || g->N < 0 || g->M < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative extent", who);
   if (g->D > kMostD) return fail(MCN_UNSUPPORTED, "%s: heads of more than %d channels", who, kMostD);
   if (g->sequences < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative number of sequences", who);
+  if (g->sequences > 1 << 28) return fail(MCN_UNSUPPORTED, "%s: too many sequences", who);
   if (g->heads && (g->keyHeads == 0 || g->heads % g->keyHeads)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %d heads over %d key heads", who, g->heads, g->keyHeads);
   if (!(g->scale >= 0) || std::isinf(g->scale)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the scale is negative or no number", who);
   // (rows of heads, and 256 positions behind the last one, are counted in 31 bits)
@@ -1318,19 +1334,19 @@ void common(AttentionP* p, const mcn_attention_geom* g, const Plan& l, const int
 }
 
 // tiles of all sequences, of `size` rows or keys
-int tiles_of(AttentionP* p, int rowsEach, int size, long long rows) {
-  if (p->qStarts) return (int)(rows / size) + p->sequences;
+long long tiles_of(AttentionP* p, int rowsEach, int size, long long rows) {
+  if (p->qStarts) return rows / size + p->sequences;
   const int each = std::max(1, div_up(rowsEach, size));
   p->byTiles = FastDiv(each);
   p->bySequences = FastDiv(p->sequences);
-  return each * p->sequences;
+  return (long long)each * p->sequences;
 }
 
 template <class V, int DW>
 int forward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   constexpr int KT = sizeof(V) == 2 ? 64 : 32;
   const long long rows = (long long)p.N * p.G;
-  const long long blocks = (long long)tiles_of(&p, p.each * p.G, 32 * l.blocks, rows) * p.keyHeads * p.slices;
+  const long long blocks = tiles_of(&p, p.each * p.G, 32 * l.blocks, rows) * p.keyHeads * p.slices;
   if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
   const dim3 grid((unsigned)blocks);
   {
@@ -1352,7 +1368,7 @@ int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   if (p.N) {
     const long long rows = (long long)p.N * p.G;
     const bool two = l.dqBlocks == 2;
-    const long long blocks = (long long)tiles_of(&p, p.each * p.G, two ? 64 : 128, rows) * p.keyHeads;
+    const long long blocks = tiles_of(&p, p.each * p.G, two ? 64 : 128, rows) * p.keyHeads;
     if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
     KernelTimer timer("attention_dq", s);
     if (two) hipLaunchKernelGGL((attention_dq<V, DW, 2, 2, 64>), dim3((unsigned)blocks), dim3(256), 0, s, p);
@@ -1363,7 +1379,7 @@ int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   if (!p.M || (!p.dk.data && !p.dv.data)) return MCN_SUCCESS;
   const bool two = l.dkvBlocks == 2;
   constexpr int AHEADX = 2;
-  const long long blocks = (long long)tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads * p.groupParts;
+  const long long blocks = tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads * p.groupParts;
   if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
   {
     KernelTimer timer("attention_dkv", s);

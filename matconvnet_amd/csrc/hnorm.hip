@@ -496,6 +496,7 @@ int check_geom(const char* who, const mcn_hnorm_geom* g) {
   if (g->D < 0 || g->heads < 0 || g->keyHeads < 0 || g->N < 0 || g->pairs < 0 || g->axes < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative extent", who);
   if (g->D > kMostD) return fail(MCN_UNSUPPORTED, "%s: heads of more than %d channels", who, kMostD);
   if (g->heads > 65536 || g->keyHeads > 65536) return fail(MCN_UNSUPPORTED, "%s: more than 65536 heads", who);
+  if (g->N > 1 << 30) return fail(MCN_UNSUPPORTED, "%s: too many positions", who);
   if (2ll * g->pairs > g->D) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %d pairs of %d channels", who, g->pairs, g->D);
   if (g->pairs && g->axes == 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: pairs, but no axes", who);
   if (g->axes > 64) return fail(MCN_UNSUPPORTED, "%s: more than 64 axes", who);

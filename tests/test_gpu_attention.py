@@ -423,3 +423,20 @@ def test_a_cache_behind_the_32nd_bit(capi):
     w = Want(q[:1, 1:2], k[:M - 700, 1:2].contiguous(), v[:M - 700, 1:2].contiguous(), q[:1, 1:2], [(1, M - 700)], False)
     near(y[:1, 1:2], w.o, w.o_off, "o")
     near(sums[:1, 1:2], w.sums, w.sums_off, "log sums")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_all_see_is_not_mended(capi, dtype):
+    """A value that is not finite in the first key reaches every row, beside one in the last key that reaches the last row alone"""
+    n = 200
+    q, k, v, dy = make(n, n, 2, 1, 128, dtype, 9)
+    v[0, :, 7], v[n - 1, :, 9] = math.nan, math.inf
+    y, sums = capi.attention_forward(q, k, v, causal=True)
+    assert bool(torch.isnan(y[:, :, 7]).all()) and bool(torch.isfinite(sums).all())
+    keep = torch.ones(128, dtype=torch.bool, device="cuda")
+    keep[7] = keep[9] = False
+    v2 = v.clone()
+    v2[0, :, 7], v2[n - 1, :, 9] = 0.0, 0.0
+    w = Want(q, k, v2, dy, [(n, n)], True)
+    near(y[:, :, keep], w.o[:, :, keep], w.o_off[:, :, keep], "o")
+    assert not bool(torch.isfinite(y[n - 1, :, 9]).any())
