@@ -882,20 +882,20 @@ def orthogonalise(x, steps=5, ws=None):
     return y
 
 
-def _heads(name, t, D=None):
-    """mcn_heads of a tensor (positions, heads, D) on the current device whose channels are neighbours; None stays none."""
-    if t is None:
-        return None
-    if t.dim() != 3 or (D is not None and t.shape[2] != D):
-        raise ValueError("%s is not a tensor (positions, heads, D) of the others' D" % name)
-    if not t.is_cuda:
-        raise ValueError("%s is not on the device" % name)
-    if t.get_device() != _torch().cuda.current_device():
-        raise ValueError("%s is on device %d, not on the current one" % (name, t.get_device()))
-    position, head, channel = t.stride()
-    if channel != 1 and t.shape[2] > 1:
-        raise ValueError("the channels of %s are not neighbours" % name)
-    return C.byref(Heads(t.data_ptr(), position, head))
+def _heads(names, *tensors):
+    """mcn_heads of tensors (positions, heads, D) on the current device whose channels are neighbours; None stays none."""
+    here, out = _torch().cuda.current_device(), []
+    for i, t in enumerate(tensors):
+        if t is None:
+            out.append(None)
+            continue
+        if t.get_device() != here:     # (-1: not on a device)
+            raise ValueError("%s is on device %d, not on the current one" % (names.split()[i], t.get_device()))
+        position, head, channel = t.stride()
+        if channel != 1 and t.shape[2] > 1:
+            raise ValueError("the channels of %s are not neighbours" % names.split()[i])
+        out.append(C.byref(Heads(t.data_ptr(), position, head)))
+    return out
 
 
 def _alike(x):
@@ -937,6 +937,9 @@ def _hnorm_geom(q, k, gq, gk, positions, frequencies, epsilon, normalise, neighb
         if g is not None and g.numel() != D:
             raise ValueError("%s does not have one value per channel" % name)
     pairs = axes = 0
+    for name, t in (("q", q), ("k", k)):
+        if t is not None and not t.is_cuda:
+            raise ValueError("%s is not on the device" % name)
     if (positions is None) != (frequencies is None):
         raise ValueError("positions and frequencies are taken together")
     if positions is not None:
@@ -970,8 +973,7 @@ def hnorm_forward(q, k, gq=None, gk=None, positions=None, frequencies=None, epsi
     write, which may be q and k."""
     g = _hnorm_geom(q, k, gq, gk, positions, frequencies, epsilon, normalise, neighbours)
     yq, yk = _outs("yq yk", out, q, k)
-    check(lib().mcn_hnorm_forward(stream(), C.byref(g), _heads("yq", yq), _heads("yk", yk), _heads("q", q, g.D), _heads("k", k, g.D), ptr(gq), ptr(gk),
-                                  ptr(positions), ptr(frequencies)))
+    check(lib().mcn_hnorm_forward(stream(), C.byref(g), *_heads("yq yk q k", yq, yk, q, k), ptr(gq), ptr(gk), ptr(positions), ptr(frequencies)))
     return yq, yk
 
 
@@ -991,16 +993,17 @@ def hnorm_backward(q, k, gq, gk, positions, frequencies, dyq, dyk, epsilon=1e-6,
     dgq, dgk = [_singles(x, g.D) if w and normalise and x is not None else None for w, x in zip(want[2:], (q, k))]
     x = q if q is not None else k
     wp, wn, held = _scratch(ws, x, lib().mcn_hnorm_workspace_bytes(C.byref(g)) if dgq is not None or dgk is not None else 0)
-    check(lib().mcn_hnorm_backward(stream(), C.byref(g), _heads("dq", dq), _heads("dk", dk), ptr(dgq), ptr(dgk), _heads("q", q, g.D), _heads("k", k, g.D),
-                                   ptr(gq), ptr(gk), ptr(positions), ptr(frequencies), _heads("dyq", dyq), _heads("dyk", dyk), wp, wn))
+    hdq, hdk, hq, hk, hdyq, hdyk = _heads("dq dk q k dyq dyk", dq, dk, q, k, dyq, dyk)
+    check(lib().mcn_hnorm_backward(stream(), C.byref(g), hdq, hdk, ptr(dgq), ptr(dgk), hq, hk, ptr(gq), ptr(gk), ptr(positions), ptr(frequencies), hdyq, hdyk,
+                                   wp, wn))
     return dq, dk, dgq, dgk
 
 
 def _attention_geom(q, k, v, sequences, q_starts, k_starts, causal, scale):
     torch = _torch()
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise ValueError("%s is not a tensor (positions, heads, D)" % name)
+        if t.dim() != 3 or not t.is_cuda:
+            raise ValueError("%s is not a tensor (positions, heads, D) on the device" % name)
     if k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError("keys and values do not have the same shape, or not the queries' D")
     if (q_starts is None) != (k_starts is None):
@@ -1038,8 +1041,8 @@ def attention_forward(q, k, v, q_starts=None, k_starts=None, sequences=None, cau
     y = _alike(q) if out is None else out
     log_sums = _singles(q, g.N, g.heads)
     wp, wn, held = _scratch(ws, q, lib().mcn_attention_workspace_bytes(C.byref(g), 0))
-    check(lib().mcn_attention_forward(stream(), C.byref(g), _heads("out", y), ptr(log_sums), _heads("q", q), _heads("k", k), _heads("v", v),
-                                      ptr(q_starts), ptr(k_starts), wp, wn))
+    hy, hq, hk, hv = _heads("out q k v", y, q, k, v)
+    check(lib().mcn_attention_forward(stream(), C.byref(g), hy, ptr(log_sums), hq, hk, hv, ptr(q_starts), ptr(k_starts), wp, wn))
     return y, log_sums
 
 
@@ -1058,8 +1061,8 @@ def attention_backward(q, k, v, y, log_sums, dy, q_starts=None, k_starts=None, s
     d = [t if w else None for w, t in zip(want, _outs("dq dk dv", out, q, k, v))] if out is not None else [
         _alike(x) if w else None for w, x in zip(want, (q, k, v))]
     wp, wn, held = _scratch(ws, q, lib().mcn_attention_workspace_bytes(C.byref(g), 1))
-    check(lib().mcn_attention_backward(stream(), C.byref(g), _heads("dq", d[0]), _heads("dk", d[1]), _heads("dv", d[2]), _heads("y", y), ptr(log_sums),
-                                       _heads("q", q), _heads("k", k), _heads("v", v), _heads("dy", dy), ptr(q_starts), ptr(k_starts), wp, wn))
+    hdq, hdk, hdv, hy, hq, hk, hv, hdy = _heads("dq dk dv y q k v dy", d[0], d[1], d[2], y, q, k, v, dy)
+    check(lib().mcn_attention_backward(stream(), C.byref(g), hdq, hdk, hdv, hy, ptr(log_sums), hq, hk, hv, hdy, ptr(q_starts), ptr(k_starts), wp, wn))
     return tuple(d)
 
 

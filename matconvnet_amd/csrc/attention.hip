@@ -1243,7 +1243,7 @@ Plan plan_of(const mcn_attention_geom* g, int backward) {
   if (backward) {
     const long long cus = std::max(1, device_compute_units());
     l.dqBlocks = split("attention_dq_split", (rows / 128 + sequences) * g->keyHeads < 2 * cus) ? 2 : 4;
-    l.dkvBlocks = split("attention_dkv_split", (g->M / 128 + sequences) * (long long)g->keyHeads < (g->N < 512ll * sequences ? 2 : l.DW == 64 ? 6 : 4) * cus) ? 2 : 4;
+    l.dkvBlocks = split("attention_dkv_split", (g->M / 128 + sequences) * (long long)g->keyHeads < (g->N < 512ll * sequences ? 2 : 4) * cus) ? 2 : 4;
     // The heads of a group in several workgroups, where there are not two rounds of them otherwise (GROUP_PARTS)
     const long long groups = std::max(1ll, ((long long)g->M / (32 * l.dkvBlocks) + sequences) * g->keyHeads), want = (l.size == 2 ? 4 : 2) * cus;
     const int forced = tunable("attention_group_parts", 0);
