@@ -618,8 +618,9 @@ MCN_API int mcn_hnorm_backward(mcn_stream_t stream, const mcn_hnorm_geom* g, con
    at most 128.
    backward: all that is asked for (derQ, derK, derV; NULL or of null data: not made) is fully overwritten for all positions of sequences; o and logSums
    as the forward call left them.  Derivatives of heads that share keys are sums without atomics: the same bits every time.
-   bfloat16: products of the bfloat16 values in single precision; exp(s - logSums) and the scores' derivatives are rounded to bfloat16
-   for the products behind them.  Single precision: products and sums in single precision.
+   bfloat16: products of the bfloat16 values in single precision; exp(s - logSums) and, for derK, the scores' derivatives are rounded to
+   bfloat16 for the products behind them; for derQ the latter are taken as two bfloat16 values.  o enters the derivatives as it is stored;
+   what its rounding puts the scores' derivatives of a row off by is taken out again for derK.  Single precision: products and sums in single precision.
    workspace: mcn_attention_workspace_bytes(g, 0 forward / 1 backward). */
 typedef struct mcn_attention_geom {
   int D, heads, keyHeads;

@@ -43,17 +43,16 @@ typedef __bf16 bfx2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
   return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2){a, b}, bfx2));
 }
-__device__ __forceinline__ float value_of(const float* p) { return *p; }
-__device__ __forceinline__ float value_of(const bf16* p) { return bits_float((unsigned)*p << 16); }
 __device__ __forceinline__ float power2(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ bool finite(float v) { return (float_bits(v) & 0x7f800000u) != 0x7f800000u; }
 
 // the other half's value of the 64 lanes (lane ^ 32)
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, kWave); }
-// whether both lanes of a row (or key) find it good
+// whether both lanes of a row (or key) find it good.  (As numbers: where each lane took its bit out of a ballot's words, whole halves of wavefronts
+// of the dq kernel came out bad now and then, all of their values being finite; the slow sums behind the loop hid that but for their time.)
 __device__ __forceinline__ bool both_good(bool good) {
-  const unsigned long long m = __ballot(good);
-  return (m & m >> 32) >> (threadIdx.x & 31) & 1;
+  const float bad = good ? 0.f : 1.f;
+  return bad + other_half(bad) == 0.f;
 }
 
 struct Tensor3 {            // heads where they lie, strides in bytes
@@ -65,7 +64,7 @@ struct AttentionP {
   Tensor3 q, k, v, o, dO, dq, dk, dv;
   float *logSums, *parts, *partSums;     // parts: a slice's o (normalised) and log sums; backward, of groupParts: [M][keyHeads][2][DW] of dk and dv
   int groupParts, headsOfPart;           // dk, dv: the group's heads in so many workgroups
-  float *statL, *statD;                  // backward, [heads][N]: -L/scale, -delta
+  float *statL, *statD;                  // backward, [heads][N]: -L (negative_sum), -delta
   const int *qStarts, *kStarts;
   int sequences, each, eachKeys;         // without starts: queries and keys of a sequence
   int D, G, heads, keyHeads, N, M, causal;
@@ -381,7 +380,7 @@ __device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
 
 // ------------------------------------------------------------------------------------------ forward
 
-constexpr int kAhead = 2;   // tiles in LDS at a time
+constexpr int kAhead = 2;   // tiles in LDS at a time: the one that is walked, the one that comes
 
 // KB blocks of 32 keys of a tile: fragments of 32 queries (q) against them.  `next` is filled meanwhile.  (A function of its own with `restrict` pointers:
 // that the loads fill none of what is read is what lets the reads go without waiting for them.)
@@ -662,10 +661,21 @@ __global__ __launch_bounds__(256) void attention_join(AttentionP p) {
 
 // ------------------------------------------------------------------------------------------ dq, and delta for dk and dv
 
+// p = exp(scale q.k - L).  bfloat16: the sum of products starts at -L/scale, which saves an addition; in single precision that would round every
+// partial sum to the places that L/scale leaves, so there it starts at 0 (dq of heads of 75 channels: off by 5e-7 instead of 1.1e-6).
+template <class V>
+__device__ constexpr bool starts_at_sum() { return sizeof(V) == 2; }
+template <class V>
+__device__ __forceinline__ float negative_sum(float logSum, float scale) {   // (a row that sees nothing: what it gives is masked)
+  return logSum == -INFINITY ? 0.f : starts_at_sum<V>() ? -logSum / scale : -logSum * kLog2e;
+}
+template <class V>
+__device__ __forceinline__ float probability(float s, float negL, float c) { return starts_at_sum<V>() ? power2(s * c) : power2(s * c + negL); }
+
 template <class V, int DW, int KB, class Bring>
 __device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const char* __restrict__ values, char* __restrict__ next, Bring bring_next,
-                                        const uintx4 (&q)[Tile<V, DW>::steps], const uintx4 (&dO)[Tile<V, DW>::steps], floatx16 (&dq)[DW / 32], float negL,
-                                        float negDelta, int j0, int limit, int last, bool edge, float c, int lane) {
+                                        const uintx4 (&q)[Tile<V, DW>::steps], const uintx4 (&dO)[Tile<V, DW>::steps], floatx16 (&dq)[DW / 32], float& rest,
+                                        float negL, float negDelta, int j0, int limit, int last, bool edge, float c, int lane) {
   typedef Tile<V, DW> T;
   bring_next(next);
   lane = fresh<V, DW>(lane);
@@ -674,20 +684,33 @@ __device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const cha
     if (b && j0 + 32 * b >= last) break;
     floatx16 s, dp;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = negL;
+    for (int r = 0; r < 16; ++r) s[r] = starts_at_sum<V>() ? negL : 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = negDelta;
-    uintx4 operand[sizeof(V) == 4 ? 4 : 2];
+    uintx4 operand[sizeof(V) == 4 ? 4 : 2], low[2];
     const auto scores = [&]() __attribute__((always_inline)) {
       float e[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c) * dp[r];
+      for (int r = 0; r < 16; ++r) e[r] = probability<V>(s[r], negL, c) * dp[r];
       if (edge) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (j0 + 32 * b + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 >= limit) e[r] = 0.f;
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rest += e[r];
       T::operand(operand, e);
+      // ds as two bfloat16 values: its sums over the keys are small beside its terms (they add up to zero against equal keys), and what one rounding
+      // of each leaves is as large as the result's own
+      if (sizeof(V) == 2) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const unsigned high = operand[r / 8 & 1][r % 8 / 2];
+          e[r] -= bits_float(high << 16);
+          e[r + 1] -= bits_float(high & 0xffff0000u);
+          low[r / 8 & 1][r % 8 / 2] = pack_bf16(e[r], e[r + 1]);
+        }
+      }
     };
     if constexpr (sizeof(V) == 2) {
       constexpr int S = T::steps, P = DW / 32 * 2;
@@ -703,6 +726,7 @@ __device__ __forceinline__ void dq_tile(const char* __restrict__ keys, const cha
             else {
               if (i == 2 * S) scores();
               dq[(i - 2 * S) / 2] = Matrix<V>::along(a, operand[i % 2], dq[(i - 2 * S) / 2]);
+              dq[(i - 2 * S) / 2] = Matrix<V>::along(a, low[i % 2], dq[(i - 2 * S) / 2]);
             }
           });
     } else {
@@ -754,17 +778,12 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     for (int s = 0; s < T::steps; ++s) q[s] = chunk_of<V>(at, 2 * s + (lane >> 5), p.D, live);
   }
   negDelta += other_half(negDelta);
-  float negL = 0.f;
-  if (live) {
-    negL = p.logSums[position * p.heads + column];
-    negL = negL == -INFINITY ? 0.f : -negL / p.scale;
-    if (lane < 32 && !share0) {
-      const long long at = (long long)column * p.N + position;
-      p.statL[at] = negL;
-      p.statD[at] = negDelta;
-    }
+  const float negL = live ? negative_sum<V>(p.logSums[position * p.heads + column], p.scale) : 0.f;
+  float rest = 0.f;
+  if (!p.dq.data && !p.dk.data) {   // (dv needs the log sums alone)
+    if (live && lane < 32 && !share0) p.statL[(long long)column * p.N + position] = negL;
+    return;
   }
-  if (!p.dq.data) return;
   const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
   const char* values = p.v.data + (long long)span.k0 * p.v.position + head * p.v.head;
   Loader<V, DW, KT, NW> loadK, loadV;
@@ -800,18 +819,21 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       before = all_finite(dq);
     }
     if (j < std::min(some, end))
-      dq_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, dO, dq, negL, negDelta, j, limit,
-                         std::min(some, end), j + 32 * KB > std::min(all, end), p.c, lane);
+      dq_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, dO, dq, rest, negL, negDelta, j,
+                         limit, std::min(some, end), j + 32 * KB > std::min(all, end), p.c, lane);
     else bring_next(to);
   }
   if (NS == 2) {
-    float* room = (float*)lds + block * DW / 32 * 16 * 64 + lane;
+    constexpr int values = DW / 32 * 16 + 1;
+    static_assert(NS == 1 || NB * values * 256 <= (int)sizeof(lds), "room");
+    float* room = (float*)lds + block * values * 64 + lane;
     __syncthreads();
     if (share0) {
 #pragma unroll
       for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) room[(16 * d + r) * 64] = dq[d][r];
+      room[(values - 1) * 64] = rest;
     }
     __syncthreads();
     if (share0) return;
@@ -819,7 +841,16 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[d][r] += room[(16 * d + r) * 64];
+    rest += room[(values - 1) * 64];
   }
+  // delta is the sum of p (do.v) over the keys, o in do.o is rounded: what ds adds up to, instead of zero, is what delta was off by
+  rest += other_half(rest);
+  if (live && lane < 32) {
+    const long long at = (long long)column * p.N + position;
+    p.statL[at] = negL;
+    p.statD[at] = negDelta - rest;
+  }
+  if (!p.dq.data) return;
   // (as in the forward pass: what is not finite is added up over the keys that a row sees)
   if (p.causal) {
     const bool good = !before || all_finite(dq);
@@ -835,7 +866,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
 #pragma unroll 1
       for (int j = 0; j < std::min(some, end); ++j) {
         const char* key = keys + (long long)j * p.k.position;
-        const float e = power2((negL + row_product<V, DW>(query, key, p.D, lane)) * p.c) *
+        const float e = probability<V>((starts_at_sum<V>() ? negL : 0.f) + row_product<V, DW>(query, key, p.D, lane), negL, p.c) *
                         (negDelta + row_product<V, DW>(der, values + (long long)j * p.v.position, p.D, lane));
         if (!good && j < limit) add_row<V, DW>(dq, key, as_operand<V>(e), p.D, lane);
       }
@@ -872,6 +903,12 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
       v[r] = l.x; v[r + 1] = l.y; v[r + 2] = l.z; v[r + 3] = l.w;
     }
   };
+  start(s, statL);
+  const floatx16 sums = s;   // (used in single precision)
+  if (!starts_at_sum<V>()) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+  }
   const auto masked = [&]() __attribute__((always_inline)) {   // (firstOf: the first position that sees this lane's key)
     if (!edge) return;
     const int here = i0 + 4 * (lane >> 5), low = firstOf - here, high = n - here;
@@ -881,7 +918,7 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
   };
   const auto probabilities = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) e[r] = power2(s[r] * c);
+    for (int r = 0; r < 16; ++r) e[r] = probability<V>(s[r], sums[r], c);
     masked();
     T::operand(operand, e);
   };
@@ -891,7 +928,6 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
     masked();
     T::operand(operand, e);
   };
-  start(s, statL);
 #pragma unroll
   for (int t = 0; t < T::steps; ++t) s = Matrix<V>::along(T::along(queries, 0, t, lane), k[t], s);
   probabilities();
@@ -907,13 +943,13 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
 
 // NB blocks of 32 keys; they walk over the positions of one head of the group after the other.  NS wavefronts share a block, each takes its 32
 // positions of every tile, and their sums are added up through LDS.
-template <class V, int DW, int NB, int NS, int AHEAD>
+template <class V, int DW, int NB, int NS>
 __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attention_dkv(AttentionP p) {
   typedef Tile<V, DW> T;
   constexpr int NW = NB * NS, RT = 32 * NS;
   constexpr int tileBytes = RT * T::rowBytes, statBytes = RT * 4, bufferBytes = 2 * tileBytes + 2 * statBytes;
   static_assert(RT <= 64, "one load brings the statistics of a tile");
-  __shared__ __attribute__((aligned(16))) char lds[AHEAD * bufferBytes];
+  __shared__ __attribute__((aligned(16))) char lds[kAhead * bufferBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = wave % NB, share0 = wave / NB * 32;
   int id = blockIdx.x;
   const int head = id % p.keyHeads;
@@ -978,18 +1014,15 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
   if (tiles) bring_tile(lds);
-  if (AHEAD == 3 && tiles > 1) bring_tile(lds + bufferBytes);
   bool edges = false, before = true;
-  int at0 = 0, i0 = last;   // where the tile that is due lies
+  int turn = 0, i0 = last;   // the tile that is due: its buffer, its first position
   for (int t = 0; t < tiles; ++t) {
-    // (three buffers: the tile behind this one may be on its way still, 2 pieces a wavefront of each tensor)
-    if (AHEAD == 3 && t + 1 < tiles) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * Loader<V, DW, RT, NW>::pieces) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    char* from = lds + at0;
-    char* to = lds + (at0 == 0 ? (AHEAD - 1) * bufferBytes : at0 - bufferBytes);   // the one of the tile before
-    at0 = at0 == (AHEAD - 1) * bufferBytes ? 0 : at0 + bufferBytes;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    char* from = lds + turn * bufferBytes;
+    char* to = lds + (turn ^ 1) * bufferBytes;
+    turn ^= 1;
     const auto bring_next = [&](char* at) __attribute__((always_inline)) {
-      if (t + AHEAD - 1 < tiles) bring_tile(at);
+      if (t + 1 < tiles) bring_tile(at);
     };
     const int i = i0 + share0;
     if (p.causal && !edges && i < all) {
@@ -1046,7 +1079,8 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
         for (int i = std::max(0, some); i < span.n; ++i) {
           const char* query = queries + (long long)i * p.q.position + h * p.q.head;
           const char* der = ders + (long long)i * p.dO.position + h * p.dO.head;
-          const float e = power2((statL[(long long)h * p.N + i] + row_product<V, DW>(keyRow, query, p.D, lane)) * p.c);
+          const float negL = statL[(long long)h * p.N + i];
+          const float e = probability<V>((starts_at_sum<V>() ? negL : 0.f) + row_product<V, DW>(keyRow, query, p.D, lane), negL, p.c);
           const float f = e * (statD[(long long)h * p.N + i] + row_product<V, DW>(valueRow, der, p.D, lane));
           if (good || i < firstOf) continue;
           add_row<V, DW>(dv, der, as_operand<V>(e), p.D, lane);
@@ -1378,13 +1412,12 @@ int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   }
   if (!p.M || (!p.dk.data && !p.dv.data)) return MCN_SUCCESS;
   const bool two = l.dkvBlocks == 2;
-  constexpr int AHEADX = 2;
   const long long blocks = tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads * p.groupParts;
   if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
   {
     KernelTimer timer("attention_dkv", s);
-    if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((attention_dkv<V, DW, 4, 1, AHEADX>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((attention_dkv<V, DW, 4, 1>), dim3((unsigned)blocks), dim3(256), 0, s, p);
   }
   int rc = check_launch(who);
   if (rc || p.groupParts == 1) return rc;
