@@ -1247,16 +1247,21 @@ struct Plan {
 };
 
 // Whether two wavefronts share a block of 32 rows or keys.  They make twice as many workgroups of half the length, which bring twice as many
-// tiles.  Rows: where the chip is not filled otherwise (one sequence of 4096, 4 heads of 128 over one, bfloat16: forward 53.8 -> 46.3 us, dq
-// 122 -> 74; 196 positions x 32 x 12 heads of 64, 768 workgroups: 18.8 -> 20.8 and 24.3 -> 29.5).  Keys: everywhere but in short sequences, whose
-// last tiles hold more that is not there (packed sequences of up to 1100, 32 heads over 8: 279 -> 251; 196 positions: 39.0 -> 42.9).
+// tiles.  Rows: where the chip is not filled otherwise (causal, bfloat16, four wavefronts alone -> two to a block.  One sequence of 4096, 4
+// heads of 128 over one: forward 50.6 -> 45.4 us, dq 114 -> 74; 4 of 512, 16 heads of 128: 19.3 -> 17.3 forward; 4 of 2048, 16 heads of 128: 90
+// -> 113, 138 -> 159; 196 positions x 32 x 12 heads of 64: 18.0 -> 19.5, 24.3 -> 31.2).  Keys, whole backward: 4 of 2048 as above 302 -> 345,
+// the one sequence 285 -> 238, 13 packed ones of up to 1100, 32 heads over 8, 354 -> 339, and the 196 positions, whose last tiles hold more that
+// is not there, 47 -> 57; the rule loses on 4096, 32 heads over 8, 552 -> 590.
 bool split(const char* name, bool rule) {
   const int forced = tunable(name, 0);
   return forced ? forced == 2 : rule;
 }
 
-// How a forward call is cut.  Rows of a sequence on average up to 32: one wavefront a workgroup, and keys are cut into slices until there
-// are workgroups for the whole chip; otherwise four wavefronts.
+// How a forward call is cut.  Rows of a sequence on average up to 32: one wavefront a workgroup, and keys are cut into slices until four of
+// those are there for every compute unit; otherwise four wavefronts, and slices until there are two workgroups for each.  A slice has four
+// tiles at least, eight where a tile takes the least time: the partial results are written, read and put together by a launch (bfloat16, heads of 128,
+// causal, slices of two workgroups a compute unit against one slice: one sequence of 8192 of 2 heads 80 and 117 us, of 2048 of 32 heads over 8
+// the same 54; with four workgroups a compute unit 73 and 76, and 4 of 512 of 32 heads over 8 56 instead of 23).
 Plan plan_of(const mcn_attention_geom* g, int backward) {
   Plan l = {};
   l.size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
@@ -1266,10 +1271,10 @@ Plan plan_of(const mcn_attention_geom* g, int backward) {
   const long long rows = (long long)g->N * l.G;
   l.slices = 1;
   if (!backward) {
-    l.blocks = rows <= 32ll * sequences ? 1 : split("attention_forward_split", (rows / 128 + sequences) * g->keyHeads * 4 < 5ll * device_compute_units()) ? 2 : 4;
-    const long long groups = (long long)div_up(rows, 32 * l.blocks) * g->keyHeads, want = 4ll * std::max(1, device_compute_units());
+    l.blocks = rows <= 32ll * sequences ? 1 : split("attention_forward_split", (rows / 128 + sequences) * g->keyHeads < 2ll * device_compute_units()) ? 2 : 4;
+    const long long groups = (long long)div_up(rows, 32 * l.blocks) * g->keyHeads, want = (l.blocks == 1 ? 4ll : 2ll) * std::max(1, device_compute_units());
     const int tile = l.size == 2 ? 64 : 32;
-    const long long most = std::max<long long>(1, g->M / sequences / (4 * tile));
+    const long long most = std::max<long long>(1, g->M / sequences / ((l.blocks == 1 || l.size == 4 ? 4 : 8) * tile));
     l.slices = (int)std::max<long long>(1, std::min<long long>({64, most, want / std::max<long long>(1, groups)}));
   }
   l.groupParts = 1;
@@ -1278,7 +1283,9 @@ Plan plan_of(const mcn_attention_geom* g, int backward) {
     const long long cus = std::max(1, device_compute_units());
     l.dqBlocks = split("attention_dq_split", (rows / 128 + sequences) * g->keyHeads < 2 * cus) ? 2 : 4;
     l.dkvBlocks = split("attention_dkv_split", (g->M / 128 + sequences) * (long long)g->keyHeads < (g->N < 512ll * sequences ? 2 : 4) * cus) ? 2 : 4;
-    // The heads of a group in several workgroups, where there are not two rounds of them otherwise (GROUP_PARTS)
+    // The heads of a group in several workgroups, whose sums are put together by one more launch, where there are not four workgroups a compute
+    // unit otherwise, two in single precision (whole backward of one sequence of 4096, causal, bfloat16, heads of 128: 4 over one 581 -> 239 us in
+    // four parts, 32 over 8 762 -> 590 in two; 13 packed sequences of 32 over 8, whose workgroups are enough, 339 -> 405 in two)
     const long long groups = std::max(1ll, ((long long)g->M / (32 * l.dkvBlocks) + sequences) * g->keyHeads), want = (l.size == 2 ? 4 : 2) * cus;
     const int forced = tunable("attention_group_parts", 0);
     const int parts = forced ? std::min(forced, l.G) : (int)std::max<long long>(1, std::min<long long>(l.G, (want + groups - 1) / groups));
