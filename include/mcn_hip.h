@@ -613,9 +613,10 @@ MCN_API int mcn_hnorm_backward(mcn_stream_t stream, const mcn_hnorm_geom* g, con
    empty; starts outside of 0..N or 0..M are taken as the nearest of these.  causal != 0: the queries are the last positions of their
    sequence, query i of n sees key j of m where j <= i + m - n.  A query that sees no key has o = 0, logSums = -infinity and gives no
    derivative.  Keys that a query does not see have no part in it, whatever they hold (and queries none in the derivatives of keys they do not
-   see); where what it does see makes it not finite in one channel, others may be not finite as well.  Rows of no sequence (before the first one's, behind the last one's) are left as they were, or with clear != 0 set to zero.
-   q, k, v, o and all derivatives are of dataType.  logSums is N x heads, a position's heads side by side.  scale 0: 1/sqrt(D).  D
-   at most 128.
+   see); where what it does see makes it not finite in one channel, others may be not finite as well.  Rows of no sequence (before the
+   first one's, behind the last one's) are left as they were, or with clear != 0 set to zero.
+   q, k, v, o and all derivatives are of dataType.  logSums is N x heads, a position's heads side by side.  scale 0: 1/sqrt(D),
+   otherwise 1e-30 to 1e30.  D at most 128.
    backward: all that is asked for (derQ, derK, derV; NULL or of null data: not made) is fully overwritten for all positions of sequences; o and logSums
    as the forward call left them.  Derivatives of heads that share keys are sums without atomics: the same bits every time.
    bfloat16: products of the bfloat16 values in single precision; exp(s - logSums) and, for derK, the scores' derivatives are rounded to

@@ -868,7 +868,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
         const char* key = keys + (long long)j * p.k.position;
         const float e = probability<V>((starts_at_sum<V>() ? negL : 0.f) + row_product<V, DW>(query, key, p.D, lane), negL, p.c) *
                         (negDelta + row_product<V, DW>(der, values + (long long)j * p.v.position, p.D, lane));
-        if (!good && j < limit) add_row<V, DW>(dq, key, as_operand<V>(e), p.D, lane);
+        if (!good && j < limit) add_row<V, DW>(dq, key, e, p.D, lane);
       }
     }
   }
@@ -1197,6 +1197,7 @@ __global__ __launch_bounds__(256) void attention_clear(ClearP p) {
 
 // ---------------------------------------------------------------------------------------------- host
 
+constexpr long long kMostThreads = 1ll << 32;   // of a launch
 constexpr size_t kAlign = 256;
 size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
@@ -1221,6 +1222,8 @@ int check_geom(const char* who, const mcn_attention_geom* g) {
   if (g->sequences > 1 << 28) return fail(MCN_UNSUPPORTED, "%s: too many sequences", who);
   if (g->heads && (g->keyHeads == 0 || g->heads % g->keyHeads)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %d heads over %d key heads", who, g->heads, g->keyHeads);
   if (!(g->scale >= 0) || std::isinf(g->scale)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the scale is negative or no number", who);
+  // (log sums are divided by it)
+  if (g->scale > 0 && (g->scale < 1e-30 || g->scale > 1e30)) return fail(MCN_UNSUPPORTED, "%s: a scale outside of 1e-30 to 1e30", who);
   // (rows of heads, and 256 positions behind the last one, are counted in 31 bits)
   if (((long long)g->N + 256) * g->heads >= (1ll << 31) || (long long)g->M + 256 >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many positions", who);
   return MCN_SUCCESS;
@@ -1388,7 +1391,7 @@ int forward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   constexpr int KT = sizeof(V) == 2 ? 64 : 32;
   const long long rows = (long long)p.N * p.G;
   const long long blocks = tiles_of(&p, p.each * p.G, 32 * l.blocks, rows) * p.keyHeads * p.slices;
-  if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+  if (blocks * (l.blocks == 1 ? 64 : 256) >= kMostThreads) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
   const dim3 grid((unsigned)blocks);
   {
     KernelTimer timer("attention_forward", s);
@@ -1410,7 +1413,7 @@ int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
     const long long rows = (long long)p.N * p.G;
     const bool two = l.dqBlocks == 2;
     const long long blocks = tiles_of(&p, p.each * p.G, two ? 64 : 128, rows) * p.keyHeads;
-    if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+    if (blocks * 256 >= kMostThreads) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
     KernelTimer timer("attention_dq", s);
     if (two) hipLaunchKernelGGL((attention_dq<V, DW, 2, 2, 64>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     else hipLaunchKernelGGL((attention_dq<V, DW, 4, 1, KT>), dim3((unsigned)blocks), dim3(256), 0, s, p);
@@ -1420,7 +1423,7 @@ int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   if (!p.M || (!p.dk.data && !p.dv.data)) return MCN_SUCCESS;
   const bool two = l.dkvBlocks == 2;
   const long long blocks = tiles_of(&p, p.eachKeys, two ? 64 : 128, p.M) * p.keyHeads * p.groupParts;
-  if (blocks >= (1ll << 31)) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
+  if (blocks * 256 >= kMostThreads) return fail(MCN_UNSUPPORTED, "%s: too many tiles", who);
   {
     KernelTimer timer("attention_dkv", s);
     if (two) hipLaunchKernelGGL((attention_dkv<V, DW, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, s, p);
@@ -1429,7 +1432,7 @@ int backward(const char* who, hipStream_t s, AttentionP& p, const Plan& l) {
   int rc = check_launch(who);
   if (rc || p.groupParts == 1) return rc;
   const long long threads = (long long)p.M * p.keyHeads * (2 * DW / 4);
-  if (threads >= (1ll << 39)) return fail(MCN_UNSUPPORTED, "%s: too many keys", who);
+  if (threads >= kMostThreads - 256) return fail(MCN_UNSUPPORTED, "%s: too many keys", who);
   KernelTimer timer("attention_dkv_join", s);
   hipLaunchKernelGGL((attention_dkv_join<V, DW>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
   return check_launch(who);
