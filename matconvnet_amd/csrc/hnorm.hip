@@ -280,7 +280,10 @@ __global__ __launch_bounds__(64 * kWaves) void hnorm_kernel(HnormP p) {
         }
       }
       float inv = 1.f;
-      if (p.normalise) inv = 1.f / sqrtf(group_sum<T>(squares) / (float)p.D + p.epsilon);
+      if (p.normalise) {
+        inv = 1.f / sqrtf(group_sum<T>(squares) / (float)p.D + p.epsilon);
+        if (BACKWARD && !mine) inv = 1.f;   // (no head: zero times what is finite, also with an epsilon of 0)
+      }
       if (!BACKWARD) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
