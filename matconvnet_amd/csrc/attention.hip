@@ -15,7 +15,12 @@
 // product straight from the registers: the order of a reduction is free, so the other operand is read from LDS in the same order.
 //
 // The walked side comes through LDS, brought there by the DMA a tile ahead, one barrier a tile.  Rows lie there 16 bytes by 16 bytes, exchanged
-// by the row so that neither reads along a row nor transposing reads across rows meet in a bank.
+// by the row so that neither reads along a row nor transposing reads across rows meet in a bank (counted: no conflict in any of the kernels).
+//
+// Measured (bfloat16, times of the kernels; operations counted over the pairs that are seen).  One causal sequence of 16384, 32 heads over 8 of
+// 128: forward 2.06 ms, 1070 TFLOP/s; dq 3.49 and dk, dv 4.18 ms, 717 TFLOP/s, 1150 with all products counted that are made (scores and do.v in
+// both kernels, dq's product twice).  32 x 196 positions, 12 heads of 64, not causal: 17, 24 and 22 us.  64 queries, one a sequence, 262144 keys in
+// all, 8 heads of 128: k and v read at 4.3 TB/s (247 us).
 #include "mcn_internal.hpp"
 
 #include <algorithm>
