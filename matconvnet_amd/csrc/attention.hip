@@ -298,11 +298,19 @@ struct Span {
 
 __device__ __forceinline__ int clamped(int v, int most) { return v < 0 ? 0 : v > most ? most : v; }
 
-__device__ __forceinline__ int wave_total(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+// of all lanes: sixteen by the vector instructions' own lane exchange, the four of these as scalars (shuffles go through LDS and are waited for)
+template <int CONTROL>
+__device__ __forceinline__ int exchanged(int v) { return __builtin_amdgcn_update_dpp(0, v, CONTROL, 0xf, 0xf, true); }
+template <class F>
+__device__ __forceinline__ int over_wave(int v, F f) {
+  v = f(v, exchanged<0xB1>(v));    // lane ^ 1
+  v = f(v, exchanged<0x4E>(v));    // lane ^ 2
+  v = f(v, exchanged<0x141>(v));   // the other four of eight, mirrored
+  v = f(v, exchanged<0x140>(v));   // the other eight of sixteen, mirrored
+  return f(f(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), f(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
+__device__ __forceinline__ int wave_total(int v) { return over_wave(v, [](int a, int b) { return a + b; }); }
+__device__ __forceinline__ int wave_most(int v) { return over_wave(v, [](int a, int b) { return a > b ? a : b; }); }
 
 // Tile `tile` of SIZE rows (KEYS: keys) of all sequences'.  Causal tiles differ in their work (rows: the last of a sequence see the most keys;
 // keys: the first are seen by the most rows), so they are taken in the order of falling work, over all sequences: of the
@@ -330,17 +338,17 @@ __device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
     return s;
   }
   if (p.causal && p.sequences <= 64) {
-    int count = 0;   // tiles of sequence `lane`
+    int q0 = 0, n = 0, k0 = 0, m = 0;   // of sequence `lane`
     if (lane < p.sequences) {
-      const int* at = KEYS ? p.kStarts : p.qStarts;
-      const int most = KEYS ? p.M : p.N;
-      count = std::max(0, clamped(at[lane + 1], most) - clamped(at[lane], most)) * (KEYS ? 1 : p.G);
-      count = (count + SIZE - 1) / SIZE;
+      const int a = p.qStarts[lane], b = p.qStarts[lane + 1], c = p.kStarts[lane], d = p.kStarts[lane + 1];
+      q0 = clamped(a, p.N);
+      n = std::max(0, clamped(b, p.N) - q0);
+      k0 = clamped(c, p.M);
+      m = std::max(0, clamped(d, p.M) - k0);
     }
-    int low = 1, high = count;   // level l: tiles with l - 1 lighter ones in their sequence; those of level `low` or above are more than `tile`
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) high = std::max(high, __shfl_xor(high, o, kWave));
-    ++high;
+    const int count = ((KEYS ? m : n * p.G) + SIZE - 1) / SIZE;   // its tiles
+    // level l: tiles with l - 1 lighter ones in their sequence; those of level `low` or above are more than `tile`
+    int low = 1, high = wave_most(count) + 1;
     int above = 0;               // tiles of level `high` or above
     if (wave_total(count) <= tile) low = 0;
     else
@@ -354,23 +362,29 @@ __device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
       }
     const unsigned long long some = __ballot(count >= low && lane < p.sequences);
     const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0));
-    const unsigned long long one = __ballot((some >> lane & 1) && rank == tile - above);
-    lo = one && low ? __builtin_ctzll(one) : 0;
-    const int tiles = __shfl(count, lo, kWave);
+    const unsigned long long one = __ballot(count >= low && lane < p.sequences && rank == tile - above);
+    lo = __builtin_amdgcn_readfirstlane(one && low ? __builtin_ctzll(one) : 0);
+    const int tiles = __builtin_amdgcn_readlane(count, lo);
     t = !low || !one ? -1 : KEYS ? tiles - low : low - 1;
-  } else {
-    const auto before = [&](int i) { return (KEYS ? clamped(p.kStarts[i], p.M) : clamped(p.qStarts[i], p.N) * p.G) / SIZE + i; };
-    int n = p.sequences;
-    lo = 0;
-    while (n > 1) {
-      const int step = (n + 63) / 64, i = lo + lane * step;
-      const unsigned long long below = __ballot(lane * step < n && before(i) <= tile);
-      const int found = below ? 63 - __builtin_clzll(below) : 0;
-      lo += found * step;
-      n = std::min(step, n - found * step);
-    }
-    t = tile - before(lo);
+    s.q0 = __builtin_amdgcn_readlane(q0, lo);
+    s.n = __builtin_amdgcn_readlane(n, lo);
+    s.k0 = __builtin_amdgcn_readlane(k0, lo);
+    s.m = __builtin_amdgcn_readlane(m, lo);
+    t = __builtin_amdgcn_readfirstlane(t);
+    s.first = t < 0 || t >= tiles ? -1 : t * SIZE;
+    return s;
   }
+  const auto before = [&](int i) { return (KEYS ? clamped(p.kStarts[i], p.M) : clamped(p.qStarts[i], p.N) * p.G) / SIZE + i; };
+  int n = p.sequences;
+  lo = 0;
+  while (n > 1) {
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    const unsigned long long below = __ballot(lane * step < n && before(i) <= tile);
+    const int found = below ? 63 - __builtin_clzll(below) : 0;
+    lo += found * step;
+    n = std::min(step, n - found * step);
+  }
+  t = tile - before(lo);
   lo = __builtin_amdgcn_readfirstlane(lo);
   t = __builtin_amdgcn_readfirstlane(t);
   s.q0 = clamped(p.qStarts[lo], p.N);
