@@ -858,6 +858,212 @@ void nnfcloss(Context& context, Allocator& allocator, int nout, Tensor* out, int
   if (rc) raise(rc > 0 && rc <= (int)VLE_Interrupted ? (ErrorCode)rc : VLE_Unknown, mcn_last_error_message());
 }
 
+bool emptyArray(Arg const& a) { return a.kind == Arg::Array && a.tensor.getNumElements() == 0; }
+double scalarOf(Arg const& a, char const* NAME) {
+  if (!(isPlainMatrix(a) && a.tensor.getNumElements() == 1)) raise(VLE_IllegalArgument, std::string(NAME) + " is not a plain scalar.");
+  return values(a)[0];
+}
+
+// channels x heads x positions x sequences, the positions of all sequences one behind the other
+mcn_heads headsOf(Tensor& t) {
+  mcn_heads h;
+  h.data = t.getMemory();
+  h.head = (long long)t.getHeight();
+  h.position = (long long)(t.getHeight() * t.getWidth());
+  return h;
+}
+void checkHeads(char const* who, Tensor const& t, char const* NAME) {
+  if (t.getDeviceType() != VLDT_GPU)
+    raise(VLE_Unsupported, std::string(who) + ": " + NAME + " is on the CPU; this library implements the GPU (HIP, gfx950) device only");
+  if (t.getDataType() != VLDT_Float) raise(VLE_Unsupported, std::string(who) + ": only single precision is implemented on the HIP device");
+  if (t.getHeight() > (std::size_t)INT_MAX || t.getWidth() > (std::size_t)INT_MAX || t.getSize() > (std::size_t)INT_MAX ||
+      t.getDepth() > (std::size_t)INT_MAX || t.getDepth() * t.getSize() > (std::size_t)INT_MAX)
+    raise(VLE_IllegalArgument, std::string(who) + ": an extent of " + NAME + " is larger than 2^31 - 1.");
+}
+
+// ------------------------------------------------------------------------------------------ vl_nnhnorm
+// (q, k, gq, gk [, dzdq, dzdk], 'epsilon', e, 'normalise', tf, 'neighbours', tf, 'positions', p, 'frequencies', f)
+
+void nnhnorm(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in) {
+  enum { optEpsilon, optNormalise, optNeighbours, optPositions, optFrequencies };
+  static OptionSpec const specs[] = {{"epsilon", true, optEpsilon}, {"normalise", true, optNormalise}, {"neighbours", true, optNeighbours},
+                                     {"positions", true, optPositions}, {"frequencies", true, optFrequencies}, {NULL, false, 0}};
+  if (nin < 4) raise(VLE_IllegalArgument, "There are less than four arguments.");
+  const bool backMode = nin > 4 && in[4].kind != Arg::String;
+  if (backMode && (nin < 6 || in[5].kind == Arg::String)) raise(VLE_IllegalArgument, "DZDQ is given without DZDK.");
+  int next = backMode ? 6 : 4;
+  mcn_hnorm_geom geom = {};
+  geom.normalise = 1;
+  geom.epsilon = 1e-6;
+  geom.dataType = MCN_FLOAT;
+  Arg const *positionsArg = NULL, *frequenciesArg = NULL;
+  int opt;
+  Arg const* value = NULL;
+  while ((opt = nextOption(in, nin, specs, &next, &value)) >= 0) {
+    switch (opt) {
+      case optEpsilon: geom.epsilon = scalarOf(*value, "EPSILON"); break;
+      case optNormalise: geom.normalise = scalarOf(*value, "NORMALISE") != 0; break;
+      case optNeighbours: geom.neighbours = scalarOf(*value, "NEIGHBOURS") != 0; break;
+      case optPositions: if (!emptyArray(*value)) positionsArg = value; break;
+      case optFrequencies: if (!emptyArray(*value)) frequenciesArg = value; break;
+    }
+  }
+  static char const* const names[2] = {"Q", "K"};
+  static char const* const multiplierNames[2] = {"GQ", "GK"};
+  static char const* const derNames[2] = {"DZDQ", "DZDK"};
+  Tensor x[2], g[2], dy[2];
+  for (int i = 0; i < 2; ++i) {
+    if (!emptyArray(in[i])) x[i] = dataTensor(in[i], names[i], 4);
+    if (!emptyArray(in[2 + i])) g[i] = dataTensor(in[2 + i], multiplierNames[i], 1);
+    if (backMode && !emptyArray(in[4 + i])) dy[i] = dataTensor(in[4 + i], derNames[i], 4);
+  }
+  Tensor const& any = x[0] ? x[0] : x[1];
+  if (!any) raise(VLE_IllegalArgument, "Q and K are both empty.");
+  if (x[0] && x[1] && (!areCompatible(x[0], x[1]) || x[0].getHeight() != x[1].getHeight() || x[0].getDepth() != x[1].getDepth() || x[0].getSize() != x[1].getSize()))
+    raise(VLE_IllegalArgument, "Q and K do not have the same channels, positions and sequences.");
+  for (int i = 0; i < 2; ++i) {
+    const std::string NAME = names[i], GNAME = multiplierNames[i], DNAME = derNames[i];
+    if (g[i] && (!x[i] || !areCompatible(x[i], g[i]) || g[i].getNumElements() != x[i].getHeight()))
+      raise(VLE_IllegalArgument, GNAME + " does not have one value per channel of " + NAME + ".");
+    if (g[i] && !geom.normalise) raise(VLE_IllegalArgument, GNAME + " is taken with NORMALISE only.");
+    if (backMode && ((bool)dy[i] != (bool)x[i] || (x[i] && (!areCompatible(x[i], dy[i]) || x[i].getShape() != dy[i].getShape()))))
+      raise(VLE_IllegalArgument, NAME + " and " + DNAME + " do not have the same size.");
+  }
+  for (int i = 0; i < 2; ++i)
+    if (x[i]) checkHeads("vl_nnhnorm", x[i], names[i]);
+  const std::size_t N = any.getDepth() * any.getSize();
+  geom.D = (int)any.getHeight();
+  geom.N = (int)N;
+  geom.heads = x[0] ? (int)x[0].getWidth() : 0;
+  geom.keyHeads = x[1] ? (int)x[1].getWidth() : 0;
+  Tensor positions, frequencies;
+  if ((positionsArg != NULL) != (frequenciesArg != NULL)) raise(VLE_IllegalArgument, "POSITIONS and FREQUENCIES are taken together.");
+  if (positionsArg) {
+    positions = dataTensor(*positionsArg, "POSITIONS", 2);      // axes x positions
+    frequencies = dataTensor(*frequenciesArg, "FREQUENCIES", 2);   // pairs x axes
+    for (Tensor const* t : {&positions, &frequencies})
+      if (t->getDataType() != VLDT_Double || t->getDeviceType() != VLDT_GPU)
+        raise(VLE_IllegalArgument, "POSITIONS and FREQUENCIES are not of class DOUBLE on the device.");
+    if (positions.getDimension(0) != frequencies.getDimension(1) || positions.getDimension(1) != N)
+      raise(VLE_IllegalArgument, "POSITIONS are not axes x positions or FREQUENCIES not pairs x axes.");
+    if (frequencies.getDimension(0) > (std::size_t)INT_MAX || frequencies.getDimension(1) > (std::size_t)INT_MAX)
+      raise(VLE_IllegalArgument, "vl_nnhnorm: more than 2^31 - 1 pairs or axes.");
+    geom.pairs = (int)frequencies.getDimension(0);
+    geom.axes = (int)frequencies.getDimension(1);
+  }
+  void* stream = context.getHipHelper().getStream();
+  Tensor y[2];
+  mcn_heads hx[2], hdy[2], hy[2];
+  for (int i = 0; i < 2; ++i) {
+    y[i] = !x[i] || (i && nout < 2) ? emptyMatrix(VLDT_Float) : newOutput(allocator, VLDT_GPU, VLDT_Float, in[i].tensor.getShape());
+    Tensor shaped(y[i]);
+    if (x[i] && !(i && nout < 2)) shaped.reshape(4);
+    hy[i] = headsOf(shaped);
+    hx[i] = headsOf(x[i]);
+    hdy[i] = headsOf(dy[i]);
+  }
+  if (!backMode && nout < 2) geom.keyHeads = 0;
+  int rc;
+  if (!backMode) {
+    rc = mcn_hnorm_forward(stream, &geom, &hy[0], &hy[1], &hx[0], &hx[1], (float const*)g[0].getMemory(), (float const*)g[1].getMemory(),
+                           (double const*)positions.getMemory(), (double const*)frequencies.getMemory());
+  } else {
+    for (int i = 0; i < 2; ++i)
+      if (nout > 2 + i) out[2 + i] = g[i] ? newOutput(allocator, VLDT_GPU, VLDT_Float, in[2 + i].tensor.getShape()) : emptyMatrix(VLDT_Float);
+    const std::size_t bytes = nout > 2 ? mcn_hnorm_workspace_bytes(&geom) : 0;
+    void* ws = callWorkspace(allocator, bytes);
+    rc = mcn_hnorm_backward(stream, &geom, &hy[0], &hy[1], nout > 2 ? (float*)out[2].getMemory() : NULL, nout > 3 ? (float*)out[3].getMemory() : NULL,
+                            &hx[0], &hx[1], (float const*)g[0].getMemory(), (float const*)g[1].getMemory(), (double const*)positions.getMemory(),
+                            (double const*)frequencies.getMemory(), &hdy[0], &hdy[1], ws, bytes);
+  }
+  if (rc) raise(rc > 0 && rc <= (int)VLE_Interrupted ? (ErrorCode)rc : VLE_Unknown, mcn_last_error_message());
+  out[0] = y[0];
+  if (nout > 1) out[1] = y[1];
+}
+
+// ------------------------------------------------------------------------------------------ vl_nnattention
+// (q, k, v [, dzdy], 'causal', tf, 'scale', s, 'output', y, 'logSums', l): vl_nnsoftmax between two products, without the scores
+
+void nnattention(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in) {
+  enum { optCausal, optScale, optOutput, optLogSums };
+  static OptionSpec const specs[] = {{"causal", true, optCausal}, {"scale", true, optScale}, {"output", true, optOutput}, {"logSums", true, optLogSums}, {NULL, false, 0}};
+  if (nin < 3) raise(VLE_IllegalArgument, "There are less than three arguments.");
+  const bool backMode = nin > 3 && in[3].kind != Arg::String;
+  int next = backMode ? 4 : 3;
+  mcn_attention_geom g = {};
+  g.dataType = MCN_FLOAT;
+  Arg const *outputArg = NULL, *sumsArg = NULL;
+  int opt;
+  Arg const* value = NULL;
+  while ((opt = nextOption(in, nin, specs, &next, &value)) >= 0) {
+    switch (opt) {
+      case optCausal: g.causal = scalarOf(*value, "CAUSAL") != 0; break;
+      case optScale: g.scale = scalarOf(*value, "SCALE"); break;
+      case optOutput: outputArg = value; break;
+      case optLogSums: sumsArg = value; break;
+    }
+  }
+  Tensor q = dataTensor(in[0], "Q", 4), k = dataTensor(in[1], "K", 4), v = dataTensor(in[2], "V", 4), dy, y, sums;
+  if (backMode) dy = dataTensor(in[3], "DZDY", 4);
+  if ((outputArg != NULL) != (sumsArg != NULL)) raise(VLE_IllegalArgument, "OUTPUT and LOGSUMS are taken together.");
+  if (outputArg && !backMode) raise(VLE_IllegalArgument, "OUTPUT and LOGSUMS are taken with DZDY only.");
+  if (outputArg) {
+    y = dataTensor(*outputArg, "OUTPUT", 4);
+    sums = dataTensor(*sumsArg, "LOGSUMS", 1);
+  }
+  if (!areCompatible(q, k) || !areCompatible(q, v)) raise(VLE_IllegalArgument, "Q, K and V do not have compatible formats.");
+  if (k.getShape() != v.getShape()) raise(VLE_IllegalArgument, "K and V do not have the same size.");
+  if (q.getHeight() != k.getHeight() || q.getSize() != k.getSize()) raise(VLE_IllegalArgument, "Q and K do not have the same channels and sequences.");
+  if (backMode && (!areCompatible(q, dy) || q.getShape() != dy.getShape())) raise(VLE_IllegalArgument, "Q and DZDY do not have the same size.");
+  const std::size_t rows = q.getWidth() * q.getDepth() * q.getSize();
+  if (outputArg && (!areCompatible(q, y) || q.getShape() != y.getShape())) raise(VLE_IllegalArgument, "Q and OUTPUT do not have the same size.");
+  if (outputArg && (!areCompatible(q, sums) || sums.getNumElements() != rows)) raise(VLE_IllegalArgument, "LOGSUMS do not have one value per head and position of Q.");
+  checkHeads("vl_nnattention", q, "Q");
+  checkHeads("vl_nnattention", k, "K");
+  g.D = (int)q.getHeight();
+  g.heads = (int)q.getWidth();
+  g.keyHeads = (int)k.getWidth();
+  g.sequences = (int)q.getSize();
+  g.N = (int)(q.getDepth() * q.getSize());
+  g.M = (int)(k.getDepth() * k.getSize());
+  void* stream = context.getHipHelper().getStream();
+  const mcn_heads hq = headsOf(q), hk = headsOf(k), hv = headsOf(v);
+  int rc = 0;
+  if (!outputArg) {   // (backward: what the forward call would have left)
+    const std::size_t bytes = mcn_attention_workspace_bytes(&g, 0);
+    void* ws = callWorkspace(allocator, bytes);
+    y = newOutput(allocator, VLDT_GPU, VLDT_Float, in[0].tensor.getShape());
+    if (backMode || nout > 1) {
+      std::size_t dims[3] = {q.getWidth(), q.getDepth(), q.getSize()};
+      sums = newOutput(allocator, VLDT_GPU, VLDT_Float, TensorShape(dims, 3));
+    }
+    Tensor shaped(y);
+    shaped.reshape(4);
+    const mcn_heads hy = headsOf(shaped);
+    rc = mcn_attention_forward(stream, &g, &hy, (float*)sums.getMemory(), &hq, &hk, &hv, NULL, NULL, ws, bytes);
+    if (!backMode) {
+      out[0] = y;
+      if (nout > 1) out[1] = sums;
+    }
+  }
+  if (!rc && backMode) {
+    const std::size_t bytes = mcn_attention_workspace_bytes(&g, 1);
+    void* ws = callWorkspace(allocator, bytes);
+    mcn_heads der[3] = {};
+    for (int i = 0; i < 3 && (i == 0 || nout > i); ++i) {
+      out[i] = newOutput(allocator, VLDT_GPU, VLDT_Float, in[i].tensor.getShape());
+      Tensor shaped(out[i]);
+      shaped.reshape(4);
+      der[i] = headsOf(shaped);
+    }
+    Tensor shaped(y);
+    shaped.reshape(4);
+    const mcn_heads hy = headsOf(shaped), hdy = headsOf(dy);
+    rc = mcn_attention_backward(stream, &g, &der[0], &der[1], &der[2], &hy, (float const*)sums.getMemory(), &hq, &hk, &hv, &hdy, NULL, NULL, ws, bytes);
+  }
+  if (rc) raise(rc > 0 && rc <= (int)VLE_Interrupted ? (ErrorCode)rc : VLE_Unknown, mcn_last_error_message());
+}
+
 typedef void (*Body)(Context&, Allocator&, int, Tensor*, int, Arg const*);
 
 ErrorCode guarded(Body body, Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
@@ -904,6 +1110,12 @@ ErrorCode vl_nnlnorm(Context& context, Allocator& allocator, int nout, Tensor* o
 }
 ErrorCode vl_nnfcloss(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in, std::string& message) {
   return guarded(nnfcloss, context, allocator, nout, out, nin, in, message);
+}
+ErrorCode vl_nnhnorm(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in, std::string& message) {
+  return guarded(nnhnorm, context, allocator, nout, out, nin, in, message);
+}
+ErrorCode vl_nnattention(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in, std::string& message) {
+  return guarded(nnattention, context, allocator, nout, out, nin, in, message);
 }
 
 } }  // namespace vl::frontend

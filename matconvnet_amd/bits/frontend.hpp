@@ -34,8 +34,8 @@ struct Arg {
   static Arg numeric(std::vector<double> const& values);
 };
 
-// Who provides memory for outputs (MATLAB's allocator in the MEX drivers), and for what vl_nnlnorm and vl_nnfcloss keep on the device
-// during a call, which may go back when the call returns, to be used again behind it on its stream.  Returning NULL = out of memory.
+// Who provides memory for outputs (MATLAB's allocator in the MEX drivers), and for what vl_nnlnorm, vl_nnfcloss, vl_nnhnorm and vl_nnattention
+// keep on the device during a call, which may go back when the call returns, to be used again behind it on its stream.  Returning NULL = out of memory.
 class Allocator {
  public:
   virtual ~Allocator() {}
@@ -54,6 +54,8 @@ class Allocator {
 //   vl_nnsoftmax: forward [y]           backward [dzdx]
 //   vl_nnlnorm: forward [y, moments]    backward [dzdx, dzdg, dzdb, moments]
 //   vl_nnfcloss: forward [y, logSums]   backward [dzdx, dzdf, dzdb]
+//   vl_nnhnorm: forward [yq, yk]        backward [dzdq, dzdk, dzdgq, dzdgk]
+//   vl_nnattention: forward [y, logSums] backward [dzdq, dzdk, dzdv]
 ErrorCode vl_nnconv(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
                     std::string& message);
 ErrorCode vl_nnconvt(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
@@ -84,6 +86,16 @@ ErrorCode vl_nnlnorm(Context& context, Allocator& allocator, int nout, Tensor* o
 // and the weights as for vl_nnloss.  logSums: the forward call's second result, which saves the backward call a third of its work.
 ErrorCode vl_nnfcloss(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
                       std::string& message);
+// vl_nnhnorm(q, k, gq, gk [, dzdq, dzdk], 'epsilon', e, 'normalise', tf, 'neighbours', tf, 'positions', p, 'frequencies', f): mcn_hnorm_*
+// (no counterpart in the reference).  q, k: channels x heads x positions x sequences, single, on the device, one of them may be empty; gq, gk: a
+// value per channel, or empty; p: axes x all positions, f: pairs x axes, both double, on the device, or neither: no rotation.
+ErrorCode vl_nnhnorm(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
+                     std::string& message);
+// vl_nnattention(q, k, v [, dzdy], 'causal', tf, 'scale', s, 'output', y, 'logSums', l): mcn_attention_* of sequences of one length (no
+// counterpart in the reference).  q: channels x heads x positions x sequences, k, v: channels x key heads x keys x sequences, single, on the
+// device; l: heads x positions x sequences.  y and l, the forward call's results, save the backward call making them again.
+ErrorCode vl_nnattention(Context& context, Allocator& allocator, int nout, Tensor* out, int nin, Arg const* in,
+                         std::string& message);
 
 } }  // namespace vl::frontend
 #endif

@@ -46,8 +46,8 @@ void fromTensor(Tensor const& t, vlh_arg* a) {
   a->text = NULL;
 }
 
-// one context per front-end function, like the static vl::MexContext of each MEX file; vl_nnlnorm and vl_nnfcloss, which keep nothing in it,
-// have one per call
+// one context per front-end function, like the static vl::MexContext of each MEX file; those from vl_nnlnorm on, which keep nothing
+// in it, have one per call
 Context& contextOf(int which) {
   static Context contexts[8];
   return contexts[which];
@@ -96,7 +96,7 @@ int vlh_call(const char* function, int nout, vlh_arg* out, int nin, const vlh_ar
     g_message = "vlh_call: null argument";
     return VLE_IllegalArgument;
   }
-  int which = !std::strcmp(function, "vl_nnconv") ? 0 : !std::strcmp(function, "vl_nnbnorm") ? 1 : !std::strcmp(function, "vl_nnpool") ? 2 : !std::strcmp(function, "vl_nnconvt") ? 3 : !std::strcmp(function, "vl_taccum") ? 4 : !std::strcmp(function, "vl_nnloss") ? 5 : !std::strcmp(function, "vl_nnrelu") ? 6 : !std::strcmp(function, "vl_nnsoftmax") ? 7 : !std::strcmp(function, "vl_nnlnorm") ? 8 : !std::strcmp(function, "vl_nnfcloss") ? 9 : -1;
+  int which = !std::strcmp(function, "vl_nnconv") ? 0 : !std::strcmp(function, "vl_nnbnorm") ? 1 : !std::strcmp(function, "vl_nnpool") ? 2 : !std::strcmp(function, "vl_nnconvt") ? 3 : !std::strcmp(function, "vl_taccum") ? 4 : !std::strcmp(function, "vl_nnloss") ? 5 : !std::strcmp(function, "vl_nnrelu") ? 6 : !std::strcmp(function, "vl_nnsoftmax") ? 7 : !std::strcmp(function, "vl_nnlnorm") ? 8 : !std::strcmp(function, "vl_nnfcloss") ? 9 : !std::strcmp(function, "vl_nnhnorm") ? 10 : !std::strcmp(function, "vl_nnattention") ? 11 : -1;
   if (which < 0) {
     g_message = std::string("vlh_call: unknown function '") + function + "'";
     return VLE_IllegalArgument;
@@ -122,6 +122,8 @@ int vlh_call(const char* function, int nout, vlh_arg* out, int nin, const vlh_ar
   else if (which == 7) e = frontend::vl_nnsoftmax(context, allocator, nout, results, nin, a, g_message);
   else if (which == 8) e = frontend::vl_nnlnorm(context, allocator, nout, results, nin, a, g_message);
   else if (which == 9) e = frontend::vl_nnfcloss(context, allocator, nout, results, nin, a, g_message);
+  else if (which == 10) e = frontend::vl_nnhnorm(context, allocator, nout, results, nin, a, g_message);
+  else if (which == 11) e = frontend::vl_nnattention(context, allocator, nout, results, nin, a, g_message);
   else e = frontend::vl_nnpool(context, allocator, nout, results, nin, a, g_message);
   for (int i = 0; i < 4; ++i) fromTensor(results[i], &out[i]);
   return (int)e;

@@ -8,6 +8,8 @@
     y / dzdx                 = vl_nnpool(x, pool[, dzdy], 'stride', s, 'pad', p, 'method', 'max'|'avg')
     y[, mom] / dzdx, ...     = vl_nnlnorm(x, g, b[, dzdy], 'epsilon', e, 'moments', m)
     y[, sums] / dzdx, ...    = vl_nnfcloss(x, f, b, c[, dzdy], 'instanceWeights', w, 'normalise', tf, 'logSums', s)
+    yq, yk / dzdq, ...       = vl_nnhnorm(q, k, gq, gk[, dzdq, dzdk], 'epsilon', e, 'positions', p, 'frequencies', f, ...)
+    y[, sums] / dzdq, ...    = vl_nnattention(q, k, v[, dzdy], 'causal', tf, 'scale', s, 'output', y, 'logSums', sums)
 
 Arguments follow the MEX drivers (matlab/src/vl_nnconv.cu, vl_nnbnorm.cu, vl_nnpool.cu): data arguments are
 torch CUDA tensors standing for MATLAB arrays -- a MATLAB array of size H x W x C x N is a contiguous
@@ -244,6 +246,24 @@ def vl_nnfcloss(*args, nout=None):
     back = len(args) > 4 and not isinstance(args[4], str) and 0 not in np.shape(args[4])
     n = nout if nout is not None else (3 if back else 1)
     r = _call("vl_nnfcloss", n, list(args))
+    return r[0] if n == 1 else tuple(r[:n])
+
+
+def vl_nnhnorm(*args, nout=None):
+    """vl_nnhnorm(q, k, gq, gk [, dzdq, dzdk], 'epsilon', e, 'normalise', tf, 'neighbours', tf, 'positions', p, 'frequencies', f): heads
+    normalised and rotated; (yq, yk), or (dzdq, dzdk, dzdgq, dzdgk) with dzdq and dzdk.  q, k: tensors (sequences, positions, heads, channels)."""
+    back = len(args) > 4 and not isinstance(args[4], str)
+    n = nout if nout is not None else (4 if back else 2)
+    r = _call("vl_nnhnorm", n, list(args))
+    return r[0] if n == 1 else tuple(r[:n])
+
+
+def vl_nnattention(*args, nout=None):
+    """vl_nnattention(q, k, v [, dzdy], 'causal', tf, 'scale', s, 'output', y, 'logSums', l): attention without the scores; y[, logSums], or dzdq,
+    dzdk, dzdv with dzdy.  q (sequences, positions, heads, channels), k, v (sequences, keys, key heads, channels)."""
+    back = len(args) > 3 and not isinstance(args[3], str)
+    n = nout if nout is not None else (3 if back else 1)
+    r = _call("vl_nnattention", n, list(args))
     return r[0] if n == 1 else tuple(r[:n])
 
 
