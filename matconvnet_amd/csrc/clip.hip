@@ -3,12 +3,12 @@
 // Bound by memory: g is read once for the norm and once for the product, y written.  Squares are summed in double from the first on
 // (gradients of 1e20 or 1e-30 neither overflow nor vanish, and hundreds of millions of terms lose nothing).
 //
-// A launch takes a table of up to kTable tensors in its arguments, so that nothing has to reach the device ahead of it and a captured
+// A launch takes a table of up to kTable entries in its arguments, so that nothing has to reach the device ahead of it and a captured
 // graph holds it all.  Every tensor is cut into runs of one length, a workgroup takes a run and leaves one partial sum; runs are as
 // long as makes about kRuns of them in all.  The second launch's workgroups each add up all partial sums, in one order, rather than
 // wait for a launch that does only that: 2048 values of 8 bytes out of the L2 for each.
-// Measured: ResNet-50's 25.6 million values, single, 74 us (two tables; a clip_squares of 11 us and a clip_scale of 20 for each: most of what
-// is read a second time comes out of the caches); 300 tensors of 600 million values in all, bfloat16 and single, 1.0 ms, 4.4 TB/s with g read twice.
+// Measured: ResNet-50's 161 tensors of 25.6 million values, single, 53 us (two launches; most of what is read a second time comes out of the
+// caches); 300 tensors of 600 million values in all, bfloat16 and single, 0.99 ms, 4.4 TB/s with g read twice.
 #include "mcn_internal.hpp"
 
 #include <algorithm>
@@ -19,27 +19,36 @@ namespace {
 
 typedef unsigned uintx4loose __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes that may start at any value
 
-constexpr int kTable = 128, kRuns = 2048;
+constexpr int kTable = 164, kFew = 32, kRuns = 2048;
 constexpr size_t kLeast = 8192;   // values of a run at least: 256 threads, 32 each
-constexpr unsigned long long kBf16Bit = 1ull << 63;
+constexpr unsigned kBf16Bit = 1u << 31;
+constexpr size_t kPiece = 1ull << 30;   // larger tensors are several entries
+constexpr size_t kMost = 1ull << 40;    // values of all tensors: a run is no longer than a piece
 
-// 28 bytes a tensor: within the 4 KB that arguments may take
+// 24 bytes an entry: as many as the 4 KB hold that arguments may take, or few, whose launch has less to copy (10
+// tensors of 70000 values: 12.9 us instead of 15.8)
+template <int ENTRIES>
 struct Table {
-  const void* der[kTable];
-  void* out[kTable];
-  unsigned long long count[kTable];   // with kBf16Bit
-  unsigned first[kTable];             // its first workgroup in this launch
+  static constexpr int most = ENTRIES;
+  const void* der[ENTRIES];
+  void* out[ENTRIES];
+  unsigned count[ENTRIES];   // with kBf16Bit
+  unsigned first[ENTRIES];   // its first workgroup in this launch
   int n;
 };
+static_assert(sizeof(Table<kTable>) + 48 <= 4096, "arguments");
 
-__device__ __forceinline__ int tensor_of(const Table& t, unsigned block) {
-  int lo = 0, hi = t.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t.first[mid] <= block) lo = mid;
-    else hi = mid - 1;
+// (every lane looks at some entries: a search by halves is eight loads one behind the other)
+template <class T>
+__device__ __forceinline__ int entry_of(const T& t, unsigned block) {
+  const int lane = threadIdx.x & 63;
+  int k = -1;
+#pragma unroll
+  for (int i = 0; i < T::most; i += 64) {
+    const bool here = i + lane < t.n && t.first[std::min(i + lane, T::most - 1)] <= block;
+    k += (int)__popcll(__ballot(here));
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(k);
 }
 
 __device__ __forceinline__ double block_sum(double v, double* slots) {
@@ -83,9 +92,10 @@ __device__ __forceinline__ double squares(const void* base, size_t first, size_t
   return s;
 }
 
-__global__ __launch_bounds__(256) void clip_squares(double* __restrict__ partials, Table t, size_t run) {
+template <int ENTRIES>
+__global__ __launch_bounds__(256) void clip_squares(double* __restrict__ partials, Table<ENTRIES> t, size_t run) {
   __shared__ double slots[4];
-  const int k = tensor_of(t, blockIdx.x);
+  const int k = entry_of(t, blockIdx.x);
   const size_t count = t.count[k] & ~kBf16Bit, first = (size_t)(blockIdx.x - t.first[k]) * run, last = std::min(first + run, count);
   const double s = block_sum(t.count[k] & kBf16Bit ? squares<true>(t.der[k], first, last) : squares<false>(t.der[k], first, last), slots);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
@@ -138,12 +148,14 @@ __device__ __forceinline__ void scale_run(void* out, const void* base, size_t fi
 }
 
 // (out may be der: a thread writes what it alone has read)
-__global__ __launch_bounds__(256) void clip_scale(float* __restrict__ norm, const double* __restrict__ partials, int parts, Table t, size_t run, double most) {
+template <int ENTRIES>
+__global__ __launch_bounds__(256) void clip_scale(float* __restrict__ norm, const double* __restrict__ partials, int parts, Table<ENTRIES> t, size_t run,
+                                                  double most) {
   __shared__ double slots[4];
   const double n = join_norm(partials, parts, 1.0, slots);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
   const double f = factor_of(n, most);
-  const int k = tensor_of(t, blockIdx.x);
+  const int k = entry_of(t, blockIdx.x);
   if (f == 1.0 && t.out[k] == t.der[k]) return;
   const size_t count = t.count[k] & ~kBf16Bit, first = (size_t)(blockIdx.x - t.first[k]) * run, last = std::min(first + run, count);
   if (t.count[k] & kBf16Bit) scale_run<true>(t.out[k], t.der[k], first, last, f);
@@ -161,21 +173,32 @@ __global__ __launch_bounds__(256) void clip_join(float* __restrict__ norm, float
 
 size_t run_of(size_t total) { return std::max(kLeast, (total / kRuns + kLeast - 1) / kLeast * kLeast); }
 
-// the tensors of one launch, from `from` on: how many, and its workgroups
-int fill(Table* t, int from, int n, void* const* out, const void* const* ders, const size_t* counts, const int* types, size_t run, unsigned* blocks) {
+// the entries of one launch, from `at` on, which is left behind them: tensors and what of them is done; its workgroups
+struct Place {
+  int tensor = 0;
+  size_t done = 0;
+};
+template <int ENTRIES>
+void fill(Table<ENTRIES>* t, Place* at, int n, void* const* out, const void* const* ders, const size_t* counts, const int* types, size_t run, unsigned* blocks) {
+  const size_t piece = std::max<size_t>(1, kPiece / run) * run;
   t->n = 0;
   *blocks = 0;
-  int i = from;
-  for (; i < n && t->n < kTable; ++i) {
-    if (counts[i] == 0) continue;
-    t->der[t->n] = ders[i];
-    t->out[t->n] = out ? out[i] : nullptr;
-    t->count[t->n] = (unsigned long long)counts[i] | (types[i] == MCN_BFLOAT16 ? kBf16Bit : 0);
-    t->first[t->n] = *blocks;
-    *blocks += (unsigned)((counts[i] + run - 1) / run);
-    ++t->n;
+  while (at->tensor < n && t->n < ENTRIES) {
+    const int i = at->tensor;
+    const size_t size = types[i] == MCN_BFLOAT16 ? 2 : 4, count = std::min(piece, counts[i] - at->done);
+    if (count) {
+      t->der[t->n] = (const char*)ders[i] + at->done * size;
+      t->out[t->n] = out ? (char*)out[i] + at->done * size : nullptr;
+      t->count[t->n] = (unsigned)count | (types[i] == MCN_BFLOAT16 ? kBf16Bit : 0);
+      t->first[t->n] = *blocks;
+      *blocks += (unsigned)((count + run - 1) / run);
+      ++t->n;
+      at->done += count;
+    }
+    if (at->done < counts[i]) continue;
+    ++at->tensor;
+    at->done = 0;
   }
-  return i;
 }
 
 struct Sizes {
@@ -192,9 +215,11 @@ Sizes sizes_of(const size_t* counts, int n) {
 int check(const char* who, const void* const* ders, const size_t* counts, const int* types, int n) {
   if (n < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative number of tensors", who);
   if (n && (!ders || !counts || !types)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null argument", who);
+  size_t total = 0;
   for (int i = 0; i < n; ++i) {
     if (types[i] != MCN_FLOAT && types[i] != MCN_BFLOAT16) return fail(MCN_ILLEGAL_ARGUMENT, "%s: unknown data type %d of tensor %d", who, types[i], i);
-    if (counts[i] > (1ull << 40)) return fail(MCN_UNSUPPORTED, "%s: tensor %d too large", who, i);
+    if (counts[i] > kMost - total) return fail(MCN_UNSUPPORTED, "%s: tensor %d too large", who, i);
+    total += counts[i];
     if (!counts[i]) continue;
     if (!ders[i]) return fail(MCN_ILLEGAL_ARGUMENT, "%s: tensor %d is null", who, i);
     if ((uintptr_t)ders[i] % (types[i] == MCN_BFLOAT16 ? 2 : 4)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: tensor %d is not aligned", who, i);
@@ -208,21 +233,41 @@ int check_workspace(const char* who, const void* workspace, size_t bytes, size_t
   return MCN_SUCCESS;
 }
 
-int squares_of_all(const char* who, hipStream_t s, double* partials, const void* const* ders, const size_t* counts, const int* types, int n, size_t run) {
-  for (int from = 0; from < n;) {
-    Table t;
+template <int ENTRIES>
+int squares_of(const char* who, hipStream_t s, double* partials, const void* const* ders, const size_t* counts, const int* types, int n, size_t run) {
+  for (Place at; at.tensor < n;) {
+    Table<ENTRIES> t;
     unsigned blocks;
-    from = fill(&t, from, n, nullptr, ders, counts, types, run, &blocks);
+    fill(&t, &at, n, nullptr, ders, counts, types, run, &blocks);
     if (!blocks) continue;
     {
       KernelTimer timer("clip_squares", s);
-      hipLaunchKernelGGL(clip_squares, dim3(blocks), dim3(256), 0, s, partials, t, run);
+      hipLaunchKernelGGL(clip_squares<ENTRIES>, dim3(blocks), dim3(256), 0, s, partials, t, run);
     }
     const int rc = check_launch(who);
     if (rc) return rc;
     partials += blocks;
   }
   return MCN_SUCCESS;
+}
+int squares_of_all(const char* who, hipStream_t s, double* partials, const void* const* ders, const size_t* counts, const int* types, int n, size_t run) {
+  return n <= kFew ? squares_of<kFew>(who, s, partials, ders, counts, types, n, run) : squares_of<kTable>(who, s, partials, ders, counts, types, n, run);
+}
+
+template <int ENTRIES>
+int scale_of(const char* who, hipStream_t s, void* const* outs, float* norm, const double* partials, const void* const* ders, const size_t* counts,
+             const int* types, int n, const Sizes& z, double most) {
+  int rc = MCN_SUCCESS;
+  for (Place at; at.tensor < n && !rc;) {
+    Table<ENTRIES> t;
+    unsigned blocks;
+    fill(&t, &at, n, outs, ders, counts, types, z.run, &blocks);
+    if (!blocks) continue;
+    KernelTimer timer("clip_scale", s);
+    hipLaunchKernelGGL(clip_scale<ENTRIES>, dim3(blocks), dim3(256), 0, s, norm, partials, (int)z.parts, t, z.run, most);
+    rc = check_launch(who);
+  }
+  return rc;
 }
 
 }  // namespace
@@ -296,16 +341,9 @@ int mcn_clip_gradients(mcn_stream_t stream, void* const* outs, float* norm, cons
   if (rc) return rc;
   hipStream_t s = as_stream(stream);
   rc = squares_of_all(who, s, (double*)workspace, ders, counts, dataTypes, n, z.run);
-  for (int from = 0; from < n && !rc;) {
-    Table t;
-    unsigned blocks;
-    from = fill(&t, from, n, outs, ders, counts, dataTypes, z.run, &blocks);
-    if (!blocks) continue;
-    KernelTimer timer("clip_scale", s);
-    hipLaunchKernelGGL(clip_scale, dim3(blocks), dim3(256), 0, s, norm, (const double*)workspace, (int)z.parts, t, z.run, maxNorm);
-    rc = check_launch(who);
-  }
-  return rc;
+  if (rc) return rc;
+  return n <= kFew ? scale_of<kFew>(who, s, outs, norm, (const double*)workspace, ders, counts, dataTypes, n, z, maxNorm)
+                   : scale_of<kTable>(who, s, outs, norm, (const double*)workspace, ders, counts, dataTypes, n, z, maxNorm);
 }
 
 }  // extern "C"
