@@ -904,7 +904,9 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
 // ------------------------------------------------------------------------------------------ dk, dv
 
 // 32 positions of a head against a wavefront's 32 keys
-template <class V, int DW, class Bring>
+// (AHEAD: LDS is read three steps ahead, where the registers for it are there and cost no wavefront: heads of 96, and of 64 where two wavefronts
+// share a block.  2 x 1024 positions, 8 heads of 64: 19.4 -> 16.9 us; with four wavefronts alone, of which three fit a SIMD as it is, 19.8 -> 23.)
+template <class V, int DW, bool AHEAD, class Bring>
 __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const char* __restrict__ ders, const float* __restrict__ statL,
                                          const float* __restrict__ statD, char* __restrict__ next, Bring bring_next, const uintx4 (&k)[Tile<V, DW>::steps],
                                          const uintx4 (&v)[Tile<V, DW>::steps], floatx16 (&dk)[DW / 32], floatx16 (&dv)[DW / 32], int i0, int n, int firstOf,
@@ -947,6 +949,29 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
     masked();
     T::operand(operand, e);
   };
+  if constexpr (AHEAD) {
+    constexpr int S = T::steps, P = DW / 32 * 2;   // steps of the products with rows as they lie, and with rows turned
+    start(dp, statD);
+    steps_ahead<3, 2 * (S + P)>(
+        [&](int i) __attribute__((always_inline)) {
+          const char* rows = (i < S || i >= 2 * S + P) ? queries : ders;
+          if (i < S || (i >= S + P && i < 2 * S + P)) return T::along(rows, 0, i < S ? i : i - S - P, lane);
+          i -= i < S + P ? S : 2 * S + P;
+          return T::turned(rows, 16 * (i % 2), i / 2, lane);
+        },
+        [&](int i, uintx4 a) __attribute__((always_inline)) {
+          if (i < S) s = Matrix<V>::along(a, k[i], s);
+          else if (i < S + P) {
+            if (i == S) probabilities();
+            dv[(i - S) / 2] = Matrix<V>::along(a, operand[i % 2], dv[(i - S) / 2]);
+          } else if (i < 2 * S + P) dp = Matrix<V>::along(a, v[i - S - P], dp);
+          else {
+            if (i == 2 * S + P) scores();
+            dk[(i - 2 * S - P) / 2] = Matrix<V>::along(a, operand[i % 2], dk[(i - 2 * S - P) / 2]);
+          }
+        });
+    return;
+  }
 #pragma unroll
   for (int t = 0; t < T::steps; ++t) s = Matrix<V>::along(T::along(queries, 0, t, lane), k[t], s);
   probabilities();
@@ -1049,7 +1074,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       before = all_finite(dk) && all_finite(dv);
     }
     if (i + 32 > some && i < span.n)
-      dkv_tile<V, DW>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, (const float*)(from + 2 * tileBytes) + share0,
+      dkv_tile<V, DW, sizeof(V) == 2 && (DW == 96 || (DW == 64 && NS == 2))>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, (const float*)(from + 2 * tileBytes) + share0,
                       (const float*)(from + 2 * tileBytes + statBytes) + share0, to, bring_next, k, v, dk, dv, i, span.n, firstOf, i < all || i + 32 > span.n, p.c,
                       lane);
     else bring_next(to);
