@@ -53,8 +53,9 @@ __device__ __forceinline__ bool finite(float v) { return (float_bits(v) & 0x7f80
 
 // the other half's value of the 64 lanes (lane ^ 32)
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, kWave); }
-// whether both lanes of a row (or key) find it good.  (As numbers: where each lane took its bit out of a ballot's words, whole halves of wavefronts
-// of the dq kernel came out bad now and then, all of their values being finite; the slow sums behind the loop hid that but for their time.)
+// whether both lanes of a row (or key) find it good.  (As numbers: a lane's own bit of a ballot takes a 64-bit shift by the lane, whose result was
+// wrong in half of a wavefront now and then where the compiler kept the amount in the last register that a wavefront has, v255 in dq; the slow
+// sums behind the loop hid that but for their time.)
 __device__ __forceinline__ bool both_good(bool good) {
   const float bad = good ? 0.f : 1.f;
   return bad + other_half(bad) == 0.f;
