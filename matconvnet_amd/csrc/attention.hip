@@ -361,8 +361,7 @@ __device__ __forceinline__ Span find(const AttentionP& p, int tile, int lane) {
           above = total;
         }
       }
-    unsigned long long some = __ballot(count >= low && lane < p.sequences);
-    asm volatile("s_nop 4" : "+s"(some));   // (lanes read its words next: more than the two steps behind which both_good's were not always right)
+    const unsigned long long some = __ballot(count >= low && lane < p.sequences);
     const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0));
     const unsigned long long one = __ballot(count >= low && lane < p.sequences && rank == tile - above);
     lo = __builtin_amdgcn_readfirstlane(one && low ? __builtin_ctzll(one) : 0);
