@@ -74,7 +74,7 @@ struct AttentionP {
   const int *qStarts, *kStarts;
   int sequences, each, eachKeys;         // without starts: queries and keys of a sequence
   int D, G, heads, keyHeads, N, M, causal;
-  int tiles, slices, vector;             // vector: outputs may be stored four values at a time
+  int slices, vector;                    // vector: outputs may be stored four values at a time
   FastDiv byG, byTiles, bySequences;     // (tiles of a sequence, sequences: without starts)
   float scale, c;                        // c = scale log2 e
 };
