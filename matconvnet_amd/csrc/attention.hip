@@ -1536,7 +1536,7 @@ using namespace mcn;
 extern "C" {
 
 size_t mcn_attention_workspace_bytes(const mcn_attention_geom* g, int backward) {
-  if (!g || g->D <= 0 || g->heads <= 0 || g->keyHeads <= 0 || g->N < 0 || g->M < 0) return 0;
+  if (!g || g->D <= 0 || g->heads <= 0 || g->keyHeads <= 0 || g->heads % g->keyHeads || g->N < 0 || g->M < 0) return 0;   // (refused by the calls)
   return plan_of(g, backward != 0).bytes;
 }
 
