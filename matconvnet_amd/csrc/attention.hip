@@ -801,7 +801,11 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
   const float negL = live ? negative_sum<V>(p.logSums[position * p.heads + column], p.scale) : 0.f;
   float rest = 0.f;
   if (!p.dq.data && !p.dk.data) {   // (dv needs the log sums alone)
-    if (live && lane < 32 && !share0) p.statL[(long long)column * p.N + position] = negL;
+    if (live && lane < 32 && !share0) {
+      const long long at = (long long)column * p.N + position;
+      p.statL[at] = negL;
+      p.statD[at] = negDelta;   // (what dk is made of and left out of)
+    }
     return;
   }
   const char* keys = p.k.data + (long long)span.k0 * p.k.position + head * p.k.head;
@@ -1059,7 +1063,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
   if (tiles) bring_tile(lds);
-  bool edges = false, before = true;
+  bool edges = false, beforeK = true, beforeV = true;
   int turn = 0, i0 = last;   // the tile that is due: its buffer, its first position
   for (int t = 0; t < tiles; ++t) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -1072,7 +1076,8 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     const int i = i0 + share0;
     if (p.causal && !edges && i < all) {
       edges = true;
-      before = all_finite(dk) && all_finite(dv);
+      beforeK = all_finite(dk);
+      beforeV = all_finite(dv);
     }
     if (i + 32 > some && i < span.n)
       dkv_tile<V, DW, sizeof(V) == 2 && (DW == 96 || (DW == 64 && NS == 2))>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, (const float*)(from + 2 * tileBytes) + share0,
@@ -1106,16 +1111,18 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
         dv[d][r] += room[(values + 16 * d + r) * 64];
       }
   }
-  // (rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN)
+  // (rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN; dk and dv each by itself: neither's bits
+  // depend on whether the other is asked for)
   if (p.causal) {
-    const bool good = !before || (all_finite(dk) && all_finite(dv));
-    if (__any(!good)) {
-      if (!good) {
+    const bool goodK = !p.dk.data || !beforeK || all_finite(dk), goodV = !p.dv.data || !beforeV || all_finite(dv);
+    if (__any(!goodK || !goodV)) {
 #pragma unroll
-        for (int d = 0; d < DW / 32; ++d)
+      for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
-      }
+        for (int r = 0; r < 16; ++r) {
+          if (!goodK) dk[d][r] = 0.f;
+          if (!goodV) dv[d][r] = 0.f;
+        }
       const char* keyRow = p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head;
       const char* valueRow = p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head;
 #pragma unroll 1
@@ -1127,9 +1134,9 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
           const float negL = statL[(long long)h * p.N + i];
           const float e = probability<V>((starts_at_sum<V>() ? negL : 0.f) + row_product<V, DW>(keyRow, query, p.D, lane), negL, p.c);
           const float f = e * (statD[(long long)h * p.N + i] + row_product<V, DW>(valueRow, der, p.D, lane));
-          if (good || i < firstOf) continue;
-          add_row<V, DW>(dv, der, as_operand<V>(e), p.D, lane);
-          add_row<V, DW>(dk, query, as_operand<V>(f), p.D, lane);
+          if (i < firstOf) continue;
+          if (!goodV) add_row<V, DW>(dv, der, as_operand<V>(e), p.D, lane);
+          if (!goodK) add_row<V, DW>(dk, query, as_operand<V>(f), p.D, lane);
         }
     }
   }

@@ -1,0 +1,52 @@
+"""Derivatives of attention one by one: what is not asked for has no part in the others, whatever the workspace holds."""
+import itertools
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+class Filled:
+    """A workspace whose memory holds `value` ahead of every call"""
+
+    def __init__(self, value):
+        self.value = value
+
+    def get(self, nbytes):
+        self.room = torch.full(((int(nbytes) + 3) // 4 + 4,), self.value, device="cuda")
+        return self.room.data_ptr(), int(nbytes)
+
+
+def make(n, heads, keyHeads, D, dtype, seed):
+    r = torch.Generator(device="cuda")
+    r.manual_seed(seed)
+    normal = lambda *s: torch.randn(s, generator=r, device="cuda")
+    return [normal(n, h, D).to(dtype) for h in (heads, keyHeads, keyHeads, heads)]
+
+
+def same(a, b):
+    """The same bits (of a NaN: that it is one)"""
+    return torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value", [math.nan, math.inf, 3e38])
+@pytest.mark.parametrize("causal", [True, False])
+def test_each_alone_in_a_workspace_of_anything(capi, causal, value, dtype):
+    """The bits of the call that makes all three; with a query behind the last keys that is not finite as well, which those keys do not see"""
+    n = 200
+    for D, heads, keyHeads, bad in ((128, 4, 2, False), (64, 2, 2, False), (128, 4, 1, True), (75, 2, 1, True)):
+        q, k, v, dy = make(n, heads, keyHeads, D, dtype, D)
+        if bad:
+            dy[150, :, 3] = math.inf
+        how = dict(causal=causal)
+        y, sums = capi.attention_forward(q, k, v, **how)
+        full = capi.attention_backward(q, k, v, y, sums, dy, **how)
+        for want in itertools.product([True, False], repeat=3):
+            got = capi.attention_backward(q, k, v, y, sums, dy, want=want, ws=Filled(value), **how)
+            for name, g, f in zip(("dq", "dk", "dv"), got, full):
+                assert g is None or same(g, f), (D, heads, keyHeads, bad, want, name)
+        if bad and causal:
+            assert bool(torch.isfinite(full[2][151:]).all())
