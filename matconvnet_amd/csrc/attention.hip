@@ -53,7 +53,7 @@ __device__ __forceinline__ bool finite(float v) { return (float_bits(v) & 0x7f80
 
 // the other half's value of the 64 lanes (lane ^ 32)
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, kWave); }
-// whether both lanes of a row (or key) find it good.  (As numbers: a lane's own bit of a ballot takes a 64-bit shift by the lane, whose result was
+// Whether both lanes of a row (or key) find it good.  (As numbers: a lane's own bit of a ballot takes a 64-bit shift by the lane, whose result was
 // wrong in half of a wavefront now and then where the compiler kept the amount in the last register that a wavefront has, v255 in dq; the slow
 // sums behind the loop hid that but for their time.)
 __device__ __forceinline__ bool both_good(bool good) {
@@ -268,6 +268,26 @@ __device__ __forceinline__ float row_product(const char* a, const char* b, int D
 #pragma unroll 1
   for (int k = 0; k < Tile<V, DW>::steps; ++k) s += Matrix<V>::dot(chunk_of<V>(a, 2 * k + (lane >> 5), D, true), chunk_of<V>(b, 2 * k + (lane >> 5), D, true));
   return s + other_half(s);
+}
+// The first (LAST: the last) row of [from, to) that holds what is not finite; none: behind (ahead of) all.  All lanes look, some rows at a time.
+__device__ __forceinline__ bool two_finite(unsigned v) { return (v & 0x7f800000u) != 0x7f800000u && (v & 0x7f80u) != 0x7f80u; }
+template <class V, int DW, bool LAST>
+__device__ __forceinline__ int bad_row(const char* rows, long long pitch, int D, int from, int to, int lane) {
+  constexpr int chunks = Tile<V, DW>::chunks, step = 64 / chunks;
+#pragma unroll 1
+  for (int j = 0; j < to - from; j += step) {
+    const int at = j + lane / chunks, row = LAST ? to - 1 - at : from + at;
+    const uintx4 v = chunk_of<V>(rows + row * pitch, lane % chunks, D, at < to - from);
+    bool good = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) good = good && (sizeof(V) == 2 ? two_finite(v[e]) : finite(bits_float(v[e])));
+    const unsigned long long bad = __ballot(!good);
+    if (bad) {
+      const int found = j + __builtin_ctzll(bad) / chunks;
+      return LAST ? to - 1 - found : from + found;
+    }
+  }
+  return LAST ? -1 : 0x7fffffff;
 }
 template <class V>
 __device__ __forceinline__ float as_operand(float v) { return sizeof(V) == 2 ? bits_float((unsigned)round_bf16(v) << 16) : v; }
@@ -553,7 +573,6 @@ __global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_
   float most = -INFINITY, sum = 0.f;
   if (begin < end) bring_tile(lds, end - begin);
   int turn = 0;
-  bool edges = false, before = true;   // tiles that not all rows see have begun; whether the row was finite then
   for (int j0 = begin; j0 < end; j0 += KT) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     char* from = lds + turn * 2 * tileBytes;
@@ -563,10 +582,6 @@ __global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_
       if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
     const int j = j0 + share0;
-    if (p.causal && !edges && j + 32 * KB > std::min(all, end)) {
-      edges = true;
-      before = all_finite(o);
-    }
     if (j < std::min(some, end))
       forward_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, o, most, sum, j, std::min(limit, end),
                               j + 32 * KB > std::min(all, end), p.c, lane);
@@ -597,12 +612,23 @@ __global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f + room[(16 * d + r) * 64] * f1;
   }
-  // A key that a row does not see has p = 0, but 0 times an infinity or a NaN of its values is NaN: a row that the tiles which not all rows see
-  // have made not finite is added up key by key, over those it sees; the others keep what they have.
+  // A key that a row does not see has p = 0, but 0 times an infinity or a NaN of its values is NaN.  A row that is not finite, and that some key of the
+  // tiles it walked which it does not see, and none that it sees, may have made so, is added up key by key over those it sees; the others keep
+  // what they have.  (Found out behind the loop, from the values themselves: what the loop would have to note on the way takes registers of
+  // it, and is lost where two wavefronts share a block.)
   if (p.causal) {
-    const bool good = !before || all_finite(o);
-    if (__any(!good)) {
-      if (!good) {
+    bool mend = live && !all_finite(o);
+    const int last = std::min(end, some + 32 * KB - 1);   // behind the last key of these tiles
+    if (__any(mend)) {   // (all lanes look)
+      const int row = bad_row<V, DW, true>(values, p.v.position, p.D, std::max(begin, all), last, lane);
+      mend = mend && row >= limit;
+    }
+    if (__any(mend)) {
+      const int row = bad_row<V, DW, false>(values, p.v.position, p.D, begin, last, lane);
+      mend = mend && row >= limit;
+    }
+    if (__any(mend)) {
+      if (mend) {
 #pragma unroll
         for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
@@ -613,7 +639,7 @@ __global__ __launch_bounds__(64 * NB * NS, NB * NS == 1 ? 1 : 2) void attention_
 #pragma unroll 1
       for (int j = begin; j < std::min(some, end); ++j) {
         const float e = power2(row_product<V, DW>(query, keys + (long long)j * p.k.position, p.D, lane) * p.c - shift);
-        if (!good && j < limit) add_row<V, DW>(o, values + (long long)j * p.v.position, as_operand<V>(e), p.D, lane);
+        if (mend && j < limit) add_row<V, DW>(o, values + (long long)j * p.v.position, as_operand<V>(e), p.D, lane);
       }
     }
   }
@@ -828,7 +854,6 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
   if (end > 0) bring_tile(lds, end);
   int turn = 0;
-  bool edges = false, before = true;
   for (int j0 = 0; j0 < end; j0 += KT) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     char* from = lds + turn * 2 * tileBytes;
@@ -838,10 +863,6 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       if (j0 + KT < end) bring_tile(at, end - j0 - KT);
     };
     const int j = j0 + share0;
-    if (p.causal && !edges && j + 32 * KB > std::min(all, end)) {
-      edges = true;
-      before = all_finite(dq);
-    }
     if (j < std::min(some, end))
       dq_tile<V, DW, KB>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, to, bring_next, q, dO, dq, rest, negL, negDelta, j,
                          limit, std::min(some, end), j + 32 * KB > std::min(all, end), p.c, lane);
@@ -875,11 +896,20 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
     p.statD[at] = negDelta - rest;
   }
   if (!p.dq.data) return;
-  // (as in the forward pass: what is not finite is added up over the keys that a row sees)
+  // (as in the forward pass, with the keys in the place of the values)
   if (p.causal) {
-    const bool good = !before || all_finite(dq);
-    if (__any(!good)) {
-      if (!good) {
+    bool mend = live && !all_finite(dq);
+    const int last = std::min(end, some + 32 * KB - 1);
+    if (__any(mend)) {
+      const int row = bad_row<V, DW, true>(keys, p.k.position, p.D, all, last, lane);
+      mend = mend && row >= limit;
+    }
+    if (__any(mend)) {
+      const int row = bad_row<V, DW, false>(keys, p.k.position, p.D, 0, last, lane);
+      mend = mend && row >= limit;
+    }
+    if (__any(mend)) {
+      if (mend) {
 #pragma unroll
         for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
@@ -892,7 +922,7 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
         const char* key = keys + (long long)j * p.k.position;
         const float e = probability<V>((starts_at_sum<V>() ? negL : 0.f) + row_product<V, DW>(query, key, p.D, lane), negL, p.c) *
                         (negDelta + row_product<V, DW>(der, values + (long long)j * p.v.position, p.D, lane));
-        if (!good && j < limit) add_row<V, DW>(dq, key, e, p.D, lane);
+        if (mend && j < limit) add_row<V, DW>(dq, key, e, p.D, lane);
       }
     }
   }
@@ -1063,7 +1093,6 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
   if (tiles) bring_tile(lds);
-  bool edges = false, beforeK = true, beforeV = true;
   int turn = 0, i0 = last;   // the tile that is due: its buffer, its first position
   for (int t = 0; t < tiles; ++t) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -1074,11 +1103,6 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
       if (t + 1 < tiles) bring_tile(at);
     };
     const int i = i0 + share0;
-    if (p.causal && !edges && i < all) {
-      edges = true;
-      beforeK = all_finite(dk);
-      beforeV = all_finite(dv);
-    }
     if (i + 32 > some && i < span.n)
       dkv_tile<V, DW, sizeof(V) == 2 && (DW == 96 || (DW == 64 && NS == 2))>(from + share0 * T::rowBytes, from + tileBytes + share0 * T::rowBytes, (const float*)(from + 2 * tileBytes) + share0,
                       (const float*)(from + 2 * tileBytes + statBytes) + share0, to, bring_next, k, v, dk, dv, i, span.n, firstOf, i < all || i + 32 > span.n, p.c,
@@ -1111,17 +1135,34 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
         dv[d][r] += room[(values + 16 * d + r) * 64];
       }
   }
-  // (rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN; dk and dv each by itself: neither's bits
-  // depend on whether the other is asked for)
+  // Rows that do not see a key have p = ds = 0, which times an infinity or a NaN of theirs is NaN: as in the forward pass, with the queries for dk and the
+  // outputs' derivatives for dv.  (Each by itself: neither's bits depend on whether the other is asked for.)
   if (p.causal) {
-    const bool goodK = !p.dk.data || !beforeK || all_finite(dk), goodV = !p.dv.data || !beforeV || all_finite(dv);
-    if (__any(!goodK || !goodV)) {
+    const auto to_mend = [&](const floatx16 (&sums)[DW / 32], const char* rows, const Tensor3& t) __attribute__((always_inline)) {
+      bool mend = live && !all_finite(sums);
+      if (!__any(mend)) return false;
+      bool unseen = false, seen = false;
+#pragma unroll 1
+      for (int h = 0; h < heads; ++h) {
+        const int row = bad_row<V, DW, false>(rows + h * t.head, t.position, p.D, std::max(0, some - 31), std::min(span.n, all), lane);
+        unseen = unseen || row < firstOf;
+      }
+      mend = mend && unseen;
+#pragma unroll 1
+      for (int h = 0; h < heads && __any(mend && !seen); ++h) {
+        const int row = bad_row<V, DW, true>(rows + h * t.head, t.position, p.D, std::max(0, some), span.n, lane);
+        seen = seen || row >= std::max(0, firstOf);
+      }
+      return mend && !seen;
+    };
+    const bool mendK = p.dk.data && to_mend(dk, queries, p.q), mendV = p.dv.data && to_mend(dv, ders, p.dO);
+    if (__any(mendK || mendV)) {
 #pragma unroll
       for (int d = 0; d < DW / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          if (!goodK) dk[d][r] = 0.f;
-          if (!goodV) dv[d][r] = 0.f;
+          if (mendK) dk[d][r] = 0.f;
+          if (mendV) dv[d][r] = 0.f;
         }
       const char* keyRow = p.k.data + (long long)(span.k0 + (live ? key : 0)) * p.k.position + head * p.k.head;
       const char* valueRow = p.v.data + (long long)(span.k0 + (live ? key : 0)) * p.v.position + head * p.v.head;
@@ -1135,8 +1176,8 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
           const float e = probability<V>((starts_at_sum<V>() ? negL : 0.f) + row_product<V, DW>(keyRow, query, p.D, lane), negL, p.c);
           const float f = e * (statD[(long long)h * p.N + i] + row_product<V, DW>(valueRow, der, p.D, lane));
           if (i < firstOf) continue;
-          if (!goodV) add_row<V, DW>(dv, der, as_operand<V>(e), p.D, lane);
-          if (!goodK) add_row<V, DW>(dk, query, as_operand<V>(f), p.D, lane);
+          if (mendV) add_row<V, DW>(dv, der, as_operand<V>(e), p.D, lane);
+          if (mendK) add_row<V, DW>(dk, query, as_operand<V>(f), p.D, lane);
         }
     }
   }
