@@ -1263,25 +1263,26 @@ __global__ __launch_bounds__(256) void attention_pack(PackP p) {
   }
 }
 
-// ------------------------------------------------------------------------------------------ rows of no sequence
+// ------------------------------------------------------------------------------------------ rows that are zero
 
 struct ClearP {
   char* data[4];
   long long position[4], head[4];   // strides in bytes
   const int* starts[4];
   int positions[4], heads[4], width[4], size[4];   // (width: values of a head)
-  int n, sequences;
+  int n, sequences, inside;
 };
 
-// Zeros for the rows before the first sequence's and behind the last one's
+// Zeros for the rows before the first sequence's and behind the last one's; inside: for those of the sequences (without starts: all)
 __global__ __launch_bounds__(256) void attention_clear(ClearP p) {
   for (int t = 0; t < p.n; ++t) {
-    const int first = clamped(p.starts[t][0], p.positions[t]), last = std::max(first, clamped(p.starts[t][p.sequences], p.positions[t]));
-    const long long rows = first + p.positions[t] - last, each = (long long)p.heads[t] * p.width[t];
+    const int first = p.starts[t] ? clamped(p.starts[t][0], p.positions[t]) : 0;
+    const int last = p.starts[t] ? std::max(first, clamped(p.starts[t][p.sequences], p.positions[t])) : p.positions[t];
+    const long long rows = p.inside ? last - first : first + p.positions[t] - last, each = (long long)p.heads[t] * p.width[t];
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * each; i += (long long)gridDim.x * 256) {
       const long long r = i / each;
       const int within = (int)(i % each), head = within / p.width[t], d = within % p.width[t];
-      char* at = p.data[t] + (r < first ? r : last + r - first) * p.position[t] + head * p.head[t];
+      char* at = p.data[t] + (p.inside ? first + r : r < first ? r : last + r - first) * p.position[t] + head * p.head[t];
       if (p.size[t] == 4) ((unsigned*)at)[d] = 0u;
       else ((unsigned short*)at)[d] = 0;
     }
@@ -1554,9 +1555,10 @@ struct Clear {
     p.width[i] = width;
     p.size[i] = size;
   }
-  int run(const char* who, hipStream_t s, const mcn_attention_geom* g) {
+  int run(const char* who, hipStream_t s, const mcn_attention_geom* g, bool inside = false) {
     if (!p.n) return MCN_SUCCESS;
     p.sequences = g->sequences;
+    p.inside = inside;
     KernelTimer timer("attention_clear", s);
     hipLaunchKernelGGL(attention_clear, dim3(256), dim3(256), 0, s, p);
     return check_launch(who);
@@ -1632,8 +1634,19 @@ int mcn_attention_backward(mcn_stream_t stream, const mcn_attention_geom* g, con
   int rc = check_geom(who, g);
   if (!rc) rc = check_starts(who, g, queryStarts, keyStarts);
   const bool wantQ = derQ && derQ->data, wantK = derK && derK->data, wantV = derV && derV->data;
-  if (rc || g->D == 0 || g->heads == 0 || (g->sequences == 0 && !(g->clear && queryStarts)) || (g->N == 0 && g->M == 0) || (!wantQ && !wantK && !wantV)) return rc;
+  if (rc || g->D == 0 || (g->sequences == 0 && !(g->clear && queryStarts)) || (g->N == 0 && g->M == 0) || (!wantQ && !wantK && !wantV)) return rc;
   const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
+  if (g->heads == 0) {   // no query sees the keys
+    Clear clear;
+    const mcn_heads* ders[2] = {wantK ? derK : nullptr, wantV ? derV : nullptr};
+    for (int i = 0; i < 2 && g->keyHeads && g->M; ++i) {
+      if (!ders[i]) continue;
+      rc = check_heads(who, i ? "values' derivative" : "keys' derivative", ders[i], g->keyHeads, g->M, g->D, size, true);
+      if (rc) return rc;
+      clear.add(in_bytes(ders[i], size), g->clear ? nullptr : keyStarts, g->M, g->keyHeads, g->D, size);
+    }
+    return clear.run(who, as_stream(stream), g, true);
+  }
   if (g->N) {
     rc = check_heads(who, "queries", q, g->heads, g->N, g->D, size, false);
     if (!rc) rc = check_heads(who, "output", o, g->heads, g->N, g->D, size, false);

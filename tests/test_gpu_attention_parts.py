@@ -50,3 +50,28 @@ def test_each_alone_in_a_workspace_of_anything(capi, causal, value, dtype):
                 assert g is None or same(g, f), (D, heads, keyHeads, bad, want, name)
         if bad and causal:
             assert bool(torch.isfinite(full[2][151:]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_keys_that_no_head_asks_for(capi, dtype):
+    """No query heads: the derivatives of keys and values are zero, of the sequences' rows or with fresh outputs of all"""
+    M, keyHeads, D = 50, 3, 24
+    q = torch.zeros(40, 0, D, dtype=dtype, device="cuda")
+    k, v = [torch.randn(M, keyHeads, D, device="cuda").to(dtype) for _ in range(2)]
+    qs, ks = torch.tensor([3, 10, 30], dtype=torch.int32, device="cuda"), torch.tensor([5, 20, 41], dtype=torch.int32, device="cuda")
+    for how in (dict(), dict(sequences=2), dict(q_starts=qs, k_starts=ks)):
+        y, sums = capi.attention_forward(q, k, v, **how)
+        assert y.shape == q.shape and sums.numel() == 0
+        for out in (None, [torch.empty_like(q)] + [torch.full_like(t, 7.0) for t in (k, v)]):
+            if out is None:     # (what a fresh tensor is made in holds something)
+                rooms = [torch.full_like(t, 9.0) for t in (k, v)]
+                del rooms
+            dq, dk, dv = capi.attention_backward(q, k, v, y, sums, torch.empty_like(q), out=out, **how)
+            assert dq.shape == q.shape
+            for t in (dk, dv):
+                inside = torch.ones(M, dtype=torch.bool, device="cuda")
+                if "q_starts" in how and out is not None:
+                    inside[:5] = inside[41:] = False
+                assert bool((t[inside] == 0).all()) and bool((t[~inside] == 7.0).all())
+        _, dk, none = capi.attention_backward(q, k, v, y, sums, torch.empty_like(q), want=(False, True, False), **how)
+        assert none is None and bool((dk == 0).all())
