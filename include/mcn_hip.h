@@ -616,7 +616,7 @@ MCN_API int mcn_hnorm_backward(mcn_stream_t stream, const mcn_hnorm_geom* g, con
    see); where what it does see makes it not finite in one channel, others may be not finite as well.  Rows of no sequence (before the
    first one's, behind the last one's) are left as they were, or with clear != 0 set to zero.
    q, k, v, o and all derivatives are of dataType.  logSums is N x heads, a position's heads side by side.  scale 0: 1/sqrt(D),
-   otherwise 1e-30 to 1e30.  D at most 128.
+   otherwise 1e-30 to 1e30.  D at most 128 (0: no log sums).
    backward: all that is asked for (derQ, derK, derV; NULL or of null data: not made) is fully overwritten for all positions of sequences; o and logSums
    as the forward call left them.  Derivatives of heads that share keys are sums without atomics: the same bits every time.
    bfloat16: products of the bfloat16 values in single precision; exp(s - logSums) and, for derK, the scores' derivatives are rounded to

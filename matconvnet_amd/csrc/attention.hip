@@ -1595,6 +1595,7 @@ int mcn_attention_forward(mcn_stream_t stream, const mcn_attention_geom* g, cons
   const char* who = "mcn_attention_forward";
   int rc = check_geom(who, g);
   if (!rc) rc = check_starts(who, g, queryStarts, keyStarts);
+  if (!rc && g->D == 0 && g->N && g->heads && logSums) rc = fail(MCN_ILLEGAL_ARGUMENT, "%s: log sums of heads of no channels", who);
   if (rc || g->D == 0 || g->N == 0 || g->heads == 0 || (g->sequences == 0 && !(g->clear && queryStarts))) return rc;
   const int size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
   rc = check_heads(who, "queries", q, g->heads, g->N, g->D, size, false);
