@@ -1050,7 +1050,7 @@ def attention_forward(q, k, v, q_starts=None, k_starts=None, sequences=None, cau
 def attention_backward(q, k, v, y, log_sums, dy, q_starts=None, k_starts=None, sequences=None, causal=False, scale=None, want=(True, True, True),
                        out=None, ws=None):
     """(dq, dk, dv) of attention_forward from what it left in y and log_sums; those not wanted are None.  out: the tensors they are
-    written to, whose rows of no sequence are left alone (fresh ones hold zeros there)."""
+    written to, or None for fresh ones; their rows of no sequence are left alone (fresh ones hold zeros there)."""
     g = _attention_geom(q, k, v, sequences, q_starts, k_starts, causal, scale)
     for name, t in (("y", y), ("dy", dy)):
         if t.shape != q.shape or t.dtype != q.dtype:
@@ -1059,8 +1059,14 @@ def attention_backward(q, k, v, y, log_sums, dy, q_starts=None, k_starts=None, s
     if log_sums.numel() != g.N * g.heads:
         raise ValueError("log_sums does not have one value per query and head")
     g.clear = int(out is None)
-    d = [t if w else None for w, t in zip(want, _outs("dq dk dv", out, q, k, v))] if out is not None else [
-        _alike(x) if w else None for w, x in zip(want, (q, k, v))]
+    if out is None:
+        d = [_alike(x) if w else None for w, x in zip(want, (q, k, v))]
+    else:
+        out = list(out)
+        d = [t if w else None for w, t in zip(want, _outs("dq dk dv", out, q, k, v))]
+        for t, given in zip(d, out):
+            if t is not None and given is None and q_starts is not None:
+                t.zero_()       # (a fresh one among the caller's)
     wp, wn, held = _scratch(ws, q, lib().mcn_attention_workspace_bytes(C.byref(g), 1))
     hdq, hdk, hdv, hy, hq, hk, hv, hdy = _heads("dq dk dv y q k v dy", d[0], d[1], d[2], y, q, k, v, dy)
     check(lib().mcn_attention_backward(stream(), C.byref(g), hdq, hdk, hdv, hy, ptr(log_sums), hq, hk, hv, hdy, ptr(q_starts), ptr(k_starts), wp, wn))

@@ -75,3 +75,24 @@ def test_keys_that_no_head_asks_for(capi, dtype):
                 assert bool((t[inside] == 0).all()) and bool((t[~inside] == 7.0).all())
         _, dk, none = capi.attention_backward(q, k, v, y, sums, torch.empty_like(q), want=(False, True, False), **how)
         assert none is None and bool((dk == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_some_outputs_of_the_callers_and_some_fresh(capi, dtype):
+    """Rows of no sequence: left alone in the caller's tensors, zero in fresh ones beside them"""
+    q, k, v, dy = make(60, 4, 2, 32, dtype, 1)
+    s = torch.tensor([7, 20, 45], dtype=torch.int32, device="cuda")
+    how = dict(q_starts=s, k_starts=s, causal=True)
+    y, sums = capi.attention_forward(q, k, v, **how)
+    full = capi.attention_backward(q, k, v, y, sums, dy, **how)
+    inside = torch.zeros(60, dtype=torch.bool, device="cuda")
+    inside[7:45] = True
+    for given in itertools.product([True, False], repeat=3):
+        rooms = [torch.full_like(t, 9.0) for t in (q, k, v)]     # (so that the memory which fresh ones get holds something)
+        del rooms
+        out = [torch.full_like(t, 7.0) if w else None for w, t in zip(given, (q, k, v))]
+        got = capi.attention_backward(q, k, v, y, sums, dy, out=out, **how)
+        for mine, g, o, f in zip(given, got, out, full):
+            assert (g is o) == mine and torch.equal(g[inside], f[inside]) and bool((g[~inside] == (7.0 if mine else 0.0)).all())
+    only = capi.attention_backward(q, k, v, y, sums, dy, want=(False, True, False), out=[None, None, None], **how)
+    assert only[0] is None and only[2] is None and torch.equal(only[1], full[1])
