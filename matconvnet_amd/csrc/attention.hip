@@ -1238,19 +1238,20 @@ struct PackP {
   const char* from[5];
   char* to[5];
   long long position[5], head[5], items[5];   // (strides in bytes) heads of all positions
-  int heads[5];
+  int positions[5];
   int D, chunks;
 };
 
-// Heads of any D and strides, laid one behind the other, each a whole number of 16 bytes, zero behind D: a thread per 16 bytes
+// Heads of any D and strides, each a whole number of 16 bytes, zero behind D: a thread per 16 bytes.  A head's positions lie one behind the other,
+// so that a tile's rows are near each other however many heads there are (their offsets and the tile's size are 32-bit numbers).
 template <class V>
 __global__ __launch_bounds__(256) void attention_pack(PackP p) {
   constexpr int W = 16 / sizeof(V);
   const int which = blockIdx.y;
   const long long all = p.items[which] * p.chunks;
   for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < all; t += (long long)gridDim.x * 256) {
-    const long long item = t / p.chunks, position = item / p.heads[which];
-    const int chunk = (int)(t % p.chunks), head = (int)(item % p.heads[which]);
+    const long long item = t / p.chunks, head = item / p.positions[which];
+    const int chunk = (int)(t % p.chunks), position = (int)(item % p.positions[which]);
     const V* from = (const V*)(p.from[which] + position * p.position[which] + head * p.head[which]) + chunk * W;
     V v[W];
 #pragma unroll
@@ -1446,8 +1447,8 @@ int place(const char* who, hipStream_t s, const mcn_attention_geom* g, const Pla
     p.position[packs] = o.t->position * l.size;
     p.head[packs] = o.t->head * l.size;
     p.items[packs] = (long long)o.positions * o.heads;
-    p.heads[packs] = std::max(1, o.heads);
-    *to[i] = {workspace + at, (long long)p.chunks * 16 * o.heads, (long long)p.chunks * 16};
+    p.positions[packs] = o.positions;
+    *to[i] = {workspace + at, p.chunks * 16ll, p.chunks * 16ll * o.positions};
     at += packed_bytes(o.positions, o.heads, g->D, l.size);
     ++packs;
   }
