@@ -162,13 +162,13 @@ __global__ __launch_bounds__(256) void clip_scale(float* __restrict__ norm, cons
   else scale_run<false>(t.out[k], t.der[k], first, last, f);
 }
 
-__global__ __launch_bounds__(256) void clip_join(float* __restrict__ norm, float* __restrict__ factor, const double* __restrict__ partials, int parts,
+__global__ __launch_bounds__(256) void clip_join(float* __restrict__ norm, double* __restrict__ factor, const double* __restrict__ partials, int parts,
                                                  double scale, double most) {
   __shared__ double slots[4];
   const double n = join_norm(partials, parts, fabs(scale), slots);
   if (threadIdx.x) return;
   if (norm) *norm = (float)n;
-  if (factor) *factor = (float)(scale * factor_of(n, most));
+  if (factor) *factor = n > most ? scale * factor_of(n, most) : (double)(float)scale;   // (not clipped: the step's own scale)
 }
 
 size_t run_of(size_t total) { return std::max(kLeast, (total / kRuns + kLeast - 1) / kLeast * kLeast); }
@@ -274,13 +274,13 @@ int scale_of(const char* who, hipStream_t s, void* const* outs, float* norm, con
 
 // for the solver's step (eltwise.hip): *factor (device) = derScale * factor of the norm of derScale * der
 size_t clip_factor_workspace(size_t count) { return sizes_of(&count, 1).parts * sizeof(double) + 16; }
-int clip_factor(const char* who, hipStream_t s, float* norm, float** factor, const float* der, size_t count, double derScale, double most, void* workspace,
+int clip_factor(const char* who, hipStream_t s, float* norm, double** factor, const float* der, size_t count, double derScale, double most, void* workspace,
                 size_t workspaceBytes) {
   const Sizes z = sizes_of(&count, 1);
   int rc = check_workspace(who, workspace, workspaceBytes, clip_factor_workspace(count));
   if (rc) return rc;
   double* partials = (double*)((char*)workspace + 16);
-  *factor = (float*)workspace;
+  *factor = (double*)workspace;
   const void* ders[1] = {der};
   const int types[1] = {MCN_FLOAT};
   rc = squares_of_all(who, s, partials, ders, &count, types, 1, z.run);
@@ -314,7 +314,7 @@ int mcn_gradient_norm(mcn_stream_t stream, float* norm, const void* const* ders,
   rc = squares_of_all(who, s, (double*)workspace, ders, counts, dataTypes, n, z.run);
   if (rc) return rc;
   KernelTimer timer("clip_join", s);
-  hipLaunchKernelGGL(clip_join, dim3(1), dim3(256), 0, s, norm, (float*)nullptr, (const double*)workspace, (int)z.parts, 1.0, 0.0);
+  hipLaunchKernelGGL(clip_join, dim3(1), dim3(256), 0, s, norm, (double*)nullptr, (const double*)workspace, (int)z.parts, 1.0, 0.0);
   return check_launch(who);
 }
 
@@ -334,7 +334,7 @@ int mcn_clip_gradients(mcn_stream_t stream, void* const* outs, float* norm, cons
   const Sizes z = sizes_of(counts, n);
   if (z.parts == 0) {   // nothing but empty tensors
     if (!norm) return MCN_SUCCESS;
-    hipLaunchKernelGGL(clip_join, dim3(1), dim3(256), 0, as_stream(stream), norm, (float*)nullptr, (const double*)nullptr, 0, 1.0, 0.0);
+    hipLaunchKernelGGL(clip_join, dim3(1), dim3(256), 0, as_stream(stream), norm, (double*)nullptr, (const double*)nullptr, 0, 1.0, 0.0);
     return check_launch(who);
   }
   rc = check_workspace(who, workspace, workspaceBytes, z.parts * sizeof(double));

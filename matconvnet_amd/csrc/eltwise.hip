@@ -71,15 +71,17 @@ __global__ __launch_bounds__(256) void eltwise_kernel(float* __restrict__ y, con
 
 // SGD with momentum over an arena of parameters: one workgroup per chunk of 1024 elements, every chunk inside one
 // parameter, whose rates come from a table.  Each element goes through the roundings of the three scaled sums the
-// reference performs one parameter at a time.  CLIPPED: the factor of the derivatives is read from the device, where the norm left it.
+// reference performs one parameter at a time.  CLIPPED: the factor of the derivatives is read from the device, where the norm left it, and multiplies
+// them in double (derivatives of 1e25 and a largest norm of 1e-20 make a factor below single precision's smallest); a factor that single
+// precision holds gives the bits of a product in single precision.
 template <bool CLIPPED>
 __global__ __launch_bounds__(256) void sgd_momentum_kernel(float* __restrict__ value, float* __restrict__ state,
                                                            const float* __restrict__ der,
                                                            const unsigned short* __restrict__ chunkParam,
                                                            const double* __restrict__ rates, double learningRate,
                                                            double weightDecay, float momentum, float derScale, int nesterov,
-                                                           const float* __restrict__ derFactor) {
-  if (CLIPPED) derScale = *derFactor;
+                                                           const double* __restrict__ derFactor) {
+  const double factor = CLIPPED ? *derFactor : 1.0;
   const int p = chunkParam[blockIdx.x];
   const float lr = (float)(learningRate * rates[2 * p]), decay = (float)(weightDecay * rates[2 * p + 1]);
   if (!(lr > 0.f || decay > 0.f)) return;
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(256) void sgd_momentum_kernel(float* __restrict__ v
   const float4 m = stream_load4((const float4*)state + i);
   float4 vo, mo;
   auto one = [&](float v1, float g1, float m1, float& vOut, float& mOut) {
-    const float t = derScale * g1;
+    const float t = CLIPPED ? (float)(factor * (double)g1) : derScale * g1;
     const float d = t + decay * v1;      // gradient, normalised, plus weight decay
     const float u = momentum * m1;
     const float mNew = u + (-1.f) * d;   // momentum
@@ -197,7 +199,7 @@ int mcn_sgd_momentum(mcn_stream_t stream, float* value, float* state, const floa
   if (rc) return rc;
   KernelTimer timer("sgd_momentum_kernel", as_stream(stream));
   hipLaunchKernelGGL(sgd_momentum_kernel<false>, dim3((unsigned)chunks), dim3(256), 0, as_stream(stream), value, state, der,
-                     chunkParam, rates, learningRate, weightDecay, (float)momentum, (float)derScale, nesterov ? 1 : 0, (const float*)nullptr);
+                     chunkParam, rates, learningRate, weightDecay, (float)momentum, (float)derScale, nesterov ? 1 : 0, (const double*)nullptr);
   return check_launch("mcn_sgd_momentum");
 }
 size_t mcn_sgd_momentum_clipped_workspace_bytes(size_t chunks) { return clip_factor_workspace(chunks * MCN_SGD_CHUNK); }
@@ -210,12 +212,12 @@ int mcn_sgd_momentum_clipped(mcn_stream_t stream, float* value, float* state, co
   int rc = chunks ? check_sgd(who, value, state, der, chunks, chunkParam, rates) : MCN_SUCCESS;
   if (rc) return rc;
   hipStream_t s = as_stream(stream);
-  float* factor;
+  double* factor;
   rc = clip_factor(who, s, norm, &factor, der, chunks * MCN_SGD_CHUNK, derScale, maxNorm, workspace, workspaceBytes);
   if (rc || chunks == 0) return rc;
   KernelTimer timer("sgd_momentum_kernel", s);
   hipLaunchKernelGGL(sgd_momentum_kernel<true>, dim3((unsigned)chunks), dim3(256), 0, s, value, state, der, chunkParam, rates, learningRate,
-                     weightDecay, (float)momentum, 0.f, nesterov ? 1 : 0, (const float*)factor);
+                     weightDecay, (float)momentum, 0.f, nesterov ? 1 : 0, (const double*)factor);
   return check_launch(who);
 }
 int mcn_convert(mcn_stream_t stream, void* dst, int dstType, const void* src, int srcType, size_t n) {

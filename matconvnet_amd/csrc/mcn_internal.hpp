@@ -44,7 +44,7 @@ class KernelTimer {
 
 // The factor that brings derScale * der under the norm `most`, times derScale, on the device (in the workspace); *norm (may be null) the norm.
 size_t clip_factor_workspace(size_t count);
-int clip_factor(const char* who, hipStream_t s, float* norm, float** factor, const float* der, size_t count, double derScale, double most, void* workspace,
+int clip_factor(const char* who, hipStream_t s, float* norm, double** factor, const float* der, size_t count, double derScale, double most, void* workspace,
                 size_t workspaceBytes);
 
 inline hipStream_t as_stream(mcn_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
