@@ -1075,11 +1075,15 @@ def attention_backward(q, k, v, y, log_sums, dy, q_starts=None, k_starts=None, s
 
 class GradientList:
     """Gradients that are clipped together, and where the clipped ones go (None: into their own places): contiguous float32 or bfloat16
-    tensors on one device, none of which overlaps another.  Holds the tensors; made once for those a program keeps."""
+    tensors on one device, none of which overlaps another.  Holds the tensors, which keep their shapes; made once for those a program keeps.
+    Where a tensor's memory has been exchanged (`.data =`, `set_`) since, a call looks the list over again."""
 
     def __init__(self, ders, outs=None):
         self.ders = list(ders)
         self.outs = self.ders if outs is None else list(outs)
+        self._look_over()
+
+    def _look_over(self):
         if len(self.outs) != len(self.ders):
             raise ValueError("there is not one output per gradient")
         self.device = None
@@ -1103,9 +1107,15 @@ class GradientList:
         self.n = n
         self.counts = (C.c_size_t * n)(*[g.numel() for g in self.ders])
         self.types = (C.c_int * n)(*[data_type(g) for g in self.ders])
-        self.der_pointers = (C.c_void_p * n)(*[g.data_ptr() for g in self.ders])
-        self.out_pointers = (C.c_void_p * n)(*[y.data_ptr() for y in self.outs])
+        self.addresses = self._addresses()
+        self.der_pointers = (C.c_void_p * n)(*self.addresses[:n])
+        self.out_pointers = (C.c_void_p * n)(*self.addresses[-n:] if n else [])
         self.workspace_bytes = lib().mcn_clip_workspace_bytes(self.counts, n)
+
+    def _addresses(self):
+        """Of all tensors (50 ns each; clipping where a tensor was would leave it as it is)"""
+        at = _torch().Tensor.data_ptr
+        return list(map(at, self.ders if self.outs is self.ders else self.ders + self.outs))
 
     def _here(self):
         torch = _torch()
@@ -1114,9 +1124,18 @@ class GradientList:
         return torch.empty(1, dtype=torch.float32, device="cuda")
 
 
+def _gradients(given):
+    """A GradientList, of where its tensors are now"""
+    if not isinstance(given, GradientList):
+        return GradientList(given)
+    if given._addresses() != given.addresses:
+        given._look_over()
+    return given
+
+
 def gradient_norm(gradients, ws=None):
     """The norm of a GradientList's (or a list's) gradients together, a one-element device tensor (include/mcn_hip.h: mcn_gradient_norm)."""
-    g = gradients if isinstance(gradients, GradientList) else GradientList(gradients)
+    g = _gradients(gradients)
     norm = g._here()
     wp, wn, held = _scratch(ws, norm, g.workspace_bytes)
     check(lib().mcn_gradient_norm(stream(), ptr(norm), g.der_pointers, g.counts, g.types, g.n, wp, wn))
@@ -1126,7 +1145,7 @@ def gradient_norm(gradients, ws=None):
 def clip_gradients(gradients, max_norm, ws=None):
     """Clips a GradientList's (or, in place, a list's) gradients to a norm of max_norm together; the norm they had, a one-element device
     tensor (include/mcn_hip.h: mcn_clip_gradients)."""
-    g = gradients if isinstance(gradients, GradientList) else GradientList(gradients)
+    g = _gradients(gradients)
     norm = g._here()
     wp, wn, held = _scratch(ws, norm, g.workspace_bytes)
     check(lib().mcn_clip_gradients(stream(), g.out_pointers, ptr(norm), g.der_pointers, g.counts, g.types, g.n, float(max_norm), wp, wn))
