@@ -7,7 +7,7 @@
 // Bound by memory: a head's channels stay in the registers of T lanes between the sum of squares and the output.  A wavefront takes
 // the heads of one position, so that the angles of a position are made once: lane by lane one pair each, the cosines and sines
 // then pass through local memory to the lanes that hold the pair in each head.  Angles are products and sums of doubles, brought to a
-// revolution in double: position 10^6 times frequency 1 keeps all of a single-precision sine.
+// revolution in double, which the sine takes in two parts: position 10^6 times frequency 1 keeps all of a single-precision sine.
 //
 // A lane holds VP pairs, 2 VP channels: the pairs' first channels and their second ones a run of pairs apart, or neighbours.  Channels of
 // no pair are held likewise and not turned.  Heads of any size and address are read four values at a time from wherever they start, what is
@@ -187,10 +187,12 @@ __device__ __forceinline__ void angles(float (*lds)[kMostD / 2], const HnormP& p
     }
     double r = angle * 0.15915494309189533577;   // revolutions
     r -= rint(r);
+    // (half revolutions in two parts: rounded to one the sine near a whole one would be off by up to 9e-8, whatever is left of it)
+    const float half = (float)(2.0 * r), rest = (float)((2.0 * r - (double)half) * 3.14159265358979323846);
     float s, c;
-    sincospif((float)(2.0 * r), &s, &c);
-    lds[0][j] = c;
-    lds[1][j] = s;
+    sincospif(half, &s, &c);
+    lds[0][j] = c - rest * s;
+    lds[1][j] = s + rest * c;
   }
   wave_order();
 }
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(256) void hnorm_join(float* __restrict__ dgq, float
 // chunks of a head: of pairs that turn, and of channels of no pair
 int chunks_of(const HnormP& p, int VP) { return div_up(p.pairs, VP) + div_up(p.D - 2 * p.pairs, 2 * VP); }
 
-// Workgroups: as many as run at once (forward 4 on a CU, backward 2), each walks over positions
+// Workgroups: as many as run at once (forward 4 on a CU, backward 3), each walks over positions
 int groups_of(long long units, int perUnit) {
   return (int)std::max<long long>(1, std::min<long long>((long long)perUnit * std::max(1, device_compute_units()), (units + kWaves - 1) / kWaves));
 }
