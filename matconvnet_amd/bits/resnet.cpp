@@ -221,6 +221,7 @@ ErrorCode ResNet50::setClip(double maxNorm) {
       return VLE_OutOfGPUMemeory;
     }
   }
+  if (clip != maxNorm) dropGraph();   // (which steps with the norm it was captured with)
   clip = maxNorm;
   return VLE_Success;
 }
@@ -290,6 +291,7 @@ ErrorCode ResNet50::losses(double* objective, double* top1Error, double* top5Err
 }
 
 void ResNet50::dropGraph() {
+  if (graphExec) (void)hipStreamSynchronize((hipStream_t)context.getHipHelper().getStream());   // (a replay may be running)
   if (graphExec) (void)hipGraphExecDestroy((hipGraphExec_t)graphExec);
   if (graph) (void)hipGraphDestroy((hipGraph_t)graph);
   graph = graphExec = NULL;

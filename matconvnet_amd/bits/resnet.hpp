@@ -69,7 +69,7 @@ class ResNet50 {
   ErrorCode lossDerivative(double derOutput = 1.0);
   ErrorCode losses(double* objective, double* top1Error, double* top5Error);
   // maxNorm > 0: sgdStep() clips the derivatives of all parameters, taken together, to that norm (it is no part of the reference's solver);
-  // the norm they had is in buffer "gradientNorm" then.  0 (the default): never.
+  // the norm they had is in buffer "gradientNorm" then.  0 (the default): never.  Another norm than before drops a captured graph.
   ErrorCode setClip(double maxNorm);
   // one update of all parameters from the derivatives backward() left (numWorkers = 1), and of the moving averages of
   // the moments from those forward() left

@@ -394,7 +394,8 @@ class ResNet50(_NamedBuffers):
         self._check(self.L.vlh_resnet50_backward(self.h))
 
     def set_clip(self, max_norm):
-        """sgd_step clips the derivatives of all parameters together to this norm (0: never); buffer "gradientNorm" holds what it was."""
+        """sgd_step clips the derivatives of all parameters together to this norm (0: never); buffer "gradientNorm" holds what it was.
+        A graph that was captured with another norm is dropped."""
         self._check(self.L.vlh_resnet50_set_clip(self.h, float(max_norm)))
 
     def sgd_step(self, learning_rate, momentum=0.9, weight_decay=1e-4):
