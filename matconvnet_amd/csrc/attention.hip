@@ -1296,18 +1296,6 @@ constexpr long long kMostThreads = 1ll << 32;   // of a launch
 constexpr size_t kAlign = 256;
 size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-int check_heads(const char* who, const char* what, const mcn_heads* t, int heads, int positions, int D, int size, bool written) {
-  if (!t || !t->data) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null %s", who, what);
-  if ((uintptr_t)t->data % size) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %s is not aligned", who, what);
-  if (t->position < 0 || t->head < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative stride of %s", who, what);
-  if (t->position > (1ll << 31) || t->head > (1ll << 40)) return fail(MCN_UNSUPPORTED, "%s: stride of %s too large", who, what);
-  if (!written) return MCN_SUCCESS;
-  const bool inside = (positions <= 1 || t->position >= (long long)(heads - 1) * t->head + D) && (heads <= 1 || t->head >= D);
-  const bool outside = (heads <= 1 || t->head >= (long long)(positions - 1) * t->position + D) && (positions <= 1 || t->position >= D);
-  if (!inside && !outside) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the heads of %s overlap", who, what);
-  return MCN_SUCCESS;
-}
-
 int check_geom(const char* who, const mcn_attention_geom* g) {
   if (!g) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null geometry", who);
   if (g->dataType != MCN_FLOAT && g->dataType != MCN_BFLOAT16) return fail(MCN_ILLEGAL_ARGUMENT, "%s: unknown data type %d", who, g->dataType);
@@ -1570,12 +1558,6 @@ int check_starts(const char* who, const mcn_attention_geom* g, const int* qStart
   if (!qStarts != !kStarts) return fail(MCN_ILLEGAL_ARGUMENT, "%s: starts of queries or of keys alone", who);
   if (!qStarts && g->sequences && (g->N % g->sequences || g->M % g->sequences))
     return fail(MCN_ILLEGAL_ARGUMENT, "%s: the positions are not %d sequences of one length", who, g->sequences);
-  return MCN_SUCCESS;
-}
-
-int check_workspace(const char* who, const void* workspace, size_t bytes, size_t need) {
-  if (need && (!workspace || bytes < need)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, bytes, need);
-  if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
   return MCN_SUCCESS;
 }
 

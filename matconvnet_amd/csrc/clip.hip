@@ -227,12 +227,6 @@ int check(const char* who, const void* const* ders, const size_t* counts, const 
   return MCN_SUCCESS;
 }
 
-int check_workspace(const char* who, const void* workspace, size_t bytes, size_t need) {
-  if (need && (!workspace || bytes < need)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, bytes, need);
-  if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
-  return MCN_SUCCESS;
-}
-
 template <int ENTRIES>
 int squares_of(const char* who, hipStream_t s, double* partials, const void* const* ders, const size_t* counts, const int* types, int n, size_t run) {
   for (Place at; at.tensor < n;) {

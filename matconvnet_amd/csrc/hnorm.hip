@@ -480,19 +480,6 @@ void choose(hipStream_t s, const HnormP& p, bool wide, bool backward, int groups
   }
 }
 
-int check_heads(const char* who, const char* what, const mcn_heads* t, int heads, int N, int D, int size, bool written) {
-  if (!t || !t->data) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null %s", who, what);
-  if ((uintptr_t)t->data % size) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %s is not aligned", who, what);
-  if (t->position < 0 || t->head < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative stride of %s", who, what);
-  if (t->position > (1ll << 31) || t->head > (1ll << 40)) return fail(MCN_UNSUPPORTED, "%s: stride of %s too large", who, what);
-  if (!written) return MCN_SUCCESS;
-  // the heads of all positions are apart
-  const bool inside = (N <= 1 || t->position >= (long long)(heads - 1) * t->head + D) && (heads <= 1 || t->head >= D);
-  const bool outside = (heads <= 1 || t->head >= (long long)(N - 1) * t->position + D) && (N <= 1 || t->position >= D);
-  if (!inside && !outside) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the heads of %s overlap", who, what);
-  return MCN_SUCCESS;
-}
-
 bool wide_heads(const mcn_heads* t, int VP) { return aligned16(t->data) && t->position % VP == 0 && t->head % VP == 0; }
 
 int check_geom(const char* who, const mcn_hnorm_geom* g) {
@@ -570,8 +557,8 @@ int run(const char* who, hipStream_t s, const mcn_hnorm_geom* g, const Call& c, 
   const bool sums = backward && p.normalise && (dgq || dgk);
   if (sums) {
     const size_t need = (size_t)groups * 2 * p.D * sizeof(float);
-    if (!workspace || workspaceBytes < need) return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, workspaceBytes, need);
-    if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
+    const int rc = check_workspace(who, workspace, workspaceBytes, need);
+    if (rc) return rc;
     p.partials = (float*)workspace;
   }
   {

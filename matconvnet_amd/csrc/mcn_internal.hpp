@@ -51,6 +51,24 @@ inline hipStream_t as_stream(mcn_stream_t s) { return reinterpret_cast<hipStream
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Heads as hnorm.hip and attention.hip take them; `written`: those of all positions have to be apart
+inline int check_heads(const char* who, const char* what, const mcn_heads* t, int heads, int positions, int D, int size, bool written) {
+  if (!t || !t->data) return fail(MCN_ILLEGAL_ARGUMENT, "%s: null %s", who, what);
+  if ((uintptr_t)t->data % size) return fail(MCN_ILLEGAL_ARGUMENT, "%s: %s is not aligned", who, what);
+  if (t->position < 0 || t->head < 0) return fail(MCN_ILLEGAL_ARGUMENT, "%s: negative stride of %s", who, what);
+  if (t->position > (1ll << 31) || t->head > (1ll << 40)) return fail(MCN_UNSUPPORTED, "%s: stride of %s too large", who, what);
+  if (!written) return MCN_SUCCESS;
+  const bool inside = (positions <= 1 || t->position >= (long long)(heads - 1) * t->head + D) && (heads <= 1 || t->head >= D);
+  const bool outside = (heads <= 1 || t->head >= (long long)(positions - 1) * t->position + D) && (positions <= 1 || t->position >= D);
+  if (!inside && !outside) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the heads of %s overlap", who, what);
+  return MCN_SUCCESS;
+}
+inline int check_workspace(const char* who, const void* workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: workspace too small (%zu < %zu bytes)", who, bytes, need);
+  if (!aligned16(workspace)) return fail(MCN_ILLEGAL_ARGUMENT, "%s: the workspace is not 16-byte aligned", who);
+  return MCN_SUCCESS;
+}
+
 inline int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Division of a non-negative 31-bit integer by a run-time constant without the ~35-instruction hardware
