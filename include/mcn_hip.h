@@ -585,10 +585,11 @@ typedef struct mcn_heads {
    pair j is channels j and pairs + j, or with neighbours != 0 channels 2j and 2j + 1; channels from 2*pairs on are not turned, pairs = 0
    turns none.  positions (N x axes, an image's row and column, a video's time, row and column...) and frequencies (axes x pairs: 0
    where an axis does not turn a pair) are doubles on the device: angles are made in double.  multipliers (NULL: ones) are D single-precision
-   values for the queries, D for the keys.  D at most 512.  Either set may have no heads.  yq may be q, yk may be k.
+   values for the queries, D for the keys.  D at most 512.  Either set may have no heads.  yq may be q, yk may be k.  Squares are summed in
+   single precision (channels of 1e19 and more overflow it).
    backward: derQ, derK (NULL or of null data: not made) may be derOutputQ, derOutputK; derMultipliers (with normalise only; NULL: not
-   made) are fully overwritten, their sums taken in one order for one shape on one kind of device; without normalise q and k
-   are not read. */
+   made) are fully overwritten, their sums taken in one order for one shape and alignment on one kind of device; without normalise
+   q and k are not read. */
 typedef struct mcn_hnorm_geom {
   int D, heads, keyHeads, N;
   int pairs, axes;
@@ -611,14 +612,14 @@ MCN_API int mcn_hnorm_backward(mcn_stream_t stream, const mcn_hnorm_geom* g, con
    i has the queries [queryStarts[i], queryStarts[i + 1]) of N and the keys [keyStarts[i], keyStarts[i + 1]) of M (device arrays of
    sequences + 1 ascending numbers, both or neither; NULL: sequences of N / sequences queries and M / sequences keys each).  Either part may be
    empty; starts outside of 0..N or 0..M are taken as the nearest of these.  causal != 0: the queries are the last positions of their
-   sequence, query i of n sees key j of m where j <= i + m - n.  A query that sees no key has o = 0, logSums = -infinity and gives no
-   derivative.  Keys that a query does not see have no part in it, whatever they hold (and queries none in the derivatives of keys they do not
+   sequence, query i of n sees key j of m where j <= i + m - n.  A query that sees no key, or none whose score is not -infinity, has
+   o = 0, logSums = -infinity and gives no derivative.  Keys that a query does not see have no part in it, whatever they hold (and queries none in the derivatives of keys they do not
    see); where what it does see makes it not finite in one channel, others may be not finite as well.  Rows of no sequence (before the
    first one's, behind the last one's) are left as they were, or with clear != 0 set to zero.
    q, k, v, o and all derivatives are of dataType.  logSums is N x heads, a position's heads side by side.  scale 0: 1/sqrt(D),
    otherwise 1e-30 to 1e30.  D at most 128 (0: no log sums).
    backward: all that is asked for (derQ, derK, derV; NULL or of null data: not made) is fully overwritten for all positions of sequences; o and logSums
-   as the forward call left them.  Derivatives of heads that share keys are sums without atomics: the same bits every time.
+   as the forward call left them.  Outputs overlap nothing that the call reads.  Derivatives of heads that share keys are sums without atomics: the same bits every time.
    bfloat16: products of the bfloat16 values in single precision; exp(s - logSums) and, for derK, the scores' derivatives are rounded to
    bfloat16 for the products behind them; for derQ the latter are taken as two bfloat16 values.  o enters the derivatives as it is stored;
    what its rounding puts the scores' derivatives of a row off by is taken out again for derK.  Single precision: products and sums in single precision.

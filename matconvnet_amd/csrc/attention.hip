@@ -18,9 +18,9 @@
 // by the row so that neither reads along a row nor transposing reads across rows meet in a bank (counted: no conflict in any of the kernels).
 //
 // Measured (bfloat16, times of the kernels; operations counted over the pairs that are seen).  One causal sequence of 16384, 32 heads over 8 of
-// 128: forward 2.06 ms, 1070 TFLOP/s; dq 3.49 and dk, dv 4.18 ms, 717 TFLOP/s, 1150 with all products counted that are made (scores and do.v in
-// both kernels, dq's product twice).  32 x 196 positions, 12 heads of 64, not causal: 17, 24 and 22 us.  64 queries, one a sequence, 262144 keys in
-// all, 8 heads of 128: k and v read at 4.3 TB/s (247 us).
+// 128: forward 2.12 ms, 1040 TFLOP/s; dq 3.64 and dk, dv 4.36 ms, 690 TFLOP/s, 1100 with all products counted that are made (scores and do.v in
+// both kernels, dq's product twice).  32 x 196 positions, 12 heads of 64, not causal: 17, 25 and 24 us.  64 queries, one a sequence, 262144 keys in
+// all, 8 heads of 128: k and v read at 4.6 TB/s (233 us).
 #include "mcn_internal.hpp"
 
 #include <algorithm>
@@ -108,8 +108,9 @@ template <> struct Matrix<float> {
   }
 };
 
-// Keeps what follows from the lane's number inside a loop's body: addresses made ahead of the loop take registers that the backward kernels do
-// not have (with 128 channels they were kept in memory, and every read of one waited for the tile that was on its way).
+// Keeps what follows from the lane's number inside a loop's body: addresses made ahead of the loop take registers that the backward kernels of 128
+// channels do not have (kept in memory, every read of one waits for the tile that is on its way).  What those kernels keep in memory all the same, 2 to
+// 13 registers, is read outside of the loops over tiles but for dk and dv with two wavefronts to a block, which reads three offsets of its loads a tile.
 template <class V, int DW>
 __device__ __forceinline__ int fresh(int lane) {
   if (sizeof(V) == 2 && DW == 128) asm volatile("" : "+v"(lane));
@@ -465,6 +466,8 @@ __device__ __forceinline__ void forward_tile(const char* __restrict__ keys, cons
     }
   };
   uintx4 operand[KB][sizeof(V) == 4 ? 4 : 2];
+  // (bfloat16: each is rounded for its product with v, and not in the sum.  The roundings are independent and partly cancel over the keys: o is off by
+  // 0.0021 of itself where its own rounding alone leaves 0.0017; a second bfloat16 part of each would be half as many products again.)
   const auto exponentials = [&](int b) __attribute__((always_inline)) {
     const float shift = most == -INFINITY ? 0.f : most * c;
     float e[16];
@@ -940,7 +943,8 @@ __global__ __launch_bounds__(64 * NB * NS, sizeof(V) == 4 ? 1 : 2) void attentio
 
 // 32 positions of a head against a wavefront's 32 keys
 // (AHEAD: LDS is read three steps ahead, where the registers for it are there and cost no wavefront: heads of 96, and of 64 where two wavefronts
-// share a block.  2 x 1024 positions, 8 heads of 64: 19.4 -> 16.9 us; with four wavefronts alone, of which three fit a SIMD as it is, 19.8 -> 23.)
+// share a block.  2 x 1024 positions, 8 heads of 64: 20.9 -> 19.0 us; with four wavefronts alone, of which three fit a SIMD as it is, 32 x 196
+// positions, 12 heads of 64: 23 -> 26.)
 template <class V, int DW, bool AHEAD, class Bring>
 __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const char* __restrict__ ders, const float* __restrict__ statL,
                                          const float* __restrict__ statD, char* __restrict__ next, Bring bring_next, const uintx4 (&k)[Tile<V, DW>::steps],
@@ -972,6 +976,7 @@ __device__ __forceinline__ void dkv_tile(const char* __restrict__ queries, const
     for (int r = 0; r < 16; ++r)
       if (8 * (r / 4) + r % 4 < low || 8 * (r / 4) + r % 4 >= high) e[r] = 0.f;
   };
+  // (bfloat16: p is rounded for dv and ds for dk, once each, as p is forward: both are off by 0.0023 of themselves)
   const auto probabilities = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) e[r] = probability<V>(s[r], sums[r], c);
@@ -1333,11 +1338,12 @@ struct Plan {
 };
 
 // Whether two wavefronts share a block of 32 rows or keys.  They make twice as many workgroups of half the length, which bring twice as many
-// tiles.  Rows: where the chip is not filled otherwise (causal, bfloat16, four wavefronts alone -> two to a block.  One sequence of 4096, 4
-// heads of 128 over one: forward 50.6 -> 45.4 us, dq 114 -> 74; 4 of 512, 16 heads of 128: 19.3 -> 17.3 forward; 4 of 2048, 16 heads of 128: 90
-// -> 113, 138 -> 159; 196 positions x 32 x 12 heads of 64: 18.0 -> 19.5, 24.3 -> 31.2).  Keys, whole backward: 4 of 2048 as above 302 -> 345,
-// the one sequence 285 -> 238, 13 packed ones of up to 1100, 32 heads over 8, 354 -> 339, and the 196 positions, whose last tiles hold more that
-// is not there, 47 -> 57; the rule loses on 4096, 32 heads over 8, 552 -> 590.
+// tiles.  Rows: where the chip is not filled otherwise (causal, bfloat16, calls with four wavefronts alone -> two to a block.  4 sequences of 512, 16
+// heads of 128: forward 16.5 -> 16.0 us, dq 24.6 -> 23.1; 2 of 1024, 8 heads of 64: 21.5 -> 20.2, 22.1 -> 17.2; 9 sequences, 6 heads of 75 over 2 in
+// single precision: 87 -> 71, 142 -> 104; one of 4096, 4 heads of 128 over one: dq 112 -> 73, but forward, which slices of keys fill the chip for as
+// well, 45 -> 50; on the other side 4 of 2048, 16 heads of 128: 89 -> 104, 137 -> 154; 196 positions x 32 x 12 heads of 64: dq 23 -> 30).  Keys,
+// whole backward: 4 of 2048 as above 293 -> 327, the one sequence 277 -> 217, 13 packed ones of up to 1100, 32 heads over 8, 331 -> 317, and the 196
+// positions, whose last tiles hold more that is not there, 45 -> 53; the rule loses on 32 heads over 8 of 4096, 559 -> 591, and of 4 x 512, 88 -> 96.
 bool split(const char* name, bool rule) {
   const int forced = tunable(name, 0);
   return forced ? forced == 2 : rule;
@@ -1346,8 +1352,9 @@ bool split(const char* name, bool rule) {
 // How a forward call is cut.  Rows of a sequence on average up to 32: one wavefront a workgroup, and keys are cut into slices until four of
 // those are there for every compute unit; otherwise four wavefronts, and slices until there are two workgroups for each.  A slice has four
 // tiles at least, eight where a tile takes the least time: the partial results are written, read and put together by a launch (bfloat16, heads of 128,
-// causal, slices of two workgroups a compute unit against one slice: one sequence of 8192 of 2 heads 80 and 117 us, of 2048 of 32 heads over 8
-// the same 54; with four workgroups a compute unit 73 and 76, and 4 of 512 of 32 heads over 8 56 instead of 23).
+// causal, slices of two workgroups a compute unit against one slice: one sequence of 8192 of 2 heads 73 and 112 us, of 2048 of 32 heads over 8
+// the same 52, but 2 of 1024 of 8 heads of 64 21 and 15; with four workgroups a compute unit 67 and 75, and 9 sequences of 6 heads of 75 over 2 in single
+// precision 90 instead of 72).
 Plan plan_of(const mcn_attention_geom* g, int backward) {
   Plan l = {};
   l.size = g->dataType == MCN_BFLOAT16 ? 2 : 4;
@@ -1370,8 +1377,8 @@ Plan plan_of(const mcn_attention_geom* g, int backward) {
     l.dqBlocks = split("attention_dq_split", (rows / 128 + sequences) * g->keyHeads < 2 * cus) ? 2 : 4;
     l.dkvBlocks = split("attention_dkv_split", (g->M / 128 + sequences) * (long long)g->keyHeads < (g->N < 512ll * sequences ? 2 : 4) * cus) ? 2 : 4;
     // The heads of a group in several workgroups, whose sums are put together by one more launch, where there are not four workgroups a compute
-    // unit otherwise, two in single precision (whole backward of one sequence of 4096, causal, bfloat16, heads of 128: 4 over one 581 -> 239 us in
-    // four parts, 32 over 8 762 -> 590 in two; 13 packed sequences of 32 over 8, whose workgroups are enough, 339 -> 405 in two)
+    // unit otherwise, two in single precision (whole backward of one sequence of 4096, causal, bfloat16, heads of 128: 4 over one 538 -> 217 us in
+    // four parts, 32 over 8 721 -> 590 in two; 13 packed sequences of 32 over 8, whose workgroups are enough, 317 -> 381 in two)
     const long long groups = std::max(1ll, ((long long)g->M / (32 * l.dkvBlocks) + sequences) * g->keyHeads), want = (l.size == 2 ? 4 : 2) * cus;
     const int forced = tunable("attention_group_parts", 0);
     const int parts = forced ? std::min(forced, l.G) : (int)std::max<long long>(1, std::min<long long>(l.G, (want + groups - 1) / groups));
